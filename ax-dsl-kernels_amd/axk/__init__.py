@@ -35,6 +35,20 @@ __all__ += ["attention", "paged_attention_decode", "paged_decode", "paged_decode
             "store_paged_kv", "paged_decode_fp8", "store_paged_kv_fp8", "paged_decode_i8", "store_paged_kv_i8",
             "paged_prefill", "paged_prefill_workspace"]
 
+from . import blocks  # noqa: E402
+from .blocks import (  # noqa: E402
+    paged_block_scores,
+    paged_decode_blocks,
+    paged_decode_blocks_workspace,
+    paged_evict_pages,
+    paged_key_bounds,
+    paged_select_blocks,
+    store_paged_kv_bounds,
+)
+
+__all__ += ["blocks", "paged_block_scores", "paged_decode_blocks", "paged_decode_blocks_workspace", "paged_evict_pages",
+            "paged_key_bounds", "paged_select_blocks", "store_paged_kv_bounds"]
+
 from . import gdn  # noqa: E402
 from .gdn import gdn_chunk_prefill, gdn_chunk_workspace, gdn_recurrent  # noqa: E402
 

@@ -204,27 +204,6 @@ struct WaveCfg {
   static_assert(RB % 64 == 0 && 1024 % RB == 0, "a tile's V rows split evenly over 1 KiB loads");
 };
 
-// Software FP32 -> E4M3 (OCP e4m3fn) with round-to-nearest-even, as torch's float8_e4m3fn cast: |v| > 464
-// (rounding to 480, past the largest finite value 448) and NaN give NaN (0x7F with the sign), values under
-// 2^-6 round onto the subnormal grid m * 2^-9.
-AXK_DEV uint32_t f32_to_e4m3(float v) {
-  const uint32_t u = __float_as_uint(v), sgn = (u >> 24) & 0x80u, a = u & 0x7fffffffu;
-  const float av = __uint_as_float(a);
-  if (a > 0x7f800000u || av > 464.0f) return sgn | 0x7fu;
-  const int e = (int)(a >> 23) - 127;
-  if (e < -6) return sgn | (uint32_t)rintf(av * 512.0f);  // 0 .. 8 (8 = the smallest normal, code 0x08)
-  const uint32_t mant = a & 0x7fffffu;
-  uint32_t m3 = mant >> 20, ex = (uint32_t)(e + 7);
-  const uint32_t rb = (mant >> 19) & 1u, sticky = mant & 0x7ffffu;
-  if (rb && (sticky || (m3 & 1u))) {
-    if (++m3 == 8u) {
-      m3 = 0u;
-      ++ex;
-    }
-  }
-  return sgn | (ex << 3) | m3;
-}
-
 typedef short axk_i16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kLocalPlanBatch = 63;  // up to this many sequences the kernels derive the plan themselves

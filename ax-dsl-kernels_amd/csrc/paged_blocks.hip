@@ -1,0 +1,1376 @@
+// Sparse attention over a paged KV cache, and eviction of its pages, for gfx950.
+//
+// A page of the cache (layout and page table as in paged_attn.hip) is cut into blocks of `block` consecutive tokens
+// (block a multiple of 16 that divides the page). For every block and KV head, bounds[P, page / block, HKV, 2, D]
+// (bf16) keeps the channel-wise minimum and maximum of the block's keys. One decode step is then
+//   1. paged_kv_write_bounds_kernel  the new tokens' K / V into the cache and into their blocks' bounds
+//      (paged_key_bounds_kernel      the bounds from the cache: after a prefill chunk, or for a whole cache)
+//   2. paged_block_scores_kernel     s[h, j] = max_g sum_d max(q_gd, 0) hi_jd + min(q_gd, 0) lo_jd, which no q_g . k of
+//                                    block j exceeds
+//   3. paged_select_blocks_kernel    the n best blocks of each (sequence, KV head), in ascending order
+//   4. paged_blocks_kernel, paged_blocks_merge_kernel   attention over those blocks (or all of them), and each page's
+//                                    share of it, w_out = decay w_in + sum over the KV head's queries
+// and, when a sequence has grown past its budget,
+//   5. paged_evict_kernel            the page table without the pages of least w.
+#include <math.h>
+
+#include "axk_common.h"
+#include "axk_host.h"
+
+namespace {
+
+constexpr int kSub = 16;       // tokens of a subtile: the rows of one MFMA operand, and the unit of the block size
+constexpr int kMaxGroup = 16;  // query heads per KV head (the other side of that operand)
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Sequence b of a page table with nnz entries: its first entry, its pages and its tokens. Offsets outside the table and
+// a last page longer than a page are clamped, so that no index built from them leaves its array.
+struct Seq {
+  int pb, np;
+  int64_t len;
+};
+AXK_DEV Seq seq_of(const int* __restrict__ indptr, const int* __restrict__ last, int b, int page, int nnz) {
+  Seq s;
+  s.pb = min(max(indptr[b], 0), nnz);
+  s.np = min(max(indptr[b + 1], s.pb), nnz) - s.pb;
+  s.len = s.np ? (int64_t)(s.np - 1) * page + min(max(last[b], 0), page) : 0;
+  return s;
+}
+
+// The sequence that holds page-table entry e (the number of sequences ending at or before it), by one wave.
+AXK_DEV int owner_of(const int* __restrict__ indptr, int batch, int e) {
+  int n = 0;
+  for (int b0 = 0; b0 < batch; b0 += 64) {
+    const int b = b0 + (int)(threadIdx.x & 63);
+    n += __popcll(__ballot(b < batch && indptr[b + 1] <= e));
+  }
+  return n;
+}
+
+// Two bf16 values (one dword) as two 16-bit integers of the same order, and back (the map is its own inverse): the 15
+// low bits of a negative value are flipped. NaN lies beyond the infinity of its sign.
+typedef short axk_s16x2 __attribute__((ext_vector_type(2)));
+AXK_DEV axk_s16x2 bf16_order(uint32_t w) {
+  const axk_s16x2 x = __builtin_bit_cast(axk_s16x2, w);
+  return x ^ ((x >> (short)15) & (short)0x7fff);
+}
+AXK_DEV uint32_t bf16_unorder(axk_s16x2 x) { return __builtin_bit_cast(uint32_t, x ^ ((x >> (short)15) & (short)0x7fff)); }
+
+// 16 bytes of stored keys as bf16 pairs in order: 4 dwords of a bf16 cache, 8 of an FP8 one (stored * inv_scale).
+template <int F8>
+AXK_DEV void stored_pairs(const axk_u32x4 w, float inv_scale, uint32_t (&out)[F8 ? 8 : 4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (F8) {
+      out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], inv_scale, false));
+      out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], inv_scale, true));
+    } else {
+      out[i] = w[i];
+    }
+  }
+}
+
+// ---- key bounds ----
+// The new rows' K / V written at loc[r] = (page, slot), and folded into the bounds of their blocks: a block that holds a
+// new row at its first slot starts afresh, every other one widens what it had. One workgroup per row; the first row of
+// the call that falls into a block folds all of them, so that rows of one block never race, and where two rows name one
+// slot the last one is stored (both are folded). Two launches' worth of work in one: a decode step pays a launch, the
+// dependent reads location, then row and bounds, and nothing else.
+template <int F8>
+__global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
+    const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, unsigned char* __restrict__ cache,
+    uint16_t* __restrict__ bounds, const int* __restrict__ loc, int rows, int hkv, int d, int page_size, int block,
+    int64_t num_pages, float kv_scale, int* __restrict__ status) {
+  __shared__ int s_rows[256];
+  __shared__ int s_count, s_first, s_fresh, s_over;
+  const int tid = threadIdx.x, r = blockIdx.x;
+  const int page = loc[2 * r], off = loc[2 * r + 1];
+  if (page < 0 || page >= num_pages || off < 0 || off >= page_size) {
+    if (status && tid == 0) *status = 1;
+    return;
+  }
+  if (tid == 0) {
+    s_first = 1;
+    s_fresh = 0;
+    s_over = 0;
+  }
+  __syncthreads();
+  const int blk = off / block;
+  // which rows of the call share the block: an earlier one owns it, a later one at the same slot is the one stored
+  for (int i = tid; i < rows; i += 256) {
+    const int p = loc[2 * i], o = loc[2 * i + 1];
+    if (p != page || o < 0 || o >= page_size || o / block != blk) continue;
+    if (i < r) s_first = 0;
+    if (o % block == 0) s_fresh = 1;
+    if (i > r && o == off) s_over = 1;
+  }
+  __syncthreads();
+  const int row = hkv * d;  // values of one token row
+  if (!s_over) {
+    for (int i = tid; i < 2 * (row / 8); i += 256) {
+      const int plane = i >= row / 8, ch = plane ? i - row / 8 : i;
+      const uint4 src = *reinterpret_cast<const uint4*>((plane ? v : k) + (int64_t)r * row + ch * 8);
+      const int64_t at = (((int64_t)page * 2 + plane) * page_size + off) * row + ch * 8;
+      if constexpr (F8) {
+        const uint32_t w[4] = {src.x, src.y, src.z, src.w};
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __uint_as_float(e & 1 ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
+          const uint32_t c = f32_to_e4m3(round_bf16(x * kv_scale));
+          if (e < 4) lo |= c << (8 * e); else hi |= c << (8 * (e - 4));
+        }
+        *reinterpret_cast<uint2*>(cache + at) = make_uint2(lo, hi);
+      } else {
+        *reinterpret_cast<uint4*>(cache + 2 * at) = src;
+      }
+    }
+  }
+  if (!s_first) return;
+  const int fresh = s_fresh;
+  uint16_t* bb = bounds + ((int64_t)page * (page_size / block) + blk) * hkv * 2 * d;
+  const float inv_scale = 1.0f / kv_scale;
+  for (int base = r & ~255; base < rows; base += 256) {  // the call's rows from this one on, 256 at a time
+    __syncthreads();
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    const int i = base + tid;
+    if (i >= r && i < rows) {
+      const int p = loc[2 * i], o = loc[2 * i + 1];
+      if (p == page && o >= 0 && o < page_size && o / block == blk) s_rows[atomicAdd(&s_count, 1)] = i;
+    }
+    __syncthreads();
+    const int n = s_count;
+    for (int c = tid; n && c < row / 8; c += 256) {  // 8 channels of one head at a time
+      const int head = c * 8 / d, ch = c * 8 - head * d;
+      uint16_t* lo_p = bb + (int64_t)head * 2 * d + ch;
+      uint4* lo4 = reinterpret_cast<uint4*>(lo_p);
+      uint4* hi4 = reinterpret_cast<uint4*>(lo_p + d);
+      axk_s16x2 lo[4], hi[4];
+      const bool from = !fresh || base > r;  // the bounds already there count (the list's first row has index >= r)
+      const uint4 l0 = *lo4, h0 = *hi4;
+      const uint32_t lw[4] = {l0.x, l0.y, l0.z, l0.w}, hw[4] = {h0.x, h0.y, h0.z, h0.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = from ? bf16_order(lw[e]) : (axk_s16x2)(short)0x7fff;
+        hi[e] = from ? bf16_order(hw[e]) : (axk_s16x2)(short)-0x8000;
+      }
+      for (int j = 0; j < n; ++j) {
+        const uint4 x4 = *reinterpret_cast<const uint4*>(k + (int64_t)s_rows[j] * row + c * 8);
+        uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (F8) {
+            const uint32_t c0 = f32_to_e4m3(round_bf16(__uint_as_float(x[e] << 16) * kv_scale));
+            const uint32_t c1 = f32_to_e4m3(round_bf16(__uint_as_float(x[e] & 0xffff0000u) * kv_scale));
+            x[e] = __builtin_bit_cast(uint32_t,
+                                      __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c0 | (c1 << 8), inv_scale, false));
+          }
+          lo[e] = __builtin_elementwise_min(lo[e], bf16_order(x[e]));
+          hi[e] = __builtin_elementwise_max(hi[e], bf16_order(x[e]));
+        }
+      }
+      *lo4 = make_uint4(bf16_unorder(lo[0]), bf16_unorder(lo[1]), bf16_unorder(lo[2]), bf16_unorder(lo[3]));
+      *hi4 = make_uint4(bf16_unorder(hi[0]), bf16_unorder(hi[1]), bf16_unorder(hi[2]), bf16_unorder(hi[3]));
+    }
+  }
+}
+
+// The bounds of every block of the page table that reaches past start[b] (all of them without start), from the cache.
+// One workgroup per block: its K rows are one contiguous run of tokens x HKV x D values, read 16 bytes a lane, a column
+// of 8 (FP8: 16) channels kept by as many lanes as the workgroup has to spare and joined through LDS. Minimum and
+// maximum are taken on the bf16 bits as ordered 16-bit integers, two values an instruction. Bound by the K bytes.
+template <int F8>
+__global__ __launch_bounds__(256) void paged_key_bounds_kernel(
+    const unsigned char* __restrict__ cache, uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
+    const int* __restrict__ indices, const int* __restrict__ last, const int* __restrict__ start, int nnz, int batch,
+    int hkv, int d, int page_size, int block, int64_t num_pages, float inv_scale, int* __restrict__ status) {
+  constexpr int N = F8 ? 8 : 4;      // dwords of bf16 pairs a lane keeps
+  constexpr int E = 2 * N;           // channels a lane keeps
+  constexpr int B = F8 ? 1 : 2;      // bytes of a stored value
+  __shared__ axk_s16x2 s_lo[256 * N], s_hi[256 * N];
+  const int tid = threadIdx.x;
+  const int bpp = page_size / block;
+  const int entry = blockIdx.x / bpp, sub = blockIdx.x - entry * bpp;
+  const int b = owner_of(indptr, batch, entry);
+  if (b >= batch) return;  // past the last sequence
+  const Seq s = seq_of(indptr, last, b, page_size, nnz);
+  const int64_t t0 = (int64_t)(entry - s.pb) * page_size + (int64_t)sub * block;
+  const int rows = (int)min((int64_t)block, s.len - t0);
+  if (entry < s.pb || rows <= 0 || (start && t0 + block <= start[b])) return;
+  const int page = indices[entry];
+  if (page < 0 || page >= num_pages) {
+    if (status && tid == 0) *status = 1;
+    return;
+  }
+  const int row = hkv * d;
+  const int cols = row / E;  // lanes that one token row takes
+  const unsigned char* src = cache + ((int64_t)page * 2 * page_size + (int64_t)sub * block) * row * B;
+  uint16_t* dst = bounds + ((int64_t)page * bpp + sub) * hkv * 2 * d;
+  for (int c0 = 0; c0 < cols; c0 += 256) {
+    const int w = min(cols - c0, 256), lanes = 256 / w;  // columns of this pass, and lanes to each
+    const int rl = tid / w, c = c0 + tid - rl * w;
+    axk_s16x2 lo[N], hi[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      lo[e] = (axk_s16x2)(short)0x7fff;
+      hi[e] = (axk_s16x2)(short)-0x8000;
+    }
+    if (rl < lanes) {
+#pragma unroll 4
+      for (int t = rl; t < rows; t += lanes) {
+        uint32_t x[N];
+        stored_pairs<F8>(load_nt(src + ((int64_t)t * row + c * E) * B), inv_scale, x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          lo[e] = __builtin_elementwise_min(lo[e], bf16_order(x[e]));
+          hi[e] = __builtin_elementwise_max(hi[e], bf16_order(x[e]));
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      s_lo[e * 256 + tid] = lo[e];
+      s_hi[e * 256 + tid] = hi[e];
+    }
+    __syncthreads();
+    for (int i = tid; i < w * N; i += 256) {
+      const int e = i / w, cc = i - e * w;
+      axk_s16x2 l = s_lo[e * 256 + cc], h = s_hi[e * 256 + cc];
+      for (int j = 1; j < lanes; ++j) {
+        l = __builtin_elementwise_min(l, s_lo[e * 256 + j * w + cc]);
+        h = __builtin_elementwise_max(h, s_hi[e * 256 + j * w + cc]);
+      }
+      const int at = (c0 + cc) * E + 2 * e, head = at / d;
+      uint32_t* o = reinterpret_cast<uint32_t*>(dst + (int64_t)head * 2 * d + (at - head * d));
+      o[0] = bf16_unorder(l);
+      o[d / 2] = bf16_unorder(h);
+    }
+  }
+}
+
+// ---- block scores ----
+// max(q lo, q hi) per channel is q+ hi + q- lo with q+ = max(q, 0), q- = min(q, 0): the score of 16 blocks for the 16
+// (padded) heads of a group is one chain of 2 D / 32 16x16x32 MFMAs, blocks as rows, and a block's bounds are read once.
+// One wave per (16 blocks, KV head); a tile that spans sequences is computed once with each one's queries.
+template <int D>
+__global__ __launch_bounds__(256) void paged_block_scores_kernel(
+    const uint16_t* __restrict__ q, const uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
+    const int* __restrict__ indices, const int* __restrict__ last, float* __restrict__ scores, int nnz, int batch,
+    int hq, int hkv, int page_size, int block, int64_t num_pages, int64_t units, int* __restrict__ status) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (unit >= units) return;
+  const int group = hq / hkv, bpp = page_size / block;
+  const int64_t total = (int64_t)nnz * bpp;
+  const int64_t tile = unit / hkv;
+  const int h = (int)(unit - tile * hkv);
+  // lane l16 of each lane group looks at block tile * 16 + l16
+  const int64_t f = tile * 16 + l16;
+  const int e = (int)(min(f, total - 1) / bpp);
+  const int first = owner_of(indptr, batch, __builtin_amdgcn_readlane(e, 0));
+  const int lastb = owner_of(indptr, batch, __builtin_amdgcn_readlane(e, 15));
+  const int id = indices[e];
+  const bool good = id >= 0 && id < num_pages;
+  const int sub = (int)(f - (int64_t)e * bpp);
+  const uint16_t* row = bounds + (((int64_t)(good ? id : 0) * bpp + (f < total ? sub : 0)) * hkv + h) * 2 * D + 8 * g;
+  axk_bf16x8 lo[D / 32], hi[D / 32];
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    lo[s] = load_bf16x8(row + 32 * s);
+    hi[s] = load_bf16x8(row + D + 32 * s);
+  }
+  for (int b = first; b <= min(lastb, batch - 1); ++b) {
+    const Seq sq = seq_of(indptr, last, b, page_size, nnz);
+    axk_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const uint16_t* qr = q + ((int64_t)b * hq + h * group + l16) * D + 8 * g;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      // bf16 sign and order agree with those of the bits as 16-bit integers
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      const s16x8 x = l16 < group ? *reinterpret_cast<const s16x8*>(qr + 32 * s) : (s16x8)(short)0;
+      const s16x8 pos = __builtin_elementwise_max(x, (s16x8)(short)0), neg = __builtin_elementwise_min(x, (s16x8)(short)0);
+      acc = mfma_bf16_16x16x32(hi[s], __builtin_bit_cast(axk_bf16x8, pos), acc);
+      acc = mfma_bf16_16x16x32(lo[s], __builtin_bit_cast(axk_bf16x8, neg), acc);
+    }
+    // acc[i]: block tile * 16 + 4 g + i, head l16: the maximum over the group's heads
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = l16 < group ? acc[i] : -INFINITY;
+      float n = x != x ? x : 0.f;  // a NaN of any head is the block's score (fmaxf would drop it)
+      x = fmaxf(x, dpp_move<0xB1>(x, x));
+      x = fmaxf(x, dpp_move<0x4E>(x, x));
+      x = fmaxf(x, dpp_move<0x141>(x, x));
+      x = fmaxf(x, dpp_move<0x140>(x, x));
+      n = group_sum<16>(n);
+      if (n != n) x = n;
+      const int64_t fi = tile * 16 + 4 * g + i;
+      const int64_t t0 = (fi - (int64_t)sq.pb * bpp) * block;  // the block's first token
+      const bool bad = __shfl((int)!good, 4 * g + i, 64) != 0;
+      if (l16 == 0 && fi < total && t0 >= 0 && t0 < (int64_t)sq.np * page_size) {
+        const bool there = t0 < sq.len;
+        scores[h * total + fi] = there && !bad ? x : -INFINITY;
+        if (there && bad && status) *status = 1;
+      }
+    }
+  }
+}
+
+// ---- the `want` largest of a row ----
+// Radix selection by one workgroup of T threads: the bits that all keys share are skipped (from their minimum and
+// maximum), then 8 bits at a time are counted in LDS until the smallest key that is taken is known, or all keys that
+// agree with it so far are taken. Up to 16 T keys stay in registers; a longer row is read again in each step. Equal keys
+// at the border are taken by the lowest index. emit(i, taken, rank) is called for every index, rank = the indices below
+// i that are taken.
+constexpr int kKeys = 16;  // keys a thread holds
+template <class Key, int T>
+struct PickLds {
+  unsigned hist[2][256];
+  Key lo[T / 64], hi[T / 64];
+  unsigned sums[T / 64];
+  unsigned digit, above, inside;
+};
+
+template <class Key, int T, class Load, class Emit>
+AXK_DEV void pick_largest(int count, int want, const Load& load, const Emit& emit, PickLds<Key, T>& lds) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tile = T * kKeys, tiles = (count + tile - 1) / tile;
+  const int per = tiles > 1 ? kKeys : (count + T - 1) / T;  // consecutive indices a thread holds
+  Key key[kKeys];
+  auto load_tile = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      const int at = t * tile + tid * per + i;
+      key[i] = i < per && at < count ? load(at) : (Key)0;
+    }
+  };
+  auto there = [&](int t, int i) { return i < per && t * tile + tid * per + i < count; };
+  if (tiles == 1) load_tile(0);
+  Key lo = ~(Key)0, hi = 0;
+  for (int t = 0; t < tiles; ++t) {
+    if (tiles > 1) load_tile(t);
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i)
+      if (there(t, i)) {
+        lo = min(lo, key[i]);
+        hi = max(hi, key[i]);
+      }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    lo = min(lo, (Key)__shfl_xor(lo, o, 64));
+    hi = max(hi, (Key)__shfl_xor(hi, o, 64));
+  }
+  if (lane == 0) {
+    lds.lo[wave] = lo;
+    lds.hi[wave] = hi;
+  }
+  for (int i = tid; i < 256; i += T) lds.hist[0][i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < T / 64; ++w) {
+    lo = min(lo, lds.lo[w]);
+    hi = max(hi, lds.hi[w]);
+  }
+  constexpr int kBits = 8 * sizeof(Key);
+  int pos = lo == hi ? 0 : kBits - (sizeof(Key) == 8 ? __clzll((long long)(lo ^ hi)) : __clz((int)(lo ^ hi)));
+  Key prefix = pos >= kBits ? (Key)0 : (hi >> pos) << pos;  // the border key's bits from `pos` up
+  unsigned remaining = (unsigned)want;                      // keys to take among those that agree with it
+  bool all = false;
+  for (int step = 0; pos > 0 && !all; ++step) {
+    const int w = min(8, pos);
+    const Key mask = pos >= kBits ? (Key)0 : ~(Key)0 << pos;
+    pos -= w;
+    unsigned* hist = lds.hist[step & 1];
+    for (int t = 0; t < tiles; ++t) {
+      if (tiles > 1) load_tile(t);
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i)
+        if (there(t, i) && ((key[i] ^ prefix) & mask) == 0)
+          atomicAdd(&hist[(unsigned)(key[i] >> pos) & ((1u << w) - 1u)], 1u);
+    }
+    __syncthreads();
+    if (wave == 0) {  // lane l: bins 255 - 4 l .. 252 - 4 l, from the top
+      unsigned c[4], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += c[i] = hist[255 - 4 * lane - i];
+      unsigned incl = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const unsigned x = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += x;
+      }
+      unsigned before = incl - sum;
+      if (before < remaining && remaining <= incl) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (before < remaining && remaining <= before + c[i]) {
+            lds.digit = 255 - 4 * lane - i;
+            lds.above = before;
+            lds.inside = c[i];
+          }
+          before += c[i];
+        }
+      }
+    } else {
+      for (int i = tid - 64; i < 256; i += T - 64) lds.hist[(step + 1) & 1][i] = 0;
+    }
+    __syncthreads();
+    prefix |= (Key)lds.digit << pos;
+    remaining -= lds.above;
+    all = lds.inside == remaining;
+  }
+  // taken: keys above the border (compared from `pos` up), and the first `remaining` of those on it
+  const Key border = prefix >> pos;
+  unsigned above0 = 0, on0 = 0;
+  for (int t = 0; t < tiles; ++t) {
+    if (tiles > 1) load_tile(t);
+    unsigned n = 0;  // above in the high half, on the border in the low half: at most 16 T < 65536 of each
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i)
+      if (there(t, i)) {
+        const Key x = key[i] >> pos;
+        n += x > border ? 0x10000u : x == border ? 1u : 0u;
+      }
+    unsigned incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned x = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += x;
+    }
+    __syncthreads();  // the sums of the tile before have been read
+    if (lane == 63) lds.sums[wave] = incl;
+    __syncthreads();
+    unsigned before = incl - n, total = 0;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) {
+      if (w < wave) before += lds.sums[w];
+      total += lds.sums[w];
+    }
+    unsigned above = above0 + (before >> 16), on = on0 + (before & 0xffffu);
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i)
+      if (there(t, i)) {
+        const Key x = key[i] >> pos;
+        emit(t * tile + tid * per + i, x > border || (x == border && on < remaining), (int)(above + min(on, remaining)));
+        above += x > border;
+        on += x == border;
+      }
+    above0 += total >> 16;
+    on0 += total & 0xffffu;
+  }
+}
+
+// Floats as integers of the same order: NaN of either sign above +inf, zeros of either sign equal.
+AXK_DEV uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  if (x != x) return 0xffffffffu;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+AXK_DEV uint64_t order_key(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+  if (x != x) return ~0ull;
+  return u >> 63 ? ~u : u | (1ull << 63);
+}
+
+// One workgroup per (sequence, KV head): its n best blocks, the first `first` and last `keep_last` always among them.
+template <int T>
+__global__ __launch_bounds__(T) void paged_select_blocks_kernel(const float* __restrict__ scores,
+                                                                const int* __restrict__ indptr,
+                                                                const int* __restrict__ last, int* __restrict__ out,
+                                                                int nnz, int hkv, int page_size, int block, int n,
+                                                                int first, int keep_last) {
+  __shared__ PickLds<uint32_t, T> lds;
+  const int tid = threadIdx.x, b = blockIdx.x / hkv, h = blockIdx.x - b * hkv;
+  const Seq s = seq_of(indptr, last, b, page_size, nnz);
+  const int bpp = page_size / block;
+  const int nb = (int)((s.len + block - 1) / block);
+  int* o = out + (int64_t)blockIdx.x * n;
+  if (nb <= n) {
+    for (int i = tid; i < n; i += T) o[i] = i < nb ? i : -1;
+    return;
+  }
+  for (int i = tid; i < first; i += T) o[i] = i;
+  for (int i = tid; i < keep_last; i += T) o[n - keep_last + i] = nb - keep_last + i;
+  const int want = n - first - keep_last;
+  if (want == 0) return;
+  const float* row = scores + (int64_t)h * nnz * bpp + (int64_t)s.pb * bpp + first;
+  pick_largest<uint32_t, T>(
+      nb - first - keep_last, want, [&](int i) { return order_key(row[i]); },
+      [&](int i, bool taken, int rank) {
+        if (taken) o[first + rank] = first + i;
+      },
+      lds);
+}
+
+// ---- decode over blocks ----
+// One query token per sequence over the listed blocks of each KV head (or all of them), split over pieces of `ps`
+// subtiles of 16 tokens. Everything a wave needs stays in its registers; it takes two subtiles (32 tokens) a step:
+//   S^T = K Q^T   16x16x32 MFMA, K rows straight from memory as the A operand (lane = token, 16 bytes of its row), Q the
+//                 B operand, the group's heads as columns;
+//   softmax       running maximum and sum per head, fp32, exp2 domain;
+//   O^T += V^T P^T  the score accumulator is the P^T operand as it stands if MFMA k index (lane group g, j) is token
+//                 4 g + j % 4 of subtile j / 4. V rows are loaded in that order, lane l16 holding D / 16 channels of eight
+//                 tokens, so that the transposition V^T needs is one byte permute per two values, without LDS.
+// The four waves of a piece take its steps in turn and are joined through LDS; pieces by the merge kernel.
+template <int D, int F8>
+struct BlkCfg {
+  static constexpr int B = F8 ? 1 : 2;             // bytes of a stored value
+  static constexpr int KL = D * B / 64;            // 16-byte K loads a lane makes per subtile
+  static constexpr int KS = D / 32;                // QK k-steps
+  static constexpr int E = F8 ? D / 16 : (D >= 128 ? 8 : D / 16);  // channels of a V load
+  static constexpr int NH = D / 16 / E;            // V loads a lane makes per token
+  static constexpr int VW = E * B / 4;             // dwords of a V load
+  static constexpr int ACC = D / 16;               // 16x16 O^T tiles
+  // The next step's K is loaded before this one's softmax where the registers hold it (bf16 at D = 256: a spill).
+  static constexpr bool AHEAD = F8 || D < 256;
+};
+
+struct BlkArgs {
+  const uint16_t* q;
+  const unsigned char* cache;
+  const int *indptr, *indices, *last;
+  const int* blocks;  // [batch, hkv, n], or null: every block
+  int n, block;
+  int nnz, batch, hq, hkv, page;
+  int64_t num_pages;
+  float scale;      // sm_scale * log2(e)
+  float inv_scale;  // of an FP8 cache
+  int ps;           // subtiles of a piece
+  int pieces;       // pieces of a row (listed blocks), or of all sequences of one KV head (every block)
+  int direct;       // every row is one piece: no merge
+  uint16_t* out;
+  float2* ml;       // [rows or hkv][pieces][group]: maximum and sum
+  float* po;        // ... [D]
+  float2* stat;     // per (row or hkv, subtile, head) reference and sum, for the page weights; null: not wanted
+  int* status;
+};
+
+// Which sequence and which of its pieces flat piece `it` of a KV head is, where every block is attended: the pieces of
+// a sequence are as many as its subtiles need. b = batch past the last one. All threads of a workgroup of 256.
+struct PieceOf {
+  int b, piece;
+};
+AXK_DEV int pieces_of(const Seq& s, int ps) { return (int)((s.len + (int64_t)kSub * ps - 1) / ((int64_t)kSub * ps)); }
+AXK_DEV PieceOf find_piece(const BlkArgs& a, int it, int* sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 256) {
+    const int b = b0 + tid;
+    const int cnt = b < a.batch ? pieces_of(seq_of(a.indptr, a.last, b, a.page, a.nnz), a.ps) : 0;
+    int incl = cnt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += x;
+    }
+    if (tid == 0) sh[4] = a.batch;
+    if (lane == 63) sh[wave] = incl;
+    __syncthreads();
+    int before = base + incl - cnt;
+    for (int w = 0; w < wave; ++w) before += sh[w];
+    if (it >= before && it < before + cnt) {
+      sh[4] = b;
+      sh[5] = it - before;
+    }
+    base += sh[0] + sh[1] + sh[2] + sh[3];
+    __syncthreads();
+    if (sh[4] < a.batch) return {sh[4], sh[5]};
+    __syncthreads();
+  }
+  return {a.batch, 0};
+}
+// Pieces of the sequences before b, where every block is attended (all threads of a workgroup of 256).
+AXK_DEV int pieces_before(const BlkArgs& a, int b, int* sh) {
+  int n = 0;
+  for (int i = threadIdx.x; i < b; i += 256) n += pieces_of(seq_of(a.indptr, a.last, i, a.page, a.nnz), a.ps);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = n;
+  __syncthreads();
+  return sh[0] + sh[1] + sh[2] + sh[3];
+}
+
+// Listed block `slot` of a row: its logical block, or -1 for padding, a block past the sequence's end, or one that does
+// not lie above its predecessor in the list (`bad` is then set, but for padding).
+AXK_DEV int listed_block(const int* __restrict__ list, int slot, int64_t nblocks, bool* bad) {
+  const int id = list[slot], prev = slot ? list[slot - 1] : -1;
+  *bad = id < -1 || id >= nblocks || (id >= 0 && slot && prev >= id);
+  return *bad ? -1 : id;
+}
+
+constexpr int kMaxPs = 128;  // subtiles of a piece, at most
+
+template <int D, int F8>
+__global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
+  using C = BlkCfg<D, F8>;
+  __shared__ __align__(16) float s_o[2][C::ACC * 256];
+  __shared__ int64_t s_base[kMaxPs];
+  __shared__ int s_valid[kMaxPs];
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ int s_find[8];
+  __shared__ int s_end;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int group = a.hq / a.hkv;
+  int b, h, piece;
+  int64_t item;
+  if (a.blocks) {
+    item = blockIdx.x;
+    const int row = blockIdx.x / a.pieces;
+    piece = blockIdx.x - row * a.pieces;
+    b = row / a.hkv;
+    h = row - b * a.hkv;
+  } else {
+    h = blockIdx.y;
+    item = (int64_t)h * a.pieces + blockIdx.x;
+    const PieceOf p = find_piece(a, blockIdx.x, s_find);
+    b = p.b;
+    piece = p.piece;
+    if (b >= a.batch) return;
+  }
+  const Seq s = seq_of(a.indptr, a.last, b, a.page, a.nnz);
+  // Q first: its loads are under way while the subtiles' places are looked up
+  axk_bf16x8 qf[C::KS];
+#pragma unroll
+  for (int i = 0; i < C::KS; ++i) {
+    const int at = F8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
+    qf[i] = l16 < group ? load_bf16x8(a.q + ((int64_t)b * a.hq + h * group + l16) * D + at) : zero_bf16x8();
+  }
+  // the piece's subtiles: where each lies in the cache, and how many of its tokens count
+  const int64_t rowb = (int64_t)a.hkv * D * C::B;  // bytes of a token row
+  const int spb = a.block / kSub, spp = a.page / kSub;
+  const int64_t nsub = a.blocks ? (int64_t)a.n * spb : (s.len + kSub - 1) / kSub;  // of the row
+  const int64_t sub0 = (int64_t)piece * a.ps;
+  const int count = (int)min((int64_t)a.ps, nsub - sub0);
+  if (tid == 0) s_end = 0;
+  __syncthreads();
+  for (int i = tid; i < a.ps; i += 256) {
+    int valid = 0;
+    int64_t base = 0;
+    if (i < count) {
+      int64_t t0 = (sub0 + i) * kSub;  // the subtile's first token
+      bool bad = false;
+      if (a.blocks) {
+        const int slot = (int)((sub0 + i) / spb);
+        const int id = listed_block(a.blocks + ((int64_t)b * a.hkv + h) * a.n, slot, (s.len + a.block - 1) / a.block, &bad);
+        t0 = id < 0 ? s.len : (int64_t)id * a.block + ((sub0 + i) - (int64_t)slot * spb) * kSub;
+      }
+      valid = (int)min(max(s.len - t0, (int64_t)0), (int64_t)kSub);
+      if (valid) {
+        const int p = (int)(t0 / a.page), id = a.indices[s.pb + p];
+        if (id < 0 || id >= a.num_pages) {
+          bad = true;
+          valid = 0;
+        } else {
+          base = ((int64_t)id * 2 * a.page + (t0 - (int64_t)p * a.page)) * rowb;
+        }
+      }
+      if (bad && a.status) *a.status = 1;
+    }
+    s_base[i] = base;
+    s_valid[i] = valid;
+    if (valid) atomicMax(&s_end, i + 1);
+  }
+  __syncthreads();
+  const int end = s_end;  // what follows is padding of the list
+  const int64_t stat_at = (a.blocks ? ((int64_t)b * a.hkv + h) * nsub : ((int64_t)h * a.nnz + s.pb) * spp) + sub0;
+  if (a.stat)
+    for (int i = ((end + 1) & ~1) * group + tid; i < count * group; i += 256)
+      a.stat[stat_at * group + i] = make_float2(0.f, 0.f);
+
+  axk_f32x4 acc[C::ACC];
+#pragma unroll
+  for (int i = 0; i < C::ACC; ++i) acc[i] = (axk_f32x4){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const unsigned char* cache_h = a.cache + (int64_t)h * D * C::B;
+  const int64_t vplane = (int64_t)a.page * rowb;
+  const uint32_t k_off = (uint32_t)(l16 * rowb + g * 16);
+  const uint32_t v_off = (uint32_t)(4 * g * rowb + l16 * C::E * C::B);
+  typedef uint32_t vload __attribute__((ext_vector_type(C::VW)));
+  axk_u32x4 kr[2][C::KL];
+  auto load_k = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const unsigned char* p = static_cast<const unsigned char*>(uniform_ptr(cache_h + s_base[2 * t + u]));
+#pragma unroll
+      for (int i = 0; i < C::KL; ++i) kr[u][i] = load_nt(p + k_off + 64 * i);
+    }
+  };
+  const int tiles = (end + 1) / 2;
+  if (C::AHEAD && wave < tiles) load_k(wave);
+  for (int t = wave; t < tiles; t += 4) {
+    if (!C::AHEAD) load_k(t);
+    const int nv0 = __builtin_amdgcn_readfirstlane(s_valid[2 * t]), nv1 = __builtin_amdgcn_readfirstlane(s_valid[2 * t + 1]);
+    vload vr[8][C::NH];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const unsigned char* p = static_cast<const unsigned char*>(uniform_ptr(cache_h + s_base[2 * t + u] + vplane));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int n = 0; n < C::NH; ++n)
+          vr[4 * u + j][n] = __builtin_nontemporal_load(
+              reinterpret_cast<const vload*>(p + v_off + j * (uint32_t)rowb + n * 16 * C::E * C::B));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    axk_f32x4 sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      sc[u] = (axk_f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < C::KL; ++i) {
+        uint32_t x[F8 ? 8 : 4];
+        stored_pairs<F8>(kr[u][i], a.inv_scale, x);
+        const axk_u32x4 x0 = {x[0], x[1], x[2], x[3]};
+        sc[u] = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, x0), qf[F8 ? 2 * i : i], sc[u]);
+        if constexpr (F8) {
+          const axk_u32x4 x1 = {x[4], x[5], x[6], x[7]};
+          sc[u] = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, x1), qf[2 * i + 1], sc[u]);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (C::AHEAD && t + 4 < tiles) load_k(t + 4);
+    __builtin_amdgcn_sched_barrier(0);
+    // sc[u][i]: token 4 g + i of subtile u, head l16
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = 4 * g + i < nv0 ? sc[0][i] * a.scale : -INFINITY;
+      x[4 + i] = 4 * g + i < nv1 ? sc[1][i] * a.scale : -INFINITY;
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    top = fmaxf(m, xor32_max(xor16_max(top)));
+    const float ref = top == -INFINITY ? 0.f : top;  // nothing counted yet: exp2(-inf) = 0 throughout
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = top;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+    const float sum0 = (x[0] + x[1]) + (x[2] + x[3]), sum1 = (x[4] + x[5]) + (x[6] + x[7]);
+    l = l * alpha + (sum0 + sum1);
+    if (a.stat) {
+      const float t0 = xor32_sum(xor16_sum(sum0)), t1 = xor32_sum(xor16_sum(sum1));
+      if (g < 2 && 2 * t + g < count && l16 < group)  // lane group 0: the first subtile, 1: the second
+        a.stat[(stat_at + 2 * t + g) * group + l16] = make_float2(ref, g ? t1 : t0);
+    }
+    if (__any(alpha != 1.0f)) {
+#pragma unroll
+      for (int i = 0; i < C::ACC; ++i) acc[i] *= alpha;
+    }
+    const axk_u32x4 pw = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                          pack_bf16x2(x[6], x[7])};
+    const axk_bf16x8 pf = __builtin_bit_cast(axk_bf16x8, pw);
+    if (nv0 < kSub || nv1 < kSub) {  // rows that do not count may hold anything: 0 * NaN is not 0
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (4 * g + (j & 3) >= (j < 4 ? nv0 : nv1))
+#pragma unroll
+          for (int n = 0; n < C::NH; ++n) vr[j][n] = (vload)0u;
+    }
+#pragma unroll
+    for (int n = 0; n < C::NH; ++n)
+#pragma unroll
+      for (int w = 0; w < C::VW; ++w) {
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (F8) {
+          uint32_t lo[4], hi[4];  // bytes (c, c + 1) of token pairs: [t.c, t'.c, t.c+1, t'.c+1]
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            lo[p] = __builtin_amdgcn_perm(vr[2 * p + 1][n][w], vr[2 * p][n][w], 0x05010400u);
+            hi[p] = __builtin_amdgcn_perm(vr[2 * p + 1][n][w], vr[2 * p][n][w], 0x07030602u);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            axk_u32x4 f;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const uint32_t src = e < 2 ? lo[p] : hi[p];
+              f[p] = __builtin_bit_cast(uint32_t, e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, a.inv_scale, true)
+                                                        : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, a.inv_scale, false));
+            }
+            axk_f32x4& o = acc[n * C::E + 4 * w + e];
+            o = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, f), pf, o);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            axk_u32x4 f;
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+              f[p] = __builtin_amdgcn_perm(vr[2 * p + 1][n][w], vr[2 * p][n][w], e ? 0x07060302u : 0x05040100u);
+            axk_f32x4& o = acc[n * C::E + 2 * w + e];
+            o = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, f), pf, o);
+          }
+        }
+      }
+  }
+
+  // the four waves' results against one maximum
+  l = xor32_sum(xor16_sum(l));
+  if (g == 0) {
+    s_m[wave][l16] = m;
+    s_l[wave][l16] = l;
+  }
+  __syncthreads();
+  float top = fmaxf(fmaxf(s_m[0][l16], s_m[1][l16]), fmaxf(s_m[2][l16], s_m[3][l16]));
+  if (top == -INFINITY) top = 0.f;
+  const float mine = __builtin_amdgcn_exp2f(m - top);
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) l += s_l[w][l16] * __builtin_amdgcn_exp2f(s_m[w][l16] - top);
+#pragma unroll
+  for (int i = 0; i < C::ACC; ++i) acc[i] *= mine;
+#pragma unroll
+  for (int half = 2; half > 0; half >>= 1) {  // waves 2, 3 into 0, 1, then 1 into 0
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < C::ACC; ++i) *reinterpret_cast<axk_f32x4*>(&s_o[wave - half][(i * 64 + lane) * 4]) = acc[i];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int i = 0; i < C::ACC; ++i) acc[i] += *reinterpret_cast<axk_f32x4*>(&s_o[wave][(i * 64 + lane) * 4]);
+    }
+    __syncthreads();
+  }
+  if (wave || l16 >= group) return;
+  // lane: head l16, channels n 16 E + E (4 g + i) + e from acc[n E + e][i]
+  if (a.direct) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint16_t* o = a.out + ((int64_t)b * a.hq + h * group + l16) * D;
+#pragma unroll
+    for (int n = 0; n < C::NH; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < C::E; e += 4)
+          *reinterpret_cast<uint2*>(o + n * 16 * C::E + C::E * (4 * g + i) + e) =
+              make_uint2(pack_bf16x2(acc[n * C::E + e][i] * inv, acc[n * C::E + e + 1][i] * inv),
+                         pack_bf16x2(acc[n * C::E + e + 2][i] * inv, acc[n * C::E + e + 3][i] * inv));
+    return;
+  }
+  if (g == 0) a.ml[item * group + l16] = make_float2(top, l);
+  float* o = a.po + (item * group + l16) * D;
+#pragma unroll
+  for (int n = 0; n < C::NH; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < C::E; e += 4)
+        *reinterpret_cast<axk_f32x4*>(o + n * 16 * C::E + C::E * (4 * g + i) + e) =
+            (axk_f32x4){acc[n * C::E + e][i], acc[n * C::E + e + 1][i], acc[n * C::E + e + 2][i], acc[n * C::E + e + 3][i]};
+}
+
+struct WeightArgs {
+  const float* in;  // [hkv, nnz], null: zeros
+  float* out;       // ..., null: not wanted
+  float decay;
+};
+
+// The joined maximum and the inverse sum of a head over its pieces (lane p of the wave looks at pieces p, p + 64, ...).
+AXK_DEV float2 head_total(const float2* __restrict__ ml, int pieces, int group, int head) {
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY, l = 0.f;
+  for (int p = lane; p < pieces; p += 64) {
+    const float2 x = ml[(int64_t)p * group + head];
+    if (x.y == 0.f) continue;  // nothing counted
+    const float top = fmaxf(m, x.x);
+    l = l * __builtin_amdgcn_exp2f(m - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
+    m = top;
+  }
+  const float top = wave_max(m);
+  l = wave_sum(m == -INFINITY ? 0.f : l * __builtin_amdgcn_exp2f(m - top));
+  return make_float2(top, l == 0.f ? 0.f : 1.0f / l);
+}
+
+// Workgroups [0, batch * hq): the output row of a (sequence, query head) from its pieces. The others: the page weights,
+// from each subtile's sum against the row's joined maximum and sum.
+template <int D>
+__global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a, const WeightArgs w) {
+  __shared__ __align__(16) float s_o[4][D];
+  __shared__ float s_top[kMaxGroup], s_inv[kMaxGroup];
+  __shared__ int s_sum[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int group = a.hq / a.hkv;
+  const bool outs = (int)blockIdx.x < a.batch * a.hq;
+  int b, h, head = 0, pieces = a.pieces, piece = 0;
+  int64_t item;
+  if (outs) {
+    b = blockIdx.x / a.hq;
+    head = blockIdx.x - b * a.hq;
+    h = head / group;
+    head -= h * group;
+    item = ((int64_t)b * a.hkv + h) * a.pieces;
+    if (!a.blocks) {
+      piece = min(pieces_before(a, b, s_sum), a.pieces);
+      item = (int64_t)h * a.pieces + piece;
+    }
+  } else {
+    const int x = blockIdx.x - a.batch * a.hq;
+    if (a.blocks) {  // one workgroup per row
+      b = x / a.hkv;
+      h = x - b * a.hkv;
+      item = (int64_t)x * a.pieces;
+    } else {  // one per piece, for the pages that begin in it
+      h = x / a.pieces;
+      const PieceOf p = find_piece(a, x - h * a.pieces, s_sum);
+      if (p.b >= a.batch) return;
+      b = p.b;
+      piece = p.piece;
+      item = x - piece;
+    }
+  }
+  const Seq s = seq_of(a.indptr, a.last, b, a.page, a.nnz);
+  // the pieces that the grid held (all of them, unless offsets of indptr overlap)
+  if (!a.blocks) pieces = min(pieces_of(s, a.ps), (int)((h + 1) * (int64_t)a.pieces - item));
+  const float2* ml = a.ml + item * group;
+  if (outs) {
+    const float2 t = head_total(ml, pieces, group, head);
+    constexpr int V = D / 64;
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = 0.f;
+#pragma unroll 4
+    for (int p = wave; p < pieces; p += 4) {
+      const float2 x = ml[(int64_t)p * group + head];
+      if (x.y == 0.f) continue;  // its partial output was not needed, and is nothing
+      const float f = __builtin_amdgcn_exp2f(x.x - t.x);
+      const float* po = a.po + ((item + p) * group + head) * D + lane * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] += f * po[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) s_o[wave][lane * V + i] = o[i];
+    __syncthreads();
+    uint16_t* out = a.out + ((int64_t)b * a.hq + h * group + head) * D;
+    for (int i = 2 * tid; i < D; i += 512)
+      *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2((s_o[0][i] + s_o[1][i] + s_o[2][i] + s_o[3][i]) * t.y,
+                                                          (s_o[0][i + 1] + s_o[1][i + 1] + s_o[2][i + 1] + s_o[3][i + 1]) * t.y);
+    return;
+  }
+  for (int i = wave; i < group; i += 4) {
+    const float2 t = head_total(ml, pieces, group, i);
+    if (lane == 0) {
+      s_top[i] = t.x;
+      s_inv[i] = t.y;
+    }
+  }
+  __syncthreads();
+  const int spp = a.page / kSub, l16 = tid & 15;
+  const float* in = w.in ? w.in + (int64_t)h * a.nnz + s.pb : nullptr;
+  float* out = w.out + (int64_t)h * a.nnz + s.pb;
+  // the share of subtiles [from, from + n) of the statistics, by 16 lanes
+  auto share = [&](int64_t from, int n) {
+    float x = 0.f;
+    const float2* st = a.stat + from * group;
+    for (int i = l16; i < n * group; i += 16) {
+      const float2 y = st[i];
+      const int hd = i % group;
+      if (y.y != 0.f) x += y.y * __builtin_amdgcn_exp2f(y.x - s_top[hd]) * s_inv[hd];
+    }
+    return group_sum<16>(x);
+  };
+  if (!a.blocks) {
+    const int64_t all = (s.len + kSub - 1) / kSub, sub0 = (int64_t)piece * a.ps;
+    const int end = (int)min((sub0 + a.ps + spp - 1) / spp, (int64_t)s.np);
+    for (int p = (int)((sub0 + spp - 1) / spp) + (tid >> 4); p < end; p += 16) {
+      const int64_t first = (int64_t)p * spp;
+      const float x = share(((int64_t)h * a.nnz + s.pb) * spp + first, (int)min((int64_t)spp, all - first));
+      if (l16 == 0) out[p] = (in ? w.decay * in[p] : 0.f) + x;
+    }
+    return;
+  }
+  for (int p = tid; p < s.np; p += 256) out[p] = in ? w.decay * in[p] : 0.f;
+  __syncthreads();
+  // the listed blocks of one page follow each other: the first of them adds them all, so that a page is added to once
+  const int spb = a.block / kSub, bpp = a.page / a.block;
+  const int64_t row = (int64_t)b * a.hkv + h, nblocks = (s.len + a.block - 1) / a.block;
+  const int* list = a.blocks + row * a.n;
+  for (int slot = tid >> 4; slot < a.n; slot += 16) {
+    bool bad;
+    const int id = listed_block(list, slot, nblocks, &bad);
+    if (id < 0) continue;
+    const int p = id / bpp;
+    if (slot) {
+      const int prev = listed_block(list, slot - 1, nblocks, &bad);
+      if (prev >= 0 && prev / bpp == p) continue;
+    }
+    float x = 0.f;
+    for (int i = slot; i < a.n; ++i) {
+      const int next = listed_block(list, i, nblocks, &bad);
+      if (next < 0 || next / bpp != p) break;
+      x += share((row * a.n + i) * spb, spb);
+    }
+    if (l16 == 0) atomicAdd(out + p, x);
+  }
+}
+
+// ---- eviction ----
+// One workgroup per sequence: its `budget` pages of largest weight (summed over the KV heads in 64 bits, so that the
+// order of the sum does not decide), the first `first` and last `keep_last` always among them, in their order into the
+// new table; the others' ids into `freed`. Every workgroup finds its places from the whole indptr, and fills as much of
+// the arrays' tails as it moved elsewhere.
+__global__ __launch_bounds__(256) void paged_evict_kernel(const float* __restrict__ w, const int* __restrict__ indptr,
+                                                          const int* __restrict__ indices, int* __restrict__ out_indptr,
+                                                          int* __restrict__ out_indices, float* __restrict__ out_w,
+                                                          int* __restrict__ freed, int nnz, int batch, int hkv,
+                                                          int budget, int first, int keep_last) {
+  __shared__ PickLds<uint64_t, 256> lds;
+  __shared__ int s_sum[4][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
+  auto ptr = [&](int i) { return min(max(indptr[i], 0), nnz); };
+  // kept and evicted pages of the sequences before b, and kept and all pages of all of them
+  int n4[4] = {0, 0, 0, 0};
+  for (int i = tid; i < batch; i += 256) {
+    const int n = max(ptr(i + 1) - ptr(i), 0), k = min(n, budget);
+    if (i < b) {
+      n4[0] += k;
+      n4[1] += n - k;
+    }
+    n4[2] += k;
+    n4[3] += n;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n4[i] += __shfl_xor(n4[i], o, 64);
+    if (lane == 0) s_sum[i][wave] = n4[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) n4[i] = s_sum[i][0] + s_sum[i][1] + s_sum[i][2] + s_sum[i][3];
+  const int kept = n4[0], gone = n4[1], all = n4[2], total = n4[3];
+  const int pb = ptr(b), np = max(ptr(b + 1) - pb, 0), keep = min(np, budget);
+  if (tid == 0) {
+    if (b == 0) out_indptr[0] = 0;
+    out_indptr[b + 1] = kept + keep;
+  }
+  auto put = [&](int i, bool taken, int rank) {
+    if (taken) {
+      if (kept + rank < nnz) {
+        out_indices[kept + rank] = indices[pb + i];
+        for (int h = 0; h < hkv; ++h) out_w[(int64_t)h * nnz + kept + rank] = w[(int64_t)h * nnz + pb + i];
+      }
+    } else if (gone + i - rank < nnz) {
+      freed[gone + i - rank] = indices[pb + i];
+    }
+  };
+  if (np <= budget) {
+    for (int i = tid; i < np; i += 256) put(i, true, i);
+  } else {
+    for (int i = tid; i < first; i += 256) put(i, true, i);
+    for (int i = tid; i < keep_last; i += 256) put(np - keep_last + i, true, budget - keep_last + i);
+    const int want = budget - first - keep_last, count = np - first - keep_last;
+    if (want == 0) {
+      for (int i = tid; i < count; i += 256) put(first + i, false, first);
+    } else {
+      pick_largest<uint64_t, 256>(
+          count, want,
+          [&](int i) {
+            double x = 0.0;
+            for (int h = 0; h < hkv; ++h) x += (double)w[(int64_t)h * nnz + pb + first + i];
+            return order_key(x);
+          },
+          [&](int i, bool taken, int rank) { put(first + i, taken, first + rank); }, lds);
+    }
+  }
+  // the tails: [all, nnz) of the table and of the weights, [total - all, nnz) of freed. A sequence's share of the first
+  // is as long as what it evicted, of the second as what it kept; the last one also fills what no sequence had
+  const int extra = b == batch - 1 ? max(nnz - total, 0) : 0;
+  for (int i = tid; i < np - keep + extra; i += 256) {
+    const int at = all + gone + i;
+    if (at >= nnz) break;
+    out_indices[at] = -1;
+    for (int h = 0; h < hkv; ++h) out_w[(int64_t)h * nnz + at] = 0.f;
+  }
+  for (int i = tid; i < keep + extra; i += 256) {
+    const int at = total - all + kept + i;
+    if (at < nnz) freed[at] = -1;
+  }
+}
+
+}  // namespace
+
+namespace {
+
+int check_blocks(int64_t batch, int64_t hkv, int64_t d, int64_t page_size, int64_t block, int64_t num_pages, int64_t nnz) {
+  AXK_REQUIRE(batch > 0 && batch <= (1 << 20) && hkv > 0 && hkv <= 4096, AXK_E_SHAPE);
+  AXK_REQUIRE(d == 64 || d == 128 || d == 256, AXK_E_SHAPE);
+  AXK_REQUIRE(page_size >= kSub && page_size % kSub == 0 && page_size <= 4096, AXK_E_SHAPE);
+  AXK_REQUIRE(block >= kSub && block % kSub == 0 && page_size % block == 0, AXK_E_SHAPE);
+  AXK_REQUIRE(num_pages > 0 && nnz >= 0 && nnz * (page_size / kSub) <= 0x7fffffff, AXK_E_SHAPE);
+  return AXK_OK;
+}
+
+// The stored type of a cache: 0 bf16, 1 FP8 E4M3 with a power-of-two scale; negative: refused.
+int cache_type(int kv_dtype, float kv_scale) {
+  if (kv_dtype == AXK_DT_BF16) return 0;
+  if (kv_dtype != AXK_DT_FP8E4M3) return -AXK_E_DTYPE;
+  int e = 0;
+  const float m = frexpf(kv_scale, &e);
+  return kv_scale > 0.f && m == 0.5f && e >= -125 && e <= 126 ? 1 : -AXK_E_SHAPE;
+}
+
+size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// How a decode over blocks is cut, from what the host knows. Pieces of at least 128 tokens, so that each wave has a step,
+// and of at most 2048; about 1024 of them.
+constexpr int64_t kPieces = 1024;
+struct BlkPlan {
+  int ps, pieces;
+  bool direct;
+  size_t ml, po, stat;  // bytes of each workspace part
+};
+BlkPlan blk_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t page, int64_t nnz, int64_t block, int64_t n,
+                 bool weights) {
+  const int64_t rows = batch * hkv, group = hq / hkv;
+  const int64_t subs = n ? n * (block / kSub) : nnz * (page / kSub);  // of a row, or of a KV head
+  const int64_t cut = n ? (kPieces + rows - 1) / rows : (kPieces + hkv - 1) / hkv;
+  int64_t ps = ((subs + cut - 1) / cut + 7) / 8 * 8;
+  ps = ps < 8 ? 8 : ps > kMaxPs ? kMaxPs : ps;
+  BlkPlan p;
+  p.ps = (int)ps;
+  p.pieces = (int)((subs + ps - 1) / ps + (n ? 0 : batch));  // a sequence's last piece may be a partial one
+  p.direct = n && p.pieces == 1 && !weights;
+  const size_t items = (size_t)(n ? rows : hkv) * p.pieces;
+  p.ml = p.direct ? 0 : round256(items * group * sizeof(float2));
+  p.po = p.direct ? 0 : round256(items * group * d * sizeof(float));
+  p.stat = weights ? round256((size_t)(n ? rows : hkv) * subs * group * sizeof(float2)) : 0;
+  return p;
+}
+
+template <int D>
+int launch_blocks(const BlkArgs& a, const WeightArgs& w, int f8, hipStream_t st) {
+  const dim3 grid = a.blocks ? dim3((unsigned)(a.batch * a.hkv * a.pieces)) : dim3((unsigned)a.pieces, (unsigned)a.hkv);
+  if (f8) hipLaunchKernelGGL((paged_blocks_kernel<D, 1>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((paged_blocks_kernel<D, 0>), grid, dim3(256), 0, st, a);
+  if (!a.direct) {
+    const int64_t wgs = (int64_t)a.batch * a.hq + (w.out ? (a.blocks ? (int64_t)a.batch : a.pieces) * a.hkv : 0);
+    hipLaunchKernelGGL((paged_blocks_merge_kernel<D>), dim3((unsigned)wgs), dim3(256), 0, st, a, w);
+  }
+  return axk_launch_status();
+}
+
+}  // namespace
+
+extern "C" int axk_paged_kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cache, int kv_dtype,
+                                         float kv_scale, uint16_t* bounds, const int32_t* cache_location, int64_t rows,
+                                         int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t block_size,
+                                         int64_t num_pages, int32_t* status, axk_stream_t stream) {
+  AXK_REQUIRE(k && v && kv_cache && bounds && cache_location, AXK_E_NULL);
+  const int rc = check_blocks(1, num_kv_heads, head_dim, page_size, block_size, num_pages, 0);
+  if (rc != AXK_OK) return rc;
+  AXK_REQUIRE(rows >= 0 && rows <= (1 << 20), AXK_E_SHAPE);
+  const int f8 = cache_type(kv_dtype, kv_scale);
+  if (f8 < 0) return -f8;
+  AXK_REQUIRE(axk_aligned(k, 16) && axk_aligned(v, 16) && axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16),
+              AXK_E_ALIGN);
+  const size_t row = (size_t)num_kv_heads * head_dim * 2, in = (size_t)rows * row;
+  const size_t cache = (size_t)num_pages * page_size * row * 2 / (f8 ? 2 : 1);
+  const size_t bb = (size_t)num_pages * (page_size / block_size) * row * 2;
+  AXK_REQUIRE(!axk_overlap(bounds, bb, kv_cache, cache) && !axk_overlap(bounds, bb, k, in) &&
+                  !axk_overlap(bounds, bb, v, in) && !axk_overlap(kv_cache, cache, k, in) &&
+                  !axk_overlap(kv_cache, cache, v, in),
+              AXK_E_ALIAS);
+  if (rows == 0) return AXK_OK;
+  AXK_LAUNCH_GATE();
+  auto* fn = f8 ? &paged_kv_write_bounds_kernel<1> : &paged_kv_write_bounds_kernel<0>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)rows), dim3(256), 0, axk_stream(stream), k, v,
+                     static_cast<unsigned char*>(kv_cache), bounds, cache_location, (int)rows, (int)num_kv_heads,
+                     (int)head_dim, (int)page_size, (int)block_size, num_pages, f8 ? kv_scale : 1.0f, status);
+  return axk_launch_status();
+}
+
+extern "C" int axk_paged_key_bounds(const void* kv_cache, int kv_dtype, float kv_scale, uint16_t* bounds,
+                                    const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len,
+                                    const int32_t* start, int64_t nnz, int64_t batch, int64_t num_kv_heads,
+                                    int64_t head_dim, int64_t page_size, int64_t block_size, int64_t num_pages,
+                                    int32_t* status, axk_stream_t stream) {
+  AXK_REQUIRE(kv_cache && bounds && indptr && (indices || nnz == 0) && last_page_len, AXK_E_NULL);
+  const int rc = check_blocks(batch, num_kv_heads, head_dim, page_size, block_size, num_pages, nnz);
+  if (rc != AXK_OK) return rc;
+  const int f8 = cache_type(kv_dtype, kv_scale);
+  if (f8 < 0) return -f8;
+  AXK_REQUIRE(axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16), AXK_E_ALIGN);
+  const size_t row = (size_t)num_kv_heads * head_dim * 2;
+  AXK_REQUIRE(!axk_overlap(bounds, (size_t)num_pages * (page_size / block_size) * row * 2, kv_cache,
+                           (size_t)num_pages * page_size * row * 2 / (f8 ? 2 : 1)),
+              AXK_E_ALIAS);
+  if (nnz == 0) return AXK_OK;
+  AXK_LAUNCH_GATE();
+  auto* fn = f8 ? &paged_key_bounds_kernel<1> : &paged_key_bounds_kernel<0>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)(nnz * (page_size / block_size))), dim3(256), 0, axk_stream(stream),
+                     static_cast<const unsigned char*>(kv_cache), bounds, indptr, indices, last_page_len, start, (int)nnz,
+                     (int)batch, (int)num_kv_heads, (int)head_dim, (int)page_size, (int)block_size, num_pages,
+                     f8 ? 1.0f / kv_scale : 1.0f, status);
+  return axk_launch_status();
+}
+
+extern "C" int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds, const int32_t* indptr,
+                                      const int32_t* indices, const int32_t* last_page_len, float* scores, int64_t nnz,
+                                      int64_t batch, int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim,
+                                      int64_t page_size, int64_t block_size, int64_t num_pages, int32_t* status,
+                                      axk_stream_t stream) {
+  AXK_REQUIRE(q && bounds && indptr && (nnz == 0 || (indices && scores)) && last_page_len, AXK_E_NULL);
+  const int rc = check_blocks(batch, num_kv_heads, head_dim, page_size, block_size, num_pages, nnz);
+  if (rc != AXK_OK) return rc;
+  AXK_REQUIRE(num_qo_heads > 0 && num_qo_heads % num_kv_heads == 0 && num_qo_heads / num_kv_heads <= kMaxGroup, AXK_E_SHAPE);
+  AXK_REQUIRE(axk_aligned(q, 16) && axk_aligned(bounds, 16) && axk_aligned(scores, 4), AXK_E_ALIGN);
+  if (nnz == 0) return AXK_OK;
+  const int64_t total = nnz * (page_size / block_size);
+  const size_t out = (size_t)num_kv_heads * total * 4;
+  AXK_REQUIRE(!axk_overlap(scores, out, q, (size_t)batch * num_qo_heads * head_dim * 2) &&
+                  !axk_overlap(scores, out, bounds,
+                               (size_t)num_pages * (page_size / block_size) * num_kv_heads * head_dim * 4),
+              AXK_E_ALIAS);
+  const int64_t units = (total + 15) / 16 * num_kv_heads;
+  AXK_REQUIRE((units + 3) / 4 <= 0x7fffffff, AXK_E_SHAPE);
+  AXK_LAUNCH_GATE();
+  auto* fn = head_dim == 64 ? &paged_block_scores_kernel<64>
+                            : head_dim == 128 ? &paged_block_scores_kernel<128> : &paged_block_scores_kernel<256>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, axk_stream(stream), q, bounds, indptr, indices,
+                     last_page_len, scores, (int)nnz, (int)batch, (int)num_qo_heads, (int)num_kv_heads, (int)page_size,
+                     (int)block_size, num_pages, units, status);
+  return axk_launch_status();
+}
+
+extern "C" int axk_paged_select_blocks(const float* scores, const int32_t* indptr, const int32_t* last_page_len,
+                                       int32_t* blocks, int64_t nnz, int64_t batch, int64_t num_kv_heads,
+                                       int64_t page_size, int64_t block_size, int64_t num_select, int64_t first,
+                                       int64_t keep_last, axk_stream_t stream) {
+  AXK_REQUIRE((scores || nnz == 0) && indptr && last_page_len && blocks, AXK_E_NULL);
+  const int rc = check_blocks(batch, num_kv_heads, 64, page_size, block_size, 1, nnz);
+  if (rc != AXK_OK) return rc;
+  AXK_REQUIRE(num_select > 0 && num_select <= (1 << 24) && first >= 0 && keep_last >= 0 &&
+                  first + keep_last <= num_select && batch * num_kv_heads <= 0x7fffffff,
+              AXK_E_SHAPE);
+  AXK_REQUIRE(axk_aligned(scores, 4) && axk_aligned(blocks, 4), AXK_E_ALIGN);
+  const int64_t total = nnz * (page_size / block_size);
+  AXK_REQUIRE(!axk_overlap(blocks, (size_t)batch * num_kv_heads * num_select * 4, scores, (size_t)num_kv_heads * total * 4),
+              AXK_E_ALIAS);
+  AXK_LAUNCH_GATE();
+  const dim3 grid((unsigned)(batch * num_kv_heads));
+  if (total <= 256 * kKeys)
+    hipLaunchKernelGGL(paged_select_blocks_kernel<256>, grid, dim3(256), 0, axk_stream(stream), scores, indptr,
+                       last_page_len, blocks, (int)nnz, (int)num_kv_heads, (int)page_size, (int)block_size,
+                       (int)num_select, (int)first, (int)keep_last);
+  else
+    hipLaunchKernelGGL(paged_select_blocks_kernel<1024>, grid, dim3(1024), 0, axk_stream(stream), scores, indptr,
+                       last_page_len, blocks, (int)nnz, (int)num_kv_heads, (int)page_size, (int)block_size,
+                       (int)num_select, (int)first, (int)keep_last);
+  return axk_launch_status();
+}
+
+extern "C" size_t axk_paged_decode_blocks_workspace_size(int64_t batch, int64_t num_qo_heads, int64_t num_kv_heads,
+                                                         int64_t head_dim, int64_t page_size, int64_t nnz,
+                                                         int64_t block_size, int64_t num_select, int with_weights) {
+  if (check_blocks(batch, num_kv_heads, head_dim, page_size, num_select ? block_size : kSub, 1, nnz) != AXK_OK) return 0;
+  if (num_qo_heads <= 0 || num_qo_heads % num_kv_heads || num_qo_heads / num_kv_heads > kMaxGroup) return 0;
+  if (num_select < 0 || num_select * (block_size / kSub) > 0x7fffffff) return 0;
+  const BlkPlan p = blk_plan(batch, num_qo_heads, num_kv_heads, head_dim, page_size, nnz, block_size, num_select,
+                             with_weights != 0);
+  return p.ml + p.po + p.stat;
+}
+
+extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, int kv_dtype, float kv_scale,
+                                       const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len,
+                                       const int32_t* blocks, int64_t block_size, int64_t num_select, uint16_t* out,
+                                       const float* weights_in, float* weights_out, float decay, int64_t nnz,
+                                       int64_t batch, int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim,
+                                       int64_t page_size, int64_t num_pages, float sm_scale, int32_t* status,
+                                       void* workspace, size_t workspace_bytes, axk_stream_t stream) {
+  AXK_REQUIRE(q && kv_cache && indptr && (indices || nnz == 0) && last_page_len && out, AXK_E_NULL);
+  if (!blocks) {
+    AXK_REQUIRE(num_select == 0, AXK_E_NULL);
+    block_size = kSub;
+  } else {
+    AXK_REQUIRE(num_select > 0, AXK_E_SHAPE);
+  }
+  const int rc = check_blocks(batch, num_kv_heads, head_dim, page_size, block_size, num_pages, nnz);
+  if (rc != AXK_OK) return rc;
+  AXK_REQUIRE(num_qo_heads > 0 && num_qo_heads % num_kv_heads == 0 && num_qo_heads / num_kv_heads <= kMaxGroup, AXK_E_SHAPE);
+  AXK_REQUIRE(num_select * (block_size / kSub) <= 0x7fffffff, AXK_E_SHAPE);
+  AXK_REQUIRE(!weights_in || weights_out, AXK_E_NULL);
+  const int f8 = cache_type(kv_dtype, kv_scale);
+  if (f8 < 0) return -f8;
+  AXK_REQUIRE(axk_aligned(q, 16) && axk_aligned(kv_cache, 16) && axk_aligned(out, 8) && axk_aligned(weights_in, 4) &&
+                  axk_aligned(weights_out, 4) && axk_aligned(blocks, 4),
+              AXK_E_ALIGN);
+  const bool weights = weights_out && nnz > 0;
+  const BlkPlan p = blk_plan(batch, num_qo_heads, num_kv_heads, head_dim, page_size, nnz, block_size, num_select, weights);
+  const size_t need = p.ml + p.po + p.stat;
+  AXK_REQUIRE(!need || (workspace && workspace_bytes >= need && axk_aligned(workspace, 256)), AXK_E_WORKSPACE);
+  const int64_t grid = blocks ? batch * num_kv_heads * p.pieces : p.pieces;
+  const int64_t wgs = batch * num_qo_heads + (weights ? (blocks ? batch : (int64_t)p.pieces) * num_kv_heads : 0);
+  AXK_REQUIRE(grid <= 0x7fffffff && wgs <= 0x7fffffff, AXK_E_SHAPE);
+  const size_t qb = (size_t)batch * num_qo_heads * head_dim * 2, wb = (size_t)num_kv_heads * nnz * 4;
+  const size_t cache = (size_t)num_pages * page_size * num_kv_heads * head_dim * (f8 ? 2 : 4);
+  AXK_REQUIRE(!axk_overlap(out, qb, q, qb) && !axk_overlap(out, qb, kv_cache, cache) && !axk_overlap(out, qb, workspace, need) &&
+                  !axk_overlap(q, qb, workspace, need) && !axk_overlap(kv_cache, cache, workspace, need),
+              AXK_E_ALIAS);
+  AXK_REQUIRE(weights_in == weights_out || !axk_overlap(weights_in, wb, weights_out, wb), AXK_E_ALIAS);
+  AXK_REQUIRE(!axk_overlap(weights_out, wb, out, qb) && !axk_overlap(weights_out, wb, q, qb) &&
+                  !axk_overlap(weights_out, wb, kv_cache, cache) && !axk_overlap(weights_out, wb, workspace, need) &&
+                  !axk_overlap(weights_in, wb, workspace, need),
+              AXK_E_ALIAS);
+  BlkArgs a;
+  a.q = q;
+  a.cache = static_cast<const unsigned char*>(kv_cache);
+  a.indptr = indptr;
+  a.indices = indices;
+  a.last = last_page_len;
+  a.blocks = blocks;
+  a.n = (int)num_select;
+  a.block = (int)block_size;
+  a.nnz = (int)nnz;
+  a.batch = (int)batch;
+  a.hq = (int)num_qo_heads;
+  a.hkv = (int)num_kv_heads;
+  a.page = (int)page_size;
+  a.num_pages = num_pages;
+  a.scale = sm_scale * kLog2e;
+  a.inv_scale = f8 ? 1.0f / kv_scale : 1.0f;
+  a.ps = p.ps;
+  a.pieces = p.pieces;
+  a.direct = p.direct;
+  a.out = out;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  a.ml = p.direct ? nullptr : reinterpret_cast<float2*>(ws);
+  a.po = p.direct ? nullptr : reinterpret_cast<float*>(ws + p.ml);
+  a.stat = weights ? reinterpret_cast<float2*>(ws + p.ml + p.po) : nullptr;
+  a.status = status;
+  const WeightArgs w = {weights_in, weights ? weights_out : nullptr, decay};
+  AXK_LAUNCH_GATE();
+  switch (head_dim) {
+    case 64: return launch_blocks<64>(a, w, f8, axk_stream(stream));
+    case 128: return launch_blocks<128>(a, w, f8, axk_stream(stream));
+    default: return launch_blocks<256>(a, w, f8, axk_stream(stream));
+  }
+}
+
+extern "C" int axk_paged_evict_pages(const float* weights, const int32_t* indptr, const int32_t* indices,
+                                     int32_t* out_indptr, int32_t* out_indices, float* out_weights, int32_t* freed,
+                                     int64_t nnz, int64_t batch, int64_t num_kv_heads, int64_t budget, int64_t first,
+                                     int64_t keep_last, axk_stream_t stream) {
+  AXK_REQUIRE(indptr && out_indptr && (nnz == 0 || (weights && indices && out_indices && out_weights && freed)), AXK_E_NULL);
+  AXK_REQUIRE(batch > 0 && batch <= (1 << 20) && num_kv_heads > 0 && num_kv_heads <= 4096 && nnz >= 0 && nnz <= 0x3fffffff,
+              AXK_E_SHAPE);
+  AXK_REQUIRE(first >= 0 && keep_last >= 1 && budget >= first + keep_last && budget <= 0x3fffffff, AXK_E_SHAPE);
+  const size_t ib = (size_t)nnz * 4, pb = (size_t)(batch + 1) * 4, wb = (size_t)num_kv_heads * nnz * 4;
+  const struct {
+    const void* p;
+    size_t n;
+  } in[3] = {{weights, wb}, {indptr, pb}, {indices, ib}}, out[4] = {{out_indptr, pb}, {out_indices, ib}, {out_weights, wb}, {freed, ib}};
+  for (int i = 0; i < 4; ++i) {
+    AXK_REQUIRE(axk_aligned(out[i].p, 4), AXK_E_ALIGN);
+    for (int j = 0; j < 3; ++j) AXK_REQUIRE(!axk_overlap(out[i].p, out[i].n, in[j].p, in[j].n), AXK_E_ALIAS);
+    for (int j = 0; j < i; ++j) AXK_REQUIRE(!axk_overlap(out[i].p, out[i].n, out[j].p, out[j].n), AXK_E_ALIAS);
+  }
+  AXK_LAUNCH_GATE();
+  hipLaunchKernelGGL(paged_evict_kernel, dim3((unsigned)batch), dim3(256), 0, axk_stream(stream), weights, indptr, indices,
+                     out_indptr, out_indices, out_weights, freed, (int)nnz, (int)batch, (int)num_kv_heads, (int)budget,
+                     (int)first, (int)keep_last);
+  return axk_launch_status();
+}

@@ -374,6 +374,95 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
                             void* workspace, size_t workspace_bytes, axk_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Sparse attention over a paged KV cache, and eviction of its pages. No counterpart in the reference.
+ *
+ * A page is cut into blocks of block_size consecutive tokens (block_size a multiple of 16 that divides page_size). For
+ * every block and KV head, bounds bf16 [num_pages, page_size / block_size, num_kv_heads, 2, head_dim] keeps the
+ * channel-wise minimum (0) and maximum (1) of the block's keys, as attention reads them. A decode step writes its tokens
+ * with axk_paged_kv_write_bounds, scores every block with axk_paged_block_scores, selects with axk_paged_select_blocks
+ * and attends the selection with axk_paged_decode_blocks, which can also add up how much attention every page received;
+ * axk_paged_evict_pages cuts a page table down to the pages that received most.
+ *
+ * Cache, page table and page size as axk_paged_decode; head_dim 64, 128 or 256; num_qo_heads / num_kv_heads <= 16;
+ * num_kv_heads <= 4096. kv_dtype: AXK_DT_BF16, or AXK_DT_FP8E4M3 for a cache of axk_paged_kv_write_fp8 with its kv_scale
+ * (a power of two; ignored for bf16). nnz: the entries of indices; offsets of indptr past it are read as nnz and a
+ * last_page_len past page_size as page_size, so that no access leaves an array; nnz * page_size / 16 < 2^31. A page id
+ * outside [0, num_pages) is skipped, never read, and sets *status (device i32, or NULL) to 1. An array per page-table entry
+ * is [num_kv_heads, nnz], one per block [num_kv_heads, nnz * page_size / block_size]: entry e's blocks at e *
+ * page_size / block_size.
+ * ------------------------------------------------------------------------------------------- */
+
+/* The new rows k, v bf16 [rows, num_kv_heads, head_dim] written at cache_location i32 [rows, 2] = (page, slot), as
+ * axk_paged_kv_write / axk_paged_kv_write_fp8, and each key (as the cache now holds it) folded into its block's bounds.
+ * A block with a new row at its first slot starts afresh; any other widens what it had, so tokens are written in order,
+ * and rows written over (rejected drafts) leave bounds that still hold but are wide, until axk_paged_key_bounds computes
+ * them again. Rows of one call may share a block; where two name one slot the last one is stored, and both are folded. A
+ * location outside the pool is skipped and sets *status. A NaN key makes the bound on its sign's side NaN. */
+int axk_paged_kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cache, int kv_dtype, float kv_scale,
+                              uint16_t* bounds, const int32_t* cache_location, int64_t rows, int64_t num_kv_heads,
+                              int64_t head_dim, int64_t page_size, int64_t block_size, int64_t num_pages,
+                              int32_t* status, axk_stream_t stream);
+
+/* The bounds computed from the cache, for the blocks of each sequence that hold a token at or after start[b] (i32
+ * [batch]; NULL: all blocks): after a prefill chunk that began at position start[b], or for a cache that came without
+ * them. Tokens past a sequence's end are not read; other blocks' bounds stay as they are. A page that several
+ * sequences share must hold as many tokens in each, or be full. */
+int axk_paged_key_bounds(const void* kv_cache, int kv_dtype, float kv_scale, uint16_t* bounds, const int32_t* indptr,
+                         const int32_t* indices, const int32_t* last_page_len, const int32_t* start, int64_t nnz,
+                         int64_t batch, int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t block_size,
+                         int64_t num_pages, int32_t* status, axk_stream_t stream);
+
+/* scores f32 [num_kv_heads, nnz * page_size / block_size]: for q bf16 [batch, num_qo_heads, head_dim], entry (h, j) is
+ *   max over the query heads g of KV head h of sum_d max(q_gd, 0) hi_jd + min(q_gd, 0) lo_jd,
+ * which no q_g . k of the block exceeds (softmax scale left out: it does not change the order). -inf for a block past its
+ * sequence's end or on a bad page; entries of no sequence (past indptr[batch]) are left as they are. */
+int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds, const int32_t* indptr, const int32_t* indices,
+                           const int32_t* last_page_len, float* scores, int64_t nnz, int64_t batch,
+                           int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                           int64_t block_size, int64_t num_pages, int32_t* status, axk_stream_t stream);
+
+/* blocks i32 [batch, num_kv_heads, num_select]: the num_select blocks of each sequence and KV head with the largest
+ * scores, as ascending block numbers within the sequence, the first `first` and last `keep_last` of its blocks always
+ * among them (first + keep_last <= num_select); equal scores by the lowest block; NaN above every number. A sequence with
+ * no more blocks than that has all of them, then -1. */
+int axk_paged_select_blocks(const float* scores, const int32_t* indptr, const int32_t* last_page_len, int32_t* blocks,
+                            int64_t nnz, int64_t batch, int64_t num_kv_heads, int64_t page_size, int64_t block_size,
+                            int64_t num_select, int64_t first, int64_t keep_last, axk_stream_t stream);
+
+/* Decode attention, as axk_paged_decode, over the listed blocks of each sequence and KV head only: blocks i32 [batch,
+ * num_kv_heads, num_select], each row strictly ascending block numbers within the sequence, then -1 (the form
+ * axk_paged_select_blocks writes). NULL with num_select 0: every block (block_size is then not read). A number past the
+ * sequence's end, or not above its predecessor in the row, is skipped and sets *status. A row that attends nothing yields
+ * zeros.
+ * weights_out f32 [num_kv_heads, nnz] (NULL: not wanted) receives, for each KV head and page-table entry,
+ *   decay * weights_in (NULL: 0) + sum over the KV head's queries of the attention the page's tokens received;
+ * weights_out may be weights_in (in place). Entries of no sequence are left as they are.
+ * workspace >= axk_paged_decode_blocks_workspace_size(...), 256-byte aligned (NULL when that is 0); with_weights: whether
+ * weights_out is given. The size is also 0 for an unsupported shape, which the call refuses. */
+size_t axk_paged_decode_blocks_workspace_size(int64_t batch, int64_t num_qo_heads, int64_t num_kv_heads,
+                                              int64_t head_dim, int64_t page_size, int64_t nnz, int64_t block_size,
+                                              int64_t num_select, int with_weights);
+int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, int kv_dtype, float kv_scale,
+                            const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len,
+                            const int32_t* blocks, int64_t block_size, int64_t num_select, uint16_t* out,
+                            const float* weights_in, float* weights_out, float decay, int64_t nnz, int64_t batch,
+                            int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                            int64_t num_pages, float sm_scale, int32_t* status, void* workspace, size_t workspace_bytes,
+                            axk_stream_t stream);
+
+/* The page table without the pages of least weight: of each sequence with more than `budget` pages, the `budget` pages
+ * with the largest weights f32 [num_kv_heads, nnz] (summed over the KV heads in 64 bits; equal sums by the lowest place;
+ * NaN above every number), the first `first` and last `keep_last` always among them (keep_last >= 1, since the last page
+ * is the one that last_page_len speaks of; first + keep_last <= budget). Every kept page keeps its order and its bytes:
+ * out_indptr i32 [batch + 1], out_indices i32 [nnz] (then -1), out_weights f32 [num_kv_heads, nnz] (then 0) and
+ * freed i32 [nnz] (the other pages' ids in table order, then -1); last_page_len stays as it is. The outputs overlap
+ * neither the inputs nor each other. The bounds go with the pages. A page that another sequence shares is freed all the
+ * same: the caller keeps count of such pages. */
+int axk_paged_evict_pages(const float* weights, const int32_t* indptr, const int32_t* indices, int32_t* out_indptr,
+                          int32_t* out_indices, float* out_weights, int32_t* freed, int64_t nnz, int64_t batch,
+                          int64_t num_kv_heads, int64_t budget, int64_t first, int64_t keep_last, axk_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Gated DeltaNet (GDN)
  * ------------------------------------------------------------------------------------------- */
 
