@@ -31,6 +31,8 @@ DECAY = 0.97  # what a page keeps of its attention weight from one step to the n
 
 
 def _axk():
+    if "axk" in sys.modules:
+        return sys.modules["axk"]
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     path = os.path.join(root, "ax-dsl-kernels_amd")
     if path not in sys.path:
