@@ -23,86 +23,91 @@ import torch
 from . import _lib
 
 
-def _check(cond: bool, msg: str) -> None:
-    if not cond:
-        raise ValueError(msg)
+# The checks build their messages only when they fail: a decode step makes these calls once a layer.
+_stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice
 
 
 def _call(name: str, tensors, *args) -> None:
     """The call on the current stream of the tensors' device, which all of them have to be on."""
-    dev = tensors[0].device
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
-    if dev.type != "cuda":
-        raise ValueError(f"axk operators take device tensors; got a tensor on {dev}")
-    if torch.cuda.current_device() == dev.index:
-        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name}: tensors on {tensors[0].device} and {t.device}")
+    if dev < 0:
+        raise ValueError(f"axk operators take device tensors; got a tensor on {tensors[0].device}")
+    if _device() == dev:
+        _lib.call(name, *args, _stream(dev))
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            _lib.call(name, *args, _stream(dev))
 
 
 def _i32(t: torch.Tensor, name: str, *shape: int) -> None:
-    _check(t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous(),
-           f"{name} must be contiguous int32 {list(shape)}")
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)}")
 
 
 def _table(indptr, last_page_len, indices=None) -> int:
     """Checks a page table and returns its sequences."""
     b = last_page_len.numel()
-    _check(b > 0, "the page table holds no sequence")
+    if b < 1:
+        raise ValueError("the page table holds no sequence")
     _i32(indptr, "indptr", b + 1)
     _i32(last_page_len, "last_page_len", b)
-    if indices is not None:
-        _check(indices.dtype == torch.int32 and indices.dim() == 1 and indices.is_contiguous(),
-               "indices must be contiguous int32 [nnz]")
+    if indices is not None and (indices.dtype != torch.int32 or indices.dim() != 1 or not indices.is_contiguous()):
+        raise ValueError("indices must be contiguous int32 [nnz]")
     return b
 
 
 def _status(status) -> None:
-    _check(status is None or (status.dtype == torch.int32 and status.numel() >= 1), "status must be int32 [1]")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise ValueError("status must be int32 [1]")
 
 
 def _sizes(page_size: int, block_size: int) -> None:
-    _check(page_size >= 16 and page_size % 16 == 0 and page_size <= 4096,
-           f"page_size {page_size} must be a multiple of 16, at most 4096")
-    _check(block_size >= 16 and block_size % 16 == 0 and page_size % block_size == 0,
-           f"block_size {block_size} must be a multiple of 16 that divides page_size {page_size}")
+    if page_size < 16 or page_size % 16 or page_size > 4096:
+        raise ValueError(f"page_size {page_size} must be a multiple of 16, at most 4096")
+    if block_size < 16 or block_size % 16 or page_size % block_size:
+        raise ValueError(f"block_size {block_size} must be a multiple of 16 that divides page_size {page_size}")
 
 
 def _cache(kv_cache, kv_scale):
     """(dtype code, scale, num_pages, page_size, HKV, D) of a bf16 or FP8 cache."""
     if kv_cache.dtype == torch.bfloat16:
-        _check(kv_scale is None, "kv_scale is for an FP8 cache")
+        if kv_scale is not None:
+            raise ValueError("kv_scale is for an FP8 cache")
         code, scale = _lib.DT_BF16, 1.0
     else:
-        _check(kv_cache.dtype in (torch.uint8, torch.float8_e4m3fn),
-               f"kv_cache must be bfloat16 or u8 / float8_e4m3fn, got {kv_cache.dtype}")
-        _check(kv_scale is not None and kv_scale > 0 and math.frexp(kv_scale)[0] == 0.5,
-               f"an FP8 cache needs its kv_scale, a power of two (got {kv_scale})")
-        code, scale = _lib.DT_FP8E4M3, float(kv_scale)
-    _check(kv_cache.dim() == 5 and kv_cache.shape[1] == 2 and kv_cache.is_contiguous(),
-           "kv_cache must be contiguous [pages, 2, page_size, HKV, D]")
+        if kv_cache.dtype not in (torch.uint8, torch.float8_e4m3fn):
+            raise ValueError(f"kv_cache must be bfloat16 or u8 / float8_e4m3fn, got {kv_cache.dtype}")
+        if kv_scale is None or not kv_scale > 0 or math.frexp(kv_scale)[0] != 0.5:
+            raise ValueError(f"an FP8 cache needs its kv_scale, a power of two (got {kv_scale})")
+        code, scale = _lib.DT_FP8E4M3, kv_scale
+    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or not kv_cache.is_contiguous():
+        raise ValueError("kv_cache must be contiguous [pages, 2, page_size, HKV, D]")
     p, _, page, hkv, d = kv_cache.shape
-    _check(d in (64, 128, 256), f"head_dim {d} not supported (64, 128, 256)")
-    _check(p > 0, "kv_cache holds no page")
+    if d not in (64, 128, 256):
+        raise ValueError(f"head_dim {d} not supported (64, 128, 256)")
+    if p < 1:
+        raise ValueError("kv_cache holds no page")
     return code, scale, p, page, hkv, d
 
 
 def _bounds(bounds, p: int, hkv: int, d: int, page_size: int) -> int:
     """Checks the bounds of a pool and returns the block size they are for."""
-    _check(bounds.dim() == 5 and bounds.dtype == torch.bfloat16 and bounds.is_contiguous() and bounds.shape[1] > 0
-           and page_size % bounds.shape[1] == 0 and bounds.shape[0] == p and tuple(bounds.shape[2:]) == (hkv, 2, d),
-           f"bounds must be contiguous bf16 [{p}, page_size / block_size, {hkv}, 2, {d}], got {tuple(bounds.shape)}")
+    if (bounds.dim() != 5 or bounds.dtype != torch.bfloat16 or not bounds.is_contiguous() or bounds.shape[1] < 1
+            or page_size % bounds.shape[1] or bounds.shape != (p, bounds.shape[1], hkv, 2, d)):
+        raise ValueError(f"bounds must be contiguous bf16 [{p}, page_size / block_size, {hkv}, 2, {d}], "
+                         f"got {tuple(bounds.shape)} {bounds.dtype}")
     block = page_size // bounds.shape[1]
     _sizes(page_size, block)
     return block
 
 
 def _heads(hq: int, hkv: int) -> None:
-    _check(hkv > 0 and hq % hkv == 0 and hq // hkv <= 16,
-           f"num_qo_heads {hq} must be a multiple (<= 16x) of num_kv_heads {hkv}")
+    if hkv < 1 or hq < 1 or hq % hkv or hq // hkv > 16:
+        raise ValueError(f"num_qo_heads {hq} must be a multiple (<= 16x) of num_kv_heads {hkv}")
 
 
 def store_paged_kv_bounds(
@@ -120,10 +125,10 @@ def store_paged_kv_bounds(
     rows); where two name one slot the last is stored."""
     code, scale, p, page, hkv, d = _cache(kv_cache, kv_scale)
     block = _bounds(bounds, p, hkv, d, page)
-    _check(k.dim() == 3 and k.shape == v.shape and tuple(k.shape[1:]) == (hkv, d) and k.dtype == torch.bfloat16
-           and v.dtype == torch.bfloat16 and k.is_contiguous() and v.is_contiguous(),
-           f"k and v must be contiguous bf16 [rows, {hkv}, {d}]")
     rows = k.shape[0]
+    if (k.shape != (rows, hkv, d) or v.shape != k.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16
+            or not k.is_contiguous() or not v.is_contiguous()):
+        raise ValueError(f"k and v must be contiguous bf16 [rows, {hkv}, {d}]")
     _i32(cache_location, "cache_location", rows, 2)
     _status(status)
     if rows:
@@ -170,19 +175,21 @@ def paged_block_scores(
     sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d over the KV head's queries of q [B, HQ, D] bf16, which no q . k in the block
     exceeds. -inf past a sequence's end. Entry e's blocks are columns e * page_size / block_size onwards."""
     b = _table(indptr, last_page_len, indices)
-    _check(q.dim() == 3 and q.shape[0] == b and q.dtype == torch.bfloat16 and q.is_contiguous(),
-           f"q must be contiguous bf16 [{b}, HQ, D]")
-    hq, d = q.shape[1:]
-    _check(d in (64, 128, 256), f"head_dim {d} not supported (64, 128, 256)")
-    _check(bounds.dim() == 5 and bounds.shape[0] > 0, "bounds must be bf16 [P, page_size / block_size, HKV, 2, D]")
+    if q.dim() != 3 or q.shape[0] != b or q.dtype != torch.bfloat16 or not q.is_contiguous():
+        raise ValueError(f"q must be contiguous bf16 [{b}, HQ, D]")
+    _, hq, d = q.shape
+    if d not in (64, 128, 256):
+        raise ValueError(f"head_dim {d} not supported (64, 128, 256)")
+    if bounds.dim() != 5 or bounds.shape[0] < 1:
+        raise ValueError("bounds must be bf16 [P, page_size / block_size, HKV, 2, D]")
     p, bpp, hkv = bounds.shape[:3]
     block = _bounds(bounds, p, hkv, d, page_size)
     _heads(hq, hkv)
     n = indices.numel() * bpp
     if output is None:
-        output = torch.empty((hkv, n), dtype=torch.float32, device=q.device)
-    _check(tuple(output.shape) == (hkv, n) and output.dtype == torch.float32 and output.is_contiguous(),
-           f"output must be contiguous float32 [{hkv}, {n}]")
+        output = q.new_empty((hkv, n), dtype=torch.float32)
+    elif output.shape != (hkv, n) or output.dtype != torch.float32 or not output.is_contiguous():
+        raise ValueError(f"output must be contiguous float32 [{hkv}, {n}]")
     _status(status)
     _call("axk_paged_block_scores", (q, bounds, indptr, indices, last_page_len, output, status), q.data_ptr(),
           bounds.data_ptr(), indptr.data_ptr(), indices.data_ptr(), last_page_len.data_ptr(), output.data_ptr(),
@@ -206,15 +213,16 @@ def paged_select_blocks(
     scores by the lowest block, NaN above every number; -1 behind the blocks of a shorter sequence."""
     b = _table(indptr, last_page_len)
     _sizes(page_size, block_size)
-    _check(scores.dim() == 2 and scores.dtype == torch.float32 and scores.is_contiguous() and scores.shape[0] > 0
-           and scores.shape[1] % (page_size // block_size) == 0,
-           "scores must be contiguous float32 [HKV, nnz * page_size / block_size]")
-    _check(first >= 0 and keep_last >= 0 and num_select > 0 and first + keep_last <= num_select,
-           f"num_select {num_select} must be positive and at least first {first} + keep_last {keep_last}")
+    if (scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous() or scores.shape[0] < 1
+            or scores.shape[1] % (page_size // block_size)):
+        raise ValueError("scores must be contiguous float32 [HKV, nnz * page_size / block_size]")
+    if first < 0 or keep_last < 0 or num_select < 1 or first + keep_last > num_select:
+        raise ValueError(f"num_select {num_select} must be positive and at least first {first} + keep_last {keep_last}")
     hkv = scores.shape[0]
     if output is None:
-        output = torch.empty((b, hkv, num_select), dtype=torch.int32, device=scores.device)
-    _i32(output, "output", b, hkv, num_select)
+        output = scores.new_empty((b, hkv, num_select), dtype=torch.int32)
+    else:
+        _i32(output, "output", b, hkv, num_select)
     _call("axk_paged_select_blocks", (scores, indptr, last_page_len, output), scores.data_ptr(), indptr.data_ptr(),
           last_page_len.data_ptr(), output.data_ptr(), scores.shape[1] // (page_size // block_size), b, hkv, page_size,
           block_size, num_select, first, keep_last)
@@ -255,13 +263,15 @@ def paged_decode_blocks(
     plus the attention that each page-table entry's tokens received, summed over the KV head's queries."""
     b = _table(indptr, last_page_len, indices)
     code, scale, p, page, hkv, d = _cache(kv_cache, kv_scale)
-    _check(q.dim() == 3 and q.shape[0] == b and q.shape[2] == d and q.dtype == torch.bfloat16 and q.is_contiguous(),
-           f"q must be contiguous bf16 [{b}, HQ, {d}]")
+    if q.dim() != 3 or q.shape[0] != b or q.shape[2] != d or q.dtype != torch.bfloat16 or not q.is_contiguous():
+        raise ValueError(f"q must be contiguous bf16 [{b}, HQ, {d}]")
     hq, nnz, n = q.shape[1], indices.numel(), 0
     _heads(hq, hkv)
     if blocks is not None:
-        _check(block_size is not None, "blocks need their block_size")
-        _check(blocks.dim() == 3 and blocks.shape[2] > 0, f"blocks must be int32 [{b}, {hkv}, n]")
+        if block_size is None:
+            raise ValueError("blocks need their block_size")
+        if blocks.dim() != 3 or blocks.shape[2] < 1:
+            raise ValueError(f"blocks must be int32 [{b}, {hkv}, n]")
         n = blocks.shape[2]
         _i32(blocks, "blocks", b, hkv, n)
     else:
@@ -271,15 +281,18 @@ def paged_decode_blocks(
         sm_scale = 1.0 / math.sqrt(d)
     if output is None:
         output = torch.empty_like(q)
-    _check(output.shape == q.shape and output.dtype == q.dtype and output.is_contiguous(), "bad output tensor")
-    _check(weights is not None or weights_in is None, "weights_in without weights")
-    for name, t in (("weights_in", weights_in), ("weights", weights)):
-        _check(t is None or (t.dtype == torch.float32 and tuple(t.shape) == (hkv, nnz) and t.is_contiguous()),
-               f"{name} must be contiguous float32 [{hkv}, {nnz}]")
+    elif output.shape != q.shape or output.dtype != q.dtype or not output.is_contiguous():
+        raise ValueError(f"output must be contiguous bf16 [{b}, {hq}, {d}]")
+    if weights is None and weights_in is not None:
+        raise ValueError("weights_in without weights")
+    for t in (weights_in, weights):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (hkv, nnz) or not t.is_contiguous()):
+            raise ValueError(f"weights_in and weights must be contiguous float32 [{hkv}, {nnz}]")
     _status(status)
     if workspace is None:
         workspace = paged_decode_blocks_workspace(b, hq, hkv, d, page, nnz, q.device, block_size, n, weights is not None)
-    _check(workspace.dtype == torch.uint8 and workspace.is_contiguous(), "workspace must be contiguous uint8")
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous uint8")
     _call("axk_paged_decode_blocks",
           (q, kv_cache, indptr, indices, last_page_len, blocks, output, weights_in, weights, status, workspace),
           q.data_ptr(), kv_cache.data_ptr(), code, scale, indptr.data_ptr(), indices.data_ptr(), last_page_len.data_ptr(),
@@ -302,15 +315,17 @@ def paged_evict_pages(
     the kept pages in their order with their weights, then -1 and 0, and the other pages' ids, then -1. last_page_len,
     the cache and the bounds stay as they are. A page that several sequences hold is freed for each that drops it."""
     b = indptr.numel() - 1
-    _check(b > 0, "the page table holds no sequence")
+    if b < 1:
+        raise ValueError("the page table holds no sequence")
     _i32(indptr, "indptr", b + 1)
-    _check(indices.dtype == torch.int32 and indices.dim() == 1 and indices.is_contiguous(),
-           "indices must be contiguous int32 [nnz]")
+    if indices.dtype != torch.int32 or indices.dim() != 1 or not indices.is_contiguous():
+        raise ValueError("indices must be contiguous int32 [nnz]")
     nnz = indices.numel()
-    _check(weights.dim() == 2 and weights.shape[0] > 0 and weights.shape[1] == nnz and weights.dtype == torch.float32
-           and weights.is_contiguous(), f"weights must be contiguous float32 [HKV, {nnz}]")
-    _check(first >= 0 and keep_last >= 1 and first + keep_last <= budget,
-           f"budget {budget} must hold first {first} (>= 0) + keep_last {keep_last} (>= 1) pages")
+    if (weights.dim() != 2 or weights.shape[0] < 1 or weights.shape[1] != nnz or weights.dtype != torch.float32
+            or not weights.is_contiguous()):
+        raise ValueError(f"weights must be contiguous float32 [HKV, {nnz}]")
+    if first < 0 or keep_last < 1 or first + keep_last > budget:
+        raise ValueError(f"budget {budget} must hold first {first} (>= 0) + keep_last {keep_last} (>= 1) pages")
     out = (torch.empty_like(indptr), torch.empty_like(indices), torch.empty_like(weights), torch.empty_like(indices))
     _call("axk_paged_evict_pages", (weights, indptr, indices, *out), weights.data_ptr(), indptr.data_ptr(),
           indices.data_ptr(), *(t.data_ptr() for t in out), nnz, b, weights.shape[0], budget, first, keep_last)

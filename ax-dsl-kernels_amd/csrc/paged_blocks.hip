@@ -29,23 +29,49 @@ struct Seq {
   int pb, np;
   int64_t len;
 };
-AXK_DEV Seq seq_of(const int* __restrict__ indptr, const int* __restrict__ last, int b, int page, int nnz) {
+AXK_DEV Seq seq_from(int lo, int hi, int last, int page, int nnz) {
   Seq s;
-  s.pb = min(max(indptr[b], 0), nnz);
-  s.np = min(max(indptr[b + 1], s.pb), nnz) - s.pb;
-  s.len = s.np ? (int64_t)(s.np - 1) * page + min(max(last[b], 0), page) : 0;
+  s.pb = min(max(lo, 0), nnz);
+  s.np = min(max(hi, s.pb), nnz) - s.pb;
+  s.len = s.np ? (int64_t)(s.np - 1) * page + min(max(last, 0), page) : 0;
   return s;
 }
-
-// The sequence that holds page-table entry e (the number of sequences ending at or before it), by one wave.
-AXK_DEV int owner_of(const int* __restrict__ indptr, int batch, int e) {
-  int n = 0;
-  for (int b0 = 0; b0 < batch; b0 += 64) {
-    const int b = b0 + (int)(threadIdx.x & 63);
-    n += __popcll(__ballot(b < batch && indptr[b + 1] <= e));
-  }
-  return n;
+AXK_DEV Seq seq_of(const int* __restrict__ indptr, const int* __restrict__ last, int b, int page, int nnz) {
+  return seq_from(indptr[b], indptr[b + 1], last[b], page, nnz);
 }
+
+// The sequence that holds page-table entry e (b = batch: none does), found by one wave: lanes hold 64 sequences at a time,
+// so that up to 64 sequences cost one round trip to memory, with the sequence's own numbers.
+struct Owner {
+  int b;
+  Seq s;
+};
+AXK_DEV Owner owner_of(const int* __restrict__ indptr, const int* __restrict__ last, int batch, int page, int nnz, int e) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < batch; b0 += 64) {
+    const int b = min(b0 + lane, batch - 1);
+    const int lo = indptr[b], hi = indptr[b + 1], tail = last[b];
+    const uint64_t after = __ballot(hi > e);  // sequences ending past e: the first of them
+    if (after) {
+      const int src = __ffsll((unsigned long long)after) - 1;
+      return {b0 + src, seq_from(__builtin_amdgcn_readlane(lo, src), __builtin_amdgcn_readlane(hi, src),
+                                 __builtin_amdgcn_readlane(tail, src), page, nnz)};
+    }
+  }
+  return {batch, {0, 0, 0}};
+}
+
+// Inclusive sum over the lanes of a wave: shifts within rows of 16 lanes, then the rows' totals passed on.
+AXK_DEV unsigned wave_scan(unsigned v) {
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+AXK_DEV int wave_total(int v) { return __builtin_amdgcn_readlane((int)wave_scan((unsigned)v), 63); }
 
 // Two bf16 values (one dword) as two 16-bit integers of the same order, and back (the map is its own inverse): the 15
 // low bits of a negative value are flipped. NaN lies beyond the infinity of its sign.
@@ -192,13 +218,13 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
   const int tid = threadIdx.x;
   const int bpp = page_size / block;
   const int entry = blockIdx.x / bpp, sub = blockIdx.x - entry * bpp;
-  const int b = owner_of(indptr, batch, entry);
-  if (b >= batch) return;  // past the last sequence
-  const Seq s = seq_of(indptr, last, b, page_size, nnz);
+  const int page = indices[entry];
+  const Owner own = owner_of(indptr, last, batch, page_size, nnz, entry);
+  if (own.b >= batch) return;  // past the last sequence
+  const Seq s = own.s;
   const int64_t t0 = (int64_t)(entry - s.pb) * page_size + (int64_t)sub * block;
   const int rows = (int)min((int64_t)block, s.len - t0);
-  if (entry < s.pb || rows <= 0 || (start && t0 + block <= start[b])) return;
-  const int page = indices[entry];
+  if (entry < s.pb || rows <= 0 || (start && t0 + block <= start[own.b])) return;
   if (page < 0 || page >= num_pages) {
     if (status && tid == 0) *status = 1;
     return;
@@ -269,9 +295,9 @@ __global__ __launch_bounds__(256) void paged_block_scores_kernel(
   // lane l16 of each lane group looks at block tile * 16 + l16
   const int64_t f = tile * 16 + l16;
   const int e = (int)(min(f, total - 1) / bpp);
-  const int first = owner_of(indptr, batch, __builtin_amdgcn_readlane(e, 0));
-  const int lastb = owner_of(indptr, batch, __builtin_amdgcn_readlane(e, 15));
   const int id = indices[e];
+  const int e0 = __builtin_amdgcn_readlane(e, 0), e1 = __builtin_amdgcn_readlane(e, 15);
+  Owner own = owner_of(indptr, last, batch, page_size, nnz, e0);
   const bool good = id >= 0 && id < num_pages;
   const int sub = (int)(f - (int64_t)e * bpp);
   const uint16_t* row = bounds + (((int64_t)(good ? id : 0) * bpp + (f < total ? sub : 0)) * hkv + h) * 2 * D + 8 * g;
@@ -281,8 +307,9 @@ __global__ __launch_bounds__(256) void paged_block_scores_kernel(
     lo[s] = load_bf16x8(row + 32 * s);
     hi[s] = load_bf16x8(row + D + 32 * s);
   }
-  for (int b = first; b <= min(lastb, batch - 1); ++b) {
-    const Seq sq = seq_of(indptr, last, b, page_size, nnz);
+  for (int b = own.b; b < batch; ++b) {  // the sequences whose entries reach into the tile
+    const Seq sq = b == own.b ? own.s : seq_of(indptr, last, b, page_size, nnz);
+    if (sq.pb > e1) break;
     axk_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     const uint16_t* qr = q + ((int64_t)b * hq + h * group + l16) * D + 8 * g;
 #pragma unroll
@@ -318,103 +345,119 @@ __global__ __launch_bounds__(256) void paged_block_scores_kernel(
 }
 
 // ---- the `want` largest of a row ----
-// Radix selection by one workgroup of T threads: the bits that all keys share are skipped (from their minimum and
-// maximum), then 8 bits at a time are counted in LDS until the smallest key that is taken is known, or all keys that
-// agree with it so far are taken. Up to 16 T keys stay in registers; a longer row is read again in each step. Equal keys
-// at the border are taken by the lowest index. emit(i, taken, rank) is called for every index, rank = the indices below
-// i that are taken.
-constexpr int kKeys = 16;  // keys a thread holds
+// Radix selection by one workgroup of T threads, K consecutive keys each in registers (a longer row is read again, T K keys
+// at a time, in each step). Keys are taken relative to the row's smallest, and log2(4 T) bits at a time, from the highest
+// that the row's range has, are counted in 4 T bins of LDS, until the smallest key that is taken is known or all keys that
+// agree with it so far are taken: two rounds as a rule. (With 256 bins of the raw bits a row of 8192 scores took 8.5 us
+// more: most scores share sign and exponent, and adds to one address wait for each other.) Equal keys at the border are
+// taken by the lowest index. load(at, n, key) fetches a thread's n keys from index `at`; emit(i, taken, rank) is called
+// for every index, rank = the indices below i that are taken; done(base, n, k) after the n indices of a tile, k of them
+// taken.
 template <class Key, int T>
 struct PickLds {
-  unsigned hist[2][256];
+  unsigned hist[4 * T];
   Key lo[T / 64], hi[T / 64];
   unsigned sums[T / 64];
   unsigned digit, above, inside;
 };
 
-template <class Key, int T, class Load, class Emit>
-AXK_DEV void pick_largest(int count, int want, const Load& load, const Emit& emit, PickLds<Key, T>& lds) {
+// A 32- or 64-bit value moved by DPP (lanes without a source keep theirs), and a wave's minimum and maximum of it.
+template <int CTRL, int ROW_MASK = 0xF>
+AXK_DEV uint32_t dpp_key(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, ROW_MASK, 0xF, false);
+}
+template <int CTRL, int ROW_MASK = 0xF>
+AXK_DEV uint64_t dpp_key(uint64_t v) {
+  return (uint64_t)dpp_key<CTRL, ROW_MASK>((uint32_t)(v >> 32)) << 32 | dpp_key<CTRL, ROW_MASK>((uint32_t)v);
+}
+AXK_DEV uint32_t lane63_key(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+AXK_DEV uint64_t lane63_key(uint64_t v) { return (uint64_t)lane63_key((uint32_t)(v >> 32)) << 32 | lane63_key((uint32_t)v); }
+template <class Key, class Op>
+AXK_DEV Key wave_key(Key v, const Op& op) {
+  v = op(v, dpp_key<0xB1>(v));
+  v = op(v, dpp_key<0x4E>(v));
+  v = op(v, dpp_key<0x141>(v));
+  v = op(v, dpp_key<0x140>(v));
+  v = op(v, dpp_key<0x142, 0xA>(v));
+  v = op(v, dpp_key<0x143, 0xC>(v));
+  return lane63_key(v);
+}
+
+template <class Key, int T, int K, class Load, class Emit, class Done>
+AXK_DEV void pick_largest(int count, int want, const Load& load, const Emit& emit, const Done& done, PickLds<Key, T>& lds) {
+  constexpr int kTile = T * K, kBits = 8 * sizeof(Key), kStep = T == 1024 ? 12 : 10;
+  static_assert(4 * T == 1 << kStep, "four bins a thread");
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int tile = T * kKeys, tiles = (count + tile - 1) / tile;
-  const int per = tiles > 1 ? kKeys : (count + T - 1) / T;  // consecutive indices a thread holds
-  Key key[kKeys];
+  const int tiles = (count + kTile - 1) / kTile;
+  const int per = tiles > 1 ? K : (count + T - 1) / T;  // consecutive indices a thread holds
+  Key key[K];
+  int mine = 0;  // how many of them there are
   auto load_tile = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < kKeys; ++i) {
-      const int at = t * tile + tid * per + i;
-      key[i] = i < per && at < count ? load(at) : (Key)0;
-    }
+    mine = min(max(count - t * kTile - tid * per, 0), per);
+    load(t * kTile + tid * per, mine, key);
   };
-  auto there = [&](int t, int i) { return i < per && t * tile + tid * per + i < count; };
   if (tiles == 1) load_tile(0);
+  *reinterpret_cast<uint4*>(&lds.hist[4 * tid]) = make_uint4(0, 0, 0, 0);
   Key lo = ~(Key)0, hi = 0;
   for (int t = 0; t < tiles; ++t) {
     if (tiles > 1) load_tile(t);
 #pragma unroll
-    for (int i = 0; i < kKeys; ++i)
-      if (there(t, i)) {
+    for (int i = 0; i < K; ++i)
+      if (i < mine) {
         lo = min(lo, key[i]);
         hi = max(hi, key[i]);
       }
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    lo = min(lo, (Key)__shfl_xor(lo, o, 64));
-    hi = max(hi, (Key)__shfl_xor(hi, o, 64));
-  }
+  lo = wave_key(lo, [](Key x, Key y) { return min(x, y); });
+  hi = wave_key(hi, [](Key x, Key y) { return max(x, y); });
   if (lane == 0) {
     lds.lo[wave] = lo;
     lds.hi[wave] = hi;
   }
-  for (int i = tid; i < 256; i += T) lds.hist[0][i] = 0;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < T / 64; ++w) {
-    lo = min(lo, lds.lo[w]);
-    hi = max(hi, lds.hi[w]);
-  }
-  constexpr int kBits = 8 * sizeof(Key);
-  int pos = lo == hi ? 0 : kBits - (sizeof(Key) == 8 ? __clzll((long long)(lo ^ hi)) : __clz((int)(lo ^ hi)));
-  Key prefix = pos >= kBits ? (Key)0 : (hi >> pos) << pos;  // the border key's bits from `pos` up
-  unsigned remaining = (unsigned)want;                      // keys to take among those that agree with it
+  lo = lds.lo[lane % (T / 64)];
+  hi = lds.hi[lane % (T / 64)];
+  lo = wave_key(lo, [](Key x, Key y) { return min(x, y); });
+  hi = wave_key(hi, [](Key x, Key y) { return max(x, y); });
+  const Key range = hi - lo;
+  int pos = range ? kBits - (sizeof(Key) == 8 ? __clzll((long long)range) : __clz((int)range)) : 0;  // bits of key - lo
+  Key prefix = 0;                       // the border key's bits from `pos` up
+  unsigned remaining = (unsigned)want;  // keys to take among those that agree with it
   bool all = false;
-  for (int step = 0; pos > 0 && !all; ++step) {
-    const int w = min(8, pos);
-    const Key mask = pos >= kBits ? (Key)0 : ~(Key)0 << pos;
+  while (pos > 0 && !all) {
+    const int w = min(kStep, pos), from = pos;
     pos -= w;
-    unsigned* hist = lds.hist[step & 1];
     for (int t = 0; t < tiles; ++t) {
       if (tiles > 1) load_tile(t);
 #pragma unroll
-      for (int i = 0; i < kKeys; ++i)
-        if (there(t, i) && ((key[i] ^ prefix) & mask) == 0)
-          atomicAdd(&hist[(unsigned)(key[i] >> pos) & ((1u << w) - 1u)], 1u);
+      for (int i = 0; i < K; ++i) {
+        const Key x = key[i] - lo;
+        if (i < mine && (from == kBits || (x ^ prefix) >> from == 0))
+          atomicAdd(&lds.hist[(unsigned)(x >> pos) & ((1u << w) - 1u)], 1u);
+      }
     }
     __syncthreads();
-    if (wave == 0) {  // lane l: bins 255 - 4 l .. 252 - 4 l, from the top
-      unsigned c[4], sum = 0;
+    // thread t: bins 4 (T - 1 - t) .. + 3, so that the scan runs from the top
+    uint4* bins = reinterpret_cast<uint4*>(&lds.hist[4 * (T - 1 - tid)]);
+    const uint4 c4 = *bins;
+    *bins = make_uint4(0, 0, 0, 0);
+    const unsigned c[4] = {c4.w, c4.z, c4.y, c4.x}, sum = c[0] + c[1] + c[2] + c[3];
+    const unsigned incl = wave_scan(sum);
+    if (lane == 63) lds.sums[wave] = incl;
+    __syncthreads();
+    unsigned before = incl - sum;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += c[i] = hist[255 - 4 * lane - i];
-      unsigned incl = sum;
+    for (int i = 0; i < T / 64; ++i) before += i < wave ? lds.sums[i] : 0u;
+    if (before < remaining && remaining <= before + sum) {
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const unsigned x = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += x;
-      }
-      unsigned before = incl - sum;
-      if (before < remaining && remaining <= incl) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (before < remaining && remaining <= before + c[i]) {
-            lds.digit = 255 - 4 * lane - i;
-            lds.above = before;
-            lds.inside = c[i];
-          }
-          before += c[i];
+      for (int i = 0; i < 4; ++i) {
+        if (before < remaining && remaining <= before + c[i]) {
+          lds.digit = 4 * (T - 1 - tid) + 3 - i;
+          lds.above = before;
+          lds.inside = c[i];
         }
+        before += c[i];
       }
-    } else {
-      for (int i = tid - 64; i < 256; i += T - 64) lds.hist[(step + 1) & 1][i] = 0;
     }
     __syncthreads();
     prefix |= (Key)lds.digit << pos;
@@ -426,39 +469,55 @@ AXK_DEV void pick_largest(int count, int want, const Load& load, const Emit& emi
   unsigned above0 = 0, on0 = 0;
   for (int t = 0; t < tiles; ++t) {
     if (tiles > 1) load_tile(t);
-    unsigned n = 0;  // above in the high half, on the border in the low half: at most 16 T < 65536 of each
+    unsigned up = 0, eq = 0;  // a bit a key: above the border, on it
 #pragma unroll
-    for (int i = 0; i < kKeys; ++i)
-      if (there(t, i)) {
-        const Key x = key[i] >> pos;
-        n += x > border ? 0x10000u : x == border ? 1u : 0u;
+    for (int i = 0; i < K; ++i)
+      if (i < mine) {
+        const Key x = (key[i] - lo) >> pos;
+        up |= (x > border ? 1u : 0u) << i;
+        eq |= (x == border ? 1u : 0u) << i;
       }
-    unsigned incl = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const unsigned x = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += x;
-    }
+    // above in the high half, on the border in the low half: at most T K < 65536 of each
+    const unsigned n = ((unsigned)__popc(up) << 16) + (unsigned)__popc(eq), incl = wave_scan(n);
     __syncthreads();  // the sums of the tile before have been read
     if (lane == 63) lds.sums[wave] = incl;
     __syncthreads();
     unsigned before = incl - n, total = 0;
 #pragma unroll
-    for (int w = 0; w < T / 64; ++w) {
-      if (w < wave) before += lds.sums[w];
-      total += lds.sums[w];
+    for (int i = 0; i < T / 64; ++i) {
+      const unsigned x = lds.sums[i];
+      before += i < wave ? x : 0u;
+      total += x;
     }
     unsigned above = above0 + (before >> 16), on = on0 + (before & 0xffffu);
-#pragma unroll
-    for (int i = 0; i < kKeys; ++i)
-      if (there(t, i)) {
-        const Key x = key[i] >> pos;
-        emit(t * tile + tid * per + i, x > border || (x == border && on < remaining), (int)(above + min(on, remaining)));
-        above += x > border;
-        on += x == border;
-      }
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      const unsigned u = (up >> i) & 1u, q = (eq >> i) & 1u;
+      emit(t * kTile + tid * per + i, u || (q && on < remaining), (int)(above + min(on, remaining)));
+      above += u;
+      on += q;
+    }
+    const unsigned before_tile = above0 + min(on0, remaining);
     above0 += total >> 16;
     on0 += total & 0xffffu;
+    done(t * kTile, min(count - t * kTile, kTile), (int)(above0 + min(on0, remaining) - before_tile));
+  }
+}
+
+// n <= K floats from p, four at a time where all K are there (p need not be 16-byte aligned)
+template <int K>
+AXK_DEV void load_run(const float* __restrict__ p, int n, float (&x)[K]) {
+  typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+  if (K % 4 == 0 && n == K) {
+#pragma unroll
+    for (int i = 0; i < K; i += 4) {
+      const f4 v = *reinterpret_cast<const f4*>(p + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i + j] = v[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < K; ++i) x[i] = i < n ? p[i] : 0.f;
   }
 }
 
@@ -475,6 +534,22 @@ AXK_DEV uint64_t order_key(double x) {
 }
 
 // One workgroup per (sequence, KV head): its n best blocks, the first `first` and last `keep_last` always among them.
+template <int T, int K>
+AXK_DEV void select_row(const float* __restrict__ row, int count, int want, int* __restrict__ out, int first,
+                        PickLds<uint32_t, T>& lds) {
+  pick_largest<uint32_t, T, K>(
+      count, want,
+      [&](int at, int n, uint32_t(&key)[K]) {
+        float x[K];
+        load_run<K>(row + at, n, x);
+#pragma unroll
+        for (int i = 0; i < K; ++i) key[i] = order_key(x[i]);
+      },
+      [&](int i, bool taken, int rank) {
+        if (taken) out[rank] = first + i;
+      },
+      [](int, int, int) {}, lds);
+}
 template <int T>
 __global__ __launch_bounds__(T) void paged_select_blocks_kernel(const float* __restrict__ scores,
                                                                 const int* __restrict__ indptr,
@@ -493,15 +568,12 @@ __global__ __launch_bounds__(T) void paged_select_blocks_kernel(const float* __r
   }
   for (int i = tid; i < first; i += T) o[i] = i;
   for (int i = tid; i < keep_last; i += T) o[n - keep_last + i] = nb - keep_last + i;
-  const int want = n - first - keep_last;
+  const int want = n - first - keep_last, count = nb - first - keep_last;
   if (want == 0) return;
   const float* row = scores + (int64_t)h * nnz * bpp + (int64_t)s.pb * bpp + first;
-  pick_largest<uint32_t, T>(
-      nb - first - keep_last, want, [&](int i) { return order_key(row[i]); },
-      [&](int i, bool taken, int rank) {
-        if (taken) o[first + rank] = first + i;
-      },
-      lds);
+  if (count <= 2 * T) select_row<T, 2>(row, count, want, o + first, first, lds);
+  else if (count <= 8 * T || T < 1024) select_row<T, 8>(row, count, want, o + first, first, lds);
+  else select_row<T, 16>(row, count, want, o + first, first, lds);
 }
 
 // ---- decode over blocks ----
@@ -548,89 +620,93 @@ struct BlkArgs {
 };
 
 // Which sequence and which of its pieces flat piece `it` of a KV head is, where every block is attended: the pieces of
-// a sequence are as many as its subtiles need. b = batch past the last one. All threads of a workgroup of 256.
+// a sequence are as many as its subtiles need. b = batch past the last one.
 struct PieceOf {
   int b, piece;
+  Seq s;
 };
 AXK_DEV int pieces_of(const Seq& s, int ps) { return (int)((s.len + (int64_t)kSub * ps - 1) / ((int64_t)kSub * ps)); }
-AXK_DEV PieceOf find_piece(const BlkArgs& a, int it, int* sh) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+AXK_DEV PieceOf find_piece(const BlkArgs& a, int it) {
+  const int lane = threadIdx.x & 63;
   int base = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 256) {
-    const int b = b0 + tid;
-    const int cnt = b < a.batch ? pieces_of(seq_of(a.indptr, a.last, b, a.page, a.nnz), a.ps) : 0;
-    int incl = cnt;
+  for (int b0 = 0; b0 < a.batch; b0 += 256) {  // 256 sequences a round trip to memory, each wave for itself
+    int lo[4], hi[4], last[4];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += x;
+    for (int i = 0; i < 4; ++i) {
+      const int b = min(b0 + 64 * i + lane, a.batch - 1);
+      lo[i] = a.indptr[b];
+      hi[i] = a.indptr[b + 1];
+      last[i] = a.last[b];
     }
-    if (tid == 0) sh[4] = a.batch;
-    if (lane == 63) sh[wave] = incl;
-    __syncthreads();
-    int before = base + incl - cnt;
-    for (int w = 0; w < wave; ++w) before += sh[w];
-    if (it >= before && it < before + cnt) {
-      sh[4] = b;
-      sh[5] = it - before;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (b0 + 64 * i >= a.batch) break;
+      const int n = b0 + 64 * i + lane < a.batch ? pieces_of(seq_from(lo[i], hi[i], last[i], a.page, a.nnz), a.ps) : 0;
+      const int before = base + (int)wave_scan((unsigned)n) - n;
+      const uint64_t mine = __ballot(it >= before && it < before + n);
+      if (mine) {
+        const int src = __ffsll((unsigned long long)mine) - 1;
+        return {b0 + 64 * i + src, it - __builtin_amdgcn_readlane(before, src),
+                seq_from(__builtin_amdgcn_readlane(lo[i], src), __builtin_amdgcn_readlane(hi[i], src),
+                         __builtin_amdgcn_readlane(last[i], src), a.page, a.nnz)};
+      }
+      base = __builtin_amdgcn_readlane(before + n, 63);
     }
-    base += sh[0] + sh[1] + sh[2] + sh[3];
-    __syncthreads();
-    if (sh[4] < a.batch) return {sh[4], sh[5]};
-    __syncthreads();
   }
-  return {a.batch, 0};
+  return {a.batch, 0, {0, 0, 0}};
 }
-// Pieces of the sequences before b, where every block is attended (all threads of a workgroup of 256).
-AXK_DEV int pieces_before(const BlkArgs& a, int b, int* sh) {
+// Pieces of the sequences before b, where every block is attended (each wave for itself).
+AXK_DEV int pieces_before(const BlkArgs& a, int b) {
   int n = 0;
-  for (int i = threadIdx.x; i < b; i += 256) n += pieces_of(seq_of(a.indptr, a.last, i, a.page, a.nnz), a.ps);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = n;
-  __syncthreads();
-  return sh[0] + sh[1] + sh[2] + sh[3];
+  for (int i = threadIdx.x & 63; i < b; i += 64) n += pieces_of(seq_of(a.indptr, a.last, i, a.page, a.nnz), a.ps);
+  return wave_total(n);
 }
 
-// Listed block `slot` of a row: its logical block, or -1 for padding, a block past the sequence's end, or one that does
-// not lie above its predecessor in the list (`bad` is then set, but for padding).
-AXK_DEV int listed_block(const int* __restrict__ list, int slot, int64_t nblocks, bool* bad) {
-  const int id = list[slot], prev = slot ? list[slot - 1] : -1;
-  *bad = id < -1 || id >= nblocks || (id >= 0 && slot && prev >= id);
-  return *bad ? -1 : id;
+// Whether a listed block is neither padding (-1) nor a block of the sequence that lies above its predecessor in the list
+// (prev: -1 for the first).
+AXK_DEV bool bad_block(int id, int prev, int64_t nblocks) {
+  return id < -1 || id >= nblocks || (id >= 0 && prev >= id);
 }
 
-constexpr int kMaxPs = 128;  // subtiles of a piece, at most
+constexpr int kMaxPs = 128;  // subtiles of a piece, at most (two a lane)
 
 template <int D, int F8>
 __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   using C = BlkCfg<D, F8>;
-  __shared__ __align__(16) float s_o[2][C::ACC * 256];
+  constexpr int Q = C::ACC / 4;  // accumulator tiles a wave gives out at the end
+  __shared__ __align__(16) float s_o[4][3][Q * 256];
   __shared__ int64_t s_base[kMaxPs];
   __shared__ int s_valid[kMaxPs];
   __shared__ float s_m[4][16], s_l[4][16];
-  __shared__ int s_find[8];
-  __shared__ int s_end;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
   const int group = a.hq / a.hkv;
   int b, h, piece;
   int64_t item;
+  Seq s;
+  const int spb = a.block / kSub;
+  int id = -1, prev = -1;  // thread i: the listed block that subtile i of the piece lies in, and the one before it
   if (a.blocks) {
     item = blockIdx.x;
     const int row = blockIdx.x / a.pieces;
     piece = blockIdx.x - row * a.pieces;
     b = row / a.hkv;
     h = row - b * a.hkv;
+    const int64_t slot = ((int64_t)piece * a.ps + tid) / spb;
+    if (tid < a.ps && slot < a.n) {
+      const int* list = a.blocks + (int64_t)row * a.n + slot;
+      id = list[0];
+      if (slot) prev = list[-1];
+    }
+    s = seq_of(a.indptr, a.last, b, a.page, a.nnz);
   } else {
     h = blockIdx.y;
     item = (int64_t)h * a.pieces + blockIdx.x;
-    const PieceOf p = find_piece(a, blockIdx.x, s_find);
+    const PieceOf p = find_piece(a, blockIdx.x);
     b = p.b;
     piece = p.piece;
+    s = p.s;
     if (b >= a.batch) return;
   }
-  const Seq s = seq_of(a.indptr, a.last, b, a.page, a.nnz);
   // Q first: its loads are under way while the subtiles' places are looked up
   axk_bf16x8 qf[C::KS];
 #pragma unroll
@@ -640,41 +716,39 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   }
   // the piece's subtiles: where each lies in the cache, and how many of its tokens count
   const int64_t rowb = (int64_t)a.hkv * D * C::B;  // bytes of a token row
-  const int spb = a.block / kSub, spp = a.page / kSub;
+  const int spp = a.page / kSub;
   const int64_t nsub = a.blocks ? (int64_t)a.n * spb : (s.len + kSub - 1) / kSub;  // of the row
   const int64_t sub0 = (int64_t)piece * a.ps;
   const int count = (int)min((int64_t)a.ps, nsub - sub0);
-  if (tid == 0) s_end = 0;
-  __syncthreads();
-  for (int i = tid; i < a.ps; i += 256) {
+  if (tid < a.ps) {
     int valid = 0;
     int64_t base = 0;
-    if (i < count) {
-      int64_t t0 = (sub0 + i) * kSub;  // the subtile's first token
+    if (tid < count) {
+      int64_t t0 = (sub0 + tid) * kSub;  // the subtile's first token
       bool bad = false;
       if (a.blocks) {
-        const int slot = (int)((sub0 + i) / spb);
-        const int id = listed_block(a.blocks + ((int64_t)b * a.hkv + h) * a.n, slot, (s.len + a.block - 1) / a.block, &bad);
-        t0 = id < 0 ? s.len : (int64_t)id * a.block + ((sub0 + i) - (int64_t)slot * spb) * kSub;
+        bad = bad_block(id, prev, (s.len + a.block - 1) / a.block);
+        t0 = bad || id < 0 ? s.len : (int64_t)id * a.block + (sub0 + tid) % spb * kSub;
       }
       valid = (int)min(max(s.len - t0, (int64_t)0), (int64_t)kSub);
       if (valid) {
-        const int p = (int)(t0 / a.page), id = a.indices[s.pb + p];
-        if (id < 0 || id >= a.num_pages) {
+        const int p = (int)(t0 / a.page), at = a.indices[s.pb + p];
+        if (at < 0 || at >= a.num_pages) {
           bad = true;
           valid = 0;
         } else {
-          base = ((int64_t)id * 2 * a.page + (t0 - (int64_t)p * a.page)) * rowb;
+          base = ((int64_t)at * 2 * a.page + (t0 - (int64_t)p * a.page)) * rowb;
         }
       }
       if (bad && a.status) *a.status = 1;
     }
-    s_base[i] = base;
-    s_valid[i] = valid;
-    if (valid) atomicMax(&s_end, i + 1);
+    s_base[tid] = base;
+    s_valid[tid] = valid;
   }
   __syncthreads();
-  const int end = s_end;  // what follows is padding of the list
+  // one past the last subtile with a token: what follows is padding of the list
+  const uint64_t low = __ballot(lane < a.ps && s_valid[lane] > 0), high = __ballot(64 + lane < a.ps && s_valid[min(64 + lane, a.ps - 1)] > 0);
+  const int end = high ? 128 - __clzll((long long)high) : low ? 64 - __clzll((long long)low) : 0;
   const int64_t stat_at = (a.blocks ? ((int64_t)b * a.hkv + h) * nsub : ((int64_t)h * a.nnz + s.pb) * spp) + sub0;
   if (a.stat)
     for (int i = ((end + 1) & ~1) * group + tid; i < count * group; i += 256)
@@ -822,160 +896,163 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   for (int w = 0; w < 4; ++w) l += s_l[w][l16] * __builtin_amdgcn_exp2f(s_m[w][l16] - top);
 #pragma unroll
   for (int i = 0; i < C::ACC; ++i) acc[i] *= mine;
+  // each wave gives out the sum of a quarter of the accumulators, and leaves the others theirs
 #pragma unroll
-  for (int half = 2; half > 0; half >>= 1) {  // waves 2, 3 into 0, 1, then 1 into 0
-    if (wave >= half && wave < 2 * half) {
+  for (int w = 0; w < 4; ++w)
+    if (w != wave) {
 #pragma unroll
-      for (int i = 0; i < C::ACC; ++i) *reinterpret_cast<axk_f32x4*>(&s_o[wave - half][(i * 64 + lane) * 4]) = acc[i];
+      for (int i = 0; i < Q; ++i)
+        *reinterpret_cast<axk_f32x4*>(&s_o[w][wave < w ? wave : wave - 1][(i * 64 + lane) * 4]) = acc[w * Q + i];
     }
-    __syncthreads();
-    if (wave < half) {
+  __syncthreads();
+  if (l16 >= group) return;
+  const float inv = !a.direct ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
+  if (!a.direct && wave == 0 && g == 0) a.ml[item * group + l16] = make_float2(top, l);
+  uint16_t* out = a.out + ((int64_t)b * a.hq + h * group + l16) * D;
+  float* po = a.po + (item * group + l16) * D;
 #pragma unroll
-      for (int i = 0; i < C::ACC; ++i) acc[i] += *reinterpret_cast<axk_f32x4*>(&s_o[wave][(i * 64 + lane) * 4]);
+  for (int w = 0; w < 4; ++w)
+    if (w == wave) {
+      // lane: head l16, channels n 16 E + E (4 g + i) + e from acc[n E + e][i]
+      axk_f32x4 o[Q];
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        o[i] = acc[w * Q + i];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) o[i] += *reinterpret_cast<axk_f32x4*>(&s_o[w][j][(i * 64 + lane) * 4]);
+        o[i] *= inv;
+      }
+      const int at = w * Q / C::E * 16 * C::E + w * Q % C::E;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = at + C::E * (4 * g + i);
+        if (a.direct) {
+          if constexpr (Q == 1) {
+            out[d] = (uint16_t)f32_to_bf16_bits(o[0][i]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < Q; e += 2) *reinterpret_cast<uint32_t*>(out + d + e) = pack_bf16x2(o[e][i], o[e + 1][i]);
+          }
+        } else {
+          typedef float fq __attribute__((ext_vector_type(Q)));
+          fq x;
+#pragma unroll
+          for (int e = 0; e < Q; ++e) x[e] = o[e][i];
+          *reinterpret_cast<fq*>(po + d) = x;
+        }
+      }
     }
-    __syncthreads();
-  }
-  if (wave || l16 >= group) return;
-  // lane: head l16, channels n 16 E + E (4 g + i) + e from acc[n E + e][i]
-  if (a.direct) {
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    uint16_t* o = a.out + ((int64_t)b * a.hq + h * group + l16) * D;
-#pragma unroll
-    for (int n = 0; n < C::NH; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < C::E; e += 4)
-          *reinterpret_cast<uint2*>(o + n * 16 * C::E + C::E * (4 * g + i) + e) =
-              make_uint2(pack_bf16x2(acc[n * C::E + e][i] * inv, acc[n * C::E + e + 1][i] * inv),
-                         pack_bf16x2(acc[n * C::E + e + 2][i] * inv, acc[n * C::E + e + 3][i] * inv));
-    return;
-  }
-  if (g == 0) a.ml[item * group + l16] = make_float2(top, l);
-  float* o = a.po + (item * group + l16) * D;
-#pragma unroll
-  for (int n = 0; n < C::NH; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < C::E; e += 4)
-        *reinterpret_cast<axk_f32x4*>(o + n * 16 * C::E + C::E * (4 * g + i) + e) =
-            (axk_f32x4){acc[n * C::E + e][i], acc[n * C::E + e + 1][i], acc[n * C::E + e + 2][i], acc[n * C::E + e + 3][i]};
 }
 
 struct WeightArgs {
   const float* in;  // [hkv, nnz], null: zeros
   float* out;       // ..., null: not wanted
   float decay;
+  int split;        // workgroups that share a row's output
 };
 
-// The joined maximum and the inverse sum of a head over its pieces (lane p of the wave looks at pieces p, p + 64, ...).
-AXK_DEV float2 head_total(const float2* __restrict__ ml, int pieces, int group, int head) {
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY, l = 0.f;
-  for (int p = lane; p < pieces; p += 64) {
-    const float2 x = ml[(int64_t)p * group + head];
-    if (x.y == 0.f) continue;  // nothing counted
-    const float top = fmaxf(m, x.x);
-    l = l * __builtin_amdgcn_exp2f(m - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
-    m = top;
-  }
-  const float top = wave_max(m);
-  l = wave_sum(m == -INFINITY ? 0.f : l * __builtin_amdgcn_exp2f(m - top));
-  return make_float2(top, l == 0.f ? 0.f : 1.0f / l);
+// Two partial softmax sums as one; a sum of zero means that nothing was counted, whatever its maximum.
+AXK_DEV float2 join(float2 x, float2 y) {
+  if (y.y == 0.f) return x;
+  if (x.y == 0.f) return y;
+  const float top = fmaxf(x.x, y.x);
+  return make_float2(top, x.y * __builtin_amdgcn_exp2f(x.x - top) + y.y * __builtin_amdgcn_exp2f(y.x - top));
 }
 
-// Workgroups [0, batch * hq): the output row of a (sequence, query head) from its pieces. The others: the page weights,
-// from each subtile's sum against the row's joined maximum and sum.
+// Workgroups [0, batch * hkv): the output rows of a (sequence, KV head) from its pieces. The others: the page weights, from
+// each subtile's sum against the row's joined maximum and sum. Every workgroup joins the pieces' sums of all heads of its
+// row first (16 lanes a piece, a head each), while the first partial outputs are on their way.
+constexpr int kListLds = 2048;  // listed blocks whose shares are kept in LDS at a time
 template <int D>
 __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a, const WeightArgs w) {
-  __shared__ __align__(16) float s_o[4][D];
+  __shared__ float2 s_part[16][16];
   __shared__ float s_top[kMaxGroup], s_inv[kMaxGroup];
-  __shared__ int s_sum[8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int group = a.hq / a.hkv;
-  const bool outs = (int)blockIdx.x < a.batch * a.hq;
-  int b, h, head = 0, pieces = a.pieces, piece = 0;
+  __shared__ axk_f32x4 s_o[4][64];
+  __shared__ float s_share[kListLds];
+  __shared__ int s_page[kListLds + 1];
+  const int tid = threadIdx.x, l16 = tid & 15, r16 = tid >> 4;
+  const int group = a.hq / a.hkv, rows = a.batch * a.hkv;
+  const bool outs = (int)blockIdx.x < rows * w.split;
+  int b, h, part = 0, pieces = a.pieces, piece = 0;
   int64_t item;
-  if (outs) {
-    b = blockIdx.x / a.hq;
-    head = blockIdx.x - b * a.hq;
-    h = head / group;
-    head -= h * group;
-    item = ((int64_t)b * a.hkv + h) * a.pieces;
-    if (!a.blocks) {
-      piece = min(pieces_before(a, b, s_sum), a.pieces);
-      item = (int64_t)h * a.pieces + piece;
-    }
-  } else {
-    const int x = blockIdx.x - a.batch * a.hq;
-    if (a.blocks) {  // one workgroup per row
-      b = x / a.hkv;
-      h = x - b * a.hkv;
-      item = (int64_t)x * a.pieces;
-    } else {  // one per piece, for the pages that begin in it
-      h = x / a.pieces;
-      const PieceOf p = find_piece(a, x - h * a.pieces, s_sum);
-      if (p.b >= a.batch) return;
-      b = p.b;
-      piece = p.piece;
-      item = x - piece;
-    }
+  Seq s;
+  if (outs || a.blocks) {
+    int row = outs ? blockIdx.x / w.split : blockIdx.x - rows * w.split;
+    part = outs ? blockIdx.x - row * w.split : 0;
+    b = row / a.hkv;
+    h = row - b * a.hkv;
+    s = seq_of(a.indptr, a.last, b, a.page, a.nnz);
+    item = (int64_t)row * a.pieces;
+    if (!a.blocks) item = (int64_t)h * a.pieces + min(pieces_before(a, b), a.pieces);
+  } else {  // one workgroup per piece, for the pages that begin in it
+    const int x = blockIdx.x - rows * w.split;
+    h = x / a.pieces;
+    const PieceOf p = find_piece(a, x - h * a.pieces);
+    if (p.b >= a.batch) return;
+    b = p.b;
+    piece = p.piece;
+    s = p.s;
+    item = x - piece;
   }
-  const Seq s = seq_of(a.indptr, a.last, b, a.page, a.nnz);
   // the pieces that the grid held (all of them, unless offsets of indptr overlap)
   if (!a.blocks) pieces = min(pieces_of(s, a.ps), (int)((h + 1) * (int64_t)a.pieces - item));
   const float2* ml = a.ml + item * group;
-  if (outs) {
-    const float2 t = head_total(ml, pieces, group, head);
-    constexpr int V = D / 64;
-    float o[V];
+  float2 t = make_float2(0.f, 0.f);
+  if (l16 < group)
+    for (int p = r16; p < pieces; p += 16) t = join(t, ml[(int64_t)p * group + l16]);
+  s_part[r16][l16] = t;
+  __syncthreads();
+  if (tid < 16) {
+    t = s_part[0][tid];
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = 0.f;
-#pragma unroll 4
-    for (int p = wave; p < pieces; p += 4) {
-      const float2 x = ml[(int64_t)p * group + head];
-      if (x.y == 0.f) continue;  // its partial output was not needed, and is nothing
-      const float f = __builtin_amdgcn_exp2f(x.x - t.x);
-      const float* po = a.po + ((item + p) * group + head) * D + lane * V;
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] += f * po[i];
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) s_o[wave][lane * V + i] = o[i];
-    __syncthreads();
-    uint16_t* out = a.out + ((int64_t)b * a.hq + h * group + head) * D;
-    for (int i = 2 * tid; i < D; i += 512)
-      *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2((s_o[0][i] + s_o[1][i] + s_o[2][i] + s_o[3][i]) * t.y,
-                                                          (s_o[0][i + 1] + s_o[1][i + 1] + s_o[2][i + 1] + s_o[3][i + 1]) * t.y);
-    return;
-  }
-  for (int i = wave; i < group; i += 4) {
-    const float2 t = head_total(ml, pieces, group, i);
-    if (lane == 0) {
-      s_top[i] = t.x;
-      s_inv[i] = t.y;
-    }
+    for (int i = 1; i < 16; ++i) t = join(t, s_part[i][tid]);
+    s_top[tid] = t.x;
+    s_inv[tid] = t.y == 0.f ? 0.f : 1.0f / t.y;
   }
   __syncthreads();
-  const int spp = a.page / kSub, l16 = tid & 15;
+  if (outs) {  // workgroup `part` of the row: 64 float4s of its group x D values, a quarter of the pieces a wave
+    const int per = group * D / 4, wave = tid >> 6, lane = tid & 63;
+    const int i = part * 64 + lane;  // per is a multiple of 16: some lanes of the last workgroup have none
+    axk_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    const int head = min(i, per - 1) / (D / 4);
+    if (i < per) {
+      const float top = s_top[head];
+      const axk_f32x4* po = reinterpret_cast<const axk_f32x4*>(a.po + item * group * D) + i;
+#pragma unroll 8
+      for (int p = wave; p < pieces; p += 4) {
+        const float2 x = ml[(int64_t)p * group + head];
+        const axk_f32x4 v = po[(int64_t)p * per];
+        o += (x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - top)) * v;  // nothing counted: a partial output of zeros
+      }
+    }
+    s_o[wave][lane] = o;
+    __syncthreads();
+    if (wave == 0 && i < per) {
+      o = ((s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane])) * s_inv[head];
+      *reinterpret_cast<uint2*>(a.out + ((int64_t)b * a.hq + h * group) * D + 4 * i) =
+          make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    }
+    return;
+  }
+  const int spp = a.page / kSub;
   const float* in = w.in ? w.in + (int64_t)h * a.nnz + s.pb : nullptr;
   float* out = w.out + (int64_t)h * a.nnz + s.pb;
   // the share of subtiles [from, from + n) of the statistics, by 16 lanes
   auto share = [&](int64_t from, int n) {
     float x = 0.f;
     const float2* st = a.stat + from * group;
+#pragma unroll 4
     for (int i = l16; i < n * group; i += 16) {
       const float2 y = st[i];
       const int hd = i % group;
-      if (y.y != 0.f) x += y.y * __builtin_amdgcn_exp2f(y.x - s_top[hd]) * s_inv[hd];
+      x += y.y == 0.f ? 0.f : y.y * __builtin_amdgcn_exp2f(y.x - s_top[hd]) * s_inv[hd];
     }
     return group_sum<16>(x);
   };
   if (!a.blocks) {
     const int64_t all = (s.len + kSub - 1) / kSub, sub0 = (int64_t)piece * a.ps;
     const int end = (int)min((sub0 + a.ps + spp - 1) / spp, (int64_t)s.np);
-    for (int p = (int)((sub0 + spp - 1) / spp) + (tid >> 4); p < end; p += 16) {
+    for (int p = (int)((sub0 + spp - 1) / spp) + r16; p < end; p += 16) {
       const int64_t first = (int64_t)p * spp;
       const float x = share(((int64_t)h * a.nnz + s.pb) * spp + first, (int)min((int64_t)spp, all - first));
       if (l16 == 0) out[p] = (in ? w.decay * in[p] : 0.f) + x;
@@ -983,27 +1060,38 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
     return;
   }
   for (int p = tid; p < s.np; p += 256) out[p] = in ? w.decay * in[p] : 0.f;
-  __syncthreads();
-  // the listed blocks of one page follow each other: the first of them adds them all, so that a page is added to once
+  // The listed blocks of one page follow each other: the first of them adds them all, so that a page is added to once.
+  // (A list out of order may name a page again: hence the atomic.) A page whose blocks straddle two rounds of the LDS is
+  // finished by the round it begins in, which looks past its end.
   const int spb = a.block / kSub, bpp = a.page / a.block;
   const int64_t row = (int64_t)b * a.hkv + h, nblocks = (s.len + a.block - 1) / a.block;
   const int* list = a.blocks + row * a.n;
-  for (int slot = tid >> 4; slot < a.n; slot += 16) {
-    bool bad;
-    const int id = listed_block(list, slot, nblocks, &bad);
-    if (id < 0) continue;
-    const int p = id / bpp;
-    if (slot) {
-      const int prev = listed_block(list, slot - 1, nblocks, &bad);
-      if (prev >= 0 && prev / bpp == p) continue;
+  for (int base = 0; base < a.n; base += kListLds - bpp) {
+    const int n = min(a.n - base, kListLds);  // the last bpp of them only to finish pages
+    __syncthreads();
+    for (int i = tid; i <= n; i += 256) {  // s_page[i]: the page of listed block base + i - 1, -1 for none
+      const int slot = base + i - 1;
+      int page = -1;
+      if (slot >= 0) {
+        const int id = list[slot];
+        if (id >= 0 && !bad_block(id, slot ? list[slot - 1] : -1, nblocks)) page = id / bpp;
+      }
+      s_page[i] = page;
     }
-    float x = 0.f;
-    for (int i = slot; i < a.n; ++i) {
-      const int next = listed_block(list, i, nblocks, &bad);
-      if (next < 0 || next / bpp != p) break;
-      x += share((row * a.n + i) * spb, spb);
+    for (int i = r16; i < n; i += 16) {
+      const float x = share((row * a.n + base + i) * spb, spb);
+      if (l16 == 0) s_share[i] = x;
     }
-    if (l16 == 0) atomicAdd(out + p, x);
+    __syncthreads();
+    const bool rest = base + n < a.n;
+    for (int i = tid; i < (rest ? kListLds - bpp : n); i += 256) {
+      const int page = s_page[i + 1];
+      if (page < 0 || s_page[i] == page) continue;
+      float x = 0.f;
+      for (int j = i; j < n && s_page[j + 1] == page; ++j) x += s_share[j];
+      atomicAdd(out + page, x);
+    }
+    if (!rest) break;
   }
 }
 
@@ -1012,18 +1100,21 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
 // order of the sum does not decide), the first `first` and last `keep_last` always among them, in their order into the
 // new table; the others' ids into `freed`. Every workgroup finds its places from the whole indptr, and fills as much of
 // the arrays' tails as it moved elsewhere.
-__global__ __launch_bounds__(256) void paged_evict_kernel(const float* __restrict__ w, const int* __restrict__ indptr,
-                                                          const int* __restrict__ indices, int* __restrict__ out_indptr,
-                                                          int* __restrict__ out_indices, float* __restrict__ out_w,
-                                                          int* __restrict__ freed, int nnz, int batch, int hkv,
-                                                          int budget, int first, int keep_last) {
-  __shared__ PickLds<uint64_t, 256> lds;
-  __shared__ int s_sum[4][4];
+constexpr int kEvict = 1024;  // threads
+constexpr int kEvictTile = 4 * kEvict;
+__global__ __launch_bounds__(kEvict) void paged_evict_kernel(const float* __restrict__ w, const int* __restrict__ indptr,
+                                                             const int* __restrict__ indices,
+                                                             int* __restrict__ out_indptr, int* __restrict__ out_indices,
+                                                             float* __restrict__ out_w, int* __restrict__ freed, int nnz,
+                                                             int batch, int hkv, int budget, int first, int keep_last) {
+  __shared__ PickLds<uint64_t, kEvict> lds;
+  __shared__ int s_sum[4][kEvict / 64];
+  __shared__ int s_list[kEvictTile];  // a tile's pages: the kept ones from the front, the others from the back
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
   auto ptr = [&](int i) { return min(max(indptr[i], 0), nnz); };
   // kept and evicted pages of the sequences before b, and kept and all pages of all of them
   int n4[4] = {0, 0, 0, 0};
-  for (int i = tid; i < batch; i += 256) {
+  for (int i = tid; i < batch; i += kEvict) {
     const int n = max(ptr(i + 1) - ptr(i), 0), k = min(n, budget);
     if (i < b) {
       n4[0] += k;
@@ -1032,60 +1123,92 @@ __global__ __launch_bounds__(256) void paged_evict_kernel(const float* __restric
     n4[2] += k;
     n4[3] += n;
   }
+  const int waves = (min(batch, kEvict) + 63) / 64;  // that had sequences to add
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) n4[i] += __shfl_xor(n4[i], o, 64);
+    n4[i] = wave_total(n4[i]);
     if (lane == 0) s_sum[i][wave] = n4[i];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) n4[i] = s_sum[i][0] + s_sum[i][1] + s_sum[i][2] + s_sum[i][3];
+  for (int i = 0; i < 4; ++i) {
+    n4[i] = 0;
+    for (int j = 0; j < waves; ++j) n4[i] += s_sum[i][j];
+  }
   const int kept = n4[0], gone = n4[1], all = n4[2], total = n4[3];
   const int pb = ptr(b), np = max(ptr(b + 1) - pb, 0), keep = min(np, budget);
   if (tid == 0) {
     if (b == 0) out_indptr[0] = 0;
     out_indptr[b + 1] = kept + keep;
   }
-  auto put = [&](int i, bool taken, int rank) {
-    if (taken) {
-      if (kept + rank < nnz) {
-        out_indices[kept + rank] = indices[pb + i];
-        for (int h = 0; h < hkv; ++h) out_w[(int64_t)h * nnz + kept + rank] = w[(int64_t)h * nnz + pb + i];
-      }
-    } else if (gone + i - rank < nnz) {
-      freed[gone + i - rank] = indices[pb + i];
+  // pages from[0 .. n) of the sequence (a null list: base, base + 1, ...) to places `at` onwards
+  auto keep_pages = [&](const int* from, int base, int n, int at) {
+    for (int i = tid; i < n; i += kEvict) {
+      const int src = pb + (from ? from[i] : base + i), dst = kept + at + i;
+      if (dst >= nnz) break;
+      out_indices[dst] = indices[src];
+#pragma unroll 4
+      for (int h = 0; h < hkv; ++h) out_w[(int64_t)h * nnz + dst] = w[(int64_t)h * nnz + src];
     }
   };
   if (np <= budget) {
-    for (int i = tid; i < np; i += 256) put(i, true, i);
+    keep_pages(nullptr, 0, np, 0);
   } else {
-    for (int i = tid; i < first; i += 256) put(i, true, i);
-    for (int i = tid; i < keep_last; i += 256) put(np - keep_last + i, true, budget - keep_last + i);
+    keep_pages(nullptr, 0, first, 0);
+    keep_pages(nullptr, np - keep_last, keep_last, budget - keep_last);
     const int want = budget - first - keep_last, count = np - first - keep_last;
     if (want == 0) {
-      for (int i = tid; i < count; i += 256) put(first + i, false, first);
+      for (int i = tid; i < count; i += kEvict)
+        if (gone + i < nnz) freed[gone + i] = indices[pb + first + i];
     } else {
-      pick_largest<uint64_t, 256>(
-          count, want,
-          [&](int i) {
-            double x = 0.0;
-            for (int h = 0; h < hkv; ++h) x += (double)w[(int64_t)h * nnz + pb + first + i];
-            return order_key(x);
-          },
-          [&](int i, bool taken, int rank) { put(first + i, taken, first + rank); }, lds);
+      int done0 = 0;  // pages kept in the tiles before
+      auto keys = [&](int at, int n, auto& key) {
+        constexpr int K = sizeof(key) / sizeof(uint64_t);
+        double x[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) x[i] = 0.0;
+        const float* row = w + pb + first + at;
+        for (int h0 = 0; h0 < hkv; h0 += 4) {  // four heads' loads under way together
+          float y[4][K];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) load_run<K>(row + (int64_t)(h0 + h) * nnz, h0 + h < hkv ? n : 0, y[h]);
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int i = 0; i < K; ++i) x[i] += (double)y[h][i];
+        }
+#pragma unroll
+        for (int i = 0; i < K; ++i) key[i] = order_key(x[i]);
+      };
+      auto list = [&](int i, bool taken, int rank) {
+        const int at = i & (kEvictTile - 1), k = rank - done0;
+        s_list[taken ? k : kEvictTile - 1 - (at - k)] = first + i;
+      };
+      auto move = [&](int base, int n, int k) {
+        __syncthreads();
+        keep_pages(s_list, 0, k, first + done0);
+        for (int i = tid; i < n - k; i += kEvict) {
+          const int dst = gone + base - done0 + i;
+          if (dst < nnz) freed[dst] = indices[pb + s_list[kEvictTile - 1 - i]];
+        }
+        done0 += k;
+        __syncthreads();
+      };
+      // a tile is at most as long as the list
+      if (count <= kEvict) pick_largest<uint64_t, kEvict, 1>(count, want, keys, list, move, lds);
+      else pick_largest<uint64_t, kEvict, 4>(count, want, keys, list, move, lds);
     }
   }
   // the tails: [all, nnz) of the table and of the weights, [total - all, nnz) of freed. A sequence's share of the first
   // is as long as what it evicted, of the second as what it kept; the last one also fills what no sequence had
   const int extra = b == batch - 1 ? max(nnz - total, 0) : 0;
-  for (int i = tid; i < np - keep + extra; i += 256) {
+  for (int i = tid; i < np - keep + extra; i += kEvict) {
     const int at = all + gone + i;
     if (at >= nnz) break;
     out_indices[at] = -1;
     for (int h = 0; h < hkv; ++h) out_w[(int64_t)h * nnz + at] = 0.f;
   }
-  for (int i = tid; i < keep + extra; i += 256) {
+  for (int i = tid; i < keep + extra; i += kEvict) {
     const int at = total - all + kept + i;
     if (at < nnz) freed[at] = -1;
   }
@@ -1115,9 +1238,9 @@ int cache_type(int kv_dtype, float kv_scale) {
 
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// How a decode over blocks is cut, from what the host knows. Pieces of at least 128 tokens, so that each wave has a step,
-// and of at most 2048; about 1024 of them.
-constexpr int64_t kPieces = 1024;
+// How a decode over blocks is cut, from what the host knows: pieces of at least 128 tokens, so that each wave has a step,
+// and of at most 2048; otherwise as many as run at once (kPieces), since a second round would pay the lookups again.
+constexpr int64_t kPieces = 512;
 struct BlkPlan {
   int ps, pieces;
   bool direct;
@@ -1127,8 +1250,10 @@ BlkPlan blk_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t page
                  bool weights) {
   const int64_t rows = batch * hkv, group = hq / hkv;
   const int64_t subs = n ? n * (block / kSub) : nnz * (page / kSub);  // of a row, or of a KV head
-  const int64_t cut = n ? (kPieces + rows - 1) / rows : (kPieces + hkv - 1) / hkv;
-  int64_t ps = ((subs + cut - 1) / cut + 7) / 8 * 8;
+  const int64_t heads = n ? rows : hkv;
+  int64_t cut = kPieces / heads;  // pieces of a row, or of a KV head, less the partial ones that sequences end in
+  if (!n) cut = cut - batch >= cut / 2 ? cut - batch : cut / 2;
+  int64_t ps = cut > 1 ? ((subs + cut - 1) / cut + 7) / 8 * 8 : kMaxPs;
   ps = ps < 8 ? 8 : ps > kMaxPs ? kMaxPs : ps;
   BlkPlan p;
   p.ps = (int)ps;
@@ -1147,7 +1272,7 @@ int launch_blocks(const BlkArgs& a, const WeightArgs& w, int f8, hipStream_t st)
   if (f8) hipLaunchKernelGGL((paged_blocks_kernel<D, 1>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((paged_blocks_kernel<D, 0>), grid, dim3(256), 0, st, a);
   if (!a.direct) {
-    const int64_t wgs = (int64_t)a.batch * a.hq + (w.out ? (a.blocks ? (int64_t)a.batch : a.pieces) * a.hkv : 0);
+    const int64_t wgs = (int64_t)a.batch * a.hkv * w.split + (w.out ? (a.blocks ? (int64_t)a.batch : a.pieces) * a.hkv : 0);
     hipLaunchKernelGGL((paged_blocks_merge_kernel<D>), dim3((unsigned)wgs), dim3(256), 0, st, a, w);
   }
   return axk_launch_status();
@@ -1252,7 +1377,7 @@ extern "C" int axk_paged_select_blocks(const float* scores, const int32_t* indpt
               AXK_E_ALIAS);
   AXK_LAUNCH_GATE();
   const dim3 grid((unsigned)(batch * num_kv_heads));
-  if (total <= 256 * kKeys)
+  if (total <= 2048)  // every row at most eight keys a thread of 256
     hipLaunchKernelGGL(paged_select_blocks_kernel<256>, grid, dim3(256), 0, axk_stream(stream), scores, indptr,
                        last_page_len, blocks, (int)nnz, (int)num_kv_heads, (int)page_size, (int)block_size,
                        (int)num_select, (int)first, (int)keep_last);
@@ -1303,7 +1428,8 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
   const size_t need = p.ml + p.po + p.stat;
   AXK_REQUIRE(!need || (workspace && workspace_bytes >= need && axk_aligned(workspace, 256)), AXK_E_WORKSPACE);
   const int64_t grid = blocks ? batch * num_kv_heads * p.pieces : p.pieces;
-  const int64_t wgs = batch * num_qo_heads + (weights ? (blocks ? batch : (int64_t)p.pieces) * num_kv_heads : 0);
+  const int split = (int)(num_qo_heads / num_kv_heads * head_dim / 4 + 63) / 64;  // four values a lane
+  const int64_t wgs = batch * num_kv_heads * split + (weights ? (blocks ? batch : (int64_t)p.pieces) * num_kv_heads : 0);
   AXK_REQUIRE(grid <= 0x7fffffff && wgs <= 0x7fffffff, AXK_E_SHAPE);
   const size_t qb = (size_t)batch * num_qo_heads * head_dim * 2, wb = (size_t)num_kv_heads * nnz * 4;
   const size_t cache = (size_t)num_pages * page_size * num_kv_heads * head_dim * (f8 ? 2 : 4);
@@ -1341,7 +1467,7 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
   a.po = p.direct ? nullptr : reinterpret_cast<float*>(ws + p.ml);
   a.stat = weights ? reinterpret_cast<float2*>(ws + p.ml + p.po) : nullptr;
   a.status = status;
-  const WeightArgs w = {weights_in, weights ? weights_out : nullptr, decay};
+  const WeightArgs w = {weights_in, weights ? weights_out : nullptr, decay, split};
   AXK_LAUNCH_GATE();
   switch (head_dim) {
     case 64: return launch_blocks<64>(a, w, f8, axk_stream(stream));
@@ -1369,7 +1495,7 @@ extern "C" int axk_paged_evict_pages(const float* weights, const int32_t* indptr
     for (int j = 0; j < i; ++j) AXK_REQUIRE(!axk_overlap(out[i].p, out[i].n, out[j].p, out[j].n), AXK_E_ALIAS);
   }
   AXK_LAUNCH_GATE();
-  hipLaunchKernelGGL(paged_evict_kernel, dim3((unsigned)batch), dim3(256), 0, axk_stream(stream), weights, indptr, indices,
+  hipLaunchKernelGGL(paged_evict_kernel, dim3((unsigned)batch), dim3(kEvict), 0, axk_stream(stream), weights, indptr, indices,
                      out_indptr, out_indices, out_weights, freed, (int)nnz, (int)batch, (int)num_kv_heads, (int)budget,
                      (int)first, (int)keep_last);
   return axk_launch_status();
