@@ -959,25 +959,30 @@ AXK_DEV float2 join(float2 x, float2 y) {
   return make_float2(top, x.y * __builtin_amdgcn_exp2f(x.x - top) + y.y * __builtin_amdgcn_exp2f(y.x - top));
 }
 
-// Workgroups [0, batch * hkv): the output rows of a (sequence, KV head) from its pieces. The others: the page weights, from
-// each subtile's sum against the row's joined maximum and sum. Every workgroup joins the pieces' sums of all heads of its
-// row first (16 lanes a piece, a head each), while the first partial outputs are on their way.
+AXK_DEV float2 join_pairs(uint2 m, uint2 l) {
+  return join(make_float2(__uint_as_float(m.x), __uint_as_float(l.x)), make_float2(__uint_as_float(m.y), __uint_as_float(l.y)));
+}
+
+// The first batch * hkv * split workgroups: the output rows of a (sequence, KV head) from its pieces, 64 float4s of its
+// group x D values each, a quarter of the pieces a wave. The others: the page weights, from each subtile's sum against the
+// row's joined maximum and sum. Every workgroup joins the pieces' sums of all heads of its row (16 lanes a piece, a head
+// each) while its other first loads are on their way: a merge is three trips to memory and little else.
 constexpr int kListLds = 2048;  // listed blocks whose shares are kept in LDS at a time
 template <int D>
 __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a, const WeightArgs w) {
-  __shared__ float2 s_part[16][16];
+  __shared__ float2 s_part[4][16];
   __shared__ float s_top[kMaxGroup], s_inv[kMaxGroup];
   __shared__ axk_f32x4 s_o[4][64];
   __shared__ float s_share[kListLds];
   __shared__ int s_page[kListLds + 1];
-  const int tid = threadIdx.x, l16 = tid & 15, r16 = tid >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = tid & 15, r16 = tid >> 4;
   const int group = a.hq / a.hkv, rows = a.batch * a.hkv;
   const bool outs = (int)blockIdx.x < rows * w.split;
   int b, h, part = 0, pieces = a.pieces, piece = 0;
   int64_t item;
   Seq s;
   if (outs || a.blocks) {
-    int row = outs ? blockIdx.x / w.split : blockIdx.x - rows * w.split;
+    const int row = outs ? blockIdx.x / w.split : blockIdx.x - rows * w.split;
     part = outs ? blockIdx.x - row * w.split : 0;
     b = row / a.hkv;
     h = row - b * a.hkv;
@@ -997,69 +1002,87 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
   // the pieces that the grid held (all of them, unless offsets of indptr overlap)
   if (!a.blocks) pieces = min(pieces_of(s, a.ps), (int)((h + 1) * (int64_t)a.pieces - item));
   const float2* ml = a.ml + item * group;
-  float2 t = make_float2(0.f, 0.f);
-  if (l16 < group)
-    for (int p = r16; p < pieces; p += 16) t = join(t, ml[(int64_t)p * group + l16]);
-  s_part[r16][l16] = t;
-  __syncthreads();
-  if (tid < 16) {
-    t = s_part[0][tid];
+  const float2 none = make_float2(0.f, 0.f);
+  float2 t = l16 < group && r16 < pieces ? ml[r16 * group + l16] : none;
+
+  // outputs: the first pieces' sums and partial outputs
+  constexpr int kFirst = 8;
+  const int per = group * D / 4, i = part * 64 + lane, head = min(i, per - 1) / (D / 4);
+  const axk_f32x4* po = reinterpret_cast<const axk_f32x4*>(a.po + item * group * D) + min(i, per - 1);
+  axk_f32x4 v[kFirst];
+  float2 x[kFirst];
+  if (outs) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) t = join(t, s_part[i][tid]);
-    s_top[tid] = t.x;
-    s_inv[tid] = t.y == 0.f ? 0.f : 1.0f / t.y;
-  }
-  __syncthreads();
-  if (outs) {  // workgroup `part` of the row: 64 float4s of its group x D values, a quarter of the pieces a wave
-    const int per = group * D / 4, wave = tid >> 6, lane = tid & 63;
-    const int i = part * 64 + lane;  // per is a multiple of 16: some lanes of the last workgroup have none
-    axk_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    const int head = min(i, per - 1) / (D / 4);
-    if (i < per) {
-      const float top = s_top[head];
-      const axk_f32x4* po = reinterpret_cast<const axk_f32x4*>(a.po + item * group * D) + i;
-#pragma unroll 8
-      for (int p = wave; p < pieces; p += 4) {
-        const float2 x = ml[(int64_t)p * group + head];
-        const axk_f32x4 v = po[(int64_t)p * per];
-        o += (x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - top)) * v;  // nothing counted: a partial output of zeros
+    for (int k = 0; k < kFirst; ++k) {
+      const int p = wave + 4 * k;
+      x[k] = none;
+      v[k] = (axk_f32x4){0.f, 0.f, 0.f, 0.f};
+      if (p < pieces) {
+        x[k] = ml[(int64_t)p * group + head];
+        v[k] = po[(int64_t)p * per];
       }
+    }
+  }
+  // page weights of listed blocks: what every page keeps
+  const int spp = a.page / kSub;
+  const float* in = w.in ? w.in + (int64_t)h * a.nnz + s.pb : nullptr;
+  float* out = w.out ? w.out + (int64_t)h * a.nnz + s.pb : nullptr;
+  if (!outs && a.blocks)
+    for (int p = tid; p < s.np; p += 256) out[p] = in ? w.decay * in[p] : 0.f;
+
+  for (int p = r16 + 16; p < pieces; p += 16)
+    if (l16 < group) t = join(t, ml[(int64_t)p * group + l16]);
+  t = join_pairs(row_pair16(t.x), row_pair16(t.y));
+  t = join_pairs(half_pair32(t.x), half_pair32(t.y));
+  if (lane < 16) s_part[wave][lane] = t;
+  __syncthreads();
+  if (outs) {
+    t = join(join(s_part[0][head], s_part[1][head]), join(s_part[2][head], s_part[3][head]));
+    axk_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kFirst; ++k) o += (x[k].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[k].x - t.x)) * v[k];
+#pragma unroll 8
+    for (int p = wave + 4 * kFirst; p < pieces; p += 4) {
+      const float2 y = ml[(int64_t)p * group + head];
+      o += (y.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(y.x - t.x)) * po[(int64_t)p * per];
     }
     s_o[wave][lane] = o;
     __syncthreads();
     if (wave == 0 && i < per) {
-      o = ((s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane])) * s_inv[head];
+      o = ((s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane])) * (t.y == 0.f ? 0.f : 1.0f / t.y);
       *reinterpret_cast<uint2*>(a.out + ((int64_t)b * a.hq + h * group) * D + 4 * i) =
           make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
     }
     return;
   }
-  const int spp = a.page / kSub;
-  const float* in = w.in ? w.in + (int64_t)h * a.nnz + s.pb : nullptr;
-  float* out = w.out + (int64_t)h * a.nnz + s.pb;
+  if (tid < 16) {
+    t = join(join(s_part[0][tid], s_part[1][tid]), join(s_part[2][tid], s_part[3][tid]));
+    s_top[tid] = t.x;
+    s_inv[tid] = t.y == 0.f ? 0.f : 1.0f / t.y;
+  }
+  __syncthreads();
   // the share of subtiles [from, from + n) of the statistics, by 16 lanes
   auto share = [&](int64_t from, int n) {
-    float x = 0.f;
+    float sum = 0.f;
     const float2* st = a.stat + from * group;
 #pragma unroll 4
-    for (int i = l16; i < n * group; i += 16) {
-      const float2 y = st[i];
-      const int hd = i % group;
-      x += y.y == 0.f ? 0.f : y.y * __builtin_amdgcn_exp2f(y.x - s_top[hd]) * s_inv[hd];
+    for (int j = l16; j < n * group; j += 16) {
+      const float2 y = st[j];
+      const int hd = j % group;
+      sum += y.y == 0.f ? 0.f : y.y * __builtin_amdgcn_exp2f(y.x - s_top[hd]) * s_inv[hd];
     }
-    return group_sum<16>(x);
+    return group_sum<16>(sum);
   };
   if (!a.blocks) {
     const int64_t all = (s.len + kSub - 1) / kSub, sub0 = (int64_t)piece * a.ps;
     const int end = (int)min((sub0 + a.ps + spp - 1) / spp, (int64_t)s.np);
     for (int p = (int)((sub0 + spp - 1) / spp) + r16; p < end; p += 16) {
       const int64_t first = (int64_t)p * spp;
-      const float x = share(((int64_t)h * a.nnz + s.pb) * spp + first, (int)min((int64_t)spp, all - first));
-      if (l16 == 0) out[p] = (in ? w.decay * in[p] : 0.f) + x;
+      const float sum = share(((int64_t)h * a.nnz + s.pb) * spp + first, (int)min((int64_t)spp, all - first));
+      if (l16 == 0) out[p] = (in ? w.decay * in[p] : 0.f) + sum;
     }
     return;
   }
-  for (int p = tid; p < s.np; p += 256) out[p] = in ? w.decay * in[p] : 0.f;
   // The listed blocks of one page follow each other: the first of them adds them all, so that a page is added to once.
   // (A list out of order may name a page again: hence the atomic.) A page whose blocks straddle two rounds of the LDS is
   // finished by the round it begins in, which looks past its end.
@@ -1069,27 +1092,27 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
   for (int base = 0; base < a.n; base += kListLds - bpp) {
     const int n = min(a.n - base, kListLds);  // the last bpp of them only to finish pages
     __syncthreads();
-    for (int i = tid; i <= n; i += 256) {  // s_page[i]: the page of listed block base + i - 1, -1 for none
-      const int slot = base + i - 1;
+    for (int j = tid; j <= n; j += 256) {  // s_page[j]: the page of listed block base + j - 1, -1 for none
+      const int slot = base + j - 1;
       int page = -1;
       if (slot >= 0) {
         const int id = list[slot];
         if (id >= 0 && !bad_block(id, slot ? list[slot - 1] : -1, nblocks)) page = id / bpp;
       }
-      s_page[i] = page;
+      s_page[j] = page;
     }
-    for (int i = r16; i < n; i += 16) {
-      const float x = share((row * a.n + base + i) * spb, spb);
-      if (l16 == 0) s_share[i] = x;
+    for (int j = r16; j < n; j += 16) {
+      const float sum = share((row * a.n + base + j) * spb, spb);
+      if (l16 == 0) s_share[j] = sum;
     }
     __syncthreads();
     const bool rest = base + n < a.n;
-    for (int i = tid; i < (rest ? kListLds - bpp : n); i += 256) {
-      const int page = s_page[i + 1];
-      if (page < 0 || s_page[i] == page) continue;
-      float x = 0.f;
-      for (int j = i; j < n && s_page[j + 1] == page; ++j) x += s_share[j];
-      atomicAdd(out + page, x);
+    for (int j = tid; j < (rest ? kListLds - bpp : n); j += 256) {
+      const int page = s_page[j + 1];
+      if (page < 0 || s_page[j] == page) continue;
+      float sum = 0.f;
+      for (int k = j; k < n && s_page[k + 1] == page; ++k) sum += s_share[k];
+      atomicAdd(out + page, sum);
     }
     if (!rest) break;
   }
