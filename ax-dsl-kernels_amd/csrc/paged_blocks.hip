@@ -36,6 +36,9 @@ AXK_DEV Seq seq_from(int lo, int hi, int last, int page, int nnz) {
   s.len = s.np ? (int64_t)(s.np - 1) * page + min(max(last, 0), page) : 0;
   return s;
 }
+// Its subtiles of 16 tokens, and blocks: 32 bits, as all that is divided here (a 64-bit division is some 130 instructions).
+AXK_DEV int subs_of(const Seq& s) { return (int)((s.len + kSub - 1) / kSub); }
+AXK_DEV int blocks_of(const Seq& s, int block) { return (int)((unsigned)(subs_of(s) + block / kSub - 1) / (unsigned)(block / kSub)); }
 AXK_DEV Seq seq_of(const int* __restrict__ indptr, const int* __restrict__ last, int b, int page, int nnz) {
   return seq_from(indptr[b], indptr[b + 1], last[b], page, nnz);
 }
@@ -284,22 +287,22 @@ template <int D>
 __global__ __launch_bounds__(256) void paged_block_scores_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
     const int* __restrict__ indices, const int* __restrict__ last, float* __restrict__ scores, int nnz, int batch,
-    int hq, int hkv, int page_size, int block, int64_t num_pages, int64_t units, int* __restrict__ status) {
+    int hq, int hkv, int page_size, int block, int64_t num_pages, unsigned units, int* __restrict__ status) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (unit >= units) return;
   const int group = hq / hkv, bpp = page_size / block;
-  const int64_t total = (int64_t)nnz * bpp;
-  const int64_t tile = unit / hkv;
-  const int h = (int)(unit - tile * hkv);
+  const int total = nnz * bpp;
+  const int tile = (int)(unit / (unsigned)hkv);
+  const int h = (int)(unit - (unsigned)tile * hkv);
   // lane l16 of each lane group looks at block tile * 16 + l16
-  const int64_t f = tile * 16 + l16;
-  const int e = (int)(min(f, total - 1) / bpp);
+  const int f = tile * 16 + l16;
+  const int e = (int)((unsigned)min(f, total - 1) / (unsigned)bpp);
   const int id = indices[e];
   const int e0 = __builtin_amdgcn_readlane(e, 0), e1 = __builtin_amdgcn_readlane(e, 15);
   Owner own = owner_of(indptr, last, batch, page_size, nnz, e0);
   const bool good = id >= 0 && id < num_pages;
-  const int sub = (int)(f - (int64_t)e * bpp);
+  const int sub = f - e * bpp;
   const uint16_t* row = bounds + (((int64_t)(good ? id : 0) * bpp + (f < total ? sub : 0)) * hkv + h) * 2 * D + 8 * g;
   axk_bf16x8 lo[D / 32], hi[D / 32];
 #pragma unroll
@@ -332,12 +335,12 @@ __global__ __launch_bounds__(256) void paged_block_scores_kernel(
       x = fmaxf(x, dpp_move<0x140>(x, x));
       n = group_sum<16>(n);
       if (n != n) x = n;
-      const int64_t fi = tile * 16 + 4 * g + i;
-      const int64_t t0 = (fi - (int64_t)sq.pb * bpp) * block;  // the block's first token
+      const int fi = tile * 16 + 4 * g + i;
+      const int64_t t0 = (int64_t)(fi - sq.pb * bpp) * block;  // the block's first token
       const bool bad = __shfl((int)!good, 4 * g + i, 64) != 0;
       if (l16 == 0 && fi < total && t0 >= 0 && t0 < (int64_t)sq.np * page_size) {
         const bool there = t0 < sq.len;
-        scores[h * total + fi] = there && !bad ? x : -INFINITY;
+        scores[(int64_t)h * total + fi] = there && !bad ? x : -INFINITY;
         if (there && bad && status) *status = 1;
       }
     }
@@ -560,7 +563,7 @@ __global__ __launch_bounds__(T) void paged_select_blocks_kernel(const float* __r
   const int tid = threadIdx.x, b = blockIdx.x / hkv, h = blockIdx.x - b * hkv;
   const Seq s = seq_of(indptr, last, b, page_size, nnz);
   const int bpp = page_size / block;
-  const int nb = (int)((s.len + block - 1) / block);
+  const int nb = blocks_of(s, block);
   int* o = out + (int64_t)blockIdx.x * n;
   if (nb <= n) {
     for (int i = tid; i < n; i += T) o[i] = i < nb ? i : -1;
@@ -579,8 +582,8 @@ __global__ __launch_bounds__(T) void paged_select_blocks_kernel(const float* __r
 // ---- decode over blocks ----
 // One query token per sequence over the listed blocks of each KV head (or all of them), split over pieces of `ps`
 // subtiles of 16 tokens. Everything a wave needs stays in its registers; it takes two subtiles (32 tokens) a step:
-//   S^T = K Q^T   16x16x32 MFMA, K rows straight from memory as the A operand (lane = token, 16 bytes of its row), Q the
-//                 B operand, the group's heads as columns;
+//   S^T = K Q^T   16x16x32 MFMA, K rows through LDS as the A operand (lane = token, 16 bytes of its row), Q the B operand,
+//                 the group's heads as columns;
 //   softmax       running maximum and sum per head, fp32, exp2 domain;
 //   O^T += V^T P^T  the score accumulator is the P^T operand as it stands if MFMA k index (lane group g, j) is token
 //                 4 g + j % 4 of subtile j / 4. V rows are loaded in that order, lane l16 holding D / 16 channels of eight
@@ -589,14 +592,21 @@ __global__ __launch_bounds__(T) void paged_select_blocks_kernel(const float* __r
 template <int D, int F8>
 struct BlkCfg {
   static constexpr int B = F8 ? 1 : 2;             // bytes of a stored value
-  static constexpr int KL = D * B / 64;            // 16-byte K loads a lane makes per subtile
+  static constexpr int RB = D * B;                 // bytes of a token's row of one head
+  static constexpr int CR = RB / 16;               // ... in 16-byte chunks
+  static constexpr int KI = 32 * RB / 1024;        // direct-to-LDS loads (64 lanes x 16 bytes) of a step's K
+  static constexpr int KL = RB / 64;               // 16-byte K fragments a lane reads per subtile
   static constexpr int KS = D / 32;                // QK k-steps
   static constexpr int E = F8 ? D / 16 : (D >= 128 ? 8 : D / 16);  // channels of a V load
   static constexpr int NH = D / 16 / E;            // V loads a lane makes per token
   static constexpr int VW = E * B / 4;             // dwords of a V load
   static constexpr int ACC = D / 16;               // 16x16 O^T tiles
-  // The next step's K is loaded before this one's softmax where the registers hold it (bf16 at D = 256: a spill).
-  static constexpr bool AHEAD = F8 || D < 256;
+  static constexpr int Q = ACC / 4;                // ... that a wave gives out at the end
+  static constexpr int KT = 32 * RB;               // bytes of a step's K in LDS, one buffer a wave
+  static constexpr int LDS = 4 * KT > 12 * Q * 1024 ? 4 * KT : 12 * Q * 1024;  // the join at the end reuses them
+  // Chunk c of row r lies at chunk c ^ swz(r) of its row in LDS: the 16 rows that lanes read one chunk of then fall on 16
+  // different 16-byte columns of the 256 bytes that LDS gives at a time.
+  static AXK_DEV int swz(int r) { return CR >= 16 ? r & 15 : r / (16 / (CR < 16 ? CR : 16)) & (CR - 1); }
 };
 
 struct BlkArgs {
@@ -625,7 +635,7 @@ struct PieceOf {
   int b, piece;
   Seq s;
 };
-AXK_DEV int pieces_of(const Seq& s, int ps) { return (int)((s.len + (int64_t)kSub * ps - 1) / ((int64_t)kSub * ps)); }
+AXK_DEV int pieces_of(const Seq& s, int ps) { return (int)((unsigned)(subs_of(s) + ps - 1) / (unsigned)ps); }
 AXK_DEV PieceOf find_piece(const BlkArgs& a, int it) {
   const int lane = threadIdx.x & 63;
   int base = 0;
@@ -664,7 +674,7 @@ AXK_DEV int pieces_before(const BlkArgs& a, int b) {
 
 // Whether a listed block is neither padding (-1) nor a block of the sequence that lies above its predecessor in the list
 // (prev: -1 for the first).
-AXK_DEV bool bad_block(int id, int prev, int64_t nblocks) {
+AXK_DEV bool bad_block(int id, int prev, int nblocks) {
   return id < -1 || id >= nblocks || (id >= 0 && prev >= id);
 }
 
@@ -673,12 +683,12 @@ constexpr int kMaxPs = 128;  // subtiles of a piece, at most (two a lane)
 template <int D, int F8>
 __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   using C = BlkCfg<D, F8>;
-  constexpr int Q = C::ACC / 4;  // accumulator tiles a wave gives out at the end
-  __shared__ __align__(16) float s_o[4][3][Q * 256];
+  constexpr int Q = C::Q;
+  extern __shared__ __align__(1024) unsigned char s_k[];  // C::LDS bytes
   __shared__ int64_t s_base[kMaxPs];
   __shared__ int s_valid[kMaxPs];
   __shared__ float s_m[4][16], s_l[4][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
   const int group = a.hq / a.hkv;
   int b, h, piece;
   int64_t item;
@@ -691,7 +701,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
     piece = blockIdx.x - row * a.pieces;
     b = row / a.hkv;
     h = row - b * a.hkv;
-    const int64_t slot = ((int64_t)piece * a.ps + tid) / spb;
+    const int slot = (int)((unsigned)(piece * a.ps + tid) / (unsigned)spb);
     if (tid < a.ps && slot < a.n) {
       const int* list = a.blocks + (int64_t)row * a.n + slot;
       id = list[0];
@@ -717,27 +727,27 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   // the piece's subtiles: where each lies in the cache, and how many of its tokens count
   const int64_t rowb = (int64_t)a.hkv * D * C::B;  // bytes of a token row
   const int spp = a.page / kSub;
-  const int64_t nsub = a.blocks ? (int64_t)a.n * spb : (s.len + kSub - 1) / kSub;  // of the row
-  const int64_t sub0 = (int64_t)piece * a.ps;
-  const int count = (int)min((int64_t)a.ps, nsub - sub0);
+  const int nsub = a.blocks ? a.n * spb : subs_of(s);  // of the row
+  const int sub0 = piece * a.ps;
+  const int count = min(a.ps, nsub - sub0);
   if (tid < a.ps) {
     int valid = 0;
     int64_t base = 0;
     if (tid < count) {
-      int64_t t0 = (sub0 + tid) * kSub;  // the subtile's first token
+      int at = sub0 + tid;  // the subtile's place in the sequence
       bool bad = false;
       if (a.blocks) {
-        bad = bad_block(id, prev, (s.len + a.block - 1) / a.block);
-        t0 = bad || id < 0 ? s.len : (int64_t)id * a.block + (sub0 + tid) % spb * kSub;
+        bad = bad_block(id, prev, blocks_of(s, a.block));
+        at = bad || id < 0 ? subs_of(s) : id * spb + (int)((unsigned)at % (unsigned)spb);
       }
-      valid = (int)min(max(s.len - t0, (int64_t)0), (int64_t)kSub);
+      valid = (int)min(max(s.len - (int64_t)at * kSub, (int64_t)0), (int64_t)kSub);
       if (valid) {
-        const int p = (int)(t0 / a.page), at = a.indices[s.pb + p];
-        if (at < 0 || at >= a.num_pages) {
+        const int p = (int)((unsigned)at / (unsigned)spp), page = a.indices[s.pb + p];
+        if (page < 0 || page >= a.num_pages) {
           bad = true;
           valid = 0;
         } else {
-          base = ((int64_t)at * 2 * a.page + (t0 - (int64_t)p * a.page)) * rowb;
+          base = ((int64_t)page * 2 * a.page + (at - p * spp) * kSub) * rowb;
         }
       }
       if (bad && a.status) *a.status = 1;
@@ -760,22 +770,28 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   float m = -INFINITY, l = 0.f;
   const unsigned char* cache_h = a.cache + (int64_t)h * D * C::B;
   const int64_t vplane = (int64_t)a.page * rowb;
-  const uint32_t k_off = (uint32_t)(l16 * rowb + g * 16);
   const uint32_t v_off = (uint32_t)(4 * g * rowb + l16 * C::E * C::B);
   typedef uint32_t vload __attribute__((ext_vector_type(C::VW)));
-  axk_u32x4 kr[2][C::KL];
+  // K of step t to this wave's buffer, whole rows an instruction (a fragment's 64 bytes of 16 rows, straight to registers,
+  // ask the L2 for every line twice). Nothing else touches the buffer, so no barrier is needed.
+  unsigned char* kbuf = s_k + wave * C::KT;
+  constexpr int kRows = 1024 / C::RB;  // rows of one load
   auto load_k = [&](int t) {
+    const unsigned char* sub[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const unsigned char* p = static_cast<const unsigned char*>(uniform_ptr(cache_h + s_base[2 * t + u]));
+    for (int u = 0; u < 2; ++u) sub[u] = static_cast<const unsigned char*>(uniform_ptr(cache_h + s_base[2 * t + u]));
 #pragma unroll
-      for (int i = 0; i < C::KL; ++i) kr[u][i] = load_nt(p + k_off + 64 * i);
+    for (int i = 0; i < C::KI; ++i) {
+      const int r = (i * kRows + lane / C::CR) % kSub;  // of its subtile
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(sub[i * kRows / kSub] + (uint32_t)(r * rowb + ((lane % C::CR) ^ C::swz(r)) * 16)),
+          (__attribute__((address_space(3))) void*)(kbuf + i * 1024), 16, 0, 2);
     }
   };
+  const uint32_t k_at = (uint32_t)(l16 * C::RB + ((g ^ C::swz(l16)) * 16));  // chunk g of row l16; chunk 4 i + g: ^ 64 i
   const int tiles = (end + 1) / 2;
-  if (C::AHEAD && wave < tiles) load_k(wave);
+  if (wave < tiles) load_k(wave);
   for (int t = wave; t < tiles; t += 4) {
-    if (!C::AHEAD) load_k(t);
     const int nv0 = __builtin_amdgcn_readfirstlane(s_valid[2 * t]), nv1 = __builtin_amdgcn_readfirstlane(s_valid[2 * t + 1]);
     vload vr[8][C::NH];
 #pragma unroll
@@ -788,6 +804,9 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
           vr[4 * u + j][n] = __builtin_nontemporal_load(
               reinterpret_cast<const vload*>(p + v_off + j * (uint32_t)rowb + n * 16 * C::E * C::B));
     }
+    // This step's K has landed in LDS (the compiler waits for registers only), and its V, which costs nothing: the other
+    // waves' loads keep the memory busy.
+    wait_vmcnt<0>();
     __builtin_amdgcn_sched_barrier(0);
     axk_f32x4 sc[2];
 #pragma unroll
@@ -796,7 +815,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
 #pragma unroll
       for (int i = 0; i < C::KL; ++i) {
         uint32_t x[F8 ? 8 : 4];
-        stored_pairs<F8>(kr[u][i], a.inv_scale, x);
+        stored_pairs<F8>(*reinterpret_cast<const axk_u32x4*>(kbuf + u * kSub * C::RB + (k_at ^ (64 * i))), a.inv_scale, x);
         const axk_u32x4 x0 = {x[0], x[1], x[2], x[3]};
         sc[u] = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, x0), qf[F8 ? 2 * i : i], sc[u]);
         if constexpr (F8) {
@@ -806,7 +825,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (C::AHEAD && t + 4 < tiles) load_k(t + 4);
+    if (t + 4 < tiles) load_k(t + 4);
     __builtin_amdgcn_sched_barrier(0);
     // sc[u][i]: token 4 g + i of subtile u, head l16
     float x[8];
@@ -897,12 +916,13 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
 #pragma unroll
   for (int i = 0; i < C::ACC; ++i) acc[i] *= mine;
   // each wave gives out the sum of a quarter of the accumulators, and leaves the others theirs
+  axk_f32x4* s_o = reinterpret_cast<axk_f32x4*>(s_k);
 #pragma unroll
   for (int w = 0; w < 4; ++w)
     if (w != wave) {
 #pragma unroll
       for (int i = 0; i < Q; ++i)
-        *reinterpret_cast<axk_f32x4*>(&s_o[w][wave < w ? wave : wave - 1][(i * 64 + lane) * 4]) = acc[w * Q + i];
+        s_o[((w * 3 + (wave < w ? wave : wave - 1)) * Q + i) * 64 + lane] = acc[w * Q + i];
     }
   __syncthreads();
   if (l16 >= group) return;
@@ -919,7 +939,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
       for (int i = 0; i < Q; ++i) {
         o[i] = acc[w * Q + i];
 #pragma unroll
-        for (int j = 0; j < 3; ++j) o[i] += *reinterpret_cast<axk_f32x4*>(&s_o[w][j][(i * 64 + lane) * 4]);
+        for (int j = 0; j < 3; ++j) o[i] += s_o[((w * 3 + j) * Q + i) * 64 + lane];
         o[i] *= inv;
       }
       const int at = w * Q / C::E * 16 * C::E + w * Q % C::E;
@@ -1024,7 +1044,7 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
     }
   }
   // page weights of listed blocks: what every page keeps
-  const int spp = a.page / kSub;
+  const unsigned spp = a.page / kSub;
   const float* in = w.in ? w.in + (int64_t)h * a.nnz + s.pb : nullptr;
   float* out = w.out ? w.out + (int64_t)h * a.nnz + s.pb : nullptr;
   if (!outs && a.blocks)
@@ -1074,11 +1094,10 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
     return group_sum<16>(sum);
   };
   if (!a.blocks) {
-    const int64_t all = (s.len + kSub - 1) / kSub, sub0 = (int64_t)piece * a.ps;
-    const int end = (int)min((sub0 + a.ps + spp - 1) / spp, (int64_t)s.np);
+    const unsigned sub0 = (unsigned)(piece * a.ps);
+    const int end = (int)min((sub0 + a.ps + spp - 1) / spp, (unsigned)s.np);
     for (int p = (int)((sub0 + spp - 1) / spp) + r16; p < end; p += 16) {
-      const int64_t first = (int64_t)p * spp;
-      const float sum = share(((int64_t)h * a.nnz + s.pb) * spp + first, (int)min((int64_t)spp, all - first));
+      const float sum = share(((int64_t)h * a.nnz + s.pb + p) * spp, min((int)spp, subs_of(s) - p * (int)spp));
       if (l16 == 0) out[p] = (in ? w.decay * in[p] : 0.f) + sum;
     }
     return;
@@ -1087,7 +1106,8 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
   // (A list out of order may name a page again: hence the atomic.) A page whose blocks straddle two rounds of the LDS is
   // finished by the round it begins in, which looks past its end.
   const int spb = a.block / kSub, bpp = a.page / a.block;
-  const int64_t row = (int64_t)b * a.hkv + h, nblocks = (s.len + a.block - 1) / a.block;
+  const int64_t row = (int64_t)b * a.hkv + h;
+  const int nblocks = blocks_of(s, a.block);
   const int* list = a.blocks + row * a.n;
   for (int base = 0; base < a.n; base += kListLds - bpp) {
     const int n = min(a.n - base, kListLds);  // the last bpp of them only to finish pages
@@ -1292,8 +1312,8 @@ BlkPlan blk_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t page
 template <int D>
 int launch_blocks(const BlkArgs& a, const WeightArgs& w, int f8, hipStream_t st) {
   const dim3 grid = a.blocks ? dim3((unsigned)(a.batch * a.hkv * a.pieces)) : dim3((unsigned)a.pieces, (unsigned)a.hkv);
-  if (f8) hipLaunchKernelGGL((paged_blocks_kernel<D, 1>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((paged_blocks_kernel<D, 0>), grid, dim3(256), 0, st, a);
+  if (f8) hipLaunchKernelGGL((paged_blocks_kernel<D, 1>), grid, dim3(256), (BlkCfg<D, 1>::LDS), st, a);
+  else hipLaunchKernelGGL((paged_blocks_kernel<D, 0>), grid, dim3(256), (BlkCfg<D, 0>::LDS), st, a);
   if (!a.direct) {
     const int64_t wgs = (int64_t)a.batch * a.hkv * w.split + (w.out ? (a.blocks ? (int64_t)a.batch : a.pieces) * a.hkv : 0);
     hipLaunchKernelGGL((paged_blocks_merge_kernel<D>), dim3((unsigned)wgs), dim3(256), 0, st, a, w);
@@ -1374,13 +1394,13 @@ extern "C" int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds,
                                (size_t)num_pages * (page_size / block_size) * num_kv_heads * head_dim * 4),
               AXK_E_ALIAS);
   const int64_t units = (total + 15) / 16 * num_kv_heads;
-  AXK_REQUIRE((units + 3) / 4 <= 0x7fffffff, AXK_E_SHAPE);
+  AXK_REQUIRE(units <= 0x7fffffff, AXK_E_SHAPE);
   AXK_LAUNCH_GATE();
   auto* fn = head_dim == 64 ? &paged_block_scores_kernel<64>
                             : head_dim == 128 ? &paged_block_scores_kernel<128> : &paged_block_scores_kernel<256>;
   hipLaunchKernelGGL(fn, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, axk_stream(stream), q, bounds, indptr, indices,
                      last_page_len, scores, (int)nnz, (int)batch, (int)num_qo_heads, (int)num_kv_heads, (int)page_size,
-                     (int)block_size, num_pages, units, status);
+                     (int)block_size, num_pages, (unsigned)units, status);
   return axk_launch_status();
 }
 
@@ -1490,6 +1510,11 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
   a.po = p.direct ? nullptr : reinterpret_cast<float*>(ws + p.ml);
   a.stat = weights ? reinterpret_cast<float2*>(ws + p.ml + p.po) : nullptr;
   a.status = status;
+  if (head_dim == 256 && !f8) {  // 64 KiB of dynamic LDS beside the static
+    static AxkOnce once;
+    if (const int e = axk_raise_lds(once, reinterpret_cast<const void*>(&paged_blocks_kernel<256, 0>), BlkCfg<256, 0>::LDS))
+      return e;
+  }
   const WeightArgs w = {weights_in, weights ? weights_out : nullptr, decay, split};
   AXK_LAUNCH_GATE();
   switch (head_dim) {
