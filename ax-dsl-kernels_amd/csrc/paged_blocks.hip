@@ -983,159 +983,193 @@ AXK_DEV float2 join_pairs(uint2 m, uint2 l) {
   return join(make_float2(__uint_as_float(m.x), __uint_as_float(l.x)), make_float2(__uint_as_float(m.y), __uint_as_float(l.y)));
 }
 
-// The first batch * hkv * split workgroups: the output rows of a (sequence, KV head) from its pieces, 64 float4s of its
-// group x D values each, a quarter of the pieces a wave. The others: the page weights, from each subtile's sum against the
-// row's joined maximum and sum. Every workgroup joins the pieces' sums of all heads of its row (16 lanes a piece, a head
-// each) while its other first loads are on their way: a merge is three trips to memory and little else.
+// A row's pieces: where they begin, how many the grid held (all of them, unless offsets of indptr overlap).
+struct Pieces {
+  int64_t item;
+  int n;
+};
+// Joins the sums of head l16 over the row's pieces (`t`: that of piece tid / 16, already loaded), a part a wave in s_part.
+AXK_DEV void join_pieces(float2 t, const float2* __restrict__ ml, int pieces, int group, float2 (*s_part)[16]) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
+  if (l16 < group)
+    for (int p = (threadIdx.x >> 4) + 16; p < pieces; p += 16) t = join(t, ml[(int64_t)p * group + l16]);
+  t = join_pairs(row_pair16(t.x), row_pair16(t.y));
+  t = join_pairs(half_pair32(t.x), half_pair32(t.y));
+  if (lane < 16) s_part[threadIdx.x >> 6][lane] = t;
+  __syncthreads();
+}
+
+// A row's output, workgroup `part`: 64 float4s of its group x D values, a quarter of the pieces a wave. The first pieces'
+// partial outputs are on their way while the sums are joined.
+template <int D>
+AXK_DEV void merge_output(const BlkArgs& a, int b, int h, int part, Pieces pc, float2 (*s_part)[16], axk_f32x4 (*s_o)[64]) {
+  constexpr int kFirst = 8;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = tid & 15, group = a.hq / a.hkv;
+  const int per = group * D / 4, i = part * 64 + lane, head = min(i, per - 1) / (D / 4);
+  const float2* ml = a.ml + pc.item * group;
+  const axk_f32x4* po = reinterpret_cast<const axk_f32x4*>(a.po + (pc.n ? pc.item : 0) * group * D) + min(i, per - 1);
+  const float2 none = make_float2(0.f, 0.f);
+  float2 t = l16 < group && (tid >> 4) < pc.n ? ml[(tid >> 4) * group + l16] : none;
+  axk_f32x4 v[kFirst];
+  float2 x[kFirst];
+#pragma unroll
+  for (int k = 0; k < kFirst; ++k) {
+    const int p = wave + 4 * k;
+    x[k] = p < pc.n ? ml[(int64_t)p * group + head] : none;
+    v[k] = po[(int64_t)max(min(p, pc.n - 1), 0) * per];  // past the end: not counted
+  }
+  join_pieces(t, ml, pc.n, group, s_part);
+  t = join(join(s_part[0][head], s_part[1][head]), join(s_part[2][head], s_part[3][head]));
+  axk_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < kFirst; ++k) o += (x[k].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[k].x - t.x)) * v[k];
+#pragma unroll 8
+  for (int p = wave + 4 * kFirst; p < pc.n; p += 4) {
+    const float2 y = ml[(int64_t)p * group + head];
+    o += (y.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(y.x - t.x)) * po[(int64_t)p * per];
+  }
+  s_o[wave][lane] = o;
+  __syncthreads();
+  if (wave == 0 && i < per) {
+    o = ((s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane])) * (t.y == 0.f ? 0.f : 1.0f / t.y);
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)b * a.hq + h * group) * D + 4 * i) =
+        make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+  }
+}
+
+// The page weights of a row (listed blocks), or of the pages that begin in piece `piece` (every block): each subtile's sum
+// against the row's joined maximum and sum. What is added up are units of subtiles (listed blocks, or pages), 64 at a time,
+// four to 16 lanes, a head a lane, four subtiles of each together; the first ones are on their way while the sums are joined.
 constexpr int kListLds = 2048;  // listed blocks whose shares are kept in LDS at a time
+AXK_DEV void merge_weights(const BlkArgs& a, const WeightArgs& w, int b, int h, int piece, const Seq& s, Pieces pc,
+                           float2 (*s_part)[16], float* s_share, int* s_page) {
+  const int tid = threadIdx.x, l16 = tid & 15, r16 = tid >> 4, group = a.hq / a.hkv;
+  const float2* ml = a.ml + pc.item * group;
+  const float2 none = make_float2(0.f, 0.f);
+  float2 t = l16 < group && r16 < pc.n ? ml[r16 * group + l16] : none;
+  const int spp = a.page / kSub, spb = a.block / kSub, bpp = a.page / a.block;
+  const float* in = w.in ? w.in + (int64_t)h * a.nnz + s.pb : nullptr;
+  float* out = w.out + (int64_t)h * a.nnz + s.pb;
+  const int p0 = (int)((unsigned)(piece * a.ps + spp - 1) / (unsigned)spp);
+  const int units = a.blocks ? a.n : min((int)((unsigned)((piece + 1) * a.ps + spp - 1) / (unsigned)spp), s.np) - p0;
+  const int span = a.blocks ? spb : spp, subs = a.blocks ? units * span : subs_of(s) - p0 * spp;
+  const float2* stat = a.stat + (subs <= 0 ? 0 : a.blocks ? ((int64_t)b * a.hkv + h) * a.n * spb : ((int64_t)h * a.nnz + s.pb + p0) * spp) * group;
+  const int top = max(subs - 1, 0);
+  float2 y[4][4];
+  auto fetch = [&](int u, int k0) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int sub = (u + 16 * q) * span + k0 + k;
+        const bool there = u + 16 * q < units && k0 + k < span && sub < subs && l16 < group;
+        // what is not there is read from the unit's own place (one address for all would hold up a channel of the L2)
+        const float2 x = stat[(int64_t)min(sub, top) * group + min(l16, group - 1)];
+        y[q][k] = make_float2(x.x, there ? x.y : 0.f);
+      }
+  };
+  // s_page[j]: the page of listed block base + j - 1, -1 for none
+  auto list_pages = [&](int base, int n) {
+    const int* list = a.blocks + ((int64_t)b * a.hkv + h) * a.n;
+    const int nblocks = blocks_of(s, a.block);
+    for (int j = tid; j <= n; j += 256) {
+      const int slot = base + j - 1, id = slot < 0 ? -1 : list[slot];
+      const bool none_here = id < 0 || bad_block(id, slot ? list[slot - 1] : -1, nblocks);
+      s_page[j] = none_here ? -1 : (int)((unsigned)id / (unsigned)bpp);
+    }
+  };
+  // The listed blocks of one page follow each other: the first of them adds them all, so that a page is added to once.
+  // (A list out of order may name a page again: hence the atomic.) A page whose blocks straddle two rounds of the LDS is
+  // finished by the round it begins in, which looks past its end.
+  for (int base = 0;; base += kListLds - bpp) {
+    const int end = a.blocks ? min(a.n, base + kListLds) : units;  // the last bpp of a round only to finish pages
+    int u = base + r16, k0 = 0;
+    fetch(u, 0);
+    if (a.blocks) {
+      __syncthreads();  // the round before has been read
+      list_pages(base, end - base);
+    }
+    if (base == 0) {
+      if (a.blocks)
+        for (int p = tid; p < s.np; p += 256) out[p] = in ? w.decay * in[p] : 0.f;  // what every page keeps
+      join_pieces(t, ml, pc.n, group, s_part);
+      t = join(join(s_part[0][l16], s_part[1][l16]), join(s_part[2][l16], s_part[3][l16]));
+      t.y = t.y == 0.f ? 0.f : 1.0f / t.y;
+    }
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    while (u < end) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          sum[q] += y[q][k].y == 0.f ? 0.f : y[q][k].y * __builtin_amdgcn_exp2f(y[q][k].x - t.x) * t.y;
+      k0 += 4;
+      if (k0 >= span) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float x = group_sum<16>(sum[q]);
+          const int unit = u + 16 * q;
+          if (l16 == 0 && unit < end) {
+            if (a.blocks) s_share[unit - base] = x;
+            else out[p0 + unit] = (in ? w.decay * in[p0 + unit] : 0.f) + x;
+          }
+          sum[q] = 0.f;
+        }
+        u += 64;
+        k0 = 0;
+      }
+      if (u < end) fetch(u, k0);
+    }
+    if (!a.blocks) return;
+    __syncthreads();
+    const int n = end - base;
+    for (int j = tid; j < (end < a.n ? n - bpp : n); j += 256) {
+      const int page = s_page[j + 1];
+      if (page < 0 || s_page[j] == page) continue;
+      float x = 0.f;
+      for (int k = j; k < n && s_page[k + 1] == page; ++k) x += s_share[k];
+      atomicAdd(out + page, x);
+    }
+    if (end == a.n) return;
+  }
+}
+
+// The first batch * hkv * split workgroups: output rows. The others: page weights. A merge is three dependent trips to
+// memory and little else.
 template <int D>
 __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a, const WeightArgs w) {
   __shared__ float2 s_part[4][16];
-  __shared__ float s_top[kMaxGroup], s_inv[kMaxGroup];
   __shared__ axk_f32x4 s_o[4][64];
   __shared__ float s_share[kListLds];
   __shared__ int s_page[kListLds + 1];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = tid & 15, r16 = tid >> 4;
-  const int group = a.hq / a.hkv, rows = a.batch * a.hkv;
-  const bool outs = (int)blockIdx.x < rows * w.split;
-  int b, h, part = 0, pieces = a.pieces, piece = 0;
-  int64_t item;
+  const int rows = a.batch * a.hkv, x = (int)blockIdx.x - rows * w.split;
+  int b, h, piece = 0;
+  Pieces pc;
   Seq s;
-  if (outs || a.blocks) {
-    const int row = outs ? blockIdx.x / w.split : blockIdx.x - rows * w.split;
-    part = outs ? blockIdx.x - row * w.split : 0;
+  if (x < 0 || a.blocks) {
+    const int row = x < 0 ? blockIdx.x / w.split : x;
     b = row / a.hkv;
     h = row - b * a.hkv;
     s = seq_of(a.indptr, a.last, b, a.page, a.nnz);
-    item = (int64_t)row * a.pieces;
-    if (!a.blocks) item = (int64_t)h * a.pieces + min(pieces_before(a, b), a.pieces);
+    pc = {(int64_t)row * a.pieces, a.pieces};
+    if (!a.blocks) {
+      const int before = min(pieces_before(a, b), a.pieces);
+      pc = {(int64_t)h * a.pieces + before, min(pieces_of(s, a.ps), a.pieces - before)};
+    }
+    if (x < 0) {
+      merge_output<D>(a, b, h, blockIdx.x - row * w.split, pc, s_part, s_o);
+      return;
+    }
   } else {  // one workgroup per piece, for the pages that begin in it
-    const int x = blockIdx.x - rows * w.split;
     h = x / a.pieces;
     const PieceOf p = find_piece(a, x - h * a.pieces);
     if (p.b >= a.batch) return;
     b = p.b;
     piece = p.piece;
     s = p.s;
-    item = x - piece;
+    pc = {x - piece, min(pieces_of(s, a.ps), (h + 1) * a.pieces - (x - piece))};
   }
-  // the pieces that the grid held (all of them, unless offsets of indptr overlap)
-  if (!a.blocks) pieces = min(pieces_of(s, a.ps), (int)((h + 1) * (int64_t)a.pieces - item));
-  const float2* ml = a.ml + item * group;
-  const float2 none = make_float2(0.f, 0.f);
-  float2 t = l16 < group && r16 < pieces ? ml[r16 * group + l16] : none;
-
-  // outputs: the first pieces' sums and partial outputs
-  constexpr int kFirst = 8;
-  const int per = group * D / 4, i = part * 64 + lane, head = min(i, per - 1) / (D / 4);
-  const axk_f32x4* po = reinterpret_cast<const axk_f32x4*>(a.po + item * group * D) + min(i, per - 1);
-  axk_f32x4 v[kFirst];
-  float2 x[kFirst];
-  if (outs) {
-#pragma unroll
-    for (int k = 0; k < kFirst; ++k) {
-      const int p = wave + 4 * k;
-      x[k] = none;
-      v[k] = (axk_f32x4){0.f, 0.f, 0.f, 0.f};
-      if (p < pieces) {
-        x[k] = ml[(int64_t)p * group + head];
-        v[k] = po[(int64_t)p * per];
-      }
-    }
-  }
-  // page weights of listed blocks: what every page keeps
-  const unsigned spp = a.page / kSub;
-  const float* in = w.in ? w.in + (int64_t)h * a.nnz + s.pb : nullptr;
-  float* out = w.out ? w.out + (int64_t)h * a.nnz + s.pb : nullptr;
-  if (!outs && a.blocks)
-    for (int p = tid; p < s.np; p += 256) out[p] = in ? w.decay * in[p] : 0.f;
-
-  for (int p = r16 + 16; p < pieces; p += 16)
-    if (l16 < group) t = join(t, ml[(int64_t)p * group + l16]);
-  t = join_pairs(row_pair16(t.x), row_pair16(t.y));
-  t = join_pairs(half_pair32(t.x), half_pair32(t.y));
-  if (lane < 16) s_part[wave][lane] = t;
-  __syncthreads();
-  if (outs) {
-    t = join(join(s_part[0][head], s_part[1][head]), join(s_part[2][head], s_part[3][head]));
-    axk_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < kFirst; ++k) o += (x[k].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[k].x - t.x)) * v[k];
-#pragma unroll 8
-    for (int p = wave + 4 * kFirst; p < pieces; p += 4) {
-      const float2 y = ml[(int64_t)p * group + head];
-      o += (y.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(y.x - t.x)) * po[(int64_t)p * per];
-    }
-    s_o[wave][lane] = o;
-    __syncthreads();
-    if (wave == 0 && i < per) {
-      o = ((s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane])) * (t.y == 0.f ? 0.f : 1.0f / t.y);
-      *reinterpret_cast<uint2*>(a.out + ((int64_t)b * a.hq + h * group) * D + 4 * i) =
-          make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
-    }
-    return;
-  }
-  if (tid < 16) {
-    t = join(join(s_part[0][tid], s_part[1][tid]), join(s_part[2][tid], s_part[3][tid]));
-    s_top[tid] = t.x;
-    s_inv[tid] = t.y == 0.f ? 0.f : 1.0f / t.y;
-  }
-  __syncthreads();
-  // the share of subtiles [from, from + n) of the statistics, by 16 lanes
-  auto share = [&](int64_t from, int n) {
-    float sum = 0.f;
-    const float2* st = a.stat + from * group;
-#pragma unroll 4
-    for (int j = l16; j < n * group; j += 16) {
-      const float2 y = st[j];
-      const int hd = j % group;
-      sum += y.y == 0.f ? 0.f : y.y * __builtin_amdgcn_exp2f(y.x - s_top[hd]) * s_inv[hd];
-    }
-    return group_sum<16>(sum);
-  };
-  if (!a.blocks) {
-    const unsigned sub0 = (unsigned)(piece * a.ps);
-    const int end = (int)min((sub0 + a.ps + spp - 1) / spp, (unsigned)s.np);
-    for (int p = (int)((sub0 + spp - 1) / spp) + r16; p < end; p += 16) {
-      const float sum = share(((int64_t)h * a.nnz + s.pb + p) * spp, min((int)spp, subs_of(s) - p * (int)spp));
-      if (l16 == 0) out[p] = (in ? w.decay * in[p] : 0.f) + sum;
-    }
-    return;
-  }
-  // The listed blocks of one page follow each other: the first of them adds them all, so that a page is added to once.
-  // (A list out of order may name a page again: hence the atomic.) A page whose blocks straddle two rounds of the LDS is
-  // finished by the round it begins in, which looks past its end.
-  const int spb = a.block / kSub, bpp = a.page / a.block;
-  const int64_t row = (int64_t)b * a.hkv + h;
-  const int nblocks = blocks_of(s, a.block);
-  const int* list = a.blocks + row * a.n;
-  for (int base = 0; base < a.n; base += kListLds - bpp) {
-    const int n = min(a.n - base, kListLds);  // the last bpp of them only to finish pages
-    __syncthreads();
-    for (int j = tid; j <= n; j += 256) {  // s_page[j]: the page of listed block base + j - 1, -1 for none
-      const int slot = base + j - 1;
-      int page = -1;
-      if (slot >= 0) {
-        const int id = list[slot];
-        if (id >= 0 && !bad_block(id, slot ? list[slot - 1] : -1, nblocks)) page = id / bpp;
-      }
-      s_page[j] = page;
-    }
-    for (int j = r16; j < n; j += 16) {
-      const float sum = share((row * a.n + base + j) * spb, spb);
-      if (l16 == 0) s_share[j] = sum;
-    }
-    __syncthreads();
-    const bool rest = base + n < a.n;
-    for (int j = tid; j < (rest ? kListLds - bpp : n); j += 256) {
-      const int page = s_page[j + 1];
-      if (page < 0 || s_page[j] == page) continue;
-      float sum = 0.f;
-      for (int k = j; k < n && s_page[k + 1] == page; ++k) sum += s_share[k];
-      atomicAdd(out + page, sum);
-    }
-    if (!rest) break;
-  }
+  merge_weights(a, w, b, h, piece, s, pc, s_part, s_share, s_page);
 }
 
 // ---- eviction ----
