@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
   constexpr int N = F8 ? 8 : 4;      // dwords of bf16 pairs a lane keeps
   constexpr int E = 2 * N;           // channels a lane keeps
   constexpr int B = F8 ? 1 : 2;      // bytes of a stored value
-  __shared__ axk_s16x2 s_lo[256 * N], s_hi[256 * N];
+  __shared__ __align__(16) axk_s16x2 s_lo[256 * N], s_hi[256 * N];
   const int tid = threadIdx.x;
   const int bpp = page_size / block;
   const int entry = blockIdx.x / bpp, sub = blockIdx.x - entry * bpp;
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
 #pragma unroll 4
       for (int t = rl; t < rows; t += lanes) {
         uint32_t x[N];
-        stored_pairs<F8>(load_nt(src + ((int64_t)t * row + c * E) * B), inv_scale, x);
+        stored_pairs<F8>(*reinterpret_cast<const axk_u32x4*>(src + ((int64_t)t * row + c * E) * B), inv_scale, x);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           lo[e] = __builtin_elementwise_min(lo[e], bf16_order(x[e]));
@@ -260,18 +260,17 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      s_lo[e * 256 + tid] = lo[e];
-      s_hi[e * 256 + tid] = hi[e];
+      s_lo[tid * N + e] = lo[e];
+      s_hi[tid * N + e] = hi[e];
     }
     __syncthreads();
-    for (int i = tid; i < w * N; i += 256) {
-      const int e = i / w, cc = i - e * w;
-      axk_s16x2 l = s_lo[e * 256 + cc], h = s_hi[e * 256 + cc];
+    for (int i = tid; i < w * N; i += 256) {  // dword i of the pass's row: consecutive lanes store consecutive dwords
+      axk_s16x2 l = s_lo[i], h = s_hi[i];
       for (int j = 1; j < lanes; ++j) {
-        l = __builtin_elementwise_min(l, s_lo[e * 256 + j * w + cc]);
-        h = __builtin_elementwise_max(h, s_hi[e * 256 + j * w + cc]);
+        l = __builtin_elementwise_min(l, s_lo[j * w * N + i]);
+        h = __builtin_elementwise_max(h, s_hi[j * w * N + i]);
       }
-      const int at = (c0 + cc) * E + 2 * e, head = at / d;
+      const int at = c0 * E + 2 * i, head = (int)((unsigned)at / (unsigned)d);
       uint32_t* o = reinterpret_cast<uint32_t*>(dst + (int64_t)head * 2 * d + (at - head * d));
       o[0] = bf16_unorder(l);
       o[d / 2] = bf16_unorder(h);
