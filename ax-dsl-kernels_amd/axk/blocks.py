@@ -26,6 +26,8 @@ from . import _lib
 # The checks build their messages only when they fail: a decode step makes these calls once a layer.
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch._C._cuda_getDevice
+_BF16, _F32, _I32, _U8, _E4M3 = torch.bfloat16, torch.float32, torch.int32, torch.uint8, torch.float8_e4m3fn
+_DT_BF16, _DT_E4M3 = _lib.DT_BF16, _lib.DT_FP8E4M3
 
 
 def _call(name: str, tensors, *args) -> None:
@@ -34,7 +36,7 @@ def _call(name: str, tensors, *args) -> None:
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{name}: tensors on {tensors[0].device} and {t.device}")
-    if dev < 0:
+    if dev < 0:  # the host
         raise ValueError(f"axk operators take device tensors; got a tensor on {tensors[0].device}")
     if _device() == dev:
         _lib.call(name, *args, _stream(dev))
@@ -44,7 +46,7 @@ def _call(name: str, tensors, *args) -> None:
 
 
 def _i32(t: torch.Tensor, name: str, *shape: int) -> None:
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not _I32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 {list(shape)}")
 
 
@@ -55,13 +57,13 @@ def _table(indptr, last_page_len, indices=None) -> int:
         raise ValueError("the page table holds no sequence")
     _i32(indptr, "indptr", b + 1)
     _i32(last_page_len, "last_page_len", b)
-    if indices is not None and (indices.dtype != torch.int32 or indices.dim() != 1 or not indices.is_contiguous()):
+    if indices is not None and (indices.dtype is not _I32 or indices.dim() != 1 or not indices.is_contiguous()):
         raise ValueError("indices must be contiguous int32 [nnz]")
     return b
 
 
 def _status(status) -> None:
-    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+    if status is not None and (status.dtype is not _I32 or status.numel() < 1):
         raise ValueError("status must be int32 [1]")
 
 
@@ -74,20 +76,21 @@ def _sizes(page_size: int, block_size: int) -> None:
 
 def _cache(kv_cache, kv_scale):
     """(dtype code, scale, num_pages, page_size, HKV, D) of a bf16 or FP8 cache."""
-    if kv_cache.dtype == torch.bfloat16:
+    dtype, shape = kv_cache.dtype, kv_cache.shape
+    if dtype is _BF16:
         if kv_scale is not None:
             raise ValueError("kv_scale is for an FP8 cache")
-        code, scale = _lib.DT_BF16, 1.0
+        code, scale = _DT_BF16, 1.0
     else:
-        if kv_cache.dtype not in (torch.uint8, torch.float8_e4m3fn):
-            raise ValueError(f"kv_cache must be bfloat16 or u8 / float8_e4m3fn, got {kv_cache.dtype}")
+        if dtype is not _U8 and dtype is not _E4M3:
+            raise ValueError(f"kv_cache must be bfloat16 or u8 / float8_e4m3fn, got {dtype}")
         if kv_scale is None or not kv_scale > 0 or math.frexp(kv_scale)[0] != 0.5:
             raise ValueError(f"an FP8 cache needs its kv_scale, a power of two (got {kv_scale})")
-        code, scale = _lib.DT_FP8E4M3, kv_scale
-    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or not kv_cache.is_contiguous():
+        code, scale = _DT_E4M3, kv_scale
+    if len(shape) != 5 or shape[1] != 2 or not kv_cache.is_contiguous():
         raise ValueError("kv_cache must be contiguous [pages, 2, page_size, HKV, D]")
-    p, _, page, hkv, d = kv_cache.shape
-    if d not in (64, 128, 256):
+    p, _, page, hkv, d = shape
+    if d != 256 and d != 128 and d != 64:
         raise ValueError(f"head_dim {d} not supported (64, 128, 256)")
     if p < 1:
         raise ValueError("kv_cache holds no page")
@@ -96,11 +99,12 @@ def _cache(kv_cache, kv_scale):
 
 def _bounds(bounds, p: int, hkv: int, d: int, page_size: int) -> int:
     """Checks the bounds of a pool and returns the block size they are for."""
-    if (bounds.dim() != 5 or bounds.dtype != torch.bfloat16 or not bounds.is_contiguous() or bounds.shape[1] < 1
-            or page_size % bounds.shape[1] or bounds.shape != (p, bounds.shape[1], hkv, 2, d)):
+    shape = bounds.shape
+    bpp = shape[1] if len(shape) == 5 else 0
+    if bpp < 1 or page_size % bpp or shape != (p, bpp, hkv, 2, d) or bounds.dtype is not _BF16 or not bounds.is_contiguous():
         raise ValueError(f"bounds must be contiguous bf16 [{p}, page_size / block_size, {hkv}, 2, {d}], "
-                         f"got {tuple(bounds.shape)} {bounds.dtype}")
-    block = page_size // bounds.shape[1]
+                         f"got {tuple(shape)} {bounds.dtype}")
+    block = page_size // bpp
     _sizes(page_size, block)
     return block
 
@@ -125,8 +129,9 @@ def store_paged_kv_bounds(
     rows); where two name one slot the last is stored."""
     code, scale, p, page, hkv, d = _cache(kv_cache, kv_scale)
     block = _bounds(bounds, p, hkv, d, page)
-    rows = k.shape[0]
-    if (k.shape != (rows, hkv, d) or v.shape != k.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16
+    shape = k.shape
+    rows = shape[0] if shape else 0
+    if (shape != (rows, hkv, d) or v.shape != shape or k.dtype is not _BF16 or v.dtype is not _BF16
             or not k.is_contiguous() or not v.is_contiguous()):
         raise ValueError(f"k and v must be contiguous bf16 [rows, {hkv}, {d}]")
     _i32(cache_location, "cache_location", rows, 2)
@@ -175,9 +180,10 @@ def paged_block_scores(
     sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d over the KV head's queries of q [B, HQ, D] bf16, which no q . k in the block
     exceeds. -inf past a sequence's end. Entry e's blocks are columns e * page_size / block_size onwards."""
     b = _table(indptr, last_page_len, indices)
-    if q.dim() != 3 or q.shape[0] != b or q.dtype != torch.bfloat16 or not q.is_contiguous():
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != b or q.dtype is not _BF16 or not q.is_contiguous():
         raise ValueError(f"q must be contiguous bf16 [{b}, HQ, D]")
-    _, hq, d = q.shape
+    _, hq, d = shape
     if d not in (64, 128, 256):
         raise ValueError(f"head_dim {d} not supported (64, 128, 256)")
     if bounds.dim() != 5 or bounds.shape[0] < 1:
@@ -188,7 +194,7 @@ def paged_block_scores(
     n = indices.numel() * bpp
     if output is None:
         output = q.new_empty((hkv, n), dtype=torch.float32)
-    elif output.shape != (hkv, n) or output.dtype != torch.float32 or not output.is_contiguous():
+    elif output.shape != (hkv, n) or output.dtype is not _F32 or not output.is_contiguous():
         raise ValueError(f"output must be contiguous float32 [{hkv}, {n}]")
     _status(status)
     _call("axk_paged_block_scores", (q, bounds, indptr, indices, last_page_len, output, status), q.data_ptr(),
@@ -213,7 +219,7 @@ def paged_select_blocks(
     scores by the lowest block, NaN above every number; -1 behind the blocks of a shorter sequence."""
     b = _table(indptr, last_page_len)
     _sizes(page_size, block_size)
-    if (scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous() or scores.shape[0] < 1
+    if (scores.dim() != 2 or scores.dtype is not _F32 or not scores.is_contiguous() or scores.shape[0] < 1
             or scores.shape[1] % (page_size // block_size)):
         raise ValueError("scores must be contiguous float32 [HKV, nnz * page_size / block_size]")
     if first < 0 or keep_last < 0 or num_select < 1 or first + keep_last > num_select:
@@ -263,9 +269,10 @@ def paged_decode_blocks(
     plus the attention that each page-table entry's tokens received, summed over the KV head's queries."""
     b = _table(indptr, last_page_len, indices)
     code, scale, p, page, hkv, d = _cache(kv_cache, kv_scale)
-    if q.dim() != 3 or q.shape[0] != b or q.shape[2] != d or q.dtype != torch.bfloat16 or not q.is_contiguous():
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != b or shape[2] != d or q.dtype is not _BF16 or not q.is_contiguous():
         raise ValueError(f"q must be contiguous bf16 [{b}, HQ, {d}]")
-    hq, nnz, n = q.shape[1], indices.numel(), 0
+    hq, nnz, n = shape[1], indices.numel(), 0
     _heads(hq, hkv)
     if blocks is not None:
         if block_size is None:
@@ -281,17 +288,17 @@ def paged_decode_blocks(
         sm_scale = 1.0 / math.sqrt(d)
     if output is None:
         output = torch.empty_like(q)
-    elif output.shape != q.shape or output.dtype != q.dtype or not output.is_contiguous():
+    elif output.shape != shape or output.dtype is not _BF16 or not output.is_contiguous():
         raise ValueError(f"output must be contiguous bf16 [{b}, {hq}, {d}]")
     if weights is None and weights_in is not None:
         raise ValueError("weights_in without weights")
     for t in (weights_in, weights):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (hkv, nnz) or not t.is_contiguous()):
+        if t is not None and (t.dtype is not _F32 or t.shape != (hkv, nnz) or not t.is_contiguous()):
             raise ValueError(f"weights_in and weights must be contiguous float32 [{hkv}, {nnz}]")
     _status(status)
     if workspace is None:
         workspace = paged_decode_blocks_workspace(b, hq, hkv, d, page, nnz, q.device, block_size, n, weights is not None)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+    elif workspace.dtype is not _U8 or not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous uint8")
     _call("axk_paged_decode_blocks",
           (q, kv_cache, indptr, indices, last_page_len, blocks, output, weights_in, weights, status, workspace),
@@ -318,10 +325,10 @@ def paged_evict_pages(
     if b < 1:
         raise ValueError("the page table holds no sequence")
     _i32(indptr, "indptr", b + 1)
-    if indices.dtype != torch.int32 or indices.dim() != 1 or not indices.is_contiguous():
+    if indices.dtype is not _I32 or indices.dim() != 1 or not indices.is_contiguous():
         raise ValueError("indices must be contiguous int32 [nnz]")
     nnz = indices.numel()
-    if (weights.dim() != 2 or weights.shape[0] < 1 or weights.shape[1] != nnz or weights.dtype != torch.float32
+    if (weights.dim() != 2 or weights.shape[0] < 1 or weights.shape[1] != nnz or weights.dtype is not _F32
             or not weights.is_contiguous()):
         raise ValueError(f"weights must be contiguous float32 [HKV, {nnz}]")
     if first < 0 or keep_last < 1 or first + keep_last > budget:

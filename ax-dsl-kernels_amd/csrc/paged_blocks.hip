@@ -100,6 +100,8 @@ AXK_DEV void stored_pairs(const axk_u32x4 w, float inv_scale, uint32_t (&out)[F8
 }
 
 // ---- key bounds ----
+constexpr int64_t kMaxRows = 16384;  // every row looks at every other's place: 2^28 reads, some 0.1 ms
+
 // The new rows' K / V written at loc[r] = (page, slot), and folded into the bounds of their blocks: a block that holds a
 // new row at its first slot starts afresh, every other one widens what it had. One workgroup per row; the first row of
 // the call that falls into a block folds all of them, so that rows of one block never race, and where two rows name one
@@ -1294,12 +1296,14 @@ __global__ __launch_bounds__(kEvict) void paged_evict_kernel(const float* __rest
 
 namespace {
 
+constexpr int64_t kMaxSubs = 1 << 30;  // subtiles of a page table, or of a row's listed blocks: sums of them fit 32 bits
+
 int check_blocks(int64_t batch, int64_t hkv, int64_t d, int64_t page_size, int64_t block, int64_t num_pages, int64_t nnz) {
   AXK_REQUIRE(batch > 0 && batch <= (1 << 20) && hkv > 0 && hkv <= 4096, AXK_E_SHAPE);
   AXK_REQUIRE(d == 64 || d == 128 || d == 256, AXK_E_SHAPE);
   AXK_REQUIRE(page_size >= kSub && page_size % kSub == 0 && page_size <= 4096, AXK_E_SHAPE);
   AXK_REQUIRE(block >= kSub && block % kSub == 0 && page_size % block == 0, AXK_E_SHAPE);
-  AXK_REQUIRE(num_pages > 0 && nnz >= 0 && nnz * (page_size / kSub) <= 0x7fffffff, AXK_E_SHAPE);
+  AXK_REQUIRE(num_pages > 0 && nnz >= 0 && nnz * (page_size / kSub) <= kMaxSubs, AXK_E_SHAPE);
   return AXK_OK;
 }
 
@@ -1363,7 +1367,7 @@ extern "C" int axk_paged_kv_write_bounds(const uint16_t* k, const uint16_t* v, v
   AXK_REQUIRE(k && v && kv_cache && bounds && cache_location, AXK_E_NULL);
   const int rc = check_blocks(1, num_kv_heads, head_dim, page_size, block_size, num_pages, 0);
   if (rc != AXK_OK) return rc;
-  AXK_REQUIRE(rows >= 0 && rows <= (1 << 20), AXK_E_SHAPE);
+  AXK_REQUIRE(rows >= 0 && rows <= kMaxRows, AXK_E_SHAPE);
   const int f8 = cache_type(kv_dtype, kv_scale);
   if (f8 < 0) return -f8;
   AXK_REQUIRE(axk_aligned(k, 16) && axk_aligned(v, 16) && axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16),
@@ -1469,7 +1473,7 @@ extern "C" size_t axk_paged_decode_blocks_workspace_size(int64_t batch, int64_t 
                                                          int64_t block_size, int64_t num_select, int with_weights) {
   if (check_blocks(batch, num_kv_heads, head_dim, page_size, num_select ? block_size : kSub, 1, nnz) != AXK_OK) return 0;
   if (num_qo_heads <= 0 || num_qo_heads % num_kv_heads || num_qo_heads / num_kv_heads > kMaxGroup) return 0;
-  if (num_select < 0 || num_select * (block_size / kSub) > 0x7fffffff) return 0;
+  if (num_select < 0 || num_select > kMaxSubs || num_select * (block_size / kSub) > kMaxSubs) return 0;
   const BlkPlan p = blk_plan(batch, num_qo_heads, num_kv_heads, head_dim, page_size, nnz, block_size, num_select,
                              with_weights != 0);
   return p.ml + p.po + p.stat;
@@ -1492,7 +1496,7 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
   const int rc = check_blocks(batch, num_kv_heads, head_dim, page_size, block_size, num_pages, nnz);
   if (rc != AXK_OK) return rc;
   AXK_REQUIRE(num_qo_heads > 0 && num_qo_heads % num_kv_heads == 0 && num_qo_heads / num_kv_heads <= kMaxGroup, AXK_E_SHAPE);
-  AXK_REQUIRE(num_select * (block_size / kSub) <= 0x7fffffff, AXK_E_SHAPE);
+  AXK_REQUIRE(num_select <= kMaxSubs && num_select * (block_size / kSub) <= kMaxSubs, AXK_E_SHAPE);
   AXK_REQUIRE(!weights_in || weights_out, AXK_E_NULL);
   const int f8 = cache_type(kv_dtype, kv_scale);
   if (f8 < 0) return -f8;
@@ -1543,9 +1547,12 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
   a.po = p.direct ? nullptr : reinterpret_cast<float*>(ws + p.ml);
   a.stat = weights ? reinterpret_cast<float2*>(ws + p.ml + p.po) : nullptr;
   a.status = status;
-  if (head_dim == 256 && !f8) {  // 64 KiB of dynamic LDS beside the static
-    static AxkOnce once;
-    if (const int e = axk_raise_lds(once, reinterpret_cast<const void*>(&paged_blocks_kernel<256, 0>), BlkCfg<256, 0>::LDS))
+  if (head_dim == 256 && !f8) {  // 64 KiB of dynamic LDS beside the static: to be allowed once on each device
+    static AxkOnce once[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return AXK_E_LAUNCH;
+    if (const int e = axk_raise_lds(once[dev & 63], reinterpret_cast<const void*>(&paged_blocks_kernel<256, 0>),
+                                    BlkCfg<256, 0>::LDS))
       return e;
   }
   const WeightArgs w = {weights_in, weights ? weights_out : nullptr, decay, split};

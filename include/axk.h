@@ -386,7 +386,7 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  * Cache, page table and page size as axk_paged_decode; head_dim 64, 128 or 256; num_qo_heads / num_kv_heads <= 16;
  * num_kv_heads <= 4096. kv_dtype: AXK_DT_BF16, or AXK_DT_FP8E4M3 for a cache of axk_paged_kv_write_fp8 with its kv_scale
  * (a power of two; ignored for bf16). nnz: the entries of indices; offsets of indptr past it are read as nnz and a
- * last_page_len past page_size as page_size, so that no access leaves an array; nnz * page_size / 16 < 2^31. A page id
+ * last_page_len past page_size as page_size, so that no access leaves an array; nnz * page_size / 16 <= 2^30. A page id
  * outside [0, num_pages) is skipped, never read, and sets *status (device i32, or NULL) to 1. An array per page-table entry
  * is [num_kv_heads, nnz], one per block [num_kv_heads, nnz * page_size / block_size]: entry e's blocks at e *
  * page_size / block_size.
@@ -397,7 +397,8 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  * A block with a new row at its first slot starts afresh; any other widens what it had, so tokens are written in order,
  * and rows written over (rejected drafts) leave bounds that still hold but are wide, until axk_paged_key_bounds computes
  * them again. Rows of one call may share a block; where two name one slot the last one is stored, and both are folded. A
- * location outside the pool is skipped and sets *status. A NaN key makes the bound on its sign's side NaN. */
+ * location outside the pool is skipped and sets *status. A NaN key makes the bound on its sign's side NaN. rows <= 16384:
+ * a longer prefill chunk is written by axk_paged_kv_write and its blocks' bounds computed by axk_paged_key_bounds. */
 int axk_paged_kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cache, int kv_dtype, float kv_scale,
                               uint16_t* bounds, const int32_t* cache_location, int64_t rows, int64_t num_kv_heads,
                               int64_t head_dim, int64_t page_size, int64_t block_size, int64_t num_pages,

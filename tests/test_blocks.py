@@ -54,12 +54,12 @@ def evict(w=at(1), ptr=at(2), idx=at(3), optr=at(4), oidx=at(5), ow=at(6), freed
     (lambda: write(k=None), NULL), (lambda: write(bounds=None), NULL), (lambda: write(loc=None), NULL),
     (lambda: write(d=96), SHAPE), (lambda: write(page=24), SHAPE), (lambda: write(block=24), SHAPE),
     (lambda: write(page=48, block=32), SHAPE), (lambda: write(page=8192, block=16), SHAPE),
-    (lambda: write(hkv=0), SHAPE), (lambda: write(pages=0), SHAPE), (lambda: write(rows=-1), SHAPE),
+    (lambda: write(hkv=0), SHAPE), (lambda: write(pages=0), SHAPE), (lambda: write(rows=-1), SHAPE), (lambda: write(rows=16385), SHAPE),
     (lambda: write(dt=_lib.DT_F16), DTYPE), (lambda: write(dt=E4M3, scale=3.0), SHAPE),
     (lambda: write(dt=E4M3, scale=float("nan")), SHAPE), (lambda: write(k=at(1, 8)), ALIGN),
     (lambda: write(bounds=at(3, 2)), ALIGN), (lambda: write(bounds=at(16)), ALIAS), (lambda: write(k=at(16)), ALIAS),
     (lambda: bounds_(cache=None), NULL), (lambda: bounds_(idx=None), NULL), (lambda: bounds_(batch=0), SHAPE),
-    (lambda: bounds_(nnz=-1), SHAPE), (lambda: bounds_(nnz=1 << 30, page=64), SHAPE), (lambda: bounds_(d=32), SHAPE),
+    (lambda: bounds_(nnz=-1), SHAPE), (lambda: bounds_(nnz=(1 << 28) + 1, page=64), SHAPE), (lambda: bounds_(d=32), SHAPE),
     (lambda: bounds_(dt=_lib.DT_U8), DTYPE), (lambda: bounds_(dt=E4M3, scale=0.0), SHAPE),
     (lambda: bounds_(cache=at(16, 8)), ALIGN), (lambda: bounds_(bounds=at(16, 4096)), ALIAS),
     (lambda: scores(out=None), NULL), (lambda: scores(q=None), NULL), (lambda: scores(hq=3), SHAPE),

@@ -231,7 +231,7 @@ def test_select(dev, kind, blocks, n, first, keep_last):
 @pytest.mark.parametrize("kv", ["bf16", "fp8"])
 @pytest.mark.parametrize("hq,hkv,d,page,block,n", [(16, 2, 256, 64, 64, 9), (16, 1, 64, 16, 16, 40), (7, 7, 64, 64, 32, 3),
                                                    (6, 2, 128, 96, 48, 12), (32, 8, 128, 256, 128, 4),
-                                                   (16, 2, 256, 64, 16, 200), (3, 1, 256, 4096, 16, 7)])
+                                                   (16, 2, 256, 64, 16, 200), (3, 1, 256, 4096, 16, 7), (16, 1, 256, 64, 32, 33)])
 def test_decode_over_listed_blocks(dev, kv, hq, hkv, d, page, block, n):
     c = make([0, 1, 17, page + 2, 1500, 3200], hq, hkv, d, page, kv, seed=n)
     blocks = random_blocks(c, block, n)
