@@ -92,6 +92,10 @@ SIGNATURES: dict[str, list] = {
     "axk_paged_decode_blocks_workspace_size": [_i64] * 8 + [_i32],
     "axk_paged_decode_blocks": [_vp, _vp, _i32, ctypes.c_float] + [_vp] * 4 + [_i64, _i64, _vp, _vp, _vp,
                                ctypes.c_float] + [_i64] * 7 + [ctypes.c_float, _vp, _vp, ctypes.c_size_t, _vp],
+    "axk_paged_kv_write_bounds_i8": [_vp] * 6 + [_i64] * 6 + [_vp, _vp],
+    "axk_paged_key_bounds_i8": [_vp] * 7 + [_i64] * 7 + [_vp, _vp],
+    "axk_paged_decode_blocks_i8": [_vp] * 7 + [_i64, _i64, _vp, _vp, _vp, ctypes.c_float] + [_i64] * 7 +
+                                  [ctypes.c_float, _vp, _vp, ctypes.c_size_t, _vp],
     "axk_paged_evict_pages": [_vp] * 7 + [_i64] * 6 + [_vp],
     "axk_gdn_recurrent": [_vp] * 10 + [_i64] * 6 + [_vp],
     "axk_gdn_chunk_workspace_size": [_i64] * 7,

@@ -9,8 +9,8 @@ decode step of a layer is then::
     out = paged_decode_blocks(q, kv_cache, indptr, indices, last, blocks, block, weights_in=w, weights=w)
 
 after a prefill chunk ``paged_key_bounds`` computes the bounds of its blocks, and ``paged_evict_pages`` cuts a page table
-down to the pages that received the most attention (``w``). Caches are those of paged_decode (bf16) and paged_decode_fp8
-(u8 / float8_e4m3fn with ``kv_scale``), page tables theirs too. Nothing is read back to the host, so a step can be
+down to the pages that received the most attention (``w``). Caches are those of paged_decode (bf16), paged_decode_fp8
+(u8 / float8_e4m3fn with ``kv_scale``) and paged_decode_i8 (int8 with ``kv_scales``), page tables theirs too. Nothing is read back to the host, so a step can be
 captured in a HIP graph. Contract violations raise ValueError.
 """
 from __future__ import annotations
@@ -26,7 +26,8 @@ from . import _lib
 # The checks build their messages only when they fail: a decode step makes these calls once a layer.
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch._C._cuda_getDevice
-_BF16, _F32, _I32, _U8, _E4M3 = torch.bfloat16, torch.float32, torch.int32, torch.uint8, torch.float8_e4m3fn
+_BF16, _F32, _I32, _I8, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.int8, torch.uint8
+_E4M3 = torch.float8_e4m3fn
 _DT_BF16, _DT_E4M3 = _lib.DT_BF16, _lib.DT_FP8E4M3
 
 
@@ -74,19 +75,9 @@ def _sizes(page_size: int, block_size: int) -> None:
         raise ValueError(f"block_size {block_size} must be a multiple of 16 that divides page_size {page_size}")
 
 
-def _cache(kv_cache, kv_scale):
-    """(dtype code, scale, num_pages, page_size, HKV, D) of a bf16 or FP8 cache."""
+def _cache(kv_cache, kv_scale, kv_scales):
+    """(entry suffix, arguments naming the stored type, num_pages, page_size, HKV, D) of a bf16, FP8 or INT8 cache."""
     dtype, shape = kv_cache.dtype, kv_cache.shape
-    if dtype is _BF16:
-        if kv_scale is not None:
-            raise ValueError("kv_scale is for an FP8 cache")
-        code, scale = _DT_BF16, 1.0
-    else:
-        if dtype is not _U8 and dtype is not _E4M3:
-            raise ValueError(f"kv_cache must be bfloat16 or u8 / float8_e4m3fn, got {dtype}")
-        if kv_scale is None or not kv_scale > 0 or math.frexp(kv_scale)[0] != 0.5:
-            raise ValueError(f"an FP8 cache needs its kv_scale, a power of two (got {kv_scale})")
-        code, scale = _DT_E4M3, kv_scale
     if len(shape) != 5 or shape[1] != 2 or not kv_cache.is_contiguous():
         raise ValueError("kv_cache must be contiguous [pages, 2, page_size, HKV, D]")
     p, _, page, hkv, d = shape
@@ -94,7 +85,22 @@ def _cache(kv_cache, kv_scale):
         raise ValueError(f"head_dim {d} not supported (64, 128, 256)")
     if p < 1:
         raise ValueError("kv_cache holds no page")
-    return code, scale, p, page, hkv, d
+    if kv_scale is not None and (dtype is _BF16 or dtype is _I8):
+        raise ValueError("kv_scale is for an FP8 cache")
+    if kv_scales is not None and dtype is not _I8:
+        raise ValueError("kv_scales are for an INT8 cache")
+    if dtype is _BF16:
+        return "", (_DT_BF16, 1.0), p, page, hkv, d
+    if dtype is _I8:
+        if (kv_scales is None or kv_scales.dtype is not _BF16 or kv_scales.shape != (p, 2, page, hkv)
+                or not kv_scales.is_contiguous()):
+            raise ValueError(f"an INT8 cache needs its kv_scales, contiguous bf16 [{p}, 2, {page}, {hkv}]")
+        return "_i8", (kv_scales.data_ptr(),), p, page, hkv, d
+    if dtype is not _U8 and dtype is not _E4M3:
+        raise ValueError(f"kv_cache must be bfloat16, u8 / float8_e4m3fn or int8, got {dtype}")
+    if kv_scale is None or not kv_scale > 0 or math.frexp(kv_scale)[0] != 0.5:
+        raise ValueError(f"an FP8 cache needs its kv_scale, a power of two (got {kv_scale})")
+    return "", (_DT_E4M3, kv_scale), p, page, hkv, d
 
 
 def _bounds(bounds, p: int, hkv: int, d: int, page_size: int) -> int:
@@ -122,12 +128,13 @@ def store_paged_kv_bounds(
     cache_location: torch.Tensor,
     kv_scale: Optional[float] = None,
     status: Optional[torch.Tensor] = None,
+    kv_scales: Optional[torch.Tensor] = None,
 ) -> None:
-    """store_paged_kv / store_paged_kv_fp8 that also folds each new key into its block's bounds, in one launch: k, v
+    """store_paged_kv / store_paged_kv_fp8 / store_paged_kv_i8 that also folds each new key into its block's bounds, in one launch: k, v
     [rows, HKV, D] bf16 go to cache_location[r] = (page, slot). bounds [P, page / block, HKV, 2, D] bf16, in place: a
     block whose first slot is written starts afresh, any other is widened. Rows of one call may share a block (draft
     rows); where two name one slot the last is stored."""
-    code, scale, p, page, hkv, d = _cache(kv_cache, kv_scale)
+    kind, stored, p, page, hkv, d = _cache(kv_cache, kv_scale, kv_scales)
     block = _bounds(bounds, p, hkv, d, page)
     shape = k.shape
     rows = shape[0] if shape else 0
@@ -137,9 +144,9 @@ def store_paged_kv_bounds(
     _i32(cache_location, "cache_location", rows, 2)
     _status(status)
     if rows:
-        _call("axk_paged_kv_write_bounds", (k, v, kv_cache, bounds, cache_location, status), k.data_ptr(), v.data_ptr(),
-              kv_cache.data_ptr(), code, scale, bounds.data_ptr(), cache_location.data_ptr(), rows, hkv, d, page, block, p,
-              _lib.ptr(status))
+        _call("axk_paged_kv_write_bounds" + kind, (k, v, kv_cache, kv_scales, bounds, cache_location, status), k.data_ptr(),
+              v.data_ptr(), kv_cache.data_ptr(), *stored, bounds.data_ptr(), cache_location.data_ptr(), rows, hkv, d, page,
+              block, p, _lib.ptr(status))
 
 
 def paged_key_bounds(
@@ -151,18 +158,19 @@ def paged_key_bounds(
     start: Optional[torch.Tensor] = None,
     kv_scale: Optional[float] = None,
     status: Optional[torch.Tensor] = None,
+    kv_scales: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """The bounds of the page table's blocks from the cache, in place: of the blocks that hold a token at or after
     start[b] (int32 [B], the position a prefill chunk began at), or of all. Returns bounds."""
-    code, scale, p, page, hkv, d = _cache(kv_cache, kv_scale)
+    kind, stored, p, page, hkv, d = _cache(kv_cache, kv_scale, kv_scales)
     block = _bounds(bounds, p, hkv, d, page)
     b = _table(indptr, last_page_len, indices)
     if start is not None:
         _i32(start, "start", b)
     _status(status)
-    _call("axk_paged_key_bounds", (kv_cache, bounds, indptr, indices, last_page_len, start, status), kv_cache.data_ptr(),
-          code, scale, bounds.data_ptr(), indptr.data_ptr(), indices.data_ptr(), last_page_len.data_ptr(),
-          _lib.ptr(start), indices.numel(), b, hkv, d, page, block, p, _lib.ptr(status))
+    _call("axk_paged_key_bounds" + kind, (kv_cache, kv_scales, bounds, indptr, indices, last_page_len, start, status),
+          kv_cache.data_ptr(), *stored, bounds.data_ptr(), indptr.data_ptr(), indices.data_ptr(),
+          last_page_len.data_ptr(), _lib.ptr(start), indices.numel(), b, hkv, d, page, block, p, _lib.ptr(status))
     return bounds
 
 
@@ -260,15 +268,16 @@ def paged_decode_blocks(
     kv_scale: Optional[float] = None,
     workspace: Optional[torch.Tensor] = None,
     status: Optional[torch.Tensor] = None,
+    kv_scales: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """paged_decode / paged_decode_fp8 over the listed blocks of each sequence and KV head: blocks int32 [B, HKV, n],
+    """paged_decode / paged_decode_fp8 / paged_decode_i8 over the listed blocks of each sequence and KV head: blocks int32 [B, HKV, n],
     strictly ascending block numbers within the sequence, then -1 (as paged_select_blocks returns them), of block_size
     tokens; None: every block. q [B, HQ, D] bf16; returns bf16 [B, HQ, D], zeros where nothing is attended.
 
     weights f32 [HKV, nnz], if given, is set to decay * weights_in (zero without weights_in; weights_in may be weights)
     plus the attention that each page-table entry's tokens received, summed over the KV head's queries."""
     b = _table(indptr, last_page_len, indices)
-    code, scale, p, page, hkv, d = _cache(kv_cache, kv_scale)
+    kind, stored, p, page, hkv, d = _cache(kv_cache, kv_scale, kv_scales)
     shape = q.shape
     if len(shape) != 3 or shape[0] != b or shape[2] != d or q.dtype is not _BF16 or not q.is_contiguous():
         raise ValueError(f"q must be contiguous bf16 [{b}, HQ, {d}]")
@@ -300,9 +309,9 @@ def paged_decode_blocks(
         workspace = paged_decode_blocks_workspace(b, hq, hkv, d, page, nnz, q.device, block_size, n, weights is not None)
     elif workspace.dtype is not _U8 or not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous uint8")
-    _call("axk_paged_decode_blocks",
-          (q, kv_cache, indptr, indices, last_page_len, blocks, output, weights_in, weights, status, workspace),
-          q.data_ptr(), kv_cache.data_ptr(), code, scale, indptr.data_ptr(), indices.data_ptr(), last_page_len.data_ptr(),
+    _call("axk_paged_decode_blocks" + kind,
+          (q, kv_cache, kv_scales, indptr, indices, last_page_len, blocks, output, weights_in, weights, status, workspace),
+          q.data_ptr(), kv_cache.data_ptr(), *stored, indptr.data_ptr(), indices.data_ptr(), last_page_len.data_ptr(),
           _lib.ptr(blocks), block_size, n, output.data_ptr(), _lib.ptr(weights_in), _lib.ptr(weights), decay, nnz, b, hq,
           hkv, d, page, p, sm_scale, _lib.ptr(status), workspace.data_ptr(), workspace.numel())
     return output

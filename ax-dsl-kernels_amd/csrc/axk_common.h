@@ -105,6 +105,16 @@ AXK_DEV uint32_t f32_to_e4m3(float v) {
   return sgn | (ex << 3) | m3;
 }
 
+// The INT8 KV cache's quantizer (models/qwen38_27b/decode/q35_group.py kv_quant_row 197-205): a row's scale
+// s = bf16(max(amax, bf16(1e-5)) * bf16(1 / 127)), and the code int8(bf16(x * r)), r = bf16(1 / s), rounded to nearest even
+// and saturated, as a float.
+AXK_DEV float kv_i8_scale(float amax) {
+  const float kFloor = __uint_as_float(0x3728u << 16);   // bf16(1e-5)
+  const float kInv127 = __uint_as_float(0x3c01u << 16);  // bf16(1 / 127)
+  return round_bf16(fmaxf(amax, kFloor) * kInv127);
+}
+AXK_DEV float kv_i8_code(float x, float r) { return fminf(fmaxf(rintf(round_bf16(x * r)), -128.0f), 127.0f); }
+
 // Eight E2M1 codes times an arbitrary fp32 scale s (an NVFP4 block's E4M3 scale) -> bf16. gfx950's scaled converts
 // apply only the exponent of their scale operand (a power of two, as MX scales are), so the codes are decoded
 // exactly at scale 1 and multiplied by s in fp32: the product of an E2M1 value (at most 2 significant bits) and an

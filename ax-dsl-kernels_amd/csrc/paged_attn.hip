@@ -2204,9 +2204,7 @@ __global__ __launch_bounds__(256) void paged_kv_write_i8_kernel(const uint16_t* 
     for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[e]));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 16));
-    const float kFloor = __uint_as_float(0x3728u << 16);    // bf16(1e-5)
-    const float kInv127 = __uint_as_float(0x3c01u << 16);   // bf16(1 / 127)
-    const float s = round_bf16(fmaxf(amax, kFloor) * kInv127);
+    const float s = kv_i8_scale(amax);
     const float r = round_bf16(1.0f / s);
     uint32_t codes[E / 4];
 #pragma unroll
@@ -2214,8 +2212,7 @@ __global__ __launch_bounds__(256) void paged_kv_write_i8_kernel(const uint16_t* 
       uint32_t word = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float y = fminf(fmaxf(rintf(round_bf16(x[4 * c4 + e] * r)), -128.0f), 127.0f);
-        word |= ((uint32_t)(int)y & 0xffu) << (8 * e);
+        word |= ((uint32_t)(int)kv_i8_code(x[4 * c4 + e], r) & 0xffu) << (8 * e);
       }
       codes[c4] = word;
     }

@@ -85,14 +85,30 @@ AXK_DEV axk_s16x2 bf16_order(uint32_t w) {
 }
 AXK_DEV uint32_t bf16_unorder(axk_s16x2 x) { return __builtin_bit_cast(uint32_t, x ^ ((x >> (short)15) & (short)0x7fff)); }
 
-// 16 bytes of stored keys as bf16 pairs in order: 4 dwords of a bf16 cache, 8 of an FP8 one (stored * inv_scale).
-template <int F8>
-AXK_DEV void stored_pairs(const axk_u32x4 w, float inv_scale, uint32_t (&out)[F8 ? 8 : 4]) {
+// What a cache stores: bf16; E4M3 bytes, attended as stored * inv_scale (a power of two: exact in bf16); or int8 codes with a
+// bf16 scale per row and KV head, attended as code * scale.
+enum { kBf16 = 0, kFp8 = 1, kI8 = 2 };
+
+// Bytes 2 hi and 2 hi + 1 of w, int8 codes, as a bf16 pair of code * s.
+AXK_DEV uint32_t i8_pair(uint32_t w, int hi, float s = 1.0f) {
+  const float x = (float)(int8_t)(w >> (16 * hi)), y = (float)(int8_t)(w >> (16 * hi + 8));
+  return pack_bf16x2(x * s, y * s);
+}
+// A dword of stored 8-bit values as two bf16 pairs (int8 codes times s).
+template <int T>
+AXK_DEV uint32_t pair_of(uint32_t w, int hi, float inv_scale, float s = 1.0f) {
+  if constexpr (T == kI8) return i8_pair(w, hi, s);
+  return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, inv_scale, true)
+                                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, inv_scale, false));
+}
+// 16 bytes of stored keys as bf16 pairs in order: 4 dwords of a bf16 cache, 8 of an 8-bit one.
+template <int T>
+AXK_DEV void stored_pairs(const axk_u32x4 w, float inv_scale, float s, uint32_t (&out)[T ? 8 : 4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (F8) {
-      out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], inv_scale, false));
-      out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], inv_scale, true));
+    if constexpr (T) {
+      out[2 * i] = pair_of<T>(w[i], 0, inv_scale, s);
+      out[2 * i + 1] = pair_of<T>(w[i], 1, inv_scale, s);
     } else {
       out[i] = w[i];
     }
@@ -107,11 +123,46 @@ constexpr int64_t kMaxRows = 16384;  // every row looks at every other's place: 
 // the call that falls into a block folds all of them, so that rows of one block never race, and where two rows name one
 // slot the last one is stored (both are folded). Two launches' worth of work in one: a decode step pays a launch, the
 // dependent reads location, then row and bounds, and nothing else.
-template <int F8>
+//
+// Eight channels of a new row as the cache keeps them: their bytes (a bf16 cache: the values themselves), the int8 scale,
+// and the key's bf16 pairs as attention reads them. The d / 8 lanes of a head's row act together.
+struct Stored {
+  uint32_t lo, hi;   // 8-bit caches: the eight bytes
+  float scale;       // int8
+  uint32_t pair[4];  // as attended
+};
+template <int T>
+AXK_DEV Stored store_eight(const uint4 src, int d, float kv_scale) {
+  const uint32_t w[4] = {src.x, src.y, src.z, src.w};
+  Stored o = {0u, 0u, 0.f, {w[0], w[1], w[2], w[3]}};
+  if constexpr (T == kBf16) return o;
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(e & 1 ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
+  float r = 0.f;
+  if constexpr (T == kI8) {
+    float amax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+    for (int m = d / 16; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));  // the row's lanes: d / 8, aligned
+    o.scale = kv_i8_scale(amax);
+    r = round_bf16(1.0f / o.scale);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t c = T == kFp8 ? f32_to_e4m3(round_bf16(x[e] * kv_scale)) : ((uint32_t)(int)kv_i8_code(x[e], r) & 0xffu);
+    if (e < 4) o.lo |= c << (8 * e); else o.hi |= c << (8 * (e - 4));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o.pair[i] = pair_of<T>(i < 2 ? o.lo : o.hi, i & 1, 1.0f / kv_scale, o.scale);
+  return o;
+}
+
+template <int T>
 __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
     const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, unsigned char* __restrict__ cache,
-    uint16_t* __restrict__ bounds, const int* __restrict__ loc, int rows, int hkv, int d, int page_size, int block,
-    int64_t num_pages, float kv_scale, int* __restrict__ status) {
+    uint16_t* __restrict__ scales, uint16_t* __restrict__ bounds, const int* __restrict__ loc, int rows, int hkv, int d,
+    int page_size, int block, int64_t num_pages, float kv_scale, int* __restrict__ status) {
   __shared__ int s_rows[256];
   __shared__ int s_count, s_first, s_fresh, s_over;
   const int tid = threadIdx.x, r = blockIdx.x;
@@ -136,31 +187,24 @@ __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
     if (i > r && o == off) s_over = 1;
   }
   __syncthreads();
-  const int row = hkv * d;  // values of one token row
+  const int row = hkv * d, chunks = row / 8;  // values of one token row, and its pieces of 8 channels
   if (!s_over) {
-    for (int i = tid; i < 2 * (row / 8); i += 256) {
-      const int plane = i >= row / 8, ch = plane ? i - row / 8 : i;
+    for (int i = tid; i < 2 * chunks; i += 256) {
+      const int plane = i >= chunks, ch = plane ? i - chunks : i;
       const uint4 src = *reinterpret_cast<const uint4*>((plane ? v : k) + (int64_t)r * row + ch * 8);
-      const int64_t at = (((int64_t)page * 2 + plane) * page_size + off) * row + ch * 8;
-      if constexpr (F8) {
-        const uint32_t w[4] = {src.x, src.y, src.z, src.w};
-        uint32_t lo = 0, hi = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = __uint_as_float(e & 1 ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
-          const uint32_t c = f32_to_e4m3(round_bf16(x * kv_scale));
-          if (e < 4) lo |= c << (8 * e); else hi |= c << (8 * (e - 4));
-        }
-        *reinterpret_cast<uint2*>(cache + at) = make_uint2(lo, hi);
-      } else {
+      const int64_t slot = ((int64_t)page * 2 + plane) * page_size + off, at = slot * row + ch * 8;
+      if constexpr (T == kBf16) {
         *reinterpret_cast<uint4*>(cache + 2 * at) = src;
+      } else {
+        const Stored o = store_eight<T>(src, d, kv_scale);
+        *reinterpret_cast<uint2*>(cache + at) = make_uint2(o.lo, o.hi);
+        if (T == kI8 && ch * 8 % d == 0) scales[slot * hkv + ch * 8 / d] = (uint16_t)f32_to_bf16_bits(o.scale);
       }
     }
   }
   if (!s_first) return;
   const int fresh = s_fresh;
   uint16_t* bb = bounds + ((int64_t)page * (page_size / block) + blk) * hkv * 2 * d;
-  const float inv_scale = 1.0f / kv_scale;
   for (int base = r & ~255; base < rows; base += 256) {  // the call's rows from this one on, 256 at a time
     __syncthreads();
     if (tid == 0) s_count = 0;
@@ -172,7 +216,7 @@ __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
     }
     __syncthreads();
     const int n = s_count;
-    for (int c = tid; n && c < row / 8; c += 256) {  // 8 channels of one head at a time
+    for (int c = tid; n && c < chunks; c += 256) {  // 8 channels of one head at a time
       const int head = c * 8 / d, ch = c * 8 - head * d;
       uint16_t* lo_p = bb + (int64_t)head * 2 * d + ch;
       uint4* lo4 = reinterpret_cast<uint4*>(lo_p);
@@ -187,18 +231,11 @@ __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
         hi[e] = from ? bf16_order(hw[e]) : (axk_s16x2)(short)-0x8000;
       }
       for (int j = 0; j < n; ++j) {
-        const uint4 x4 = *reinterpret_cast<const uint4*>(k + (int64_t)s_rows[j] * row + c * 8);
-        uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
+        const Stored o = store_eight<T>(*reinterpret_cast<const uint4*>(k + (int64_t)s_rows[j] * row + c * 8), d, kv_scale);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (F8) {
-            const uint32_t c0 = f32_to_e4m3(round_bf16(__uint_as_float(x[e] << 16) * kv_scale));
-            const uint32_t c1 = f32_to_e4m3(round_bf16(__uint_as_float(x[e] & 0xffff0000u) * kv_scale));
-            x[e] = __builtin_bit_cast(uint32_t,
-                                      __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c0 | (c1 << 8), inv_scale, false));
-          }
-          lo[e] = __builtin_elementwise_min(lo[e], bf16_order(x[e]));
-          hi[e] = __builtin_elementwise_max(hi[e], bf16_order(x[e]));
+          lo[e] = __builtin_elementwise_min(lo[e], bf16_order(o.pair[e]));
+          hi[e] = __builtin_elementwise_max(hi[e], bf16_order(o.pair[e]));
         }
       }
       *lo4 = make_uint4(bf16_unorder(lo[0]), bf16_unorder(lo[1]), bf16_unorder(lo[2]), bf16_unorder(lo[3]));
@@ -209,16 +246,16 @@ __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
 
 // The bounds of every block of the page table that reaches past start[b] (all of them without start), from the cache.
 // One workgroup per block: its K rows are one contiguous run of tokens x HKV x D values, read 16 bytes a lane, a column
-// of 8 (FP8: 16) channels kept by as many lanes as the workgroup has to spare and joined through LDS. Minimum and
+// of 8 (8-bit caches: 16) channels kept by as many lanes as the workgroup has to spare and joined through LDS. Minimum and
 // maximum are taken on the bf16 bits as ordered 16-bit integers, two values an instruction. Bound by the K bytes.
-template <int F8>
+template <int T>
 __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
-    const unsigned char* __restrict__ cache, uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
+    const unsigned char* __restrict__ cache, const uint16_t* __restrict__ scales, uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
     const int* __restrict__ indices, const int* __restrict__ last, const int* __restrict__ start, int nnz, int batch,
     int hkv, int d, int page_size, int block, int64_t num_pages, float inv_scale, int* __restrict__ status) {
-  constexpr int N = F8 ? 8 : 4;      // dwords of bf16 pairs a lane keeps
+  constexpr int N = T ? 8 : 4;      // dwords of bf16 pairs a lane keeps
   constexpr int E = 2 * N;           // channels a lane keeps
-  constexpr int B = F8 ? 1 : 2;      // bytes of a stored value
+  constexpr int B = T ? 1 : 2;      // bytes of a stored value
   __shared__ __align__(16) axk_s16x2 s_lo[256 * N], s_hi[256 * N];
   const int tid = threadIdx.x;
   const int bpp = page_size / block;
@@ -236,11 +273,13 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
   }
   const int row = hkv * d;
   const int cols = row / E;  // lanes that one token row takes
-  const unsigned char* src = cache + ((int64_t)page * 2 * page_size + (int64_t)sub * block) * row * B;
+  const int64_t first = (int64_t)page * 2 * page_size + (int64_t)sub * block;  // the block's first K row
+  const unsigned char* src = cache + first * row * B;
   uint16_t* dst = bounds + ((int64_t)page * bpp + sub) * hkv * 2 * d;
   for (int c0 = 0; c0 < cols; c0 += 256) {
     const int w = min(cols - c0, 256), lanes = 256 / w;  // columns of this pass, and lanes to each
     const int rl = tid / w, c = c0 + tid - rl * w;
+    const uint16_t* sc = T == kI8 ? scales + first * hkv + (unsigned)(c * E) / (unsigned)d : nullptr;  // a lane's head
     axk_s16x2 lo[N], hi[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -251,7 +290,8 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
 #pragma unroll 4
       for (int t = rl; t < rows; t += lanes) {
         uint32_t x[N];
-        stored_pairs<F8>(*reinterpret_cast<const axk_u32x4*>(src + ((int64_t)t * row + c * E) * B), inv_scale, x);
+        const float s = T == kI8 ? bf16_bits_to_f32(sc[(int64_t)t * hkv]) : 1.0f;
+        stored_pairs<T>(*reinterpret_cast<const axk_u32x4*>(src + ((int64_t)t * row + c * E) * B), inv_scale, s, x);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           lo[e] = __builtin_elementwise_min(lo[e], bf16_order(x[e]));
@@ -590,15 +630,15 @@ __global__ __launch_bounds__(T) void paged_select_blocks_kernel(const float* __r
 //                 4 g + j % 4 of subtile j / 4. V rows are loaded in that order, lane l16 holding D / 16 channels of eight
 //                 tokens, so that the transposition V^T needs is one byte permute per two values, without LDS.
 // The four waves of a piece take its steps in turn and are joined through LDS; pieces by the merge kernel.
-template <int D, int F8>
+template <int D, int T>
 struct BlkCfg {
-  static constexpr int B = F8 ? 1 : 2;             // bytes of a stored value
+  static constexpr int B = T ? 1 : 2;              // bytes of a stored value
   static constexpr int RB = D * B;                 // bytes of a token's row of one head
   static constexpr int CR = RB / 16;               // ... in 16-byte chunks
   static constexpr int KI = 32 * RB / 1024;        // direct-to-LDS loads (64 lanes x 16 bytes) of a step's K
   static constexpr int KL = RB / 64;               // 16-byte K fragments a lane reads per subtile
   static constexpr int KS = D / 32;                // QK k-steps
-  static constexpr int E = F8 ? D / 16 : (D >= 128 ? 8 : D / 16);  // channels of a V load
+  static constexpr int E = T ? D / 16 : (D >= 128 ? 8 : D / 16);  // channels of a V load
   static constexpr int NH = D / 16 / E;            // V loads a lane makes per token
   static constexpr int VW = E * B / 4;             // dwords of a V load
   static constexpr int ACC = D / 16;               // 16x16 O^T tiles
@@ -613,6 +653,7 @@ struct BlkCfg {
 struct BlkArgs {
   const uint16_t* q;
   const unsigned char* cache;
+  const uint16_t* kv_scales;  // of an int8 cache
   const int *indptr, *indices, *last;
   const int* blocks;  // [batch, hkv, n], or null: every block
   int n, block;
@@ -679,14 +720,19 @@ AXK_DEV bool bad_block(int id, int prev, int nblocks) {
   return id < -1 || id >= nblocks || (id >= 0 && prev >= id);
 }
 
+// A wave-uniform 64-bit value in scalar registers.
+AXK_DEV int64_t uniform_i64(int64_t x) {
+  return (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+
 constexpr int kMaxPs = 128;  // subtiles of a piece, at most (two a lane)
 
-template <int D, int F8>
+template <int D, int T>
 __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
-  using C = BlkCfg<D, F8>;
+  using C = BlkCfg<D, T>;
   constexpr int Q = C::Q;
   extern __shared__ __align__(1024) unsigned char s_k[];  // C::LDS bytes
-  __shared__ int64_t s_base[kMaxPs];
+  __shared__ int64_t s_row[kMaxPs];
   __shared__ int s_valid[kMaxPs];
   __shared__ float s_m[4][16], s_l[4][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
@@ -722,7 +768,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   axk_bf16x8 qf[C::KS];
 #pragma unroll
   for (int i = 0; i < C::KS; ++i) {
-    const int at = F8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
+    const int at = T ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
     qf[i] = l16 < group ? load_bf16x8(a.q + ((int64_t)b * a.hq + h * group + l16) * D + at) : zero_bf16x8();
   }
   // the piece's subtiles: where each lies in the cache, and how many of its tokens count
@@ -748,12 +794,12 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
           bad = true;
           valid = 0;
         } else {
-          base = ((int64_t)page * 2 * a.page + (at - p * spp) * kSub) * rowb;
+          base = (int64_t)page * 2 * a.page + (at - p * spp) * kSub;
         }
       }
       if (bad && a.status) *a.status = 1;
     }
-    s_base[tid] = base;
+    s_row[tid] = base;
     s_valid[tid] = valid;
   }
   __syncthreads();
@@ -770,7 +816,6 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   for (int i = 0; i < C::ACC; ++i) acc[i] = (axk_f32x4){0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   const unsigned char* cache_h = a.cache + (int64_t)h * D * C::B;
-  const int64_t vplane = (int64_t)a.page * rowb;
   const uint32_t v_off = (uint32_t)(4 * g * rowb + l16 * C::E * C::B);
   typedef uint32_t vload __attribute__((ext_vector_type(C::VW)));
   // K of step t to this wave's buffer, whole rows an instruction (a fragment's 64 bytes of 16 rows, straight to registers,
@@ -780,7 +825,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   auto load_k = [&](int t) {
     const unsigned char* sub[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) sub[u] = static_cast<const unsigned char*>(uniform_ptr(cache_h + s_base[2 * t + u]));
+    for (int u = 0; u < 2; ++u) sub[u] = cache_h + uniform_i64(s_row[2 * t + u]) * rowb;
 #pragma unroll
     for (int i = 0; i < C::KI; ++i) {
       const int r = (i * kRows + lane / C::CR) % kSub;  // of its subtile
@@ -797,7 +842,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
     vload vr[8][C::NH];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const unsigned char* p = static_cast<const unsigned char*>(uniform_ptr(cache_h + s_base[2 * t + u] + vplane));
+      const unsigned char* p = cache_h + (uniform_i64(s_row[2 * t + u]) + a.page) * rowb;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -805,21 +850,35 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
           vr[4 * u + j][n] = __builtin_nontemporal_load(
               reinterpret_cast<const vload*>(p + v_off + j * (uint32_t)rowb + n * 16 * C::E * C::B));
     }
+    // int8: lane (plane, subtile, token) loads one scale, zero where the token does not count
+    float ks[8], vs[8], own = 0.f;
+    if constexpr (T == kI8) {
+      const int u = g & 1, plane = g >> 1;
+      if (l16 < (u ? nv1 : nv0))
+        own = bf16_bits_to_f32(a.kv_scales[(s_row[2 * t + u] + plane * a.page + l16) * a.hkv + h]);
+    }
     // This step's K has landed in LDS (the compiler waits for registers only), and its V, which costs nothing: the other
     // waves' loads keep the memory busy.
     wait_vmcnt<0>();
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (T == kI8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {  // the scales of this lane's tokens: 4 g + j % 4 of subtile j / 4
+        ks[j] = __shfl(own, (j >> 2) * 16 + 4 * g + (j & 3), 64);
+        vs[j] = __shfl(own, 32 + (j >> 2) * 16 + 4 * g + (j & 3), 64);
+      }
+    }
     axk_f32x4 sc[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       sc[u] = (axk_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < C::KL; ++i) {
-        uint32_t x[F8 ? 8 : 4];
-        stored_pairs<F8>(*reinterpret_cast<const axk_u32x4*>(kbuf + u * kSub * C::RB + (k_at ^ (64 * i))), a.inv_scale, x);
+        uint32_t x[T ? 8 : 4];
+        stored_pairs<T>(*reinterpret_cast<const axk_u32x4*>(kbuf + u * kSub * C::RB + (k_at ^ (64 * i))), a.inv_scale, 1.0f, x);
         const axk_u32x4 x0 = {x[0], x[1], x[2], x[3]};
-        sc[u] = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, x0), qf[F8 ? 2 * i : i], sc[u]);
-        if constexpr (F8) {
+        sc[u] = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, x0), qf[T ? 2 * i : i], sc[u]);
+        if constexpr (T != kBf16) {
           const axk_u32x4 x1 = {x[4], x[5], x[6], x[7]};
           sc[u] = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, x1), qf[2 * i + 1], sc[u]);
         }
@@ -832,6 +891,10 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if constexpr (T == kI8) {
+        sc[0][i] *= ks[i];
+        sc[1][i] *= ks[4 + i];
+      }
       x[i] = 4 * g + i < nv0 ? sc[0][i] * a.scale : -INFINITY;
       x[4 + i] = 4 * g + i < nv1 ? sc[1][i] * a.scale : -INFINITY;
     }
@@ -853,6 +916,10 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
 #pragma unroll
       for (int i = 0; i < C::ACC; ++i) acc[i] *= alpha;
     }
+    if constexpr (T == kI8) {  // V's scales go with the probabilities
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= vs[i];
+    }
     const axk_u32x4 pw = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
                           pack_bf16x2(x[6], x[7])};
     const axk_bf16x8 pf = __builtin_bit_cast(axk_bf16x8, pw);
@@ -868,7 +935,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
 #pragma unroll
       for (int w = 0; w < C::VW; ++w) {
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (F8) {
+        if constexpr (T != kBf16) {
           uint32_t lo[4], hi[4];  // bytes (c, c + 1) of token pairs: [t.c, t'.c, t.c+1, t'.c+1]
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
@@ -880,9 +947,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
             axk_u32x4 f;
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-              const uint32_t src = e < 2 ? lo[p] : hi[p];
-              f[p] = __builtin_bit_cast(uint32_t, e & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, a.inv_scale, true)
-                                                        : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, a.inv_scale, false));
+              f[p] = pair_of<T>(e < 2 ? lo[p] : hi[p], e & 1, a.inv_scale);
             }
             axk_f32x4& o = acc[n * C::E + 4 * w + e];
             o = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, f), pf, o);
@@ -1307,13 +1372,13 @@ int check_blocks(int64_t batch, int64_t hkv, int64_t d, int64_t page_size, int64
   return AXK_OK;
 }
 
-// The stored type of a cache: 0 bf16, 1 FP8 E4M3 with a power-of-two scale; negative: refused.
+// The stored type of a cache by its dtype code (kBf16 or kFp8, the latter with a power-of-two scale); negative: refused.
 int cache_type(int kv_dtype, float kv_scale) {
-  if (kv_dtype == AXK_DT_BF16) return 0;
+  if (kv_dtype == AXK_DT_BF16) return kBf16;
   if (kv_dtype != AXK_DT_FP8E4M3) return -AXK_E_DTYPE;
   int e = 0;
   const float m = frexpf(kv_scale, &e);
-  return kv_scale > 0.f && m == 0.5f && e >= -125 && e <= 126 ? 1 : -AXK_E_SHAPE;
+  return kv_scale > 0.f && m == 0.5f && e >= -125 && e <= 126 ? kFp8 : -AXK_E_SHAPE;
 }
 
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -1347,10 +1412,11 @@ BlkPlan blk_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t page
 }
 
 template <int D>
-int launch_blocks(const BlkArgs& a, const WeightArgs& w, int f8, hipStream_t st) {
+int launch_blocks(const BlkArgs& a, const WeightArgs& w, int type, hipStream_t st) {
   const dim3 grid = a.blocks ? dim3((unsigned)(a.batch * a.hkv * a.pieces)) : dim3((unsigned)a.pieces, (unsigned)a.hkv);
-  if (f8) hipLaunchKernelGGL((paged_blocks_kernel<D, 1>), grid, dim3(256), (BlkCfg<D, 1>::LDS), st, a);
-  else hipLaunchKernelGGL((paged_blocks_kernel<D, 0>), grid, dim3(256), (BlkCfg<D, 0>::LDS), st, a);
+  if (type == kI8) hipLaunchKernelGGL((paged_blocks_kernel<D, kI8>), grid, dim3(256), (BlkCfg<D, kI8>::LDS), st, a);
+  else if (type == kFp8) hipLaunchKernelGGL((paged_blocks_kernel<D, kFp8>), grid, dim3(256), (BlkCfg<D, kFp8>::LDS), st, a);
+  else hipLaunchKernelGGL((paged_blocks_kernel<D, kBf16>), grid, dim3(256), (BlkCfg<D, kBf16>::LDS), st, a);
   if (!a.direct) {
     const int64_t wgs = (int64_t)a.batch * a.hkv * w.split + (w.out ? (a.blocks ? (int64_t)a.batch : a.pieces) * a.hkv : 0);
     hipLaunchKernelGGL((paged_blocks_merge_kernel<D>), dim3((unsigned)wgs), dim3(256), 0, st, a, w);
@@ -1360,32 +1426,83 @@ int launch_blocks(const BlkArgs& a, const WeightArgs& w, int f8, hipStream_t st)
 
 }  // namespace
 
+namespace {
+
+int kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cache, int type, float kv_scale, uint16_t* kv_scales,
+                    uint16_t* bounds, const int32_t* loc, int64_t rows, int64_t hkv, int64_t d, int64_t page_size,
+                    int64_t block_size, int64_t num_pages, int32_t* status, axk_stream_t stream) {
+  AXK_REQUIRE(k && v && kv_cache && bounds && loc && (kv_scales || type != kI8), AXK_E_NULL);
+  const int rc = check_blocks(1, hkv, d, page_size, block_size, num_pages, 0);
+  if (rc != AXK_OK) return rc;
+  AXK_REQUIRE(rows >= 0 && rows <= kMaxRows, AXK_E_SHAPE);
+  if (type < 0) return -type;
+  AXK_REQUIRE(axk_aligned(k, 16) && axk_aligned(v, 16) && axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16) &&
+                  axk_aligned(kv_scales, 2),
+              AXK_E_ALIGN);
+  const size_t row = (size_t)hkv * d, slots = (size_t)num_pages * page_size * 2;
+  const struct {
+    const void* p;
+    size_t n;
+  } out[3] = {{kv_cache, slots * row * (type ? 1 : 2)}, {bounds, (size_t)num_pages * (page_size / block_size) * row * 4},
+              {kv_scales, slots * hkv * 2}};
+  for (int i = 0; i < 3; ++i) {
+    AXK_REQUIRE(!axk_overlap(out[i].p, out[i].n, k, rows * row * 2) && !axk_overlap(out[i].p, out[i].n, v, rows * row * 2),
+                AXK_E_ALIAS);
+    for (int j = 0; j < i; ++j) AXK_REQUIRE(!axk_overlap(out[i].p, out[i].n, out[j].p, out[j].n), AXK_E_ALIAS);
+  }
+  if (rows == 0) return AXK_OK;
+  AXK_LAUNCH_GATE();
+  auto* fn = type == kI8 ? &paged_kv_write_bounds_kernel<kI8>
+                         : type == kFp8 ? &paged_kv_write_bounds_kernel<kFp8> : &paged_kv_write_bounds_kernel<kBf16>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)rows), dim3(256), 0, axk_stream(stream), k, v,
+                     static_cast<unsigned char*>(kv_cache), kv_scales, bounds, loc, (int)rows, (int)hkv, (int)d,
+                     (int)page_size, (int)block_size, num_pages, type == kFp8 ? kv_scale : 1.0f, status);
+  return axk_launch_status();
+}
+
+int key_bounds(const void* kv_cache, int type, float kv_scale, const uint16_t* kv_scales, uint16_t* bounds,
+               const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len, const int32_t* start,
+               int64_t nnz, int64_t batch, int64_t hkv, int64_t d, int64_t page_size, int64_t block_size,
+               int64_t num_pages, int32_t* status, axk_stream_t stream) {
+  AXK_REQUIRE(kv_cache && bounds && indptr && (indices || nnz == 0) && last_page_len && (kv_scales || type != kI8),
+              AXK_E_NULL);
+  const int rc = check_blocks(batch, hkv, d, page_size, block_size, num_pages, nnz);
+  if (rc != AXK_OK) return rc;
+  if (type < 0) return -type;
+  AXK_REQUIRE(axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16) && axk_aligned(kv_scales, 2), AXK_E_ALIGN);
+  const size_t row = (size_t)hkv * d, slots = (size_t)num_pages * page_size * 2;
+  const size_t bb = (size_t)num_pages * (page_size / block_size) * row * 4;
+  AXK_REQUIRE(!axk_overlap(bounds, bb, kv_cache, slots * row * (type ? 1 : 2)) &&
+                  !axk_overlap(bounds, bb, kv_scales, slots * hkv * 2),
+              AXK_E_ALIAS);
+  if (nnz == 0) return AXK_OK;
+  AXK_LAUNCH_GATE();
+  auto* fn = type == kI8 ? &paged_key_bounds_kernel<kI8>
+                         : type == kFp8 ? &paged_key_bounds_kernel<kFp8> : &paged_key_bounds_kernel<kBf16>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)(nnz * (page_size / block_size))), dim3(256), 0, axk_stream(stream),
+                     static_cast<const unsigned char*>(kv_cache), kv_scales, bounds, indptr, indices, last_page_len, start,
+                     (int)nnz, (int)batch, (int)hkv, (int)d, (int)page_size, (int)block_size, num_pages,
+                     type == kFp8 ? 1.0f / kv_scale : 1.0f, status);
+  return axk_launch_status();
+}
+
+}  // namespace
+
 extern "C" int axk_paged_kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cache, int kv_dtype,
                                          float kv_scale, uint16_t* bounds, const int32_t* cache_location, int64_t rows,
                                          int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t block_size,
                                          int64_t num_pages, int32_t* status, axk_stream_t stream) {
-  AXK_REQUIRE(k && v && kv_cache && bounds && cache_location, AXK_E_NULL);
-  const int rc = check_blocks(1, num_kv_heads, head_dim, page_size, block_size, num_pages, 0);
-  if (rc != AXK_OK) return rc;
-  AXK_REQUIRE(rows >= 0 && rows <= kMaxRows, AXK_E_SHAPE);
-  const int f8 = cache_type(kv_dtype, kv_scale);
-  if (f8 < 0) return -f8;
-  AXK_REQUIRE(axk_aligned(k, 16) && axk_aligned(v, 16) && axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16),
-              AXK_E_ALIGN);
-  const size_t row = (size_t)num_kv_heads * head_dim * 2, in = (size_t)rows * row;
-  const size_t cache = (size_t)num_pages * page_size * row * 2 / (f8 ? 2 : 1);
-  const size_t bb = (size_t)num_pages * (page_size / block_size) * row * 2;
-  AXK_REQUIRE(!axk_overlap(bounds, bb, kv_cache, cache) && !axk_overlap(bounds, bb, k, in) &&
-                  !axk_overlap(bounds, bb, v, in) && !axk_overlap(kv_cache, cache, k, in) &&
-                  !axk_overlap(kv_cache, cache, v, in),
-              AXK_E_ALIAS);
-  if (rows == 0) return AXK_OK;
-  AXK_LAUNCH_GATE();
-  auto* fn = f8 ? &paged_kv_write_bounds_kernel<1> : &paged_kv_write_bounds_kernel<0>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)rows), dim3(256), 0, axk_stream(stream), k, v,
-                     static_cast<unsigned char*>(kv_cache), bounds, cache_location, (int)rows, (int)num_kv_heads,
-                     (int)head_dim, (int)page_size, (int)block_size, num_pages, f8 ? kv_scale : 1.0f, status);
-  return axk_launch_status();
+  return kv_write_bounds(k, v, kv_cache, cache_type(kv_dtype, kv_scale), kv_scale, nullptr, bounds, cache_location, rows,
+                         num_kv_heads, head_dim, page_size, block_size, num_pages, status, stream);
+}
+
+extern "C" int axk_paged_kv_write_bounds_i8(const uint16_t* k, const uint16_t* v, int8_t* kv_cache, uint16_t* kv_scales,
+                                            uint16_t* bounds, const int32_t* cache_location, int64_t rows,
+                                            int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                            int64_t block_size, int64_t num_pages, int32_t* status,
+                                            axk_stream_t stream) {
+  return kv_write_bounds(k, v, kv_cache, kI8, 1.0f, kv_scales, bounds, cache_location, rows, num_kv_heads, head_dim,
+                         page_size, block_size, num_pages, status, stream);
 }
 
 extern "C" int axk_paged_key_bounds(const void* kv_cache, int kv_dtype, float kv_scale, uint16_t* bounds,
@@ -1393,24 +1510,17 @@ extern "C" int axk_paged_key_bounds(const void* kv_cache, int kv_dtype, float kv
                                     const int32_t* start, int64_t nnz, int64_t batch, int64_t num_kv_heads,
                                     int64_t head_dim, int64_t page_size, int64_t block_size, int64_t num_pages,
                                     int32_t* status, axk_stream_t stream) {
-  AXK_REQUIRE(kv_cache && bounds && indptr && (indices || nnz == 0) && last_page_len, AXK_E_NULL);
-  const int rc = check_blocks(batch, num_kv_heads, head_dim, page_size, block_size, num_pages, nnz);
-  if (rc != AXK_OK) return rc;
-  const int f8 = cache_type(kv_dtype, kv_scale);
-  if (f8 < 0) return -f8;
-  AXK_REQUIRE(axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16), AXK_E_ALIGN);
-  const size_t row = (size_t)num_kv_heads * head_dim * 2;
-  AXK_REQUIRE(!axk_overlap(bounds, (size_t)num_pages * (page_size / block_size) * row * 2, kv_cache,
-                           (size_t)num_pages * page_size * row * 2 / (f8 ? 2 : 1)),
-              AXK_E_ALIAS);
-  if (nnz == 0) return AXK_OK;
-  AXK_LAUNCH_GATE();
-  auto* fn = f8 ? &paged_key_bounds_kernel<1> : &paged_key_bounds_kernel<0>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)(nnz * (page_size / block_size))), dim3(256), 0, axk_stream(stream),
-                     static_cast<const unsigned char*>(kv_cache), bounds, indptr, indices, last_page_len, start, (int)nnz,
-                     (int)batch, (int)num_kv_heads, (int)head_dim, (int)page_size, (int)block_size, num_pages,
-                     f8 ? 1.0f / kv_scale : 1.0f, status);
-  return axk_launch_status();
+  return key_bounds(kv_cache, cache_type(kv_dtype, kv_scale), kv_scale, nullptr, bounds, indptr, indices, last_page_len,
+                    start, nnz, batch, num_kv_heads, head_dim, page_size, block_size, num_pages, status, stream);
+}
+
+extern "C" int axk_paged_key_bounds_i8(const int8_t* kv_cache, const uint16_t* kv_scales, uint16_t* bounds,
+                                       const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len,
+                                       const int32_t* start, int64_t nnz, int64_t batch, int64_t num_kv_heads,
+                                       int64_t head_dim, int64_t page_size, int64_t block_size, int64_t num_pages,
+                                       int32_t* status, axk_stream_t stream) {
+  return key_bounds(kv_cache, kI8, 1.0f, kv_scales, bounds, indptr, indices, last_page_len, start, nnz, batch,
+                    num_kv_heads, head_dim, page_size, block_size, num_pages, status, stream);
 }
 
 extern "C" int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds, const int32_t* indptr,
@@ -1479,14 +1589,16 @@ extern "C" size_t axk_paged_decode_blocks_workspace_size(int64_t batch, int64_t 
   return p.ml + p.po + p.stat;
 }
 
-extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, int kv_dtype, float kv_scale,
-                                       const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len,
-                                       const int32_t* blocks, int64_t block_size, int64_t num_select, uint16_t* out,
-                                       const float* weights_in, float* weights_out, float decay, int64_t nnz,
-                                       int64_t batch, int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim,
-                                       int64_t page_size, int64_t num_pages, float sm_scale, int32_t* status,
-                                       void* workspace, size_t workspace_bytes, axk_stream_t stream) {
-  AXK_REQUIRE(q && kv_cache && indptr && (indices || nnz == 0) && last_page_len && out, AXK_E_NULL);
+namespace {
+
+int decode_blocks(const uint16_t* q, const void* kv_cache, int type, float kv_scale, const uint16_t* kv_scales,
+                  const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len, const int32_t* blocks,
+                  int64_t block_size, int64_t num_select, uint16_t* out, const float* weights_in, float* weights_out,
+                  float decay, int64_t nnz, int64_t batch, int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim,
+                  int64_t page_size, int64_t num_pages, float sm_scale, int32_t* status, void* workspace,
+                  size_t workspace_bytes, axk_stream_t stream) {
+  AXK_REQUIRE(q && kv_cache && indptr && (indices || nnz == 0) && last_page_len && out && (kv_scales || type != kI8),
+              AXK_E_NULL);
   if (!blocks) {
     AXK_REQUIRE(num_select == 0, AXK_E_NULL);
     block_size = kSub;
@@ -1498,10 +1610,9 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
   AXK_REQUIRE(num_qo_heads > 0 && num_qo_heads % num_kv_heads == 0 && num_qo_heads / num_kv_heads <= kMaxGroup, AXK_E_SHAPE);
   AXK_REQUIRE(num_select <= kMaxSubs && num_select * (block_size / kSub) <= kMaxSubs, AXK_E_SHAPE);
   AXK_REQUIRE(!weights_in || weights_out, AXK_E_NULL);
-  const int f8 = cache_type(kv_dtype, kv_scale);
-  if (f8 < 0) return -f8;
+  if (type < 0) return -type;
   AXK_REQUIRE(axk_aligned(q, 16) && axk_aligned(kv_cache, 16) && axk_aligned(out, 8) && axk_aligned(weights_in, 4) &&
-                  axk_aligned(weights_out, 4) && axk_aligned(blocks, 4),
+                  axk_aligned(weights_out, 4) && axk_aligned(blocks, 4) && axk_aligned(kv_scales, 2),
               AXK_E_ALIGN);
   const bool weights = weights_out && nnz > 0;
   const BlkPlan p = blk_plan(batch, num_qo_heads, num_kv_heads, head_dim, page_size, nnz, block_size, num_select, weights);
@@ -1512,7 +1623,7 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
   const int64_t wgs = batch * num_kv_heads * split + (weights ? (blocks ? batch : (int64_t)p.pieces) * num_kv_heads : 0);
   AXK_REQUIRE(grid <= 0x7fffffff && wgs <= 0x7fffffff, AXK_E_SHAPE);
   const size_t qb = (size_t)batch * num_qo_heads * head_dim * 2, wb = (size_t)num_kv_heads * nnz * 4;
-  const size_t cache = (size_t)num_pages * page_size * num_kv_heads * head_dim * (f8 ? 2 : 4);
+  const size_t cache = (size_t)num_pages * page_size * num_kv_heads * head_dim * (type ? 2 : 4);
   AXK_REQUIRE(!axk_overlap(out, qb, q, qb) && !axk_overlap(out, qb, kv_cache, cache) && !axk_overlap(out, qb, workspace, need) &&
                   !axk_overlap(q, qb, workspace, need) && !axk_overlap(kv_cache, cache, workspace, need),
               AXK_E_ALIAS);
@@ -1536,8 +1647,9 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
   a.hkv = (int)num_kv_heads;
   a.page = (int)page_size;
   a.num_pages = num_pages;
+  a.kv_scales = kv_scales;
   a.scale = sm_scale * kLog2e;
-  a.inv_scale = f8 ? 1.0f / kv_scale : 1.0f;
+  a.inv_scale = type == kFp8 ? 1.0f / kv_scale : 1.0f;
   a.ps = p.ps;
   a.pieces = p.pieces;
   a.direct = p.direct;
@@ -1547,21 +1659,47 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
   a.po = p.direct ? nullptr : reinterpret_cast<float*>(ws + p.ml);
   a.stat = weights ? reinterpret_cast<float2*>(ws + p.ml + p.po) : nullptr;
   a.status = status;
-  if (head_dim == 256 && !f8) {  // 64 KiB of dynamic LDS beside the static: to be allowed once on each device
+  if (head_dim == 256 && type == kBf16) {  // 64 KiB of dynamic LDS beside the static: to be allowed once on each device
     static AxkOnce once[64];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return AXK_E_LAUNCH;
-    if (const int e = axk_raise_lds(once[dev & 63], reinterpret_cast<const void*>(&paged_blocks_kernel<256, 0>),
-                                    BlkCfg<256, 0>::LDS))
+    if (const int e = axk_raise_lds(once[dev & 63], reinterpret_cast<const void*>(&paged_blocks_kernel<256, kBf16>),
+                                    BlkCfg<256, kBf16>::LDS))
       return e;
   }
   const WeightArgs w = {weights_in, weights ? weights_out : nullptr, decay, split};
   AXK_LAUNCH_GATE();
   switch (head_dim) {
-    case 64: return launch_blocks<64>(a, w, f8, axk_stream(stream));
-    case 128: return launch_blocks<128>(a, w, f8, axk_stream(stream));
-    default: return launch_blocks<256>(a, w, f8, axk_stream(stream));
+    case 64: return launch_blocks<64>(a, w, type, axk_stream(stream));
+    case 128: return launch_blocks<128>(a, w, type, axk_stream(stream));
+    default: return launch_blocks<256>(a, w, type, axk_stream(stream));
   }
+}
+
+}  // namespace
+
+extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, int kv_dtype, float kv_scale,
+                                       const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len,
+                                       const int32_t* blocks, int64_t block_size, int64_t num_select, uint16_t* out,
+                                       const float* weights_in, float* weights_out, float decay, int64_t nnz,
+                                       int64_t batch, int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim,
+                                       int64_t page_size, int64_t num_pages, float sm_scale, int32_t* status,
+                                       void* workspace, size_t workspace_bytes, axk_stream_t stream) {
+  return decode_blocks(q, kv_cache, cache_type(kv_dtype, kv_scale), kv_scale, nullptr, indptr, indices, last_page_len,
+                       blocks, block_size, num_select, out, weights_in, weights_out, decay, nnz, batch, num_qo_heads,
+                       num_kv_heads, head_dim, page_size, num_pages, sm_scale, status, workspace, workspace_bytes, stream);
+}
+
+extern "C" int axk_paged_decode_blocks_i8(const uint16_t* q, const int8_t* kv_cache, const uint16_t* kv_scales,
+                                          const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len,
+                                          const int32_t* blocks, int64_t block_size, int64_t num_select, uint16_t* out,
+                                          const float* weights_in, float* weights_out, float decay, int64_t nnz,
+                                          int64_t batch, int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim,
+                                          int64_t page_size, int64_t num_pages, float sm_scale, int32_t* status,
+                                          void* workspace, size_t workspace_bytes, axk_stream_t stream) {
+  return decode_blocks(q, kv_cache, kI8, 1.0f, kv_scales, indptr, indices, last_page_len, blocks, block_size, num_select,
+                       out, weights_in, weights_out, decay, nnz, batch, num_qo_heads, num_kv_heads, head_dim, page_size,
+                       num_pages, sm_scale, status, workspace, workspace_bytes, stream);
 }
 
 extern "C" int axk_paged_evict_pages(const float* weights, const int32_t* indptr, const int32_t* indices,

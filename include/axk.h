@@ -385,7 +385,8 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  *
  * Cache, page table and page size as axk_paged_decode; head_dim 64, 128 or 256; num_qo_heads / num_kv_heads <= 16;
  * num_kv_heads <= 4096. kv_dtype: AXK_DT_BF16, or AXK_DT_FP8E4M3 for a cache of axk_paged_kv_write_fp8 with its kv_scale
- * (a power of two; ignored for bf16). nnz: the entries of indices; offsets of indptr past it are read as nnz and a
+ * (a power of two; ignored for bf16). The entries ending in _i8 take the int8 cache and bf16 scales of
+ * axk_paged_kv_write_i8, read as code * scale (head_dim 64 too). nnz: the entries of indices; offsets of indptr past it are read as nnz and a
  * last_page_len past page_size as page_size, so that no access leaves an array; nnz * page_size / 16 <= 2^30. A page id
  * outside [0, num_pages) is skipped, never read, and sets *status (device i32, or NULL) to 1. An array per page-table entry
  * is [num_kv_heads, nnz], one per block [num_kv_heads, nnz * page_size / block_size]: entry e's blocks at e *
@@ -403,6 +404,10 @@ int axk_paged_kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cac
                               uint16_t* bounds, const int32_t* cache_location, int64_t rows, int64_t num_kv_heads,
                               int64_t head_dim, int64_t page_size, int64_t block_size, int64_t num_pages,
                               int32_t* status, axk_stream_t stream);
+int axk_paged_kv_write_bounds_i8(const uint16_t* k, const uint16_t* v, int8_t* kv_cache, uint16_t* kv_scales,
+                                 uint16_t* bounds, const int32_t* cache_location, int64_t rows, int64_t num_kv_heads,
+                                 int64_t head_dim, int64_t page_size, int64_t block_size, int64_t num_pages,
+                                 int32_t* status, axk_stream_t stream);
 
 /* The bounds computed from the cache, for the blocks of each sequence that hold a token at or after start[b] (i32
  * [batch]; NULL: all blocks): after a prefill chunk that began at position start[b], or for a cache that came without
@@ -412,6 +417,10 @@ int axk_paged_key_bounds(const void* kv_cache, int kv_dtype, float kv_scale, uin
                          const int32_t* indices, const int32_t* last_page_len, const int32_t* start, int64_t nnz,
                          int64_t batch, int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t block_size,
                          int64_t num_pages, int32_t* status, axk_stream_t stream);
+int axk_paged_key_bounds_i8(const int8_t* kv_cache, const uint16_t* kv_scales, uint16_t* bounds, const int32_t* indptr,
+                            const int32_t* indices, const int32_t* last_page_len, const int32_t* start, int64_t nnz,
+                            int64_t batch, int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t block_size,
+                            int64_t num_pages, int32_t* status, axk_stream_t stream);
 
 /* scores f32 [num_kv_heads, nnz * page_size / block_size]: for q bf16 [batch, num_qo_heads, head_dim], entry (h, j) is
  *   max over the query heads g of KV head h of sum_d max(q_gd, 0) hi_jd + min(q_gd, 0) lo_jd,
@@ -450,6 +459,13 @@ int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, int kv_dtyp
                             int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
                             int64_t num_pages, float sm_scale, int32_t* status, void* workspace, size_t workspace_bytes,
                             axk_stream_t stream);
+int axk_paged_decode_blocks_i8(const uint16_t* q, const int8_t* kv_cache, const uint16_t* kv_scales,
+                               const int32_t* indptr, const int32_t* indices, const int32_t* last_page_len,
+                               const int32_t* blocks, int64_t block_size, int64_t num_select, uint16_t* out,
+                               const float* weights_in, float* weights_out, float decay, int64_t nnz, int64_t batch,
+                               int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                               int64_t num_pages, float sm_scale, int32_t* status, void* workspace,
+                               size_t workspace_bytes, axk_stream_t stream);
 
 /* The page table without the pages of least weight: of each sequence with more than `budget` pages, the `budget` pages
  * with the largest weights f32 [num_kv_heads, nnz] (summed over the KV heads in 64 bits; equal sums by the lowest place;

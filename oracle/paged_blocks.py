@@ -11,11 +11,14 @@ import math
 
 import torch
 
-from .paged_attn import seq_lens
+from .paged_attn import quant_kv_i8, seq_lens
 
 
 def attended(x: torch.Tensor, kv_scale=None) -> torch.Tensor:
-    """Stored cache values as attention reads them, in 64 bits."""
+    """Stored cache values as attention reads them, in 64 bits. kv_scale: None for bf16, the static scale of FP8 bytes, or
+    the scales of int8 codes, one per row of the last dimension."""
+    if isinstance(kv_scale, torch.Tensor):
+        return x.double() * kv_scale.double()[..., None]
     return x.double() if kv_scale is None else x.view(torch.float8_e4m3fn).double() / kv_scale
 
 
@@ -25,7 +28,9 @@ def seq_rows(cache, indptr, indices, last, b: int, kv_scale=None):
     n = seq_lens(indptr, last, page)[b]
     ids = indices[int(indptr[b]):int(indptr[b + 1])].long()
     good = (ids >= 0) & (ids < p)
-    kv = attended(cache[torch.where(good, ids, 0)], kv_scale).transpose(0, 1).reshape(2, -1, hkv, d)[:, :n]
+    at = torch.where(good, ids, 0)
+    kv = attended(cache[at], kv_scale[at] if isinstance(kv_scale, torch.Tensor) else kv_scale)
+    kv = kv.transpose(0, 1).reshape(2, -1, hkv, d)[:, :n]
     return kv[0], kv[1], good.repeat_interleave(page)[:n]
 
 
@@ -46,7 +51,7 @@ def key_bounds(cache, bounds, indptr, indices, last, start=None, kv_scale=None) 
 
 
 def store(k, v, cache, bounds, loc, kv_scale=None):
-    """(cache, bounds) after the rows are written in order."""
+    """(cache, bounds) after the rows are written in order; an int8 cache's scales, kv_scale, are written in place."""
     cache, out = cache.clone(), bounds.double()
     p, _, page = cache.shape[:3]
     block = page // bounds.shape[1]
@@ -55,12 +60,15 @@ def store(k, v, cache, bounds, loc, kv_scale=None):
     begun = set()
     for r, a, o in good:
         for i, x in enumerate((k, v)):
-            row = x[r]
-            if kv_scale is not None:
+            row, s = x[r], kv_scale
+            if isinstance(kv_scale, torch.Tensor):
+                row, s = quant_kv_i8(row)
+                kv_scale[a, i, o] = s
+            elif kv_scale is not None:
                 row = (row.float() * kv_scale).to(torch.bfloat16).to(torch.float8_e4m3fn).view(torch.uint8)
             cache[a, i, o] = row
             if i == 0:
-                key = attended(row, kv_scale)
+                key = attended(row, s).to(torch.bfloat16).double()
         at = (a, o // block)
         if at in fresh and at not in begun:
             out[at] = torch.stack([key, key], 1)

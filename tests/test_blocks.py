@@ -50,7 +50,27 @@ def evict(w=at(1), ptr=at(2), idx=at(3), optr=at(4), oidx=at(5), ow=at(6), freed
                                              None)
 
 
+def write_i8(cache=at(16), scales=at(24), bounds=at(3), rows=2, d=64, hkv=2):
+    return _lib.load().axk_paged_kv_write_bounds_i8(at(1), at(2), cache, scales, bounds, at(4), rows, hkv, d, 32, 16, 8, None,
+                                                    None)
+
+
+def bounds_i8(scales=at(24), bounds=at(3), d=64):
+    return _lib.load().axk_paged_key_bounds_i8(at(16), scales, bounds, at(4), at(5), at(6), None, 8, 2, 2, d, 32, 16, 8,
+                                               None, None)
+
+
+def decode_i8(scales=at(24), out=at(8), ws=at(32), d=64):
+    return _lib.load().axk_paged_decode_blocks_i8(at(1), at(16), scales, at(4), at(5), at(6), None, 0, 0, out, None, None,
+                                                  1.0, 8, 2, 4, 2, d, 32, 8, 0.125, None, ws, 1 << 24, None)
+
+
 @pytest.mark.parametrize("call,code", [
+    (lambda: write_i8(scales=None), NULL), (lambda: write_i8(scales=at(24, 1)), ALIGN), (lambda: write_i8(scales=at(16)), ALIAS),
+    (lambda: write_i8(bounds=at(24)), ALIAS), (lambda: write_i8(d=80), SHAPE), (lambda: write_i8(rows=1 << 15), SHAPE),
+    (lambda: bounds_i8(scales=None), NULL), (lambda: bounds_i8(bounds=at(24)), ALIAS), (lambda: bounds_i8(d=512), SHAPE),
+    (lambda: decode_i8(scales=None), NULL), (lambda: decode_i8(scales=at(24, 1)), ALIGN), (lambda: decode_i8(ws=None), WORKSPACE),
+    (lambda: decode_i8(out=at(16)), ALIAS),
     (lambda: write(k=None), NULL), (lambda: write(bounds=None), NULL), (lambda: write(loc=None), NULL),
     (lambda: write(d=96), SHAPE), (lambda: write(page=24), SHAPE), (lambda: write(block=24), SHAPE),
     (lambda: write(page=48, block=32), SHAPE), (lambda: write(page=8192, block=16), SHAPE),
@@ -116,8 +136,14 @@ U8 = torch.zeros(4, 2, 32, 2, 64, dtype=torch.uint8)
      "kv_scale"),
     (lambda t: axk.store_paged_kv_bounds(bf(2, 2, 64), bf(2, 2, 64), CACHE, BOUNDS, torch.zeros(2, 2, dtype=torch.int32),
                                          kv_scale=8.0), "kv_scale"),
+    (lambda t: axk.store_paged_kv_bounds(bf(2, 2, 64), bf(2, 2, 64), CACHE.to(torch.int16), BOUNDS,
+                                         torch.zeros(2, 2, dtype=torch.int32)), "bfloat16, u8"),
     (lambda t: axk.store_paged_kv_bounds(bf(2, 2, 64), bf(2, 2, 64), CACHE.to(torch.int8), BOUNDS,
-                                         torch.zeros(2, 2, dtype=torch.int32)), "bfloat16 or u8"),
+                                         torch.zeros(2, 2, dtype=torch.int32)), "kv_scales"),
+    (lambda t: axk.paged_key_bounds(CACHE.to(torch.int8), BOUNDS, *t, kv_scales=bf(4, 2, 32, 3)), "kv_scales"),
+    (lambda t: axk.paged_key_bounds(CACHE, BOUNDS, *t, kv_scales=bf(4, 2, 32, 2)), "INT8"),
+    (lambda t: axk.paged_decode_blocks(bf(2, 4, 64), CACHE.to(torch.int8), *t, kv_scale=8.0, kv_scales=bf(4, 2, 32, 2)),
+     "FP8"),
     (lambda t: axk.store_paged_kv_bounds(bf(2, 2, 64), bf(2, 2, 64), CACHE, BOUNDS, torch.zeros(3, 2, dtype=torch.int32)),
      "cache_location"),
     (lambda t: axk.store_paged_kv_bounds(bf(2, 3, 64), bf(2, 3, 64), CACHE, BOUNDS, torch.zeros(2, 2, dtype=torch.int32)),

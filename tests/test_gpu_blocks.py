@@ -32,14 +32,26 @@ def make(lens, hq, hkv, d, page, kv="bf16", seed=0, extra=3):
         scale = 8.0
         x = (x * scale).to(torch.float8_e4m3fn).view(torch.uint8)
         x.masked_fill_(~used[:, None, :, None, None], 0x7F)
-    else:
+    elif kv == "bf16":
         x.masked_fill_(~used[:, None, :, None, None], NAN)
+    if kv == "i8":
+        codes, scale = paged_attn.quant_kv_i8(x)
+        x = codes.masked_fill(~used[:, None, :, None, None], 127)
+        scale.masked_fill_(~used[:, None, :, None], NAN)
     q = (1.5 * torch.randn(len(lens), hq, d, generator=g)).to(torch.bfloat16)
     return dict(lens=lens, q=q, cache=x, ptr=ptr, idx=idx, last=last, scale=scale, page=page, hkv=hkv, d=d)
 
 
 def table(c, dev):
     return c["ptr"].to(dev), c["idx"].to(dev), c["last"].to(dev)
+
+
+def kv_of(c, dev=None):
+    """The scale arguments of the operators for this cache (an int8 cache's scales on the device)."""
+    s = c["scale"]
+    if isinstance(s, torch.Tensor):
+        return {"kv_scales": s.to(dev)}
+    return {"kv_scale": s}
 
 
 def empty_bounds(c, block, fill=0.0):
@@ -76,7 +88,7 @@ def check_decode(c, dev, blocks=None, block=16, weights=True, decay=0.75, sm_sca
     out = axk.paged_decode_blocks(c["q"].to(dev), c["cache"].to(dev), *table(c, dev),
                                   blocks=None if blocks is None else blocks.to(dev), block_size=block, sm_scale=sm_scale,
                                   weights_in=w0.to(dev) if weights and win else None, weights=w, decay=decay,
-                                  kv_scale=c["scale"], status=status)
+                                  status=status, **kv_of(c, dev))
     within(out, ref, slack + ref.abs() * 2.0 ** -8)
     if weights:
         within(w, rw, wslack)
@@ -84,7 +96,7 @@ def check_decode(c, dev, blocks=None, block=16, weights=True, decay=0.75, sm_sca
 
 
 # ---- key bounds ----
-@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "i8"])
 @pytest.mark.parametrize("hkv,d,page,block", [(2, 256, 64, 64), (1, 64, 16, 16), (3, 64, 96, 48), (8, 128, 256, 128),
                                               (16, 256, 32, 16), (5, 128, 64, 32)])
 def test_bounds_from_the_cache(dev, kv, hkv, d, page, block):
@@ -92,7 +104,7 @@ def test_bounds_from_the_cache(dev, kv, hkv, d, page, block):
     fill = empty_bounds(c, block, 7.0)
     for start in (None, torch.tensor([0, 0, block, page, 2 * page - block - 1, block + 1], dtype=torch.int32)):
         ref = ob.key_bounds(c["cache"], fill, c["ptr"], c["idx"], c["last"], start, c["scale"])
-        got = axk.paged_key_bounds(c["cache"].to(dev), fill.to(dev), *table(c, dev), kv_scale=c["scale"],
+        got = axk.paged_key_bounds(c["cache"].to(dev), fill.to(dev), *table(c, dev), **kv_of(c, dev),
                                    start=None if start is None else start.to(dev)).cpu()
         assert torch.equal(got, ref)
 
@@ -109,7 +121,7 @@ def test_bounds_skip_pages_outside_the_pool_and_padding(dev):
     assert torch.equal(got, ob.key_bounds(c["cache"], fill, c["ptr"], c["idx"], c["last"])) and int(status) == 1
 
 
-@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "i8"])
 @pytest.mark.parametrize("hkv,d,page,block,rows", [(2, 256, 64, 64, 1), (1, 64, 16, 16, 5), (3, 64, 96, 48, 3),
                                                    (16, 256, 32, 16, 2)])
 def test_store_folds_rows_in_order(dev, kv, hkv, d, page, block, rows):
@@ -118,6 +130,7 @@ def test_store_folds_rows_in_order(dev, kv, hkv, d, page, block, rows):
     c = make([n] * bsz, hkv, hkv, d, page, kv)
     cache = torch.zeros_like(c["cache"]).to(dev)
     bounds = empty_bounds(c, block, 9.0).to(dev)
+    kvs = kv_of(c, dev)
     g = torch.Generator().manual_seed(1)
     for at in range(0, n, rows):
         t = list(range(at, min(n, at + rows)))
@@ -125,9 +138,11 @@ def test_store_folds_rows_in_order(dev, kv, hkv, d, page, block, rows):
         loc = torch.tensor([[int(c["idx"][int(c["ptr"][b]) + i // page]), i % page] for b in range(bsz) for i in t],
                            dtype=torch.int32)
         rc, rb = ob.store(k, v, cache.cpu(), bounds.cpu(), loc, c["scale"])
-        axk.store_paged_kv_bounds(k.to(dev), v.to(dev), cache, bounds, loc.to(dev), kv_scale=c["scale"])
+        axk.store_paged_kv_bounds(k.to(dev), v.to(dev), cache, bounds, loc.to(dev), **kvs)
         assert torch.equal(cache.cpu().view(torch.uint8), rc.view(torch.uint8)) and torch.equal(bounds.cpu(), rb)
-    used = axk.paged_key_bounds(cache, bounds.clone(), *table(c, dev), kv_scale=c["scale"])
+    if kv == "i8":
+        assert torch.equal(kvs["kv_scales"].cpu().view(torch.int16), c["scale"].view(torch.int16))
+    used = axk.paged_key_bounds(cache, bounds.clone(), *table(c, dev), **kvs)
     assert torch.equal(used, bounds)
 
 
@@ -156,6 +171,11 @@ def test_store_matches_the_plain_writes_and_handles_shared_slots(dev):
         else:
             axk.store_paged_kv_fp8(k[:4].to(dev), v[:4].to(dev), b, loc, scale)
         assert torch.equal(a, b)
+    a, b = (torch.zeros(pool, 2, page, hkv, d, dtype=torch.int8, device=dev) for _ in range(2))
+    sa, sb = (torch.zeros(pool, 2, page, hkv, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    axk.store_paged_kv_bounds(k[:4].to(dev), v[:4].to(dev), a, gb, loc, kv_scales=sa)
+    axk.store_paged_kv_i8(k[:4].to(dev), v[:4].to(dev), b, sb, loc)
+    assert torch.equal(a, b) and torch.equal(sa, sb)
     axk.store_paged_kv_bounds(k[:0].to(dev), v[:0].to(dev), gc, gb, loc[:0])  # no rows: nothing happens
 
 
@@ -228,7 +248,7 @@ def test_select(dev, kind, blocks, n, first, keep_last):
 
 
 # ---- decode ----
-@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "i8"])
 @pytest.mark.parametrize("hq,hkv,d,page,block,n", [(16, 2, 256, 64, 64, 9), (16, 1, 64, 16, 16, 40), (7, 7, 64, 64, 32, 3),
                                                    (6, 2, 128, 96, 48, 12), (32, 8, 128, 256, 128, 4),
                                                    (16, 2, 256, 64, 16, 200), (3, 1, 256, 4096, 16, 7), (16, 1, 256, 64, 32, 33)])
@@ -244,7 +264,7 @@ def test_decode_over_listed_blocks(dev, kv, hq, hkv, d, page, block, n):
         assert torch.equal(a, x)
 
 
-@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "i8"])
 @pytest.mark.parametrize("hq,hkv,d,page", [(16, 2, 256, 64), (16, 1, 64, 16), (7, 7, 64, 64), (6, 2, 128, 96),
                                            (16, 4, 256, 256)])
 def test_decode_over_every_block(dev, kv, hq, hkv, d, page):
@@ -393,14 +413,14 @@ def test_evict_a_table_with_room_to_spare(dev):
 
 
 # ---- together ----
-@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "i8"])
 def test_decode_steps_with_eviction(dev, kv):
     """Prefilled sequences decoded for some steps: write, score, select, attend, add weights; then evicted and decoded on,
     every operator's result checked against the oracle on the state the GPU had before it."""
     page, block, hq, hkv, d, n = 32, 16, 8, 2, 128, 6
     lens = [150, 31, 96]
     c = make([x + 8 for x in lens], hq, hkv, d, page, kv)  # pages for what is to come
-    cache, scale = c["cache"].to(dev), c["scale"]
+    cache, scale, kvs = c["cache"].to(dev), c["scale"], kv_of(c, dev)
     ptr, idx, _ = table(c, dev)
     last = torch.tensor([(x - 1) % page + 1 for x in lens], dtype=torch.int32, device=dev)
     ptr_used = torch.tensor([0] + [-(-x // page) for x in lens]).cumsum(0).int()
@@ -408,7 +428,7 @@ def test_decode_steps_with_eviction(dev, kv):
     used = [r[:-(-x // page)] for r, x in zip(rows, lens)]
     ptr, idx = ptr_used.to(dev), torch.tensor(sum(used, []), dtype=torch.int32, device=dev)
     bounds = empty_bounds(c, block).to(dev)
-    axk.paged_key_bounds(cache, bounds, ptr, idx, last, kv_scale=scale)
+    axk.paged_key_bounds(cache, bounds, ptr, idx, last, **kvs)
     w = torch.zeros(hkv, idx.numel(), device=dev)
     g = torch.Generator().manual_seed(9)
     for step in range(6):
@@ -429,7 +449,7 @@ def test_decode_steps_with_eviction(dev, kv):
         q = (1.5 * torch.randn(3, hq, d, generator=g)).to(torch.bfloat16)
         loc = torch.tensor([[u[-1], int(last[b]) - 1] for b, u in enumerate(used)], dtype=torch.int32)
         rc, rb = ob.store(k, v, cache.cpu(), bounds.cpu(), loc, scale)
-        axk.store_paged_kv_bounds(k.to(dev), v.to(dev), cache, bounds, loc.to(dev), kv_scale=scale)
+        axk.store_paged_kv_bounds(k.to(dev), v.to(dev), cache, bounds, loc.to(dev), **kvs)
         assert torch.equal(cache.cpu().view(torch.uint8), rc.view(torch.uint8)) and torch.equal(bounds.cpu(), rb)
         s = axk.paged_block_scores(q.to(dev), bounds, ptr, idx, last, page)
         blocks = axk.paged_select_blocks(s, ptr, last, page, block, n)
@@ -437,7 +457,7 @@ def test_decode_steps_with_eviction(dev, kv):
         ref, rw, slack, wslack = ob.decode_blocks(q, cache.cpu(), ptr.cpu(), idx.cpu(), last.cpu(), blocks.cpu(), block,
                                                   None, w.cpu(), 0.9, scale)
         out = axk.paged_decode_blocks(q.to(dev), cache, ptr, idx, last, blocks, block, weights_in=w, weights=w, decay=0.9,
-                                      kv_scale=scale)
+                                      **kvs)
         within(out, ref, slack + ref.abs() * 2.0 ** -8)
         within(w, rw, wslack)
         if step == 3:
