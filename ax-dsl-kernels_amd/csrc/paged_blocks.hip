@@ -116,7 +116,7 @@ AXK_DEV void stored_pairs(const axk_u32x4 w, float inv_scale, float s, uint32_t 
 }
 
 // ---- key bounds ----
-constexpr int64_t kMaxRows = 16384;  // every row looks at every other's place: 2^28 reads, some 0.1 ms
+constexpr int64_t kMaxRows = 16384;  // every row looks at every other's place: 16384 rows take 0.22 ms, 1024 10.6 us
 
 // The new rows' K / V written at loc[r] = (page, slot), and folded into the bounds of their blocks: a block that holds a
 // new row at its first slot starts afresh, every other one widens what it had. One workgroup per row; the first row of
@@ -230,12 +230,20 @@ __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
         lo[e] = from ? bf16_order(lw[e]) : (axk_s16x2)(short)0x7fff;
         hi[e] = from ? bf16_order(hw[e]) : (axk_s16x2)(short)-0x8000;
       }
-      for (int j = 0; j < n; ++j) {
-        const Stored o = store_eight<T>(*reinterpret_cast<const uint4*>(k + (int64_t)s_rows[j] * row + c * 8), d, kv_scale);
+      for (int j0 = 0; j0 < n; j0 += 8) {  // eight rows' loads under way together
+        uint4 x[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          lo[e] = __builtin_elementwise_min(lo[e], bf16_order(o.pair[e]));
-          hi[e] = __builtin_elementwise_max(hi[e], bf16_order(o.pair[e]));
+        for (int j = 0; j < 8; ++j)
+          if (j0 + j < n) x[j] = *reinterpret_cast<const uint4*>(k + (int64_t)s_rows[j0 + j] * row + c * 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j0 + j >= n) break;
+          const Stored o = store_eight<T>(x[j], d, kv_scale);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            lo[e] = __builtin_elementwise_min(lo[e], bf16_order(o.pair[e]));
+            hi[e] = __builtin_elementwise_max(hi[e], bf16_order(o.pair[e]));
+          }
         }
       }
       *lo4 = make_uint4(bf16_unorder(lo[0]), bf16_unorder(lo[1]), bf16_unorder(lo[2]), bf16_unorder(lo[3]));
