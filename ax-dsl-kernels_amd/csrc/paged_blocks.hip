@@ -1094,13 +1094,18 @@ AXK_DEV void merge_output(const BlkArgs& a, int b, int h, int part, Pieces pc, f
   }
   join_pieces(t, ml, pc.n, group, s_part);
   t = join(join(s_part[0][head], s_part[1][head]), join(s_part[2][head], s_part[3][head]));
-  axk_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const axk_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  axk_f32x4 o = zero;
 #pragma unroll
-  for (int k = 0; k < kFirst; ++k) o += (x[k].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[k].x - t.x)) * v[k];
+  for (int k = 0; k < kFirst; ++k) {
+    const axk_f32x4 y = __builtin_amdgcn_exp2f(x[k].x - t.x) * v[k];
+    o += x[k].y == 0.f ? zero : y;  // a selection: what was not counted may be anything, and 0 * NaN is not 0
+  }
 #pragma unroll 8
   for (int p = wave + 4 * kFirst; p < pc.n; p += 4) {
     const float2 y = ml[(int64_t)p * group + head];
-    o += (y.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(y.x - t.x)) * po[(int64_t)p * per];
+    const axk_f32x4 z = __builtin_amdgcn_exp2f(y.x - t.x) * po[(int64_t)p * per];
+    o += y.y == 0.f ? zero : z;
   }
   s_o[wave][lane] = o;
   __syncthreads();

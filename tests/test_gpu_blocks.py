@@ -85,7 +85,10 @@ def check_decode(c, dev, blocks=None, block=16, weights=True, decay=0.75, sm_sca
                                               w0, decay, c["scale"])
     w = torch.full((c["hkv"], c["idx"].numel()), NAN, device=dev) if weights else None
     status = torch.zeros(1, dtype=torch.int32, device=dev)
-    out = axk.paged_decode_blocks(c["q"].to(dev), c["cache"].to(dev), *table(c, dev),
+    ws = axk.paged_decode_blocks_workspace(len(c["lens"]), c["q"].shape[1], c["hkv"], c["d"], c["page"], c["idx"].numel(), dev,
+                                           block, 0 if blocks is None else blocks.shape[2], weights)
+    ws.fill_(255)  # NaNs: nothing may be read that the call has not written
+    out = axk.paged_decode_blocks(c["q"].to(dev), c["cache"].to(dev), *table(c, dev), workspace=ws,
                                   blocks=None if blocks is None else blocks.to(dev), block_size=block, sm_scale=sm_scale,
                                   weights_in=w0.to(dev) if weights and win else None, weights=w, decay=decay,
                                   status=status, **kv_of(c, dev))
@@ -286,12 +289,47 @@ def test_decode_over_every_block_agrees_with_paged_decode(dev):
                                                                         1 / 16).float(), rtol=2e-2, atol=1e-2)
 
 
+@pytest.mark.parametrize("lens", [[0], [0, 0, 700], [700, 0]])
+def test_decode_of_empty_sequences_beside_others(dev, lens):
+    """Empty sequences yield zeros whatever the workspace or another sequence's values hold."""
+    c = make(lens, 4, 2, 128, 32)
+    check_decode(c, dev)
+    check_decode(c, dev, random_blocks(c, 16, 40), 16)
+    if max(lens):
+        c["cache"][:, 1] = math.inf
+        out = axk.paged_decode_blocks(c["q"].to(dev), c["cache"].to(dev), *table(c, dev)).cpu()
+        for b, n in enumerate(lens):
+            assert (out[b] == (math.inf if n else 0.0)).all()
+
+
 @pytest.mark.parametrize("batch", [1, 63, 64, 300, 700])
 def test_decode_many_short_sequences(dev, batch):
     rng = random.Random(batch)
     c = make([rng.choice([0, 1, 5, 16, 40, 130]) for _ in range(batch)], 4, 2, 64, 16, seed=batch)
     check_decode(c, dev)
     check_decode(c, dev, random_blocks(c, 16, 3), 16)
+
+
+@pytest.mark.parametrize("page,block", [(64, 16), (4096, 16), (48, 48)])
+def test_decode_over_a_long_list(dev, page, block):
+    """Lists longer than the merge keeps in LDS (2048 blocks), whose pages straddle its rounds."""
+    c = make([50000, 33, 40000], 2, 1, 64, page, seed=page)
+    blocks = torch.full((3, 1, 50000 // block + 3), -1, dtype=torch.int32)
+    g = torch.Generator().manual_seed(0)
+    for b, n in enumerate(c["lens"]):
+        nb = -(-n // block)
+        got = torch.arange(nb)[torch.rand(nb, generator=g) < 0.9]
+        blocks[b, 0, :len(got)] = got.int()
+    check_decode(c, dev, blocks, block)
+
+
+def test_decode_of_more_rows_than_run_at_once(dev):
+    """520 (sequence, KV head) rows: pieces of 2048 tokens, in the listed form and over every block."""
+    lens = [20] * 130
+    lens[3], lens[70], lens[129] = 2100, 4500, 2048
+    c = make(lens, 8, 4, 64, 64)
+    check_decode(c, dev, random_blocks(c, 32, 150), 32)
+    check_decode(c, dev)
 
 
 def test_decode_skips_bad_pages_and_bad_lists(dev):
