@@ -685,7 +685,8 @@ struct PieceOf {
   int b, piece;
   Seq s;
 };
-AXK_DEV int pieces_of(const Seq& s, int ps) { return (int)((unsigned)(subs_of(s) + ps - 1) / (unsigned)ps); }
+// (One at least where it has pages, so that pages without a token get their weights too.)
+AXK_DEV int pieces_of(const Seq& s, int ps) { return s.np ? max((int)((unsigned)(subs_of(s) + ps - 1) / (unsigned)ps), 1) : 0; }
 AXK_DEV PieceOf find_piece(const BlkArgs& a, int it) {
   const int lane = threadIdx.x & 63;
   int base = 0;
@@ -1130,7 +1131,7 @@ AXK_DEV void merge_weights(const BlkArgs& a, const WeightArgs& w, int b, int h, 
   const float* in = w.in ? w.in + (int64_t)h * a.nnz + s.pb : nullptr;
   float* out = w.out + (int64_t)h * a.nnz + s.pb;
   const int p0 = (int)((unsigned)(piece * a.ps + spp - 1) / (unsigned)spp);
-  const int units = a.blocks ? a.n : min((int)((unsigned)((piece + 1) * a.ps + spp - 1) / (unsigned)spp), s.np) - p0;
+  const int units = a.blocks ? a.n : (piece == pc.n - 1 ? s.np : (int)((unsigned)((piece + 1) * a.ps + spp - 1) / (unsigned)spp)) - p0;
   const int span = a.blocks ? spb : spp, subs = a.blocks ? units * span : subs_of(s) - p0 * spp;
   const float2* stat = a.stat + (subs <= 0 ? 0 : a.blocks ? ((int64_t)b * a.hkv + h) * a.n * spb : ((int64_t)h * a.nnz + s.pb + p0) * spp) * group;
   const int top = max(subs - 1, 0);

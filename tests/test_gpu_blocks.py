@@ -358,6 +358,33 @@ def test_decode_extreme_scores(dev):
     check_decode(c, dev, random_blocks(c, 32, 6), 32)
 
 
+def test_a_last_page_without_a_token(dev):
+    """last_page_len 0: the page counts for nothing, keeps its weight, and its blocks score -inf."""
+    for lens in ([1024, 33, 64], [64, 2048]):
+        c = make(lens, 6, 2, 64, 64)
+        extra = c["cache"].shape[0] - c["idx"].numel()
+        ptr, idx, free = [0], [], sorted(set(range(c["cache"].shape[0])) - set(c["idx"].tolist()))[:extra]
+        for b, n in enumerate(lens):  # the first and last sequences get a page with nothing in it
+            idx += c["idx"][int(c["ptr"][b]):int(c["ptr"][b + 1])].tolist()
+            if b != 1 or len(lens) == 2:
+                idx.append(free.pop())
+                c["last"][b] = 0
+            ptr.append(len(idx))
+        idx.append(free.pop())  # and a sequence of one empty page
+        c["ptr"] = torch.tensor(ptr + [len(idx)], dtype=torch.int32)
+        c["idx"], c["last"] = torch.tensor(idx, dtype=torch.int32), torch.cat([c["last"], torch.zeros(1, dtype=torch.int32)])
+        c["q"], c["lens"] = torch.cat([c["q"], c["q"][:1]]), lens + [0]
+        out, _, status = check_decode(c, dev)
+        assert status == 0 and not out[-1].any()
+        check_decode(c, dev, random_blocks(c, 16, 9), 16)
+        bounds = ob.key_bounds(c["cache"], empty_bounds(c, 32, 1.0), c["ptr"], c["idx"], c["last"])
+        assert torch.equal(axk.paged_key_bounds(c["cache"].to(dev), empty_bounds(c, 32, 1.0).to(dev), *table(c, dev)).cpu(),
+                           bounds)
+        got = axk.paged_block_scores(c["q"].to(dev), bounds.to(dev), *table(c, dev), 64).cpu()
+        ref, _ = ob.block_scores(c["q"], bounds, c["ptr"], c["idx"], c["last"], 64)
+        assert torch.equal(got == -math.inf, ref == -math.inf)
+
+
 def test_infinite_and_nan_rows_stay_where_they_are(dev):
     """Blocks that the list leaves out may hold anything; a NaN value that is attended reaches its own heads only."""
     c = make([640, 640], 4, 2, 64, 64)
