@@ -1121,8 +1121,10 @@ AXK_DEV void merge_output(const BlkArgs& a, int b, int h, int part, Pieces pc, f
 // against the row's joined maximum and sum. What is added up are units of subtiles (listed blocks, or pages), 64 at a time,
 // four to 16 lanes, a head a lane, four subtiles of each together; the first ones are on their way while the sums are joined.
 constexpr int kListLds = 2048;  // listed blocks whose shares are kept in LDS at a time
+template <bool LISTED>
 AXK_DEV void merge_weights(const BlkArgs& a, const WeightArgs& w, int b, int h, int piece, const Seq& s, Pieces pc,
                            float2 (*s_part)[16], float* s_share, int* s_page) {
+  constexpr int NQ = LISTED ? 4 : 1;
   const int tid = threadIdx.x, l16 = tid & 15, r16 = tid >> 4, group = a.hq / a.hkv;
   const float2* ml = a.ml + pc.item * group;
   const float2 none = make_float2(0.f, 0.f);
@@ -1130,15 +1132,22 @@ AXK_DEV void merge_weights(const BlkArgs& a, const WeightArgs& w, int b, int h, 
   const int spp = a.page / kSub, spb = a.block / kSub, bpp = a.page / a.block;
   const float* in = w.in ? w.in + (int64_t)h * a.nnz + s.pb : nullptr;
   float* out = w.out + (int64_t)h * a.nnz + s.pb;
-  const int p0 = (int)((unsigned)(piece * a.ps + spp - 1) / (unsigned)spp);
-  const int units = a.blocks ? a.n : (piece == pc.n - 1 ? s.np : (int)((unsigned)((piece + 1) * a.ps + spp - 1) / (unsigned)spp)) - p0;
-  const int span = a.blocks ? spb : spp, subs = a.blocks ? units * span : subs_of(s) - p0 * spp;
-  const float2* stat = a.stat + (subs <= 0 ? 0 : a.blocks ? ((int64_t)b * a.hkv + h) * a.n * spb : ((int64_t)h * a.nnz + s.pb + p0) * spp) * group;
+  // where the units' statistics begin, their subtiles, and all of these
+  int p0 = 0, units = a.n, span = spb, subs = a.n * spb;
+  int64_t from = ((int64_t)b * a.hkv + h) * a.n * spb;
+  if constexpr (!LISTED) {
+    p0 = (int)((unsigned)(piece * a.ps + spp - 1) / (unsigned)spp);
+    units = (piece == pc.n - 1 ? s.np : (int)((unsigned)((piece + 1) * a.ps + spp - 1) / (unsigned)spp)) - p0;
+    span = spp;
+    subs = subs_of(s) - p0 * spp;
+    from = subs > 0 ? ((int64_t)h * a.nnz + s.pb + p0) * spp : 0;
+  }
+  const float2* stat = a.stat + from * group;
   const int top = max(subs - 1, 0);
-  float2 y[4][4];
+  float2 y[NQ][4];
   auto fetch = [&](int u, int k0) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < NQ; ++q)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int sub = (u + 16 * q) * span + k0 + k;
@@ -1162,45 +1171,45 @@ AXK_DEV void merge_weights(const BlkArgs& a, const WeightArgs& w, int b, int h, 
   // (A list out of order may name a page again: hence the atomic.) A page whose blocks straddle two rounds of the LDS is
   // finished by the round it begins in, which looks past its end.
   for (int base = 0;; base += kListLds - bpp) {
-    const int end = a.blocks ? min(a.n, base + kListLds) : units;  // the last bpp of a round only to finish pages
+    const int end = LISTED ? min(a.n, base + kListLds) : units;  // the last bpp of a round only to finish pages
     int u = base + r16, k0 = 0;
     fetch(u, 0);
-    if (a.blocks) {
+    if (LISTED) {
       __syncthreads();  // the round before has been read
       list_pages(base, end - base);
     }
     if (base == 0) {
-      if (a.blocks)
+      if (LISTED)
         for (int p = tid; p < s.np; p += 256) out[p] = in ? w.decay * in[p] : 0.f;  // what every page keeps
       join_pieces(t, ml, pc.n, group, s_part);
       t = join(join(s_part[0][l16], s_part[1][l16]), join(s_part[2][l16], s_part[3][l16]));
       t.y = t.y == 0.f ? 0.f : 1.0f / t.y;
     }
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    float sum[NQ] = {};
     while (u < end) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int q = 0; q < NQ; ++q)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           sum[q] += y[q][k].y == 0.f ? 0.f : y[q][k].y * __builtin_amdgcn_exp2f(y[q][k].x - t.x) * t.y;
       k0 += 4;
       if (k0 >= span) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < NQ; ++q) {
           const float x = group_sum<16>(sum[q]);
           const int unit = u + 16 * q;
           if (l16 == 0 && unit < end) {
-            if (a.blocks) s_share[unit - base] = x;
+            if (LISTED) s_share[unit - base] = x;
             else out[p0 + unit] = (in ? w.decay * in[p0 + unit] : 0.f) + x;
           }
           sum[q] = 0.f;
         }
-        u += 64;
+        u += 16 * NQ;
         k0 = 0;
       }
       if (u < end) fetch(u, k0);
     }
-    if (!a.blocks) return;
+    if (!LISTED) return;
     __syncthreads();
     const int n = end - base;
     for (int j = tid; j < (end < a.n ? n - bpp : n); j += 256) {
@@ -1216,23 +1225,23 @@ AXK_DEV void merge_weights(const BlkArgs& a, const WeightArgs& w, int b, int h, 
 
 // The first batch * hkv * split workgroups: output rows. The others: page weights. A merge is three dependent trips to
 // memory and little else.
-template <int D>
+template <int D, bool LISTED>
 __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a, const WeightArgs w) {
   __shared__ float2 s_part[4][16];
   __shared__ axk_f32x4 s_o[4][64];
-  __shared__ float s_share[kListLds];
-  __shared__ int s_page[kListLds + 1];
+  __shared__ float s_share[LISTED ? kListLds : 1];
+  __shared__ int s_page[LISTED ? kListLds + 1 : 1];
   const int rows = a.batch * a.hkv, x = (int)blockIdx.x - rows * w.split;
   int b, h, piece = 0;
   Pieces pc;
   Seq s;
-  if (x < 0 || a.blocks) {
+  if (x < 0 || LISTED) {
     const int row = x < 0 ? blockIdx.x / w.split : x;
     b = row / a.hkv;
     h = row - b * a.hkv;
     s = seq_of(a.indptr, a.last, b, a.page, a.nnz);
     pc = {(int64_t)row * a.pieces, a.pieces};
-    if (!a.blocks) {
+    if (!LISTED) {
       const int before = min(pieces_before(a, b), a.pieces);
       pc = {(int64_t)h * a.pieces + before, min(pieces_of(s, a.ps), a.pieces - before)};
     }
@@ -1249,7 +1258,7 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
     s = p.s;
     pc = {x - piece, min(pieces_of(s, a.ps), (h + 1) * a.pieces - (x - piece))};
   }
-  merge_weights(a, w, b, h, piece, s, pc, s_part, s_share, s_page);
+  merge_weights<LISTED>(a, w, b, h, piece, s, pc, s_part, s_share, s_page);
 }
 
 // ---- eviction ----
@@ -1433,7 +1442,8 @@ int launch_blocks(const BlkArgs& a, const WeightArgs& w, int type, hipStream_t s
   else hipLaunchKernelGGL((paged_blocks_kernel<D, kBf16>), grid, dim3(256), (BlkCfg<D, kBf16>::LDS), st, a);
   if (!a.direct) {
     const int64_t wgs = (int64_t)a.batch * a.hkv * w.split + (w.out ? (a.blocks ? (int64_t)a.batch : a.pieces) * a.hkv : 0);
-    hipLaunchKernelGGL((paged_blocks_merge_kernel<D>), dim3((unsigned)wgs), dim3(256), 0, st, a, w);
+    if (a.blocks) hipLaunchKernelGGL((paged_blocks_merge_kernel<D, true>), dim3((unsigned)wgs), dim3(256), 0, st, a, w);
+    else hipLaunchKernelGGL((paged_blocks_merge_kernel<D, false>), dim3((unsigned)wgs), dim3(256), 0, st, a, w);
   }
   return axk_launch_status();
 }
