@@ -121,8 +121,8 @@ constexpr int64_t kMaxRows = 16384;  // every row looks at every other's place: 
 // The new rows' K / V written at loc[r] = (page, slot), and folded into the bounds of their blocks: a block that holds a
 // new row at its first slot starts afresh, every other one widens what it had. One workgroup per row; the first row of
 // the call that falls into a block folds all of them, so that rows of one block never race, and where two rows name one
-// slot the last one is stored (both are folded). Two launches' worth of work in one: a decode step pays a launch, the
-// dependent reads location, then row and bounds, and nothing else.
+// slot the last one is stored (both are folded). Bound by its chain: launch, locations, then row and bounds; 3.4 us for the
+// 16 rows of a decode step (HKV 2, D 256), 2.3 without the bounds, 4.5 for 16 rows of one block.
 //
 // Eight channels of a new row as the cache keeps them: their bytes (a bf16 cache: the values themselves), the int8 scale,
 // and the key's bf16 pairs as attention reads them. The d / 8 lanes of a head's row act together.
@@ -255,7 +255,9 @@ __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
 // The bounds of every block of the page table that reaches past start[b] (all of them without start), from the cache.
 // One workgroup per block: its K rows are one contiguous run of tokens x HKV x D values, read 16 bytes a lane, a column
 // of 8 (8-bit caches: 16) channels kept by as many lanes as the workgroup has to spare and joined through LDS. Minimum and
-// maximum are taken on the bf16 bits as ordered 16-bit integers, two values an instruction. Bound by the K bytes.
+// maximum are taken on the bf16 bits as ordered 16-bit integers, two values an instruction. Bound by the K bytes: 136,000
+// tokens of an FP8 cache (HKV 2, D 256, blocks of 32) 18.7 us, 84 MB at 4.5 TB/s; without minimum and maximum at all 4%
+// less, with non-temporal loads 8% more, and 1.5 us more while lanes stored dwords 32 bytes apart.
 template <int T>
 __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
     const unsigned char* __restrict__ cache, const uint16_t* __restrict__ scales, uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
@@ -331,7 +333,10 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
 // ---- block scores ----
 // max(q lo, q hi) per channel is q+ hi + q- lo with q+ = max(q, 0), q- = min(q, 0): the score of 16 blocks for the 16
 // (padded) heads of a group is one chain of 2 D / 32 16x16x32 MFMAs, blocks as rows, and a block's bounds are read once.
-// One wave per (16 blocks, KV head); a tile that spans sequences is computed once with each one's queries.
+// One wave per (16 blocks, KV head); a tile that spans sequences is computed once with each one's queries. Bound by the
+// bounds' bytes: 8 sequences of 131072 tokens in blocks of 64 (HKV 4, D 256) 16.3 us, 67 MB at 4.1 TB/s, all of its waves
+// at once. With the rows through LDS as in the decode below the same took 18.2 us, since half as many waves fit (and one
+// sequence of 5003 tokens 4.6 against 5.5).
 template <int D>
 __global__ __launch_bounds__(256) void paged_block_scores_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
@@ -400,8 +405,9 @@ __global__ __launch_bounds__(256) void paged_block_scores_kernel(
 // Radix selection by one workgroup of T threads, K consecutive keys each in registers (a longer row is read again, T K keys
 // at a time, in each step). Keys are taken relative to the row's smallest, and log2(4 T) bits at a time, from the highest
 // that the row's range has, are counted in 4 T bins of LDS, until the smallest key that is taken is known or all keys that
-// agree with it so far are taken: two rounds as a rule. (With 256 bins of the raw bits a row of 8192 scores took 8.5 us
-// more: most scores share sign and exponent, and adds to one address wait for each other.) Equal keys at the border are
+// agree with it so far are taken: two rounds as a rule. Bound by its barriers: 256 of 8192 scores 9.7 us, 64 of 313 4.0.
+// (With 256 bins of the raw bits the former took 19.6: most scores share sign and exponent, and adds to one address wait
+// for each other.) Equal keys at the border are
 // taken by the lowest index. load(at, n, key) fetches a thread's n keys from index `at`; emit(i, taken, rank) is called
 // for every index, rank = the indices below i that are taken; done(base, n, k) after the n indices of a tile, k of them
 // taken.
@@ -638,6 +644,10 @@ __global__ __launch_bounds__(T) void paged_select_blocks_kernel(const float* __r
 //                 4 g + j % 4 of subtile j / 4. V rows are loaded in that order, lane l16 holding D / 16 channels of eight
 //                 tokens, so that the transposition V^T needs is one byte permute per two values, without LDS.
 // The four waves of a piece take its steps in turn and are joined through LDS; pieces by the merge kernel.
+// Bound by HBM: 64 blocks of 64 for 8 sequences of 131072 tokens (HQ 32, HKV 4, D 256) 28.3 us, 134 MB at 4.7 TB/s; the
+// whole FP8 cache of 16 sequences (HQ 16, HKV 2) 30.2 us, 139 MB at 4.6 TB/s; of these some 5 us are the chain of lookups
+// before the first load (list, page, rows) and the join after the last. As many pieces as run at once are best: with three
+// quarters of them the former took 17% longer, with half as many again 3%, and the latter 25%.
 template <int D, int T>
 struct BlkCfg {
   static constexpr int B = T ? 1 : 2;              // bytes of a stored value
@@ -1224,7 +1234,7 @@ AXK_DEV void merge_weights(const BlkArgs& a, const WeightArgs& w, int b, int h, 
 }
 
 // The first batch * hkv * split workgroups: output rows. The others: page weights. A merge is three dependent trips to
-// memory and little else.
+// memory and little else: 4 us for one sequence's 64 pieces, 5.9 for 512 pieces of 8 sequences with their weights.
 template <int D, bool LISTED>
 __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a, const WeightArgs w) {
   __shared__ float2 s_part[4][16];
@@ -1265,7 +1275,8 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
 // One workgroup per sequence: its `budget` pages of largest weight (summed over the KV heads in 64 bits, so that the
 // order of the sum does not decide), the first `first` and last `keep_last` always among them, in their order into the
 // new table; the others' ids into `freed`. Every workgroup finds its places from the whole indptr, and fills as much of
-// the arrays' tails as it moved elsewhere.
+// the arrays' tails as it moved elsewhere. Bound by the selection's barriers: 64 sequences of up to 2048 pages 11.6 us
+// (26 us while a thread summed its pages' heads one after the other).
 constexpr int kEvict = 1024;  // threads
 constexpr int kEvictTile = 4 * kEvict;
 __global__ __launch_bounds__(kEvict) void paged_evict_kernel(const float* __restrict__ w, const int* __restrict__ indptr,
@@ -1407,7 +1418,8 @@ int cache_type(int kv_dtype, float kv_scale) {
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // How a decode over blocks is cut, from what the host knows: pieces of at least 128 tokens, so that each wave has a step,
-// and of at most 2048; otherwise as many as run at once (kPieces), since a second round would pay the lookups again.
+// and of at most 2048; otherwise as many as run at once (two workgroups a CU), since a second round would pay the lookups
+// again.
 constexpr int64_t kPieces = 512;
 struct BlkPlan {
   int ps, pieces;
