@@ -10,8 +10,8 @@ decode step of a layer is then::
 
 after a prefill chunk ``paged_key_bounds`` computes the bounds of its blocks, and ``paged_evict_pages`` cuts a page table
 down to the pages that received the most attention (``w``). Caches are those of paged_decode (bf16), paged_decode_fp8
-(u8 / float8_e4m3fn with ``kv_scale``) and paged_decode_i8 (int8 with ``kv_scales``), page tables theirs too. Nothing is read back to the host, so a step can be
-captured in a HIP graph. Contract violations raise ValueError.
+(u8 / float8_e4m3fn with ``kv_scale``) and paged_decode_i8 (int8 with ``kv_scales``), page tables theirs too. Nothing is
+read back to the host, so a step can be captured in a HIP graph. Contract violations raise ValueError.
 """
 from __future__ import annotations
 
@@ -130,10 +130,10 @@ def store_paged_kv_bounds(
     status: Optional[torch.Tensor] = None,
     kv_scales: Optional[torch.Tensor] = None,
 ) -> None:
-    """store_paged_kv / store_paged_kv_fp8 / store_paged_kv_i8 that also folds each new key into its block's bounds, in one launch: k, v
-    [rows, HKV, D] bf16 go to cache_location[r] = (page, slot). bounds [P, page / block, HKV, 2, D] bf16, in place: a
-    block whose first slot is written starts afresh, any other is widened. Rows of one call may share a block (draft
-    rows); where two name one slot the last is stored."""
+    """store_paged_kv / store_paged_kv_fp8 / store_paged_kv_i8 that also folds each new key into its block's bounds, in
+    one launch: k, v [rows, HKV, D] bf16 go to cache_location[r] = (page, slot). bounds [P, page / block, HKV, 2, D] bf16,
+    in place: a block whose first slot is written starts afresh, any other is widened. Rows of one call may share a block
+    (draft rows); where two name one slot the last is stored."""
     kind, stored, p, page, hkv, d = _cache(kv_cache, kv_scale, kv_scales)
     block = _bounds(bounds, p, hkv, d, page)
     shape = k.shape
@@ -270,9 +270,9 @@ def paged_decode_blocks(
     status: Optional[torch.Tensor] = None,
     kv_scales: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """paged_decode / paged_decode_fp8 / paged_decode_i8 over the listed blocks of each sequence and KV head: blocks int32 [B, HKV, n],
-    strictly ascending block numbers within the sequence, then -1 (as paged_select_blocks returns them), of block_size
-    tokens; None: every block. q [B, HQ, D] bf16; returns bf16 [B, HQ, D], zeros where nothing is attended.
+    """paged_decode / paged_decode_fp8 / paged_decode_i8 over the listed blocks of each sequence and KV head: blocks int32
+    [B, HKV, n], strictly ascending block numbers within the sequence, then -1 (as paged_select_blocks returns them), of
+    block_size tokens; None: every block. q [B, HQ, D] bf16; returns bf16 [B, HQ, D], zeros where nothing is attended.
 
     weights f32 [HKV, nnz], if given, is set to decay * weights_in (zero without weights_in; weights_in may be weights)
     plus the attention that each page-table entry's tokens received, summed over the KV head's queries."""

@@ -407,10 +407,9 @@ __global__ __launch_bounds__(256) void paged_block_scores_kernel(
 // that the row's range has, are counted in 4 T bins of LDS, until the smallest key that is taken is known or all keys that
 // agree with it so far are taken: two rounds as a rule. Bound by its barriers: 256 of 8192 scores 9.7 us, 64 of 313 4.0.
 // (With 256 bins of the raw bits the former took 19.6: most scores share sign and exponent, and adds to one address wait
-// for each other.) Equal keys at the border are
-// taken by the lowest index. load(at, n, key) fetches a thread's n keys from index `at`; emit(i, taken, rank) is called
-// for every index, rank = the indices below i that are taken; done(base, n, k) after the n indices of a tile, k of them
-// taken.
+// for each other.) Equal keys at the border are taken by the lowest index. load(at, n, key) fetches a thread's n keys from
+// index `at`; emit(i, taken, rank) is called for every index, rank = the indices below i that are taken; done(base, n, k)
+// after the n indices of a tile, k of them taken.
 template <class Key, int T>
 struct PickLds {
   unsigned hist[4 * T];
@@ -733,10 +732,11 @@ AXK_DEV int pieces_before(const BlkArgs& a, int b) {
   return wave_total(n);
 }
 
-// Whether a listed block is neither padding (-1) nor a block of the sequence that lies above its predecessor in the list
-// (prev: -1 for the first).
+// Whether a listed block is neither padding (-1) nor a block of the sequence that lies above its predecessor in the list,
+// which is no padding either (prev: kNoPrev for the first).
+constexpr int kNoPrev = -2;
 AXK_DEV bool bad_block(int id, int prev, int nblocks) {
-  return id < -1 || id >= nblocks || (id >= 0 && prev >= id);
+  return id < -1 || id >= nblocks || (id >= 0 && (prev >= id || prev == -1));
 }
 
 // A wave-uniform 64-bit value in scalar registers.
@@ -760,7 +760,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
   int64_t item;
   Seq s;
   const int spb = a.block / kSub;
-  int id = -1, prev = -1;  // thread i: the listed block that subtile i of the piece lies in, and the one before it
+  int id = -1, prev = kNoPrev;  // thread i: the listed block that subtile i of the piece lies in, and the one before it
   if (a.blocks) {
     item = blockIdx.x;
     const int row = blockIdx.x / a.pieces;
@@ -1173,7 +1173,7 @@ AXK_DEV void merge_weights(const BlkArgs& a, const WeightArgs& w, int b, int h, 
     const int nblocks = blocks_of(s, a.block);
     for (int j = tid; j <= n; j += 256) {
       const int slot = base + j - 1, id = slot < 0 ? -1 : list[slot];
-      const bool none_here = id < 0 || bad_block(id, slot ? list[slot - 1] : -1, nblocks);
+      const bool none_here = id < 0 || bad_block(id, slot ? list[slot - 1] : kNoPrev, nblocks);
       s_page[j] = none_here ? -1 : (int)((unsigned)id / (unsigned)bpp);
     }
   };

@@ -386,11 +386,11 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  * Cache, page table and page size as axk_paged_decode; head_dim 64, 128 or 256; num_qo_heads / num_kv_heads <= 16;
  * num_kv_heads <= 4096. kv_dtype: AXK_DT_BF16, or AXK_DT_FP8E4M3 for a cache of axk_paged_kv_write_fp8 with its kv_scale
  * (a power of two; ignored for bf16). The entries ending in _i8 take the int8 cache and bf16 scales of
- * axk_paged_kv_write_i8, read as code * scale (head_dim 64 too). nnz: the entries of indices; offsets of indptr past it are read as nnz and a
- * last_page_len past page_size as page_size, so that no access leaves an array; nnz * page_size / 16 <= 2^30. A page id
- * outside [0, num_pages) is skipped, never read, and sets *status (device i32, or NULL) to 1. An array per page-table entry
- * is [num_kv_heads, nnz], one per block [num_kv_heads, nnz * page_size / block_size]: entry e's blocks at e *
- * page_size / block_size.
+ * axk_paged_kv_write_i8, read as code * scale (head_dim 64 too). nnz: the entries of indices; offsets of indptr past it
+ * are read as nnz and a last_page_len past page_size as page_size, so that no access leaves an array;
+ * nnz * page_size / 16 <= 2^30. A page id outside [0, num_pages) is skipped, never read, and sets *status (device i32, or
+ * NULL) to 1. An array per page-table entry is [num_kv_heads, nnz], one per block
+ * [num_kv_heads, nnz * page_size / block_size]: entry e's blocks at e * page_size / block_size.
  * ------------------------------------------------------------------------------------------- */
 
 /* The new rows k, v bf16 [rows, num_kv_heads, head_dim] written at cache_location i32 [rows, 2] = (page, slot), as
@@ -442,8 +442,8 @@ int axk_paged_select_blocks(const float* scores, const int32_t* indptr, const in
 /* Decode attention, as axk_paged_decode, over the listed blocks of each sequence and KV head only: blocks i32 [batch,
  * num_kv_heads, num_select], each row strictly ascending block numbers within the sequence, then -1 (the form
  * axk_paged_select_blocks writes). NULL with num_select 0: every block (block_size is then not read). A number past the
- * sequence's end, or not above its predecessor in the row, is skipped and sets *status. A row that attends nothing yields
- * zeros.
+ * sequence's end, not above its predecessor in the row, or right behind a -1 is skipped and sets *status. A row that
+ * attends nothing yields zeros.
  * weights_out f32 [num_kv_heads, nnz] (NULL: not wanted) receives, for each KV head and page-table entry,
  *   decay * weights_in (NULL: 0) + sum over the KV head's queries of the attention the page's tokens received;
  * weights_out may be weights_in (in place). Entries of no sequence are left as they are.

@@ -148,7 +148,7 @@ def decode_blocks(q, cache, indptr, indices, last, blocks=None, block: int = 16,
             if blocks is not None:
                 ids, prev = [], -1
                 for slot, i in enumerate(blocks[b, h].tolist()):
-                    if 0 <= i < -(-n // block) and (slot == 0 or i > prev):
+                    if 0 <= i < -(-n // block) and (slot == 0 or (i > prev and prev != -1)):
                         ids.append(i)
                     prev = i
                 rows = rows[torch.isin(rows // block, torch.tensor(ids, dtype=torch.long))]

@@ -342,6 +342,9 @@ def test_decode_skips_bad_pages_and_bad_lists(dev):
     blocks[1, 1] = torch.tensor([1, 2, 3, 10, 12, 13, 5, -1])
     _, _, status = check_decode(c, dev, blocks, 16)
     assert status == 1
+    blocks[:, :] = torch.tensor([2, 5, -1, 2, 5, -1, -1, 7])  # blocks behind padding, some of them twice
+    _, _, status = check_decode(c, dev, blocks, 16, weights=True)
+    assert status == 1
     c["idx"][:] = -1  # nothing left to attend
     out, w, status = check_decode(c, dev, blocks, 16)
     assert status == 1 and not out.any()
