@@ -713,7 +713,8 @@ AXK_DEV PieceOf find_piece(const BlkArgs& a, int it) {
       if (b0 + 64 * i >= a.batch) break;
       const int n = b0 + 64 * i + lane < a.batch ? pieces_of(seq_from(lo[i], hi[i], last[i], a.page, a.nnz), a.ps) : 0;
       const int before = base + (int)wave_scan((unsigned)n) - n;
-      const uint64_t mine = __ballot(it >= before && it < before + n);
+      // (offsets of indptr that fall back can make the sums pass 32 bits: such pieces are nobody's)
+      const uint64_t mine = __ballot(before >= 0 && it >= before && it - before < n);
       if (mine) {
         const int src = __ffsll((unsigned long long)mine) - 1;
         return {b0 + 64 * i + src, it - __builtin_amdgcn_readlane(before, src),
@@ -1252,7 +1253,7 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
     s = seq_of(a.indptr, a.last, b, a.page, a.nnz);
     pc = {(int64_t)row * a.pieces, a.pieces};
     if (!LISTED) {
-      const int before = min(pieces_before(a, b), a.pieces);
+      const int before = (int)min((unsigned)pieces_before(a, b), (unsigned)a.pieces);
       pc = {(int64_t)h * a.pieces + before, min(pieces_of(s, a.ps), a.pieces - before)};
     }
     if (x < 0) {
@@ -1285,14 +1286,15 @@ __global__ __launch_bounds__(kEvict) void paged_evict_kernel(const float* __rest
                                                              float* __restrict__ out_w, int* __restrict__ freed, int nnz,
                                                              int batch, int hkv, int budget, int first, int keep_last) {
   __shared__ PickLds<uint64_t, kEvict> lds;
-  __shared__ int s_sum[4][kEvict / 64];
+  __shared__ unsigned s_sum[4][kEvict / 64];
   __shared__ int s_list[kEvictTile];  // a tile's pages: the kept ones from the front, the others from the back
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
   auto ptr = [&](int i) { return min(max(indptr[i], 0), nnz); };
-  // kept and evicted pages of the sequences before b, and kept and all pages of all of them
-  int n4[4] = {0, 0, 0, 0};
+  // kept and evicted pages of the sequences before b, and kept and all pages of all of them. (Unsigned, as every place made
+  // of them is checked: where offsets of indptr fall back, the sums can be anything.)
+  unsigned n4[4] = {0, 0, 0, 0};
   for (int i = tid; i < batch; i += kEvict) {
-    const int n = max(ptr(i + 1) - ptr(i), 0), k = min(n, budget);
+    const unsigned n = max(ptr(i + 1) - ptr(i), 0), k = min(n, (unsigned)budget);
     if (i < b) {
       n4[0] += k;
       n4[1] += n - k;
@@ -1303,7 +1305,7 @@ __global__ __launch_bounds__(kEvict) void paged_evict_kernel(const float* __rest
   const int waves = (min(batch, kEvict) + 63) / 64;  // that had sequences to add
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    n4[i] = wave_total(n4[i]);
+    n4[i] = (unsigned)wave_total((int)n4[i]);
     if (lane == 0) s_sum[i][wave] = n4[i];
   }
   __syncthreads();
@@ -1312,17 +1314,18 @@ __global__ __launch_bounds__(kEvict) void paged_evict_kernel(const float* __rest
     n4[i] = 0;
     for (int j = 0; j < waves; ++j) n4[i] += s_sum[i][j];
   }
-  const int kept = n4[0], gone = n4[1], all = n4[2], total = n4[3];
+  const unsigned kept = n4[0], gone = n4[1], all = n4[2], total = n4[3], table = (unsigned)nnz;
   const int pb = ptr(b), np = max(ptr(b + 1) - pb, 0), keep = min(np, budget);
   if (tid == 0) {
     if (b == 0) out_indptr[0] = 0;
-    out_indptr[b + 1] = kept + keep;
+    out_indptr[b + 1] = (int)(kept + keep);
   }
   // pages from[0 .. n) of the sequence (a null list: base, base + 1, ...) to places `at` onwards
   auto keep_pages = [&](const int* from, int base, int n, int at) {
     for (int i = tid; i < n; i += kEvict) {
-      const int src = pb + (from ? from[i] : base + i), dst = kept + at + i;
-      if (dst >= nnz) break;
+      const int src = pb + (from ? from[i] : base + i);
+      const unsigned dst = kept + at + i;
+      if (dst >= table) break;
       out_indices[dst] = indices[src];
 #pragma unroll 4
       for (int h = 0; h < hkv; ++h) out_w[(int64_t)h * nnz + dst] = w[(int64_t)h * nnz + src];
@@ -1336,7 +1339,7 @@ __global__ __launch_bounds__(kEvict) void paged_evict_kernel(const float* __rest
     const int want = budget - first - keep_last, count = np - first - keep_last;
     if (want == 0) {
       for (int i = tid; i < count; i += kEvict)
-        if (gone + i < nnz) freed[gone + i] = indices[pb + first + i];
+        if (gone + i < table) freed[gone + i] = indices[pb + first + i];
     } else {
       int done0 = 0;  // pages kept in the tiles before
       auto keys = [&](int at, int n, auto& key) {
@@ -1365,8 +1368,8 @@ __global__ __launch_bounds__(kEvict) void paged_evict_kernel(const float* __rest
         __syncthreads();
         keep_pages(s_list, 0, k, first + done0);
         for (int i = tid; i < n - k; i += kEvict) {
-          const int dst = gone + base - done0 + i;
-          if (dst < nnz) freed[dst] = indices[pb + s_list[kEvictTile - 1 - i]];
+          const unsigned dst = gone + base - done0 + i;
+          if (dst < table) freed[dst] = indices[pb + s_list[kEvictTile - 1 - i]];
         }
         done0 += k;
         __syncthreads();
@@ -1378,16 +1381,16 @@ __global__ __launch_bounds__(kEvict) void paged_evict_kernel(const float* __rest
   }
   // the tails: [all, nnz) of the table and of the weights, [total - all, nnz) of freed. A sequence's share of the first
   // is as long as what it evicted, of the second as what it kept; the last one also fills what no sequence had
-  const int extra = b == batch - 1 ? max(nnz - total, 0) : 0;
+  const int extra = b == batch - 1 && total < table ? (int)(table - total) : 0;
   for (int i = tid; i < np - keep + extra; i += kEvict) {
-    const int at = all + gone + i;
-    if (at >= nnz) break;
+    const unsigned at = all + gone + i;
+    if (at >= table) break;
     out_indices[at] = -1;
     for (int h = 0; h < hkv; ++h) out_w[(int64_t)h * nnz + at] = 0.f;
   }
   for (int i = tid; i < keep + extra; i += kEvict) {
-    const int at = total - all + kept + i;
-    if (at < nnz) freed[at] = -1;
+    const unsigned at = total - all + kept + i;
+    if (at < table) freed[at] = -1;
   }
 }
 

@@ -387,7 +387,8 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  * num_kv_heads <= 4096. kv_dtype: AXK_DT_BF16, or AXK_DT_FP8E4M3 for a cache of axk_paged_kv_write_fp8 with its kv_scale
  * (a power of two; ignored for bf16). The entries ending in _i8 take the int8 cache and bf16 scales of
  * axk_paged_kv_write_i8, read as code * scale (head_dim 64 too). nnz: the entries of indices; offsets of indptr past it
- * are read as nnz and a last_page_len past page_size as page_size, so that no access leaves an array;
+ * are read as nnz, negative ones as 0, and a last_page_len past page_size as page_size, so that no access leaves an array
+ * (of sequences whose entries overlap or fall back, results are undefined where they meet);
  * nnz * page_size / 16 <= 2^30. A page id outside [0, num_pages) is skipped, never read, and sets *status (device i32, or
  * NULL) to 1. An array per page-table entry is [num_kv_heads, nnz], one per block
  * [num_kv_heads, nnz * page_size / block_size]: entry e's blocks at e * page_size / block_size.

@@ -350,6 +350,46 @@ def test_decode_skips_bad_pages_and_bad_lists(dev):
     assert status == 1 and not out.any()
 
 
+def test_offsets_that_fall_back_or_leave_the_table(dev):
+    """Sequences overlap, run backwards or end past the table: nothing leaves an array, and what does not meet is right."""
+    c = make([150, 150, 150, 150, 150, 150], 4, 2, 64, 32)
+    nnz = c["idx"].numel()
+    c["cache"].nan_to_num_(0.5)
+    c["ptr"] = torch.tensor([0, 5, -4, 3, 2**31 - 1, 1, nnz], dtype=torch.int32)
+    c["last"][:] = torch.tensor([32, 9, 40, -3, 5, 2**31 - 1], dtype=torch.int32)
+    spans = [(0, 5), (5, 5), (0, 3), (3, nnz), (nnz, nnz), (1, nnz)]
+    blocks = torch.tensor([0, 1, 3, 5, -1], dtype=torch.int32).expand(6, 2, 5).contiguous()
+    t = table(c, dev)
+    cache, q = c["cache"].to(dev), c["q"].to(dev)
+    got = axk.paged_decode_blocks(q, cache, *t, blocks=blocks.to(dev), block_size=16)
+    for b, (lo, hi) in enumerate(spans):
+        last = min(max(int(c["last"][b]), 0), 32) if hi > lo else 0
+        ref, _, slack, _ = ob.decode_blocks(c["q"][b:b + 1], c["cache"], torch.tensor([0, hi - lo]), c["idx"][lo:hi],
+                                            torch.tensor([last]), blocks[b:b + 1], 16)
+        within(got[b:b + 1], ref, slack + ref.abs() * 2.0 ** -8)
+    w = torch.ones(2, nnz, device=dev)
+    axk.paged_decode_blocks(q, cache, *t, weights_in=w, weights=w)
+    bounds = axk.paged_key_bounds(cache, empty_bounds(c, 16).to(dev), *t)
+    scores = axk.paged_block_scores(q, bounds, *t, 32)
+    picked = axk.paged_select_blocks(scores, t[0], t[2], 32, 16, 4).cpu()
+    for b, (lo, hi) in enumerate(spans):
+        assert (picked[b] < 2 * (hi - lo)).all() and (picked[b] >= -1).all()
+    p, i, ww, f = axk.paged_evict_pages(torch.rand(2, nnz, device=dev), t[0], t[1], 3)
+    assert p.tolist() == [0, 3, 3, 6, 9, 9, 12]
+    assert set(i.tolist()) <= set(c["idx"].tolist()) | {-1}
+
+
+def test_evict_offsets_whose_sums_pass_32_bits(dev):
+    n = 1 << 18
+    ptr = torch.zeros(20001, dtype=torch.int32)
+    ptr[1::2] = n  # 10000 sequences of the whole table, and as many that fall back
+    idx = torch.arange(n, dtype=torch.int32, device=dev)
+    for budget in (n, 300):
+        p, i, w, f = axk.paged_evict_pages(torch.ones(1, n, device=dev), ptr.to(dev), idx, budget)
+        assert p[:3].tolist() == [0, budget, budget]
+        assert int(i.min()) >= -1 and int(i.max()) < n and int(f.min()) >= -1 and int(f.max()) < n
+
+
 def test_decode_extreme_scores(dev):
     """Scores of thousands, all equal ones, and a sign-flipped scale."""
     c = make([500, 33], 16, 2, 128, 64)
