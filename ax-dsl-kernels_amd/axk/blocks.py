@@ -1,7 +1,7 @@
 """Sparse attention over a paged KV cache on gfx950, and eviction of its pages.
 
-A page is cut into blocks of consecutive tokens; ``bounds`` keeps every block's channel-wise minimum and maximum key. One
-decode step of a layer is then::
+A page is cut into blocks of consecutive tokens; ``bounds`` keeps every block's channel-wise minimum and maximum key
+(rounded outward to bf16 where it holds more bits, in an INT8 cache). One decode step of a layer is then::
 
     store_paged_kv_bounds(k, v, kv_cache, bounds, cache_location)          # the new tokens
     scores = paged_block_scores(q, bounds, indptr, indices, last, page)    # an upper bound of q . k per block

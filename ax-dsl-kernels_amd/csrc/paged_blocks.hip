@@ -2,7 +2,8 @@
 //
 // A page of the cache (layout and page table as in paged_attn.hip) is cut into blocks of `block` consecutive tokens
 // (block a multiple of 16 that divides the page). For every block and KV head, bounds[P, page / block, HKV, 2, D]
-// (bf16) keeps the channel-wise minimum and maximum of the block's keys. One decode step is then
+// (bf16) keeps the channel-wise minimum and maximum of the block's keys, rounded outward where bf16 does not hold them
+// (int8 caches). One decode step is then
 //   1. paged_kv_write_bounds_kernel  the new tokens' K / V into the cache and into their blocks' bounds
 //      (paged_key_bounds_kernel      the bounds from the cache: after a prefill chunk, or for a whole cache)
 //   2. paged_block_scores_kernel     s[h, j] = max_g sum_d max(q_gd, 0) hi_jd + min(q_gd, 0) lo_jd, which no q_g . k of
@@ -89,26 +90,36 @@ AXK_DEV uint32_t bf16_unorder(axk_s16x2 x) { return __builtin_bit_cast(uint32_t,
 // bf16 scale per row and KV head, attended as code * scale.
 enum { kBf16 = 0, kFp8 = 1, kI8 = 2 };
 
-// Bytes 2 hi and 2 hi + 1 of w, int8 codes, as a bf16 pair of code * s.
-AXK_DEV uint32_t i8_pair(uint32_t w, int hi, float s = 1.0f) {
-  const float x = (float)(int8_t)(w >> (16 * hi)), y = (float)(int8_t)(w >> (16 * hi + 8));
-  return pack_bf16x2(x * s, y * s);
-}
-// A dword of stored 8-bit values as two bf16 pairs (int8 codes times s).
+// Byte i of w, an int8 code, as a float.
+AXK_DEV float i8_code(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
+// A dword of stored 8-bit values as two bf16 pairs (int8: the codes, exact in bf16).
 template <int T>
-AXK_DEV uint32_t pair_of(uint32_t w, int hi, float inv_scale, float s = 1.0f) {
-  if constexpr (T == kI8) return i8_pair(w, hi, s);
+AXK_DEV uint32_t pair_of(uint32_t w, int hi, float inv_scale) {
+  if constexpr (T == kI8) return pack_bf16x2(i8_code(w, 2 * hi), i8_code(w, 2 * hi + 1));
   return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, inv_scale, true)
                                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, inv_scale, false));
 }
+// An int8 key, code * scale, has up to 16 significant bits and is attended unrounded, so its bf16 bounds are rounded
+// outward: x down and up to bf16, in the high half of a dword (a magnitude's low half carries into the high one where the
+// value moves away from zero). NaN goes past the infinity of either side.
+AXK_DEV uint32_t bf16_down(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return x != x ? 0xffff0000u : u + ((uint32_t)((int)u >> 31) >> 16);
+}
+AXK_DEV uint32_t bf16_up(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return x != x ? 0x7fff0000u : u + (~(uint32_t)((int)u >> 31) >> 16);
+}
+AXK_DEV uint32_t high_halves(uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x07060302u); }
+
 // 16 bytes of stored keys as bf16 pairs in order: 4 dwords of a bf16 cache, 8 of an 8-bit one.
 template <int T>
-AXK_DEV void stored_pairs(const axk_u32x4 w, float inv_scale, float s, uint32_t (&out)[T ? 8 : 4]) {
+AXK_DEV void stored_pairs(const axk_u32x4 w, float inv_scale, uint32_t (&out)[T ? 8 : 4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (T) {
-      out[2 * i] = pair_of<T>(w[i], 0, inv_scale, s);
-      out[2 * i + 1] = pair_of<T>(w[i], 1, inv_scale, s);
+      out[2 * i] = pair_of<T>(w[i], 0, inv_scale);
+      out[2 * i + 1] = pair_of<T>(w[i], 1, inv_scale);
     } else {
       out[i] = w[i];
     }
@@ -125,16 +136,17 @@ constexpr int64_t kMaxRows = 16384;  // every row looks at every other's place: 
 // 16 rows of a decode step (HKV 2, D 256), 2.3 without the bounds, 4.5 for 16 rows of one block.
 //
 // Eight channels of a new row as the cache keeps them: their bytes (a bf16 cache: the values themselves), the int8 scale,
-// and the key's bf16 pairs as attention reads them. The d / 8 lanes of a head's row act together.
+// and the key's bf16 pairs as attention reads them, rounded down and up where they have more bits (int8). The d / 8 lanes of
+// a head's row act together.
 struct Stored {
-  uint32_t lo, hi;   // 8-bit caches: the eight bytes
-  float scale;       // int8
-  uint32_t pair[4];  // as attended
+  uint32_t lo, hi;            // 8-bit caches: the eight bytes
+  float scale;                // int8
+  uint32_t down[4], up[4];
 };
 template <int T>
 AXK_DEV Stored store_eight(const uint4 src, int d, float kv_scale) {
   const uint32_t w[4] = {src.x, src.y, src.z, src.w};
-  Stored o = {0u, 0u, 0.f, {w[0], w[1], w[2], w[3]}};
+  Stored o = {0u, 0u, 0.f, {w[0], w[1], w[2], w[3]}, {w[0], w[1], w[2], w[3]}};
   if constexpr (T == kBf16) return o;
   float x[8];
 #pragma unroll
@@ -154,7 +166,16 @@ AXK_DEV Stored store_eight(const uint4 src, int d, float kv_scale) {
     if (e < 4) o.lo |= c << (8 * e); else o.hi |= c << (8 * (e - 4));
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o.pair[i] = pair_of<T>(i < 2 ? o.lo : o.hi, i & 1, 1.0f / kv_scale, o.scale);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = i < 2 ? o.lo : o.hi;
+    if constexpr (T == kI8) {
+      const float y0 = i8_code(b, 2 * (i & 1)) * o.scale, y1 = i8_code(b, 2 * (i & 1) + 1) * o.scale;
+      o.down[i] = high_halves(bf16_down(y0), bf16_down(y1));
+      o.up[i] = high_halves(bf16_up(y0), bf16_up(y1));
+    } else {
+      o.down[i] = o.up[i] = pair_of<T>(b, i & 1, 1.0f / kv_scale);
+    }
+  }
   return o;
 }
 
@@ -241,8 +262,8 @@ __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
           const Stored o = store_eight<T>(x[j], d, kv_scale);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            lo[e] = __builtin_elementwise_min(lo[e], bf16_order(o.pair[e]));
-            hi[e] = __builtin_elementwise_max(hi[e], bf16_order(o.pair[e]));
+            lo[e] = __builtin_elementwise_min(lo[e], bf16_order(o.down[e]));
+            hi[e] = __builtin_elementwise_max(hi[e], bf16_order(o.up[e]));
           }
         }
       }
@@ -255,9 +276,11 @@ __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
 // The bounds of every block of the page table that reaches past start[b] (all of them without start), from the cache.
 // One workgroup per block: its K rows are one contiguous run of tokens x HKV x D values, read 16 bytes a lane, a column
 // of 8 (8-bit caches: 16) channels kept by as many lanes as the workgroup has to spare and joined through LDS. Minimum and
-// maximum are taken on the bf16 bits as ordered 16-bit integers, two values an instruction. Bound by the K bytes: 136,000
+// maximum are taken on the bf16 bits as ordered 16-bit integers, two values an instruction; of an int8 cache in fp32, which
+// holds code * scale exactly, and rounded outward once a lane. Bound by the K bytes: 136,000
 // tokens of an FP8 cache (HKV 2, D 256, blocks of 32) 18.7 us, 84 MB at 4.5 TB/s; without minimum and maximum at all 4%
-// less, with non-temporal loads 8% more, and 1.5 us more while lanes stored dwords 32 bytes apart.
+// less, with non-temporal loads 8% more, and 1.5 us more while lanes stored dwords 32 bytes apart. As an int8 cache the
+// same tokens take 25.3 us (22.8 with keys rounded to nearest, which bounds nothing).
 template <int T>
 __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
     const unsigned char* __restrict__ cache, const uint16_t* __restrict__ scales, uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
@@ -296,17 +319,42 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
       lo[e] = (axk_s16x2)(short)0x7fff;
       hi[e] = (axk_s16x2)(short)-0x8000;
     }
+    float lof[T == kI8 ? E : 1], hif[T == kI8 ? E : 1];  // int8 keys in fp32, where the product is exact; NaN stays
+    if constexpr (T == kI8) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        lof[e] = INFINITY;
+        hif[e] = -INFINITY;
+      }
+    }
     if (rl < lanes) {
 #pragma unroll 4
       for (int t = rl; t < rows; t += lanes) {
-        uint32_t x[N];
-        const float s = T == kI8 ? bf16_bits_to_f32(sc[(int64_t)t * hkv]) : 1.0f;
-        stored_pairs<T>(*reinterpret_cast<const axk_u32x4*>(src + ((int64_t)t * row + c * E) * B), inv_scale, s, x);
+        const axk_u32x4 w4 = *reinterpret_cast<const axk_u32x4*>(src + ((int64_t)t * row + c * E) * B);
+        if constexpr (T == kI8) {
+          const float s = bf16_bits_to_f32(sc[(int64_t)t * hkv]);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          lo[e] = __builtin_elementwise_min(lo[e], bf16_order(x[e]));
-          hi[e] = __builtin_elementwise_max(hi[e], bf16_order(x[e]));
+          for (int e = 0; e < E; ++e) {
+            const float x = i8_code(w4[e / 4], e % 4) * s;
+            lof[e] = __builtin_elementwise_minimum(lof[e], x);
+            hif[e] = __builtin_elementwise_maximum(hif[e], x);
+          }
+        } else {
+          uint32_t x[N];
+          stored_pairs<T>(w4, inv_scale, x);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            lo[e] = __builtin_elementwise_min(lo[e], bf16_order(x[e]));
+            hi[e] = __builtin_elementwise_max(hi[e], bf16_order(x[e]));
+          }
         }
+      }
+    }
+    if constexpr (T == kI8) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        lo[e] = bf16_order(high_halves(bf16_down(lof[2 * e]), bf16_down(lof[2 * e + 1])));
+        hi[e] = bf16_order(high_halves(bf16_up(hif[2 * e]), bf16_up(hif[2 * e + 1])));
       }
     }
     __syncthreads();
@@ -895,7 +943,7 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
 #pragma unroll
       for (int i = 0; i < C::KL; ++i) {
         uint32_t x[T ? 8 : 4];
-        stored_pairs<T>(*reinterpret_cast<const axk_u32x4*>(kbuf + u * kSub * C::RB + (k_at ^ (64 * i))), a.inv_scale, 1.0f, x);
+        stored_pairs<T>(*reinterpret_cast<const axk_u32x4*>(kbuf + u * kSub * C::RB + (k_at ^ (64 * i))), a.inv_scale, x);
         const axk_u32x4 x0 = {x[0], x[1], x[2], x[3]};
         sc[u] = mfma_bf16_16x16x32(__builtin_bit_cast(axk_bf16x8, x0), qf[T ? 2 * i : i], sc[u]);
         if constexpr (T != kBf16) {

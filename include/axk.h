@@ -378,7 +378,8 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  *
  * A page is cut into blocks of block_size consecutive tokens (block_size a multiple of 16 that divides page_size). For
  * every block and KV head, bounds bf16 [num_pages, page_size / block_size, num_kv_heads, 2, head_dim] keeps the
- * channel-wise minimum (0) and maximum (1) of the block's keys, as attention reads them. A decode step writes its tokens
+ * channel-wise minimum (0) and maximum (1) of the block's keys, as attention reads them; an int8 key, code * scale, has up
+ * to 16 significant bits, so that its minimum is rounded down and its maximum up. A decode step writes its tokens
  * with axk_paged_kv_write_bounds, scores every block with axk_paged_block_scores, selects with axk_paged_select_blocks
  * and attends the selection with axk_paged_decode_blocks, which can also add up how much attention every page received;
  * axk_paged_evict_pages cuts a page table down to the pages that received most.
@@ -399,7 +400,7 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  * A block with a new row at its first slot starts afresh; any other widens what it had, so tokens are written in order,
  * and rows written over (rejected drafts) leave bounds that still hold but are wide, until axk_paged_key_bounds computes
  * them again. Rows of one call may share a block; where two name one slot the last one is stored, and both are folded. A
- * location outside the pool is skipped and sets *status. A NaN key makes the bound on its sign's side NaN. rows <= 16384:
+ * location outside the pool is skipped and sets *status. A NaN key makes the bound on its sign's side NaN (int8: both). rows <= 16384:
  * a longer prefill chunk is written by axk_paged_kv_write and its blocks' bounds computed by axk_paged_key_bounds. */
 int axk_paged_kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cache, int kv_dtype, float kv_scale,
                               uint16_t* bounds, const int32_t* cache_location, int64_t rows, int64_t num_kv_heads,

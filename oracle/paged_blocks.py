@@ -34,6 +34,13 @@ def seq_rows(cache, indptr, indices, last, b: int, kv_scale=None):
     return kv[0], kv[1], good.repeat_interleave(page)[:n]
 
 
+def outward(lo: torch.Tensor, hi: torch.Tensor):
+    """(lo rounded down, hi rounded up) to bf16, so that they still contain what they bounded; NaN stays."""
+    a, b = lo.to(torch.bfloat16), hi.to(torch.bfloat16)
+    a = torch.where(a.double() > lo, torch.nextafter(a, torch.full_like(a, -math.inf)), a)
+    return a, torch.where(b.double() < hi, torch.nextafter(b, torch.full_like(b, math.inf)), b)
+
+
 def key_bounds(cache, bounds, indptr, indices, last, start=None, kv_scale=None) -> torch.Tensor:
     out = bounds.clone()
     page = cache.shape[2]
@@ -46,7 +53,7 @@ def key_bounds(cache, bounds, indptr, indices, last, start=None, kv_scale=None) 
                 continue
             rows = k[j * block:min(n, (j + 1) * block)]
             at = int(indices[int(indptr[b]) + j // bpp])
-            out[at, j % bpp] = torch.stack([rows.amin(0), rows.amax(0)], 1).to(torch.bfloat16)
+            out[at, j % bpp] = torch.stack(outward(rows.amin(0), rows.amax(0)), 1)
     return out
 
 
@@ -68,14 +75,14 @@ def store(k, v, cache, bounds, loc, kv_scale=None):
                 row = (row.float() * kv_scale).to(torch.bfloat16).to(torch.float8_e4m3fn).view(torch.uint8)
             cache[a, i, o] = row
             if i == 0:
-                key = attended(row, s).to(torch.bfloat16).double()
+                key = attended(row, s)
         at = (a, o // block)
         if at in fresh and at not in begun:
             out[at] = torch.stack([key, key], 1)
         else:
             out[at] = torch.stack([torch.minimum(out[at][:, 0], key), torch.maximum(out[at][:, 1], key)], 1)
         begun.add(at)
-    return cache, out.to(torch.bfloat16)
+    return cache, torch.stack(outward(out[:, :, :, 0], out[:, :, :, 1]), 3)
 
 
 def block_scores(q, bounds, indptr, indices, last, page: int):

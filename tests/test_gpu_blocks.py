@@ -652,3 +652,62 @@ def test_an_empty_table(dev):
     assert not axk.paged_decode_blocks(q, cache, ptr, idx, last, bl, 16, weights=w).any()
     p, i, ww, f = axk.paged_evict_pages(w, ptr, idx, 4)
     assert not p.any() and i.numel() == ww.numel() == f.numel() == 0
+
+
+# ---- what the bounds promise ----
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "i8"])
+@pytest.mark.parametrize("hq,hkv,d,page,block", [(6, 2, 64, 32, 16), (8, 8, 128, 96, 48), (16, 1, 256, 64, 64)])
+def test_bounds_contain_the_keys_and_scores_bound_the_products(dev, kv, hq, hkv, d, page, block):
+    """In every kind of cache, from the cache and at the write: lo <= key <= hi for the keys as attention reads them, and
+    q . k <= score but for the roundings of the score's fp32 sum."""
+    lens = [1, 16, block + 1, 2 * page + 3, 500]
+    c = make(lens, hq, hkv, d, page, kv, seed=3)
+    bounds = axk.paged_key_bounds(c["cache"].to(dev), empty_bounds(c, block).to(dev), *table(c, dev), **kv_of(c, dev))
+    # the same keys written again, row by row
+    loc = torch.tensor([[int(c["idx"][int(c["ptr"][b]) + t // page]), t % page] for b, n in enumerate(lens)
+                        for t in range(n)], dtype=torch.int32)
+    k = torch.randn(len(loc), hkv, d, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    cache, kvs, folded = c["cache"].to(dev), kv_of(c, dev), empty_bounds(c, block).to(dev)
+    axk.store_paged_kv_bounds(k.to(dev), k.to(dev), cache, folded, loc.to(dev), **kvs)
+    again = dict(c, cache=cache.cpu(), scale=kvs["kv_scales"].cpu() if kv == "i8" else c["scale"])
+    for x, got in ((c, bounds), (again, folded)):
+        scores = axk.paged_block_scores(c["q"].to(dev), got, *table(c, dev), page).cpu().double()
+        got = got.cpu()
+        _, mag = ob.block_scores(c["q"], got, c["ptr"], c["idx"], c["last"], page)
+        for b, n in enumerate(lens):
+            key, _, _ = ob.seq_rows(x["cache"], c["ptr"], c["idx"], c["last"], b, x["scale"])
+            t = torch.arange(n)
+            e, s = int(c["ptr"][b]) + t // page, t % page // block
+            bb = got[c["idx"][e].long(), s].double()
+            assert (bb[:, :, 0] <= key).all() and (key <= bb[:, :, 1]).all()
+            prod = (c["q"][b].double().view(1, hkv, hq // hkv, d) * key[:, :, None]).sum(3).amax(2)
+            at = e * (page // block) + s
+            assert (prod.t() <= scores[:, at] + 2 * d * 2.0 ** -24 * mag[:, at]).all()
+
+
+def test_int8_scales_that_are_not_finite(dev):
+    """A key that is NaN makes both bounds of its channel NaN, at the write as from the cache; infinite keys stay."""
+    page, hkv, d = 32, 2, 64
+    codes = torch.randint(-127, 128, (2, 2, page, hkv, d), generator=torch.Generator().manual_seed(1), dtype=torch.int8)
+    codes[0, 0, 3, 0, :4] = torch.tensor([0, 5, -5, 0], dtype=torch.int8)
+    scales = torch.full((2, 2, page, hkv), 0.0625, dtype=torch.bfloat16)
+    scales[0, 0, 3, 0] = math.inf  # keys NaN, inf, -inf, NaN, ...
+    scales[1, 0, 20, 1] = NAN
+    ptr, idx, last = (torch.tensor(x, dtype=torch.int32) for x in ([0, 2], [0, 1], [page]))
+    empty = torch.zeros(2, 2, hkv, 2, d, dtype=torch.bfloat16)
+    ref = ob.key_bounds(codes, empty, ptr, idx, last, kv_scale=scales)
+    got = axk.paged_key_bounds(codes.to(dev), empty.to(dev), ptr.to(dev), idx.to(dev), last.to(dev),
+                               kv_scales=scales.to(dev)).cpu()
+    assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got.nan_to_num(0.5), ref.nan_to_num(0.5))
+    assert got[0, 0, 0, :, 0].isnan().all() and got[1, 1, 1].isnan().all()
+    assert got[0, 0, 0, 1, 1] == math.inf and got[0, 0, 0, 0, 2] == -math.inf
+    # a row with an infinite value is stored with an infinite scale: code 0 where it was finite
+    k = torch.randn(16, hkv, d, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    k[5, 1, 7] = math.inf
+    loc = torch.tensor([[1, t] for t in range(16)], dtype=torch.int32, device=dev)
+    gc, gs, gb = codes.to(dev), scales.to(dev), empty.to(dev)
+    axk.store_paged_kv_bounds(k.to(dev), k.to(dev), gc, gb, loc, kv_scales=gs)
+    one = torch.tensor([0, 1], dtype=torch.int32)
+    ref = ob.key_bounds(gc.cpu(), empty, one, idx[1:], torch.tensor([16], dtype=torch.int32), kv_scale=gs.cpu())
+    assert torch.equal(gb[1, 0].cpu().isnan(), ref[1, 0].isnan()) and ref[1, 0].isnan().any()
+    assert torch.equal(gb[1, 0].cpu().nan_to_num(0.5), ref[1, 0].nan_to_num(0.5))

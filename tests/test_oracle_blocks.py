@@ -96,3 +96,51 @@ def test_evict_keeps_budget_pages_and_frees_the_rest():
     p, i, ww, f = ob.evict_pages(w, ptr, idx, 3)
     assert p.tolist() == [0, 3, 3, 5] and i.tolist() == [10, 13, 14, 15, 16, -1, -1]
     assert f.tolist() == [11, 12, -1, -1, -1, -1, -1] and ww[0].tolist() == [5, 3, 9, 0, 7, 0, 0]
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "i8"])
+@pytest.mark.parametrize("page,block", [(32, 16), (48, 48), (16, 16)])
+def test_bounds_contain_and_scores_bound_in_every_cache(kv, page, block):
+    """lo <= key <= hi and q . k <= score for the keys as attention reads them (int8: code * scale, unrounded), where the
+    bounds come from the cache and where they are folded at the write, one-token blocks among them."""
+    lens, hq, hkv, d = [1, 16, 70, 33], 6, 2, 64
+    c = case(lens, hq, hkv, d, page, seed=7)
+    cache, ptr, idx, last, scale = c["cache"], c["indptr"], c["indices"], c["last_page_len"], None
+    if kv == "fp8":
+        scale = 8.0
+        cache = (cache * scale).to(torch.float8_e4m3fn).view(torch.uint8)
+    elif kv == "i8":
+        cache, scale = paged_attn.quant_kv_i8(cache)
+    empty = torch.zeros(cache.shape[0], page // block, hkv, 2, d, dtype=torch.bfloat16)
+    read = ob.key_bounds(cache, empty, ptr, idx, last, kv_scale=scale)
+    loc = torch.tensor([[int(idx[int(ptr[b]) + t // page]), t % page] for b, n in enumerate(lens) for t in range(n)],
+                       dtype=torch.int32)
+    written, folded = ob.store(*c["cache"][loc[:, 0].long(), :, loc[:, 1].long()].unbind(1), cache, empty, loc, scale)
+    assert torch.equal(written.view(torch.uint8), cache.view(torch.uint8)) and torch.equal(folded, read)
+    scores, mag = ob.block_scores(c["q"], read, ptr, idx, last, page)
+    bpp = page // block
+    for b, n in enumerate(lens):
+        k, _, _ = ob.seq_rows(cache, ptr, idx, last, b, scale)
+        prod = (c["q"][b].double().view(1, hkv, hq // hkv, d) * k[:, :, None]).sum(3).amax(2)  # [t, HKV]
+        for t in range(n):
+            e, s = int(ptr[b]) + t // page, t % page // block
+            bb = read[idx[e].long(), s].double()
+            assert (bb[:, 0] <= k[t]).all() and (k[t] <= bb[:, 1]).all()
+            # sums of D terms in 64 bits on both sides
+            assert (prod[t] <= scores[:, e * bpp + s] + 2 * d * 2.0 ** -53 * mag[:, e * bpp + s]).all()
+
+
+def test_bounds_of_an_int8_cache_are_the_tightest_in_bf16():
+    """The minimum rounded down and the maximum rounded up by less than a step; a NaN key makes both NaN."""
+    x = torch.tensor([-3.0, -1.00390625, -1.0, -0.0, 0.0, 1.0, 1.00390625, 3.0], dtype=torch.float64)
+    lo, hi = ob.outward(x, x)
+    assert lo.dtype == hi.dtype == torch.bfloat16
+    assert lo.tolist() == [-3.0, -1.0078125, -1.0, 0.0, 0.0, 1.0, 1.0, 3.0]
+    assert hi.tolist() == [-3.0, -1.0, -1.0, 0.0, 0.0, 1.0, 1.0078125, 3.0]
+    top = torch.finfo(torch.bfloat16).max  # past it: the largest finite value inside, infinity outside
+    assert [float(t) for t in ob.outward(*2 * [torch.tensor(1.001 * top, dtype=torch.float64)])] == [top, math.inf]
+    y = torch.randn(4096, generator=torch.Generator().manual_seed(0)).double()
+    lo, hi = ob.outward(y, y)
+    step = torch.where(lo.double() == y, 0.0, y.abs() * 2.0 ** -7)
+    assert (lo.double() <= y).all() and (y <= hi.double()).all() and (hi.double() - lo.double() <= step).all()
+    assert all(t.isnan().all() for t in ob.outward(torch.tensor([math.nan]).double(), torch.tensor([math.nan]).double()))
