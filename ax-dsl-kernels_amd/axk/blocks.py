@@ -185,7 +185,7 @@ def paged_block_scores(
     status: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """f32 [HKV, nnz * page_size / block_size]: for each KV head and block of the page table, the largest
-    sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d over the KV head's queries of q [B, HQ, D] bf16, which no q . k in the block
+    sum_d max(q_d lo_d, q_d hi_d) over the KV head's queries of q [B, HQ, D] bf16, which no q . k in the block
     exceeds. -inf past a sequence's end. Entry e's blocks are columns e * page_size / block_size onwards."""
     b = _table(indptr, last_page_len, indices)
     shape = q.shape

@@ -6,8 +6,7 @@
 // (int8 caches). One decode step is then
 //   1. paged_kv_write_bounds_kernel  the new tokens' K / V into the cache and into their blocks' bounds
 //      (paged_key_bounds_kernel      the bounds from the cache: after a prefill chunk, or for a whole cache)
-//   2. paged_block_scores_kernel     s[h, j] = max_g sum_d max(q_gd, 0) hi_jd + min(q_gd, 0) lo_jd, which no q_g . k of
-//                                    block j exceeds
+//   2. paged_block_scores_kernel     s[h, j] = max_g sum_d max(q_gd lo_jd, q_gd hi_jd), which no q_g . k of block j exceeds
 //   3. paged_select_blocks_kernel    the n best blocks of each (sequence, KV head), in ascending order
 //   4. paged_blocks_kernel, paged_blocks_merge_kernel   attention over those blocks (or all of them), and each page's
 //                                    share of it, w_out = decay w_in + sum over the KV head's queries
@@ -385,6 +384,27 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
 // bounds' bytes: 8 sequences of 131072 tokens in blocks of 64 (HKV 4, D 256) 16.3 us, 67 MB at 4.1 TB/s, all of its waves
 // at once. With the rows through LDS as in the decode below the same took 18.2 us, since half as many waves fit (and one
 // sequence of 5003 tokens 4.6 against 5.5).
+//
+// Where a bound is infinite, the product that the split leaves at zero is 0 inf = NaN, though max(q lo, q hi) is not. So a
+// block whose sum came out NaN is summed again as the formula stands, head by head, after the others: a lane's block and
+// channels as there, its bounds read again (kept, they would cost every wave registers: 160 instead of 92 at D 256).
+template <int D>
+AXK_DEV float plain_score(const uint16_t* __restrict__ q, const uint16_t* __restrict__ row, int group) {
+  float best = -INFINITY;
+#pragma unroll 1
+  for (int head = 0; head < group; ++head) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < D; d += 32) {
+      const axk_bf16x8 x = load_bf16x8(q + (int64_t)head * D + d), lo = load_bf16x8(row + d), hi = load_bf16x8(row + D + d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += __builtin_elementwise_maximum((float)x[e] * (float)lo[e], (float)x[e] * (float)hi[e]);
+    }
+    best = __builtin_elementwise_maximum(best, xor32_sum(xor16_sum(sum)));
+  }
+  return best;
+}
+
 template <int D>
 __global__ __launch_bounds__(256) void paged_block_scores_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
@@ -412,6 +432,7 @@ __global__ __launch_bounds__(256) void paged_block_scores_kernel(
     lo[s] = load_bf16x8(row + 32 * s);
     hi[s] = load_bf16x8(row + D + 32 * s);
   }
+  int again = 0;  // lane 16 g, bit i: the sum of block 4 g + i came out NaN
   for (int b = own.b; b < batch; ++b) {  // the sequences whose entries reach into the tile
     const Seq sq = b == own.b ? own.s : seq_of(indptr, last, b, page_size, nnz);
     if (sq.pb > e1) break;
@@ -444,8 +465,19 @@ __global__ __launch_bounds__(256) void paged_block_scores_kernel(
         const bool there = t0 < sq.len;
         scores[(int64_t)h * total + fi] = there && !bad ? x : -INFINITY;
         if (there && bad && status) *status = 1;
+        if (there && !bad && x != x) again |= 1 << i;
       }
     }
+  }
+  if (!__any(again)) return;
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");  // the NaNs are stored before what replaces them
+  again = __shfl(again, 16 * (l16 >> 2), 64) >> (l16 & 3) & 1;  // of this lane's block
+  for (int b = own.b; b < batch; ++b) {
+    const Seq sq = seq_of(indptr, last, b, page_size, nnz);
+    if (sq.pb > e1) break;
+    const float x = plain_score<D>(q + ((int64_t)b * hq + h * group) * D + 8 * g, row, group);
+    const int64_t t0 = (int64_t)(f - sq.pb * bpp) * block;
+    if (g == 0 && again && t0 >= 0 && t0 < sq.len) scores[(int64_t)h * total + f] = x;
   }
 }
 

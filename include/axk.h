@@ -425,7 +425,7 @@ int axk_paged_key_bounds_i8(const int8_t* kv_cache, const uint16_t* kv_scales, u
                             int64_t num_pages, int32_t* status, axk_stream_t stream);
 
 /* scores f32 [num_kv_heads, nnz * page_size / block_size]: for q bf16 [batch, num_qo_heads, head_dim], entry (h, j) is
- *   max over the query heads g of KV head h of sum_d max(q_gd, 0) hi_jd + min(q_gd, 0) lo_jd,
+ *   max over the query heads g of KV head h of sum_d max(q_gd lo_jd, q_gd hi_jd),
  * which no q_g . k of the block exceeds (softmax scale left out: it does not change the order). -inf for a block past its
  * sequence's end or on a bad page; entries of no sequence (past indptr[batch]) are left as they are. */
 int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds, const int32_t* indptr, const int32_t* indices,

@@ -711,3 +711,30 @@ def test_int8_scales_that_are_not_finite(dev):
     ref = ob.key_bounds(gc.cpu(), empty, one, idx[1:], torch.tensor([16], dtype=torch.int32), kv_scale=gs.cpu())
     assert torch.equal(gb[1, 0].cpu().isnan(), ref[1, 0].isnan()) and ref[1, 0].isnan().any()
     assert torch.equal(gb[1, 0].cpu().nan_to_num(0.5), ref[1, 0].nan_to_num(0.5))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (7, 1, 128), (32, 2, 256)])
+def test_scores_of_infinite_bounds(dev, hq, hkv, d):
+    """max(q lo, q hi) is finite, or infinite, where one bound is infinite; NaN only where q is zero there or infinities of
+    both signs meet. The other blocks of a tile and the other heads are not touched."""
+    page, block = 64, 16
+    c = make([500, 40], hq, hkv, d, page, seed=d)
+    bounds = ob.key_bounds(c["cache"], empty_bounds(c, block), c["ptr"], c["idx"], c["last"])
+    p = c["idx"].long()
+    c["q"][:, :, :4] = torch.tensor([2.0, -2.0, 0.0, 1.0]).to(torch.bfloat16)
+    bounds[p[0], 0, :, 0, 0] = -math.inf  # finite: the other bound decides
+    bounds[p[0], 1, :, 1, 1] = math.inf   # finite
+    bounds[p[0], 2, :, 1, 0] = math.inf   # +inf
+    bounds[p[0], 3, :, :, 0] = -math.inf  # -inf
+    bounds[p[1], 0, :, 0, 2] = -math.inf  # 0 * inf
+    bounds[p[1], 1, :, 1, 0], bounds[p[1], 1, :, 1, 1] = math.inf, -math.inf
+    bounds[p[1], 1, :, 0, 1] = -math.inf  # +inf twice
+    bounds[p[1], 2, :, 1, 0], bounds[p[1], 2, :, :, 3] = math.inf, -math.inf  # inf - inf
+    bounds[p[1], 3, 0, 0, 0] = -math.inf  # one KV head only
+    ref, mag = ob.block_scores(c["q"], bounds, c["ptr"], c["idx"], c["last"], page)
+    got = axk.paged_block_scores(c["q"].to(dev), bounds.to(dev), *table(c, dev), page).cpu().double()
+    assert ref[0, [0, 1, 7]].isfinite().all() and ref[0, 2] == ref[0, 5] == math.inf and ref[0, 3] == -math.inf
+    assert ref[0, 4].isnan() and ref[0, 6].isnan()
+    there = ref.isfinite()
+    assert torch.equal(got[~there].nan_to_num(0.5), ref[~there].nan_to_num(0.5))
+    assert ((got - ref).abs()[there] <= (2 * d * 2.0 ** -24 * mag)[there]).all()
