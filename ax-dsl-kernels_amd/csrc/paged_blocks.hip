@@ -1480,6 +1480,9 @@ namespace {
 
 constexpr int64_t kMaxSubs = 1 << 30;  // subtiles of a page table, or of a row's listed blocks: sums of them fit 32 bits
 
+// Whether a dimension of a launch holds these workgroups: its threads are counted in 32 bits.
+bool launch_fits(int64_t workgroups, int threads) { return workgroups <= (int64_t)0xffffffff / threads; }
+
 int check_blocks(int64_t batch, int64_t hkv, int64_t d, int64_t page_size, int64_t block, int64_t num_pages, int64_t nnz) {
   AXK_REQUIRE(batch > 0 && batch <= (1 << 20) && hkv > 0 && hkv <= 4096, AXK_E_SHAPE);
   AXK_REQUIRE(d == 64 || d == 128 || d == 256, AXK_E_SHAPE);
@@ -1506,7 +1509,9 @@ size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 constexpr int64_t kPieces = 512;
 struct BlkPlan {
   int ps, pieces;
+  int split;            // workgroups of the merge that share a row's output, four values a lane
   bool direct;
+  bool fits;            // both launches
   size_t ml, po, stat;  // bytes of each workspace part
 };
 BlkPlan blk_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t page, int64_t nnz, int64_t block, int64_t n,
@@ -1526,6 +1531,9 @@ BlkPlan blk_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t page
   p.ml = p.direct ? 0 : round256(items * group * sizeof(float2));
   p.po = p.direct ? 0 : round256(items * group * d * sizeof(float));
   p.stat = weights ? round256((size_t)(n ? rows : hkv) * subs * group * sizeof(float2)) : 0;
+  p.split = (int)((group * d / 4 + 63) / 64);
+  p.fits = launch_fits(n ? rows * p.pieces : p.pieces, 256) &&
+           (p.direct || launch_fits(rows * p.split + (weights ? (n ? rows : hkv * p.pieces) : 0), 256));
   return p;
 }
 
@@ -1587,6 +1595,7 @@ int key_bounds(const void* kv_cache, int type, float kv_scale, const uint16_t* k
               AXK_E_NULL);
   const int rc = check_blocks(batch, hkv, d, page_size, block_size, num_pages, nnz);
   if (rc != AXK_OK) return rc;
+  AXK_REQUIRE(launch_fits(nnz * (page_size / block_size), 256), AXK_E_SHAPE);
   if (type < 0) return -type;
   AXK_REQUIRE(axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16) && axk_aligned(kv_scales, 2), AXK_E_ALIGN);
   const size_t row = (size_t)hkv * d, slots = (size_t)num_pages * page_size * 2;
@@ -1651,16 +1660,15 @@ extern "C" int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds,
   const int rc = check_blocks(batch, num_kv_heads, head_dim, page_size, block_size, num_pages, nnz);
   if (rc != AXK_OK) return rc;
   AXK_REQUIRE(num_qo_heads > 0 && num_qo_heads % num_kv_heads == 0 && num_qo_heads / num_kv_heads <= kMaxGroup, AXK_E_SHAPE);
+  const int64_t total = nnz * (page_size / block_size), units = (total + 15) / 16 * num_kv_heads;
+  AXK_REQUIRE(launch_fits((units + 3) / 4, 256), AXK_E_SHAPE);
   AXK_REQUIRE(axk_aligned(q, 16) && axk_aligned(bounds, 16) && axk_aligned(scores, 4), AXK_E_ALIGN);
   if (nnz == 0) return AXK_OK;
-  const int64_t total = nnz * (page_size / block_size);
   const size_t out = (size_t)num_kv_heads * total * 4;
   AXK_REQUIRE(!axk_overlap(scores, out, q, (size_t)batch * num_qo_heads * head_dim * 2) &&
                   !axk_overlap(scores, out, bounds,
                                (size_t)num_pages * (page_size / block_size) * num_kv_heads * head_dim * 4),
               AXK_E_ALIAS);
-  const int64_t units = (total + 15) / 16 * num_kv_heads;
-  AXK_REQUIRE(units <= 0x7fffffff, AXK_E_SHAPE);
   AXK_LAUNCH_GATE();
   auto* fn = head_dim == 64 ? &paged_block_scores_kernel<64>
                             : head_dim == 128 ? &paged_block_scores_kernel<128> : &paged_block_scores_kernel<256>;
@@ -1678,15 +1686,17 @@ extern "C" int axk_paged_select_blocks(const float* scores, const int32_t* indpt
   const int rc = check_blocks(batch, num_kv_heads, 64, page_size, block_size, 1, nnz);
   if (rc != AXK_OK) return rc;
   AXK_REQUIRE(num_select > 0 && num_select <= (1 << 24) && first >= 0 && keep_last >= 0 &&
-                  first + keep_last <= num_select && batch * num_kv_heads <= 0x7fffffff,
+                  first + keep_last <= num_select,
               AXK_E_SHAPE);
-  AXK_REQUIRE(axk_aligned(scores, 4) && axk_aligned(blocks, 4), AXK_E_ALIGN);
   const int64_t total = nnz * (page_size / block_size);
+  const bool small = total <= 2048;  // every row at most eight keys a thread of 256
+  AXK_REQUIRE(launch_fits(batch * num_kv_heads, small ? 256 : 1024), AXK_E_SHAPE);
+  AXK_REQUIRE(axk_aligned(scores, 4) && axk_aligned(blocks, 4), AXK_E_ALIGN);
   AXK_REQUIRE(!axk_overlap(blocks, (size_t)batch * num_kv_heads * num_select * 4, scores, (size_t)num_kv_heads * total * 4),
               AXK_E_ALIAS);
   AXK_LAUNCH_GATE();
   const dim3 grid((unsigned)(batch * num_kv_heads));
-  if (total <= 2048)  // every row at most eight keys a thread of 256
+  if (small)
     hipLaunchKernelGGL(paged_select_blocks_kernel<256>, grid, dim3(256), 0, axk_stream(stream), scores, indptr,
                        last_page_len, blocks, (int)nnz, (int)num_kv_heads, (int)page_size, (int)block_size,
                        (int)num_select, (int)first, (int)keep_last);
@@ -1705,7 +1715,7 @@ extern "C" size_t axk_paged_decode_blocks_workspace_size(int64_t batch, int64_t 
   if (num_select < 0 || num_select > kMaxSubs || num_select * (block_size / kSub) > kMaxSubs) return 0;
   const BlkPlan p = blk_plan(batch, num_qo_heads, num_kv_heads, head_dim, page_size, nnz, block_size, num_select,
                              with_weights != 0);
-  return p.ml + p.po + p.stat;
+  return p.fits ? p.ml + p.po + p.stat : 0;
 }
 
 namespace {
@@ -1735,12 +1745,9 @@ int decode_blocks(const uint16_t* q, const void* kv_cache, int type, float kv_sc
               AXK_E_ALIGN);
   const bool weights = weights_out && nnz > 0;
   const BlkPlan p = blk_plan(batch, num_qo_heads, num_kv_heads, head_dim, page_size, nnz, block_size, num_select, weights);
+  AXK_REQUIRE(p.fits, AXK_E_SHAPE);
   const size_t need = p.ml + p.po + p.stat;
   AXK_REQUIRE(!need || (workspace && workspace_bytes >= need && axk_aligned(workspace, 256)), AXK_E_WORKSPACE);
-  const int64_t grid = blocks ? batch * num_kv_heads * p.pieces : p.pieces;
-  const int split = (int)(num_qo_heads / num_kv_heads * head_dim / 4 + 63) / 64;  // four values a lane
-  const int64_t wgs = batch * num_kv_heads * split + (weights ? (blocks ? batch : (int64_t)p.pieces) * num_kv_heads : 0);
-  AXK_REQUIRE(grid <= 0x7fffffff && wgs <= 0x7fffffff, AXK_E_SHAPE);
   const size_t qb = (size_t)batch * num_qo_heads * head_dim * 2, wb = (size_t)num_kv_heads * nnz * 4;
   const size_t cache = (size_t)num_pages * page_size * num_kv_heads * head_dim * (type ? 2 : 4);
   AXK_REQUIRE(!axk_overlap(out, qb, q, qb) && !axk_overlap(out, qb, kv_cache, cache) && !axk_overlap(out, qb, workspace, need) &&
@@ -1786,7 +1793,7 @@ int decode_blocks(const uint16_t* q, const void* kv_cache, int type, float kv_sc
                                     BlkCfg<256, kBf16>::LDS))
       return e;
   }
-  const WeightArgs w = {weights_in, weights ? weights_out : nullptr, decay, split};
+  const WeightArgs w = {weights_in, weights ? weights_out : nullptr, decay, p.split};
   AXK_LAUNCH_GATE();
   switch (head_dim) {
     case 64: return launch_blocks<64>(a, w, type, axk_stream(stream));

@@ -390,8 +390,10 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  * axk_paged_kv_write_i8, read as code * scale (head_dim 64 too). nnz: the entries of indices; offsets of indptr past it
  * are read as nnz, negative ones as 0, and a last_page_len past page_size as page_size, so that no access leaves an array
  * (of sequences whose entries overlap or fall back, results are undefined where they meet);
- * nnz * page_size / 16 <= 2^30. A page id outside [0, num_pages) is skipped, never read, and sets *status (device i32, or
- * NULL) to 1. An array per page-table entry is [num_kv_heads, nnz], one per block
+ * nnz * page_size / 16 <= 2^30, batch <= 2^20, and a launch holds fewer than 2^32 threads: more is refused with AXK_E_SHAPE
+ * (key bounds: 2^24 blocks in the table; scores: 2^26 times 16 blocks of a head; selection: 2^22 rows, 2^24 of up to 2048
+ * blocks in the table; decode: 2^24 pieces, of 128 to 2048 tokens). A page id outside [0, num_pages) is skipped, never read,
+ * and sets *status (device i32, or NULL) to 1. An array per page-table entry is [num_kv_heads, nnz], one per block
  * [num_kv_heads, nnz * page_size / block_size]: entry e's blocks at e * page_size / block_size.
  * ------------------------------------------------------------------------------------------- */
 
@@ -400,8 +402,9 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  * A block with a new row at its first slot starts afresh; any other widens what it had, so tokens are written in order,
  * and rows written over (rejected drafts) leave bounds that still hold but are wide, until axk_paged_key_bounds computes
  * them again. Rows of one call may share a block; where two name one slot the last one is stored, and both are folded. A
- * location outside the pool is skipped and sets *status. A NaN key makes the bound on its sign's side NaN (int8: both). rows <= 16384:
- * a longer prefill chunk is written by axk_paged_kv_write and its blocks' bounds computed by axk_paged_key_bounds. */
+ * location outside the pool is skipped and sets *status. A NaN key makes the bound on its sign's side NaN (int8: both).
+ * rows <= 16384: a longer prefill chunk is written by axk_paged_kv_write and its blocks' bounds computed by
+ * axk_paged_key_bounds. */
 int axk_paged_kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cache, int kv_dtype, float kv_scale,
                               uint16_t* bounds, const int32_t* cache_location, int64_t rows, int64_t num_kv_heads,
                               int64_t head_dim, int64_t page_size, int64_t block_size, int64_t num_pages,
@@ -435,7 +438,7 @@ int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds, const int3
 
 /* blocks i32 [batch, num_kv_heads, num_select]: the num_select blocks of each sequence and KV head with the largest
  * scores, as ascending block numbers within the sequence, the first `first` and last `keep_last` of its blocks always
- * among them (first + keep_last <= num_select); equal scores by the lowest block; NaN above every number. A sequence with
+ * among them (first + keep_last <= num_select <= 2^24); equal scores by the lowest block; NaN above every number. A sequence with
  * no more blocks than that has all of them, then -1. */
 int axk_paged_select_blocks(const float* scores, const int32_t* indptr, const int32_t* last_page_len, int32_t* blocks,
                             int64_t nnz, int64_t batch, int64_t num_kv_heads, int64_t page_size, int64_t block_size,

@@ -183,3 +183,25 @@ U8 = torch.zeros(4, 2, 32, 2, 64, dtype=torch.uint8)
 def test_python_layer_raises_value_error(call, match):
     with pytest.raises(ValueError, match=match):
         call(table())
+
+
+@pytest.mark.parametrize("call", [
+    # a launch holds fewer than 2^32 threads: 256 a block of bounds, 64 for 16 blocks' scores of a head, 256 or 1024 a
+    # selected row, 256 a piece of a decode and a part of its merge
+    lambda: bounds_(nnz=1 << 24, page=16, block=16),
+    lambda: bounds_(nnz=1 << 20, page=256, block=16),
+    lambda: scores(nnz=1 << 20, hq=1024, hkv=1024, page=16, block=16),
+    lambda: select(nnz=4096, batch=1 << 20, hkv=4),
+    lambda: select(nnz=8, batch=1 << 20, hkv=16),
+    lambda: decode(batch=1 << 16, hq=16, hkv=16, n=1 << 13),
+    lambda: decode(batch=1 << 20, hq=16, hkv=16, n=1),
+    lambda: decode(batch=1 << 20, hq=256, hkv=16, d=256, blocks=None, n=0),
+])
+def test_launches_that_do_not_fit_are_refused(call):
+    assert call() == SHAPE
+
+
+def test_workspace_of_a_launch_that_does_not_fit():
+    size = _lib.load().axk_paged_decode_blocks_workspace_size
+    assert size(1 << 16, 16, 16, 64, 32, 8, 16, 1 << 13, 0) == 0
+    assert size(1 << 10, 16, 16, 64, 32, 8, 16, 1 << 13, 0) > 0
