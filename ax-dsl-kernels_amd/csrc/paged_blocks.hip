@@ -1480,6 +1480,22 @@ namespace {
 
 constexpr int64_t kMaxSubs = 1 << 30;  // subtiles of a page table, or of a row's listed blocks: sums of them fit 32 bits
 
+// Arrays that a call writes overlap neither what it reads nor each other.
+struct Span {
+  const void* p;
+  size_t n;
+};
+template <int W, int R>
+bool disjoint(const Span (&writes)[W], const Span (&reads)[R]) {
+  for (int i = 0; i < W; ++i) {
+    for (const Span& r : reads)
+      if (axk_overlap(writes[i].p, writes[i].n, r.p, r.n)) return false;
+    for (int j = 0; j < i; ++j)
+      if (axk_overlap(writes[i].p, writes[i].n, writes[j].p, writes[j].n)) return false;
+  }
+  return true;
+}
+
 // Whether a dimension of a launch holds these workgroups: its threads are counted in 32 bits.
 bool launch_fits(int64_t workgroups, int threads) { return workgroups <= (int64_t)0xffffffff / threads; }
 
@@ -1567,16 +1583,10 @@ int kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cache, int ty
                   axk_aligned(kv_scales, 2),
               AXK_E_ALIGN);
   const size_t row = (size_t)hkv * d, slots = (size_t)num_pages * page_size * 2;
-  const struct {
-    const void* p;
-    size_t n;
-  } out[3] = {{kv_cache, slots * row * (type ? 1 : 2)}, {bounds, (size_t)num_pages * (page_size / block_size) * row * 4},
-              {kv_scales, slots * hkv * 2}};
-  for (int i = 0; i < 3; ++i) {
-    AXK_REQUIRE(!axk_overlap(out[i].p, out[i].n, k, rows * row * 2) && !axk_overlap(out[i].p, out[i].n, v, rows * row * 2),
-                AXK_E_ALIAS);
-    for (int j = 0; j < i; ++j) AXK_REQUIRE(!axk_overlap(out[i].p, out[i].n, out[j].p, out[j].n), AXK_E_ALIAS);
-  }
+  const Span writes[] = {{kv_cache, slots * row * (type ? 1 : 2)},
+                         {bounds, (size_t)num_pages * (page_size / block_size) * row * 4}, {kv_scales, slots * hkv * 2}};
+  const Span reads[] = {{k, rows * row * 2}, {v, rows * row * 2}, {loc, (size_t)rows * 8}};
+  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
   if (rows == 0) return AXK_OK;
   AXK_LAUNCH_GATE();
   auto* fn = type == kI8 ? &paged_kv_write_bounds_kernel<kI8>
@@ -1599,10 +1609,11 @@ int key_bounds(const void* kv_cache, int type, float kv_scale, const uint16_t* k
   if (type < 0) return -type;
   AXK_REQUIRE(axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16) && axk_aligned(kv_scales, 2), AXK_E_ALIGN);
   const size_t row = (size_t)hkv * d, slots = (size_t)num_pages * page_size * 2;
-  const size_t bb = (size_t)num_pages * (page_size / block_size) * row * 4;
-  AXK_REQUIRE(!axk_overlap(bounds, bb, kv_cache, slots * row * (type ? 1 : 2)) &&
-                  !axk_overlap(bounds, bb, kv_scales, slots * hkv * 2),
-              AXK_E_ALIAS);
+  const size_t tb = (size_t)batch * 4;
+  const Span writes[] = {{bounds, (size_t)num_pages * (page_size / block_size) * row * 4}};
+  const Span reads[] = {{kv_cache, slots * row * (type ? 1 : 2)}, {kv_scales, slots * hkv * 2}, {indptr, tb + 4},
+                        {indices, (size_t)nnz * 4}, {last_page_len, tb}, {start, tb}};
+  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
   if (nnz == 0) return AXK_OK;
   AXK_LAUNCH_GATE();
   auto* fn = type == kI8 ? &paged_key_bounds_kernel<kI8>
@@ -1664,11 +1675,12 @@ extern "C" int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds,
   AXK_REQUIRE(launch_fits((units + 3) / 4, 256), AXK_E_SHAPE);
   AXK_REQUIRE(axk_aligned(q, 16) && axk_aligned(bounds, 16) && axk_aligned(scores, 4), AXK_E_ALIGN);
   if (nnz == 0) return AXK_OK;
-  const size_t out = (size_t)num_kv_heads * total * 4;
-  AXK_REQUIRE(!axk_overlap(scores, out, q, (size_t)batch * num_qo_heads * head_dim * 2) &&
-                  !axk_overlap(scores, out, bounds,
-                               (size_t)num_pages * (page_size / block_size) * num_kv_heads * head_dim * 4),
-              AXK_E_ALIAS);
+  const size_t tb = (size_t)batch * 4;
+  const Span writes[] = {{scores, (size_t)num_kv_heads * total * 4}};
+  const Span reads[] = {{q, tb / 2 * num_qo_heads * head_dim},
+                        {bounds, (size_t)num_pages * (page_size / block_size) * num_kv_heads * head_dim * 4},
+                        {indptr, tb + 4}, {indices, (size_t)nnz * 4}, {last_page_len, tb}};
+  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
   AXK_LAUNCH_GATE();
   auto* fn = head_dim == 64 ? &paged_block_scores_kernel<64>
                             : head_dim == 128 ? &paged_block_scores_kernel<128> : &paged_block_scores_kernel<256>;
@@ -1692,8 +1704,10 @@ extern "C" int axk_paged_select_blocks(const float* scores, const int32_t* indpt
   const bool small = total <= 2048;  // every row at most eight keys a thread of 256
   AXK_REQUIRE(launch_fits(batch * num_kv_heads, small ? 256 : 1024), AXK_E_SHAPE);
   AXK_REQUIRE(axk_aligned(scores, 4) && axk_aligned(blocks, 4), AXK_E_ALIGN);
-  AXK_REQUIRE(!axk_overlap(blocks, (size_t)batch * num_kv_heads * num_select * 4, scores, (size_t)num_kv_heads * total * 4),
-              AXK_E_ALIAS);
+  const size_t tb = (size_t)batch * 4;
+  const Span writes[] = {{blocks, tb * num_kv_heads * num_select}};
+  const Span reads[] = {{scores, (size_t)num_kv_heads * total * 4}, {indptr, tb + 4}, {last_page_len, tb}};
+  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
   AXK_LAUNCH_GATE();
   const dim3 grid((unsigned)(batch * num_kv_heads));
   if (small)
@@ -1748,16 +1762,14 @@ int decode_blocks(const uint16_t* q, const void* kv_cache, int type, float kv_sc
   AXK_REQUIRE(p.fits, AXK_E_SHAPE);
   const size_t need = p.ml + p.po + p.stat;
   AXK_REQUIRE(!need || (workspace && workspace_bytes >= need && axk_aligned(workspace, 256)), AXK_E_WORKSPACE);
-  const size_t qb = (size_t)batch * num_qo_heads * head_dim * 2, wb = (size_t)num_kv_heads * nnz * 4;
-  const size_t cache = (size_t)num_pages * page_size * num_kv_heads * head_dim * (type ? 2 : 4);
-  AXK_REQUIRE(!axk_overlap(out, qb, q, qb) && !axk_overlap(out, qb, kv_cache, cache) && !axk_overlap(out, qb, workspace, need) &&
-                  !axk_overlap(q, qb, workspace, need) && !axk_overlap(kv_cache, cache, workspace, need),
-              AXK_E_ALIAS);
-  AXK_REQUIRE(weights_in == weights_out || !axk_overlap(weights_in, wb, weights_out, wb), AXK_E_ALIAS);
-  AXK_REQUIRE(!axk_overlap(weights_out, wb, out, qb) && !axk_overlap(weights_out, wb, q, qb) &&
-                  !axk_overlap(weights_out, wb, kv_cache, cache) && !axk_overlap(weights_out, wb, workspace, need) &&
-                  !axk_overlap(weights_in, wb, workspace, need),
-              AXK_E_ALIAS);
+  // (The merge reads the page table and the lists again, after the first kernel has written the workspace.)
+  const size_t tb = (size_t)batch * 4, qb = tb / 2 * num_qo_heads * head_dim, wb = (size_t)num_kv_heads * nnz * 4;
+  const size_t slots = (size_t)num_pages * page_size * 2 * num_kv_heads;
+  const Span writes[] = {{out, qb}, {weights_out, wb}, {workspace, need}};
+  const Span reads[] = {{q, qb}, {kv_cache, slots * head_dim * (type ? 1 : 2)}, {kv_scales, slots * 2}, {indptr, tb + 4},
+                        {indices, (size_t)nnz * 4}, {last_page_len, tb}, {blocks, tb * num_kv_heads * num_select},
+                        {weights_in == weights_out ? nullptr : weights_in, wb}};
+  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
   BlkArgs a;
   a.q = q;
   a.cache = static_cast<const unsigned char*>(kv_cache);
@@ -1837,15 +1849,11 @@ extern "C" int axk_paged_evict_pages(const float* weights, const int32_t* indptr
               AXK_E_SHAPE);
   AXK_REQUIRE(first >= 0 && keep_last >= 1 && budget >= first + keep_last && budget <= 0x3fffffff, AXK_E_SHAPE);
   const size_t ib = (size_t)nnz * 4, pb = (size_t)(batch + 1) * 4, wb = (size_t)num_kv_heads * nnz * 4;
-  const struct {
-    const void* p;
-    size_t n;
-  } in[3] = {{weights, wb}, {indptr, pb}, {indices, ib}}, out[4] = {{out_indptr, pb}, {out_indices, ib}, {out_weights, wb}, {freed, ib}};
-  for (int i = 0; i < 4; ++i) {
-    AXK_REQUIRE(axk_aligned(out[i].p, 4), AXK_E_ALIGN);
-    for (int j = 0; j < 3; ++j) AXK_REQUIRE(!axk_overlap(out[i].p, out[i].n, in[j].p, in[j].n), AXK_E_ALIAS);
-    for (int j = 0; j < i; ++j) AXK_REQUIRE(!axk_overlap(out[i].p, out[i].n, out[j].p, out[j].n), AXK_E_ALIAS);
-  }
+  AXK_REQUIRE(axk_aligned(out_indptr, 4) && axk_aligned(out_indices, 4) && axk_aligned(out_weights, 4) && axk_aligned(freed, 4),
+              AXK_E_ALIGN);
+  const Span writes[] = {{out_indptr, pb}, {out_indices, ib}, {out_weights, wb}, {freed, ib}};
+  const Span reads[] = {{weights, wb}, {indptr, pb}, {indices, ib}};
+  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
   AXK_LAUNCH_GATE();
   hipLaunchKernelGGL(paged_evict_kernel, dim3((unsigned)batch), dim3(kEvict), 0, axk_stream(stream), weights, indptr, indices,
                      out_indptr, out_indices, out_weights, freed, (int)nnz, (int)batch, (int)num_kv_heads, (int)budget,

@@ -394,7 +394,8 @@ int axk_paged_prefill_split(const uint16_t* q, const uint16_t* kv_cache, const i
  * (key bounds: 2^24 blocks in the table; scores: 2^26 times 16 blocks of a head; selection: 2^22 rows, 2^24 of up to 2048
  * blocks in the table; decode: 2^24 pieces, of 128 to 2048 tokens). A page id outside [0, num_pages) is skipped, never read,
  * and sets *status (device i32, or NULL) to 1. An array per page-table entry is [num_kv_heads, nnz], one per block
- * [num_kv_heads, nnz * page_size / block_size]: entry e's blocks at e * page_size / block_size.
+ * [num_kv_heads, nnz * page_size / block_size]: entry e's blocks at e * page_size / block_size. What a
+ * call writes, its workspace too, overlaps neither what it reads nor each other (AXK_E_ALIAS; weights_out may be weights_in).
  * ------------------------------------------------------------------------------------------- */
 
 /* The new rows k, v bf16 [rows, num_kv_heads, head_dim] written at cache_location i32 [rows, 2] = (page, slot), as
@@ -438,8 +439,8 @@ int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds, const int3
 
 /* blocks i32 [batch, num_kv_heads, num_select]: the num_select blocks of each sequence and KV head with the largest
  * scores, as ascending block numbers within the sequence, the first `first` and last `keep_last` of its blocks always
- * among them (first + keep_last <= num_select <= 2^24); equal scores by the lowest block; NaN above every number. A sequence with
- * no more blocks than that has all of them, then -1. */
+ * among them (first + keep_last <= num_select <= 2^24); equal scores by the lowest block; NaN above every number. A
+ * sequence with no more blocks than that has all of them, then -1. */
 int axk_paged_select_blocks(const float* scores, const int32_t* indptr, const int32_t* last_page_len, int32_t* blocks,
                             int64_t nnz, int64_t batch, int64_t num_kv_heads, int64_t page_size, int64_t block_size,
                             int64_t num_select, int64_t first, int64_t keep_last, axk_stream_t stream);
@@ -477,9 +478,8 @@ int axk_paged_decode_blocks_i8(const uint16_t* q, const int8_t* kv_cache, const 
  * NaN above every number), the first `first` and last `keep_last` always among them (keep_last >= 1, since the last page
  * is the one that last_page_len speaks of; first + keep_last <= budget). Every kept page keeps its order and its bytes:
  * out_indptr i32 [batch + 1], out_indices i32 [nnz] (then -1), out_weights f32 [num_kv_heads, nnz] (then 0) and
- * freed i32 [nnz] (the other pages' ids in table order, then -1); last_page_len stays as it is. The outputs overlap
- * neither the inputs nor each other. The bounds go with the pages. A page that another sequence shares is freed all the
- * same: the caller keeps count of such pages. */
+ * freed i32 [nnz] (the other pages' ids in table order, then -1); last_page_len stays as it is. The bounds go with the pages.
+ * A page that another sequence shares is freed all the same: the caller keeps count of such pages. */
 int axk_paged_evict_pages(const float* weights, const int32_t* indptr, const int32_t* indices, int32_t* out_indptr,
                           int32_t* out_indices, float* out_weights, int32_t* freed, int64_t nnz, int64_t batch,
                           int64_t num_kv_heads, int64_t budget, int64_t first, int64_t keep_last, axk_stream_t stream);

@@ -205,3 +205,29 @@ def test_workspace_of_a_launch_that_does_not_fit():
     size = _lib.load().axk_paged_decode_blocks_workspace_size
     assert size(1 << 16, 16, 16, 64, 32, 8, 16, 1 << 13, 0) == 0
     assert size(1 << 10, 16, 16, 64, 32, 8, 16, 1 << 13, 0) > 0
+
+
+W = dict(wout=at(9))
+
+
+@pytest.mark.parametrize("call", [
+    # the tables that a call reads, or that its second kernel reads again, under what it writes
+    lambda: write(loc=at(16)), lambda: write(loc=at(3)),
+    lambda: bounds_(ptr=at(3)), lambda: bounds_(idx=at(3, 16)), lambda: bounds_(last=at(3)),
+    lambda: bounds_with_start(at(3)),
+    lambda: scores(out=at(4)), lambda: scores(out=at(5)), lambda: scores(out=at(6)),
+    lambda: select(out=at(4)), lambda: select(out=at(6)),
+    lambda: decode(out=at(4, 8)), lambda: decode(out=at(5)), lambda: decode(out=at(6)), lambda: decode(out=at(7)),
+    lambda: decode(wout=at(4)), lambda: decode(wout=at(5)), lambda: decode(wout=at(6)), lambda: decode(wout=at(7)),
+    lambda: decode(ws=at(4), **W), lambda: decode(ws=at(5), **W), lambda: decode(ws=at(6), **W), lambda: decode(ws=at(7), **W),
+    lambda: decode(out=at(10), win=at(10), **W),
+    lambda: decode_i8(out=at(24)), lambda: decode_i8(ws=at(24)),
+    lambda: write_i8(scales=at(4)),
+])
+def test_overlapping_arrays_are_refused(call):
+    assert call() == ALIAS
+
+
+def bounds_with_start(start):
+    return _lib.load().axk_paged_key_bounds(at(16), BF16, 1.0, at(3), at(4), at(5), at(6), start, 8, 2, 2, 64, 32, 16, 8,
+                                            None, None)
