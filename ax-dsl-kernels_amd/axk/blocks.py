@@ -23,9 +23,8 @@ import torch
 from . import _lib
 
 
-# The checks build their messages only when they fail: a decode step makes these calls once a layer.
-_stream = torch._C._cuda_getCurrentRawStream
-_device = torch._C._cuda_getDevice
+# The checks build their messages only when they fail, and the stream comes straight from torch's extension module: a
+# decode step makes these calls once a layer. (Looked up in the call, as a torch built without a GPU has no such function.)
 _BF16, _F32, _I32, _I8, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.int8, torch.uint8
 _E4M3 = torch.float8_e4m3fn
 _DT_BF16, _DT_E4M3 = _lib.DT_BF16, _lib.DT_FP8E4M3
@@ -39,11 +38,12 @@ def _call(name: str, tensors, *args) -> None:
             raise ValueError(f"{name}: tensors on {tensors[0].device} and {t.device}")
     if dev < 0:  # the host
         raise ValueError(f"axk operators take device tensors; got a tensor on {tensors[0].device}")
-    if _device() == dev:
-        _lib.call(name, *args, _stream(dev))
+    c = torch._C
+    if c._cuda_getDevice() == dev:
+        _lib.call(name, *args, c._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, _stream(dev))
+            _lib.call(name, *args, c._cuda_getCurrentRawStream(dev))
 
 
 def _i32(t: torch.Tensor, name: str, *shape: int) -> None:

@@ -1,6 +1,9 @@
 """Refusals of the block operators, before anything is launched (CPU): the C entries' status codes, with pointers that are
 never followed, and the Python layer's ValueErrors."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -231,3 +234,15 @@ def test_overlapping_arrays_are_refused(call):
 def bounds_with_start(start):
     return _lib.load().axk_paged_key_bounds(at(16), BF16, 1.0, at(3), at(4), at(5), at(6), start, 8, 2, 2, 64, 32, 16, 8,
                                             None, None)
+
+
+def test_import_beside_a_torch_that_was_built_without_a_gpu():
+    """Such a torch lacks the stream functions of its extension module: the codecs and configs import all the same."""
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]: delattr(torch._C, n)\n"
+            "import axk\n"
+            "from axk import configs\n"
+            "print(axk.quantize_nvfp4(torch.ones(16, 32))[0].shape, len(dir(configs)) > 0)\n")
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(os.path.abspath(axk.__file__))))
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env, timeout=300)
+    assert got.returncode == 0, got.stderr
