@@ -448,8 +448,8 @@ int axk_paged_select_blocks(const float* scores, const int32_t* indptr, const in
 /* Decode attention, as axk_paged_decode, over the listed blocks of each sequence and KV head only: blocks i32 [batch,
  * num_kv_heads, num_select], each row strictly ascending block numbers within the sequence, then -1 (the form
  * axk_paged_select_blocks writes). NULL with num_select 0: every block (block_size is then not read). A number past the
- * sequence's end, not above its predecessor in the row, or right behind a -1 is skipped and sets *status. A row that
- * attends nothing yields zeros.
+ * sequence's end, not above its predecessor in the row, or right behind a -1 is skipped and sets *status (a block
+ * named again further on is attended again). A row that attends nothing yields zeros.
  * weights_out f32 [num_kv_heads, nnz] (NULL: not wanted) receives, for each KV head and page-table entry,
  *   decay * weights_in (NULL: 0) + sum over the KV head's queries of the attention the page's tokens received;
  * weights_out may be weights_in (in place). Entries of no sequence are left as they are.

@@ -158,7 +158,7 @@ def decode_blocks(q, cache, indptr, indices, last, blocks=None, block: int = 16,
                     if 0 <= i < -(-n // block) and (slot == 0 or (i > prev and prev != -1)):
                         ids.append(i)
                     prev = i
-                rows = rows[torch.isin(rows // block, torch.tensor(ids, dtype=torch.long))]
+                rows = torch.cat([rows[rows // block == i] for i in ids] or [rows[:0]])
             if not len(rows):
                 continue
             x = q[b, h * group:(h + 1) * group].double()

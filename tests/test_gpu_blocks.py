@@ -738,3 +738,16 @@ def test_scores_of_infinite_bounds(dev, hq, hkv, d):
     there = ref.isfinite()
     assert torch.equal(got[~there].nan_to_num(0.5), ref[~there].nan_to_num(0.5))
     assert ((got - ref).abs()[there] <= (2 * d * 2.0 ** -24 * mag)[there]).all()
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_lists_that_name_a_block_again(dev, weights):
+    """Behind a fall of the list, or behind padding and a block that is skipped, a block may come a second time: flagged, and
+    attended again."""
+    c = make([300, 200], 4, 2, 64, 32)
+    blocks = torch.tensor([[[0, 5, 2, 5, 7, -1], [3, 9, -1, 4, 9, 11]], [[6, 2, 6, 7, 3, 7], [1, 1, 2, 2, 12, 0]]], dtype=torch.int32)
+    _, _, status = check_decode(c, dev, blocks, 16, weights=weights)
+    assert status == 1
+    long = blocks.repeat(1, 1, 40)  # over several pieces
+    _, _, status = check_decode(c, dev, long, 16, weights=weights)
+    assert status == 1

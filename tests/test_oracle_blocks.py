@@ -144,3 +144,16 @@ def test_bounds_of_an_int8_cache_are_the_tightest_in_bf16():
     step = torch.where(lo.double() == y, 0.0, y.abs() * 2.0 ** -7)
     assert (lo.double() <= y).all() and (y <= hi.double()).all() and (hi.double() - lo.double() <= step).all()
     assert all(t.isnan().all() for t in ob.outward(torch.tensor([math.nan]).double(), torch.tensor([math.nan]).double()))
+
+
+def test_a_block_named_again_behind_a_fall_counts_again():
+    """[0, 2, 1, 2]: 1 is skipped, and 2, above its predecessor, is attended a second time."""
+    c = case([64], 4, 2, 64, 32, seed=5)
+    args = [c[n] for n in ("q", "cache", "indptr", "indices", "last_page_len")]
+    blocks = torch.tensor([[[0, 2, 1, 2], [0, 2, -1, -1]]], dtype=torch.int32)
+    out, w, _, _ = ob.decode_blocks(*args, blocks=blocks, block=16)
+    k, v, _ = ob.seq_rows(c["cache"], c["indptr"], c["indices"], c["last_page_len"], 0)
+    for h, rows in enumerate(([*range(16), *range(32, 48), *range(32, 48)], [*range(16), *range(32, 48)])):
+        p = torch.softmax(c["q"][0, 2 * h:2 * h + 2].double() @ k[rows, h].t() / 8, 1)
+        torch.testing.assert_close(out[0, 2 * h:2 * h + 2], p @ v[rows, h])
+        torch.testing.assert_close(w[h], torch.stack([p[:, :16].sum(), p[:, 16:].sum()]))
