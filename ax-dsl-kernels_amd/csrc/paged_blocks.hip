@@ -132,7 +132,8 @@ constexpr int64_t kMaxRows = 16384;  // every row looks at every other's place: 
 // new row at its first slot starts afresh, every other one widens what it had. One workgroup per row; the first row of
 // the call that falls into a block folds all of them, so that rows of one block never race, and where two rows name one
 // slot the last one is stored (both are folded). Bound by its chain: launch, locations, then row and bounds; 3.4 us for the
-// 16 rows of a decode step (HKV 2, D 256), 2.3 without the bounds, 4.5 for 16 rows of one block.
+// 16 rows of a decode step (HKV 2, D 256), 2.3 without the bounds, 4.5 for 16 rows of one block; into an int8 cache 4.7 and
+// 14.5, as a row is quantized once for the cache and once for the bounds.
 //
 // Eight channels of a new row as the cache keeps them: their bytes (a bf16 cache: the values themselves), the int8 scale,
 // and the key's bf16 pairs as attention reads them, rounded down and up where they have more bits (int8). The d / 8 lanes of
@@ -276,10 +277,10 @@ __global__ __launch_bounds__(256) void paged_kv_write_bounds_kernel(
 // One workgroup per block: its K rows are one contiguous run of tokens x HKV x D values, read 16 bytes a lane, a column
 // of 8 (8-bit caches: 16) channels kept by as many lanes as the workgroup has to spare and joined through LDS. Minimum and
 // maximum are taken on the bf16 bits as ordered 16-bit integers, two values an instruction; of an int8 cache in fp32, which
-// holds code * scale exactly, and rounded outward once a lane. Bound by the K bytes: 136,000
-// tokens of an FP8 cache (HKV 2, D 256, blocks of 32) 18.7 us, 84 MB at 4.5 TB/s; without minimum and maximum at all 4%
+// holds code * scale exactly, and rounded outward once a lane. Bound by the K bytes: 145,592
+// tokens of an FP8 cache (HKV 2, D 256, blocks of 32) 18.6 us, 84 MB at 4.5 TB/s; without minimum and maximum at all 4%
 // less, with non-temporal loads 8% more, and 1.5 us more while lanes stored dwords 32 bytes apart. As an int8 cache the
-// same tokens take 25.3 us (22.8 with keys rounded to nearest, which bounds nothing).
+// same tokens take 26.4 us, 84 MB at 3.2 TB/s: a convert, a product, a minimum and a maximum a value in fp32.
 template <int T>
 __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
     const unsigned char* __restrict__ cache, const uint16_t* __restrict__ scales, uint16_t* __restrict__ bounds, const int* __restrict__ indptr,
@@ -381,9 +382,9 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(
 // max(q lo, q hi) per channel is q+ hi + q- lo with q+ = max(q, 0), q- = min(q, 0): the score of 16 blocks for the 16
 // (padded) heads of a group is one chain of 2 D / 32 16x16x32 MFMAs, blocks as rows, and a block's bounds are read once.
 // One wave per (16 blocks, KV head); a tile that spans sequences is computed once with each one's queries. Bound by the
-// bounds' bytes: 8 sequences of 131072 tokens in blocks of 64 (HKV 4, D 256) 16.3 us, 67 MB at 4.1 TB/s, all of its waves
+// bounds' bytes: 8 sequences of 131072 tokens in blocks of 64 (HKV 4, D 256) 16.5 us, 68 MB at 4.1 TB/s, all of its waves
 // at once. With the rows through LDS as in the decode below the same took 18.2 us, since half as many waves fit (and one
-// sequence of 5003 tokens 4.6 against 5.5).
+// sequence of 5003 tokens 4.6 against 5.6).
 //
 // Where a bound is infinite, the product that the split leaves at zero is 0 inf = NaN, though max(q lo, q hi) is not. So a
 // block whose sum came out NaN is summed again as the formula stands, head by head, after the others: a lane's block and
@@ -485,7 +486,8 @@ __global__ __launch_bounds__(256) void paged_block_scores_kernel(
 // Radix selection by one workgroup of T threads, K consecutive keys each in registers (a longer row is read again, T K keys
 // at a time, in each step). Keys are taken relative to the row's smallest, and log2(4 T) bits at a time, from the highest
 // that the row's range has, are counted in 4 T bins of LDS, until the smallest key that is taken is known or all keys that
-// agree with it so far are taken: two rounds as a rule. Bound by its barriers: 256 of 8192 scores 9.7 us, 64 of 313 4.0.
+// agree with it so far are taken: two rounds as a rule. 256 of 8192 scores for 32 rows 9.7 us, 64 of 313 4.0: latency, as
+// the bytes take 0.2 us; how it divides between loads, counts, scans and barriers has not been measured for this form.
 // (With 256 bins of the raw bits the former took 19.6: most scores share sign and exponent, and adds to one address wait
 // for each other.) Equal keys at the border are taken by the lowest index. load(at, n, key) fetches a thread's n keys from
 // index `at`; emit(i, taken, rank) is called for every index, rank = the indices below i that are taken; done(base, n, k)
@@ -723,9 +725,10 @@ __global__ __launch_bounds__(T) void paged_select_blocks_kernel(const float* __r
 //                 4 g + j % 4 of subtile j / 4. V rows are loaded in that order, lane l16 holding D / 16 channels of eight
 //                 tokens, so that the transposition V^T needs is one byte permute per two values, without LDS.
 // The four waves of a piece take its steps in turn and are joined through LDS; pieces by the merge kernel.
-// Bound by HBM: 64 blocks of 64 for 8 sequences of 131072 tokens (HQ 32, HKV 4, D 256) 28.3 us, 134 MB at 4.7 TB/s; the
-// whole FP8 cache of 16 sequences (HQ 16, HKV 2) 30.2 us, 139 MB at 4.6 TB/s; of these some 5 us are the chain of lookups
-// before the first load (list, page, rows) and the join after the last. As many pieces as run at once are best: with three
+// Bound by HBM: 64 blocks of 64 for 8 sequences of 131072 tokens (HQ 32, HKV 4, D 256) 28.2 us, 134 MB at 4.8 TB/s; all
+// 145,592 tokens of 16 sequences (HQ 16, HKV 2) of an FP8 cache 29.9 us, 149 MB at 5.0 TB/s, of an int8 cache 32.9 us, 151 MB
+// at 4.6; of these some 5 us are the chain of lookups before the first load (list, page, rows) and the join after the last.
+// (The decode over whole bf16 caches in paged_attn.hip reads 6.1 TB/s.) As many pieces as run at once are best: with three
 // quarters of them the former took 17% longer, with half as many again 3%, and the latter 25%.
 template <int D, int T>
 struct BlkCfg {
@@ -957,8 +960,8 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
       if (l16 < (u ? nv1 : nv0))
         own = bf16_bits_to_f32(a.kv_scales[(s_row[2 * t + u] + plane * a.page + l16) * a.hkv + h]);
     }
-    // This step's K has landed in LDS (the compiler waits for registers only), and its V, which costs nothing: the other
-    // waves' loads keep the memory busy.
+    // This step's K has landed in LDS (the compiler waits for registers only), and its V with it. (The other waves' loads keep
+    // the memory busy meanwhile; a wait for K alone has not been measured.)
     wait_vmcnt<0>();
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (T == kI8) {
@@ -1020,6 +1023,8 @@ __global__ __launch_bounds__(256, 2) void paged_blocks_kernel(const BlkArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] *= vs[i];
     }
+    // Probabilities meet V in bf16, as V itself is held (half a step, 2^-8 of each, which averages out over the tokens:
+    // outputs are off by 1.7e-3 of their size, those of fp32 probabilities by as much, their own rounding). l keeps fp32.
     const axk_u32x4 pw = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
                           pack_bf16x2(x[6], x[7])};
     const axk_bf16x8 pf = __builtin_bit_cast(axk_bf16x8, pw);
@@ -1315,7 +1320,7 @@ AXK_DEV void merge_weights(const BlkArgs& a, const WeightArgs& w, int b, int h, 
 }
 
 // The first batch * hkv * split workgroups: output rows. The others: page weights. A merge is three dependent trips to
-// memory and little else: 4 us for one sequence's 64 pieces, 5.9 for 512 pieces of 8 sequences with their weights.
+// memory: 4 us for one sequence's 64 pieces, 5.8 for 512 pieces of 8 sequences with their weights.
 template <int D, bool LISTED>
 __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a, const WeightArgs w) {
   __shared__ float2 s_part[4][16];
@@ -1356,7 +1361,7 @@ __global__ __launch_bounds__(256) void paged_blocks_merge_kernel(const BlkArgs a
 // One workgroup per sequence: its `budget` pages of largest weight (summed over the KV heads in 64 bits, so that the
 // order of the sum does not decide), the first `first` and last `keep_last` always among them, in their order into the
 // new table; the others' ids into `freed`. Every workgroup finds its places from the whole indptr, and fills as much of
-// the arrays' tails as it moved elsewhere. Bound by the selection's barriers: 64 sequences of up to 2048 pages 11.6 us
+// the arrays' tails as it moved elsewhere. Bound by the selection's latency: 64 sequences of up to 2048 pages 11.6 us
 // (26 us while a thread summed its pages' heads one after the other).
 constexpr int kEvict = 1024;  // threads
 constexpr int kEvictTile = 4 * kEvict;
@@ -1520,8 +1525,8 @@ int cache_type(int kv_dtype, float kv_scale) {
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // How a decode over blocks is cut, from what the host knows: pieces of at least 128 tokens, so that each wave has a step,
-// and of at most 2048; otherwise as many as run at once (two workgroups a CU), since a second round would pay the lookups
-// again.
+// and of at most 2048; otherwise as many as run at once at D = 256, two workgroups a CU, since a second round would pay the
+// lookups again. (Smaller heads leave room for more workgroups; their cut has not been measured apart.)
 constexpr int64_t kPieces = 512;
 struct BlkPlan {
   int ps, pieces;
