@@ -49,6 +49,18 @@ from .blocks import (  # noqa: E402
 __all__ += ["blocks", "paged_block_scores", "paged_decode_blocks", "paged_decode_blocks_workspace", "paged_evict_pages",
             "paged_key_bounds", "paged_select_blocks", "store_paged_kv_bounds"]
 
+from . import tree  # noqa: E402
+from .tree import (  # noqa: E402
+    gdn_tree_commit,
+    gdn_tree_verify,
+    paged_tree_verify,
+    paged_tree_verify_workspace,
+    store_paged_kv_rope,
+)
+
+__all__ += ["tree", "gdn_tree_commit", "gdn_tree_verify", "paged_tree_verify", "paged_tree_verify_workspace",
+            "store_paged_kv_rope"]
+
 from . import gdn  # noqa: E402
 from .gdn import gdn_chunk_prefill, gdn_chunk_workspace, gdn_recurrent  # noqa: E402
 

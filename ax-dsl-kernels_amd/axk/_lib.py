@@ -97,6 +97,16 @@ SIGNATURES: dict[str, list] = {
     "axk_paged_decode_blocks_i8": [_vp] * 7 + [_i64, _i64, _vp, _vp, _vp, ctypes.c_float] + [_i64] * 7 +
                                   [ctypes.c_float, _vp, _vp, ctypes.c_size_t, _vp],
     "axk_paged_evict_pages": [_vp] * 7 + [_i64] * 6 + [_vp],
+    "axk_paged_kv_write_rope": [_vp, _i64, _i64] * 3 + [_vp] * 4 + [_i32, _i64] + [_vp] * 4 + [_i32, ctypes.c_float] +
+                               [_i64] * 7 + [ctypes.c_float, _vp, _vp],
+    "axk_paged_kv_write_rope_i8": [_vp, _i64, _i64] * 3 + [_vp] * 4 + [_i32, _i64] + [_vp] * 5 + [_i64] * 7 +
+                                  [ctypes.c_float, _vp, _vp],
+    "axk_paged_tree_verify_workspace_size": [_i64] * 5,
+    "axk_paged_tree_verify": [_vp, _vp, _i32, ctypes.c_float] + [_vp] * 5 + [_i64] * 8 +
+                             [ctypes.c_float, _vp, _vp, ctypes.c_size_t, _vp],
+    "axk_paged_tree_verify_i8": [_vp] * 8 + [_i64] * 8 + [ctypes.c_float, _vp, _vp, ctypes.c_size_t, _vp],
+    "axk_gdn_tree_verify": [_vp] * 12 + [_i64] * 6 + [_vp, _vp],
+    "axk_gdn_tree_commit": [_vp] * 7 + [_i64] * 6 + [_vp, _vp],
     "axk_gdn_recurrent": [_vp] * 10 + [_i64] * 6 + [_vp],
     "axk_gdn_chunk_workspace_size": [_i64] * 7,
     "axk_gdn_chunk_prefill": [_vp] * 10 + [_i64] * 7 + [_vp, ctypes.c_size_t, _vp],
@@ -149,6 +159,7 @@ _RESTYPES = {
     "axk_paged_decode_workspace_size": ctypes.c_size_t,
     "axk_paged_prefill_workspace_size": ctypes.c_size_t,
     "axk_paged_decode_blocks_workspace_size": ctypes.c_size_t,
+    "axk_paged_tree_verify_workspace_size": ctypes.c_size_t,
     "axk_moe_workspace_size": ctypes.c_size_t,
     "axk_gdn_chunk_workspace_size": ctypes.c_size_t,
     "axk_gdn_layer_workspace_size": ctypes.c_size_t,

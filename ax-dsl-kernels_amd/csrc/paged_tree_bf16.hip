@@ -1,0 +1,6 @@
+// paged_tree.h for a cache of this stored type (a file of its own, so that the three compile side by side).
+#include "paged_tree.h"
+
+namespace axk_tree {
+int launch_bf16(const TreeArgs& a, int d, int wr, hipStream_t st) { return launch_type<kBf16>(a, d, wr, st); }
+}  // namespace axk_tree

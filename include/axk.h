@@ -485,6 +485,92 @@ int axk_paged_evict_pages(const float* weights, const int32_t* indptr, const int
                           int64_t num_kv_heads, int64_t budget, int64_t first, int64_t keep_last, axk_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Verifying a tree of drafted tokens. No counterpart in the reference (whose verify path checks chains).
+ *
+ * A sequence's tree of up to `nodes` <= 64 drafted tokens is parents i32 [batch, nodes]: node t's parent, a node before it,
+ * or -1 (the last token of the history), or -2 (no node: rows behind a smaller tree, whose outputs are zero). Any other value,
+ * or a parent that is no node, makes t no node and sets *status (device i32, or NULL) to 1. A verify step appends the nodes'
+ * rows to the paged cache (axk_paged_kv_write_rope), attends (axk_paged_tree_verify) or runs the delta rule
+ * (axk_gdn_tree_verify) over every branch at once; when a branch has been accepted its rows are written to their final places
+ * (axk_paged_kv_write_rope with page -1 for the other rows) and the states are brought to its last node
+ * (axk_gdn_tree_commit).
+ *
+ * What a call writes, its workspace and *status too, overlaps neither what it reads nor each other (AXK_E_ALIAS). A launch
+ * holds fewer than 2^32 threads (AXK_E_SHAPE). kv_dtype: AXK_DT_BF16, or AXK_DT_FP8E4M3 with its kv_scale (a power of two;
+ * ignored for bf16); the entries ending in _i8 take the int8 cache and bf16 scales of axk_paged_kv_write_i8, read as
+ * code * scale. head_dim 64, 128 or 256.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Rows of k and v [rows, num_kv_heads, head_dim] appended to a paged cache, and of q [rows, num_qo_heads, head_dim] (NULL with
+ * num_qo_heads 0: none) into q_out, contiguous, with the normalisation and position rotation applied on the way. bf16 operands
+ * with row strides ld* and head strides hd* in elements (multiples of 8, 16-byte aligned: views of a fused projection, also of
+ * its [q | gate] heads); they are only read and may overlap each other.
+ *   y = x rsqrt(mean(x^2) + eps) w for q and k with their weights q_norm / k_norm f32 [head_dim] (16-byte aligned), y = x
+ *   without (NULL); channels i and i + rot / 2, i < rot / 2: (y_i cos_i - y_j sin_i, y_j cos_i + y_i sin_i); the rest as is.
+ * cos, sin [table_rows, rot / 2], both bf16 or both f32 (table_dtype AXK_DT_BF16 / AXK_DT_F32), 16-byte aligned, row
+ * positions[r] (NULL: row r); rot a multiple of 16, 0 for no rotation (cos and sin may then be NULL). All in fp32, rounded
+ * once to what is stored: bf16, e4m3(y * kv_scale) (NaN past 464), or int8 codes with the scale of the row and head
+ * (axk_paged_kv_write_i8's quantizer, on the fp32 values).
+ * cache_location i32 [rows, 2] = (page, slot) of row r's k and v; page -1: not stored, q still written. positions[r] = -1: no
+ * row, nothing is written. Any other location outside the pool leaves k and v out, any other position outside the table the
+ * whole row, and sets *status. The locations of one call are distinct (where two rows name one slot, each 16-byte piece of it
+ * is one row's). rows <= 2^24; num_qo_heads, num_kv_heads <= 4096; page_size <= 2^24. */
+int axk_paged_kv_write_rope(const uint16_t* q, int64_t ldq, int64_t hdq, const uint16_t* k, int64_t ldk, int64_t hdk,
+                            const uint16_t* v, int64_t ldv, int64_t hdv, const float* q_norm, const float* k_norm,
+                            const void* cos, const void* sin, int table_dtype, int64_t table_rows, const int32_t* positions,
+                            const int32_t* cache_location, uint16_t* q_out, void* kv_cache, int kv_dtype, float kv_scale,
+                            int64_t rows, int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim, int64_t rot,
+                            int64_t page_size, int64_t num_pages, float eps, int32_t* status, axk_stream_t stream);
+int axk_paged_kv_write_rope_i8(const uint16_t* q, int64_t ldq, int64_t hdq, const uint16_t* k, int64_t ldk, int64_t hdk,
+                               const uint16_t* v, int64_t ldv, int64_t hdv, const float* q_norm, const float* k_norm,
+                               const void* cos, const void* sin, int table_dtype, int64_t table_rows, const int32_t* positions,
+                               const int32_t* cache_location, uint16_t* q_out, int8_t* kv_cache, uint16_t* kv_scales,
+                               int64_t rows, int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim, int64_t rot,
+                               int64_t page_size, int64_t num_pages, float eps, int32_t* status, axk_stream_t stream);
+
+/* Attention of a tree's nodes over the paged cache: q, out bf16 [batch, nodes, num_qo_heads, head_dim]. The page table covers
+ * the history and the sequence's n nodes (those up to its last that is one), whose K / V are its last n cached tokens, node t
+ * at n - t from the end; node t attends the history, its ancestors and itself. Rows that attend nothing are zero. A chain
+ * (parents -1, 0, 1, ..) is axk_paged_prefill over the same rows. Cache, page table and page size as axk_paged_decode;
+ * num_qo_heads / num_kv_heads <= 16, num_kv_heads <= 4096, batch <= 2^20. nnz: the entries of indices; offsets of indptr past it
+ * are read as nnz, negative ones as 0, a last_page_len past page_size as page_size; nnz * page_size < 2^31 - 256. A page id
+ * outside [0, num_pages) is skipped, never read, and a sequence of fewer cached tokens than nodes gets zeros; both set *status.
+ * workspace: the fp32 partial outputs of sequences that are cut into pieces, 256-byte aligned, of
+ * axk_paged_tree_verify_workspace_size bytes (0: may be NULL, or an unsupported shape); it carries nothing from call to call,
+ * and calls that may run at the same time need one each. Equal calls give equal bits. */
+size_t axk_paged_tree_verify_workspace_size(int64_t batch, int64_t nodes, int64_t num_qo_heads, int64_t num_kv_heads,
+                                            int64_t head_dim);
+int axk_paged_tree_verify(const uint16_t* q, const void* kv_cache, int kv_dtype, float kv_scale, const int32_t* indptr,
+                          const int32_t* indices, const int32_t* last_page_len, const int32_t* parents, uint16_t* out,
+                          int64_t nnz, int64_t batch, int64_t nodes, int64_t num_qo_heads, int64_t num_kv_heads,
+                          int64_t head_dim, int64_t page_size, int64_t num_pages, float sm_scale, int32_t* status,
+                          void* workspace, size_t workspace_bytes, axk_stream_t stream);
+int axk_paged_tree_verify_i8(const uint16_t* q, const int8_t* kv_cache, const uint16_t* kv_scales, const int32_t* indptr,
+                             const int32_t* indices, const int32_t* last_page_len, const int32_t* parents, uint16_t* out,
+                             int64_t nnz, int64_t batch, int64_t nodes, int64_t num_qo_heads, int64_t num_kv_heads,
+                             int64_t head_dim, int64_t page_size, int64_t num_pages, float sm_scale, int32_t* status,
+                             void* workspace, size_t workspace_bytes, axk_stream_t stream);
+
+/* axk_gdn_recurrent along every branch of a tree: q, k bf16 [batch, nodes, num_k_heads, 128], v [batch, nodes, num_v_heads,
+ * 128], a, b [batch, nodes, num_v_heads]; node t continues the state after its parent, a node with parent -1 state f32 [batch,
+ * num_v_heads, 128, 128], which is only read. out bf16 like v; updates f32 like v, each node's rank-1 update u = beta (v - k^T
+ * S); gates f32 [batch, nodes, num_v_heads], its log decay g; all zero where there is no node. A chain's outputs are those of
+ * axk_gdn_recurrent. Value head h reads key head h / (num_v_heads / num_k_heads). batch * num_v_heads <= 2^20. */
+int axk_gdn_tree_verify(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* a, const uint16_t* b,
+                        const float* a_log, const float* dt_bias, const float* state, const int32_t* parents, uint16_t* out,
+                        float* updates, float* gates, int64_t batch, int64_t nodes, int64_t num_k_heads, int64_t num_v_heads,
+                        int64_t head_k_dim, int64_t head_v_dim, int32_t* status, axk_stream_t stream);
+
+/* The state after node accepted[b] (i32 [batch]; -1: none, the state as it was) of each tree, from axk_gdn_tree_verify's inputs
+ * k and parents and its updates and gates: state_out = e^(sum g) state_in + sum over the node and its ancestors i of
+ * e^(sum of g after i) k_i u_i^T, k normalised. state_out may be state_in (in place). An accepted entry that is no node leaves
+ * the state as it was and sets *status. */
+int axk_gdn_tree_commit(const float* state_in, const uint16_t* k, const float* updates, const float* gates,
+                        const int32_t* parents, const int32_t* accepted, float* state_out, int64_t batch, int64_t nodes,
+                        int64_t num_k_heads, int64_t num_v_heads, int64_t head_k_dim, int64_t head_v_dim, int32_t* status,
+                        axk_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Gated DeltaNet (GDN)
  * ------------------------------------------------------------------------------------------- */
 
