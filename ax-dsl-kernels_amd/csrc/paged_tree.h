@@ -72,9 +72,10 @@ AXK_DEV int wave_scan(int v) {
   return v;
 }
 
-// How the batch is cut: every sequence into pieces of P pairs, P such that all pieces of all row blocks and KV heads fill the
-// chip once (total / den pairs; a sequence's last piece is shorter, so there are at most den + batch pieces). Every wave of
-// both launches derives the same cut from the page table: the total is a float sum in a fixed order.
+// How the batch is cut: every sequence into pieces of P pairs, P such that the pieces of all row blocks and KV heads run at
+// once: total / den pairs, or more until no more than den pieces come out (a sequence's last piece is shorter, so there are at
+// most den + batch). Every wave of both launches derives the same cut from the page table: the total is a float sum in a fixed
+// order.
 struct Piece {
   int b;       // sequence (-1: none)
   int j, ns;   // piece of the sequence, and how many it has
@@ -101,16 +102,24 @@ AXK_DEV Piece find_piece(const TreeArgs& a, int want, bool by_piece, int kg) {
   Piece k;
   k.b = -1;
   k.size = 0x40000000;
+  auto pieces = [&](int b0, int size) {  // at least one each, which writes the zeros of a sequence without tokens
+    return b0 + lane < a.batch ? max(1, (int)((unsigned)(pairs_at(b0) + size - 1) / (unsigned)size)) : 0;
+  };
   if (a.split) {
-    const int p = max(a.min_piece, (int)(total / (float)a.den) + 1);
+    int p = max(a.min_piece, (int)(total / (float)a.den) + 1);
     k.size = (p + kg - 1) / kg * kg;
+    if (a.batch <= 64)  // (a larger batch has up to den + batch pieces)
+      for (int i = 0; i < 8; ++i) {
+        const int n = __builtin_amdgcn_readlane(wave_scan(pieces(0, k.size)), 63);
+        if (n <= a.den || k.size >= (int)total) break;
+        p = (int)((float)k.size * (float)n / (float)a.den) + 1;
+        k.size = (p + kg - 1) / kg * kg;
+      }
   }
   int base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     if (a.batch > 64) load(b0);
-    const int pairs = pairs_at(b0);
-    // at least one piece, which writes the zeros of a sequence without tokens
-    const int n = b0 + lane < a.batch ? max(1, (int)((unsigned)(pairs + k.size - 1) / (unsigned)k.size)) : 0;
+    const int n = pieces(b0, k.size);
     const int incl = wave_scan(n), excl = base + incl - n;
     const bool mine = by_piece ? n > 0 && want >= excl && want < excl + n : b0 + lane == want;
     const uint64_t hit = __ballot(mine);
@@ -129,57 +138,86 @@ AXK_DEV Piece find_piece(const TreeArgs& a, int want, bool by_piece, int kg) {
   return k;
 }
 
-template <int D>
+// RT row tiles of 32 a wave, WR waves over the rows and KG = 4 / WR over the tokens.
+template <int D, int T, int RT, int WR>
 struct TreeCfg {
-  static constexpr int KS = D / 16;   // 16-deep MFMA steps of Q K^T
-  static constexpr int DT = D / 32;   // 32-wide tiles of O
-  static constexpr int RB = D * 2;    // bytes of a bf16 row
-  static constexpr int NCH = RB / 16; // its 16-byte chunks
-  static constexpr int PLANE = kPair * RB;
-  static constexpr int BUF = 2 * PLANE + 2 * kPair * 4;  // K, V, and the int8 scales of both
-  // Chunk c of K row r is kept at chunk c ^ (r mod 16) and of V row r at c ^ 4 (r mod 4), so that a K fragment read (32 rows,
-  // one chunk each) and a transposing V read (4 rows, 64 bytes each) cover all LDS banks.
-  static AXK_DEV int kswz(int r) { return r & (NCH < 16 ? NCH - 1 : 15); }
-  static AXK_DEV int vswz(int r) { return 4 * (NCH < 16 ? ((r >> 1) & 1) : (r & 3)); }
-  static constexpr int OLD = D + 4;   // floats of an O row in LDS
+  static constexpr int KG = 4 / WR;
+  static constexpr int RB = 32 * RT * WR;          // rows of a workgroup
+  static constexpr int KS = D / 16;                // 16-deep MFMA steps of Q K^T
+  static constexpr int DT = D / 32;                // 32-wide tiles of O
+  static constexpr int RBY = T == kBf16 ? 2 * D : D;  // bytes of a stored row
+  static constexpr int NCH = RBY / 16;             // its 16-byte chunks
+  static constexpr int RPI = 1024 / RBY;           // rows of one direct-to-LDS instruction (64 lanes x 16 B)
+  static constexpr int IPP = kTile / RPI;          // instructions of a tile's K (or V)
+  static constexpr int IPW = 4 * IPP / WR;         // a wave's, of a pair
+  static constexpr int TILE = kTile * RBY, PLANE = 2 * TILE;
+  static constexpr int OCC = RT == 1 && D <= 128 ? 2 : 1;  // workgroups a CU (registers: Q and O take 3 RT D / 4 of a wave's)
+  // Pairs of K, and of V, that a group holds in LDS: K is scored one pair ahead of the V that is weighted.
+  static constexpr int LDS_MAX = (OCC == 2 ? 80 : 160) * 1024 - 4096;
+  static constexpr int NS = KG * 8 * PLANE <= LDS_MAX ? 4 : 2;
+  static constexpr int SCALES = T == kI8 ? 8 * 256 : 0;  // a group's scales: of eight pairs' K and V rows
+  static constexpr int GROUP = 2 * NS * PLANE + SCALES;
+  static constexpr int RING = KG * GROUP;
+  static constexpr int JOIN = KG == 2 ? WR * RT * 32 * (D * 4 + 8) : 0;  // one group's results
+  static constexpr int LDS = (RING > JOIN ? RING : JOIN) + kMaxNodes * 8;  // and the ancestors
+  static_assert(KG * 4 * PLANE <= LDS_MAX && LDS <= 160 * 1024 && KG <= 2 && NS < 8, "LDS");
+  // Where chunk c of a tile's row r is kept: K fragment reads (32 rows, one or two chunks each) and transposing V reads (4 rows
+  // x 64 bytes of bf16, 8 rows x 32 bytes of 8 bits) then cover all LDS banks.
+  static AXK_DEV int kswz(int r) { return NCH == 4 ? (r >> 1) & 3 : r & (NCH < 16 ? NCH - 1 : 15); }
+  static AXK_DEV int vswz(int r) {
+    if constexpr (T == kBf16) return 4 * (NCH < 16 ? (r >> 1) & 1 : r & 3);
+    return 2 * (NCH < 8 ? (r >> 1) & 1 : r & 3);
+  }
 };
 
 AXK_DEV axk_f32x16 mfma_bf16_32x32x16(axk_bf16x8 a, axk_bf16x8 b, axk_f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// 16 stored bytes as bf16 chunks: one (bf16) or two (8-bit; int8: the codes, exact in bf16).
+// Eight stored 8-bit values (two dwords) as bf16: E4M3 times a power of two, or int8 codes, both exact.
 template <int T>
-AXK_DEV void as_bf16(const axk_u32x4 w, float inv_scale, axk_u32x4 (&out)[T == kBf16 ? 1 : 2]) {
-  if constexpr (T == kBf16) {
-    out[0] = w;
-  } else {
+AXK_DEV axk_bf16x8 bf16_of(uint32_t w0, uint32_t w1, float inv_scale) {
+  axk_u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t x = w[i / 2];
-      uint32_t r;
-      if constexpr (T == kFp8)
-        r = __builtin_bit_cast(uint32_t, i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, inv_scale, true)
-                                               : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, inv_scale, false));
-      else
-        r = pack_bf16x2((float)(int8_t)(x >> (16 * (i & 1))), (float)(int8_t)(x >> (16 * (i & 1) + 8)));
-      out[i / 4][i % 4] = r;
-    }
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = i < 2 ? w0 : w1;
+    if constexpr (T == kFp8)
+      r[i] = __builtin_bit_cast(uint32_t, i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, inv_scale, true)
+                                                : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, inv_scale, false));
+    else
+      r[i] = pack_bf16x2((float)(int8_t)(x >> (16 * (i & 1))), (float)(int8_t)(x >> (16 * (i & 1) + 8)));
   }
+  return __builtin_bit_cast(axk_bf16x8, r);
 }
 
-template <int D, int T, int WR>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tree_kernel(TreeArgs a) {
-  using C = TreeCfg<D>;
-  constexpr int KG = 4 / WR, NT = 64 * WR, RB = 32 * WR;
-  constexpr int CPU = T == kBf16 ? 1 : 2;           // bf16 chunks of a 16-byte load
-  constexpr int LPR = C::NCH / CPU;                 // loads of a row
-  constexpr int RPU = NT / LPR < kPair ? NT / LPR : kPair;  // rows of one load of all the group's threads
-  constexpr int UNITS = kPair / RPU;                // loads a thread and plane
-  constexpr int LOADERS = RPU * LPR;                // threads of the group that load (all but for 8-bit rows of 64 bytes)
-  static_assert(NT % LPR == 0 && UNITS * RPU == kPair, "a pair divides over the group's threads");
-  constexpr int SLOTS = WR == 1 ? 1 : 2;            // pairs of a group in LDS
+// A 2-byte value a lane, zero-extended, into LDS at lds_base + 4 * lane.
+AXK_DEV void lds_dma2(const void* gptr, uint32_t lds_base_any) {
+  const uint32_t lds_base = __builtin_amdgcn_readfirstlane(lds_base_any);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_ushort %1, off"
+      :
+      : "s"(lds_base), "v"(gptr)
+      : "memory");
+}
+
+// f(std::integral_constant<int, 0>) .. f(<N - 1>): an unrolled loop whose index is a constant expression.
+template <typename F, int... I>
+AXK_DEV void for_each_index_of(F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+AXK_DEV void for_each_index(F&& f) {
+  for_each_index_of(f, std::make_integer_sequence<int, N>{});
+}
+
+template <int D, int T, int RT, int WR>
+__global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_kernel(TreeArgs a) {
+  using C = TreeCfg<D, T, RT, WR>;
+  constexpr int KG = C::KG, RB = C::RB, KS = C::KS, DT = C::DT, NS = C::NS;
   extern __shared__ __align__(16) unsigned char smem[];
+  uint64_t* const s_anc = reinterpret_cast<uint64_t*>(smem + C::LDS - kMaxNodes * 8);
 
   const int sl = blockIdx.x >> 3;
   const int gi = sl / a.nb * 8 + (blockIdx.x & 7), blk = sl % a.nb;
@@ -188,7 +226,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tree_kernel(TreeA
   const Piece k = find_piece(a, gi / a.hkv, true, KG);
   if (k.b < 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kg = wave / WR, wr = wave % WR, gt = threadIdx.x - kg * NT;
+  const int kg = wave / WR, wr = wave % WR;
   const int l16 = lane & 15, l32 = lane & 31, h = lane >> 5;
   const int group = a.hq / a.hkv, rows = a.nodes * group;
 
@@ -196,354 +234,561 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tree_kernel(TreeA
   const int n = node_count(parent);
   const int base = k.s.len - n;  // the first node's position
   if (base < 0 && a.status && threadIdx.x == 0) *a.status = 1;
-
-  // this lane's row (lanes l and l + 32 share it)
-  const int r = blk * RB + 32 * wr + l32;
-  const bool inside = r < rows;
-  const int node = inside ? r / group : 0;
-  const int64_t qrow = ((int64_t)k.b * a.nodes + node) * a.hq + kvh * group + (inside ? r - node * group : 0);
   if (blk * RB >= n * group) {  // no node of this block is one
     if (k.ns == 1)
-      for (int i = threadIdx.x; i < RB * C::NCH; i += 256) {
-        const int rr = blk * RB + i / C::NCH;
+      for (int i = threadIdx.x; i < RB * D / 8; i += 256) {
+        const int rr = blk * RB + i / (D / 8);
         if (rr < rows) {
           const int t = rr / group;
-          const int64_t at = (((int64_t)k.b * a.nodes + t) * a.hq + kvh * group + rr - t * group) * D + i % C::NCH * 8;
+          const int64_t at = (((int64_t)k.b * a.nodes + t) * a.hq + kvh * group + rr - t * group) * D + i % (D / 8) * 8;
           *reinterpret_cast<axk_u32x4*>(a.out + at) = axk_u32x4{0u, 0u, 0u, 0u};
         }
       }
     return;
   }
-  const uint64_t anc_lane = ancestors(parent, a.nodes, a.status);
-  uint64_t anc = ((uint64_t)__shfl((uint32_t)(anc_lane >> 32), node) << 32) | __shfl((uint32_t)anc_lane, node);
-  const bool live = inside && anc != 0 && base >= 0;
 
-  // a negative scale moves into Q's signs and a zero scale into zero rows, so that scores keep their order
+  // this lane's rows (lanes l and l + 32 share them), and their q as the B operand
   const float c = a.scale == 0.f ? 1.0f : fabsf(a.scale);
-  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, keep = live && a.scale != 0.f ? 0xffffffffu : 0u;
-  axk_bf16x8 qb[C::KS];
+  // a negative scale moves into Q's signs and a zero scale into zero rows, so that scores keep their order
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, keep = a.scale != 0.f ? 0xffffffffu : 0u;
+  int node[RT];
+  int64_t qrow[RT];
+  axk_bf16x8 qb[RT][KS];
 #pragma unroll
-  for (int s = 0; s < C::KS; ++s) {
-    axk_u32x4 w = *reinterpret_cast<const axk_u32x4*>(a.q + qrow * D + 16 * s + 8 * h);
+  for (int t = 0; t < RT; ++t) {
+    const int r = blk * RB + 32 * (RT * wr + t) + l32, rr = min(r, rows - 1);
+    node[t] = r < rows ? r / group : -1;
+    const int nd = rr / group;
+    qrow[t] = ((int64_t)k.b * a.nodes + nd) * a.hq + kvh * group + rr - nd * group;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = (w[e] ^ flip) & keep;
-    qb[s] = __builtin_bit_cast(axk_bf16x8, w);
+    for (int s = 0; s < KS; ++s) {
+      // element (h, j) of step s: channel 16 s + 8 h + j; 8-bit rows are read 16 bytes a lane, two steps at a time:
+      // 32 (s / 2) + 16 h + 8 (s % 2) + j
+      const int ch = T == kBf16 ? 16 * s + 8 * h : 32 * (s / 2) + 16 * h + 8 * (s % 2);
+      axk_u32x4 w = *reinterpret_cast<const axk_u32x4*>(a.q + qrow[t] * D + ch);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = (w[e] ^ flip) & keep;
+      qb[t][s] = __builtin_bit_cast(axk_bf16x8, w);
+    }
   }
 
   // this group's pairs p_beg + kg, + KG, .. before p_end
-  const int p_all = pairs_of(k.s);
-  const int p_beg = k.j * k.size, p_end = min(p_all, p_beg + k.size);
-  const int steps = (p_end - p_beg + KG - 1) / KG;
+  const int p_beg = k.j * k.size + kg, p_end = min(pairs_of(k.s), k.j * k.size + k.size);
+  const int steps = p_end > p_beg ? (p_end - p_beg + KG - 1) / KG : 0;
+  const int all_steps = (max(p_end - k.j * k.size, 0) + KG - 1) / KG;  // of the workgroup (kg = 0)
   const int tpp = a.page / kTile;
-  const int64_t row_bytes = (int64_t)a.hkv * D * (T == kBf16 ? 2 : 1), plane_bytes = (int64_t)a.page * row_bytes;
-  const unsigned char* const head0 = a.cache + (int64_t)kvh * D * (T == kBf16 ? 2 : 1);
+  const int64_t row_bytes = (int64_t)a.hkv * C::RBY, plane_bytes = (int64_t)a.page * row_bytes, tile_bytes = kTile * row_bytes;
+  const unsigned char* const head0 = a.cache + (int64_t)kvh * C::RBY;
 
-  // page ids, 64 at a time: lane l holds that of the sequence's page 64 chunk + l
-  int chunk = -1, ids = 0;
-  auto page_id = [&](int lp) {
-    if ((lp >> 6) != chunk) {
-      chunk = lp >> 6;
-      const int j = (chunk << 6) + lane;
-      ids = j < k.s.np ? a.indices[k.s.pb + j] : 0;
-    }
-    return __builtin_amdgcn_readlane(ids, lp & 63);
+  // 64 pages of the sequence at a time: lane l holds the address of page 64 chunk + l; bad: the lanes whose page lies outside
+  // the pool (they hold page 0's)
+  int chunk = -1;
+  uint32_t pg_lo = 0, pg_hi = 0, pg_id = 0;
+  uint64_t bad = 0;
+  auto set_chunk = [&](int ck) {
+    chunk = ck;
+    const int j = (ck << 6) + lane;
+    const int pid = j < k.s.np ? a.indices[k.s.pb + j] : 0;
+    const bool out = pid < 0 || pid >= a.num_pages;
+    bad = __ballot(out);
+    if (bad && a.status && lane == 0) *a.status = 1;
+    pg_id = out ? 0 : pid;
+    const uint64_t at = (uint64_t)(uintptr_t)(head0 + (int64_t)pg_id * 2 * plane_bytes);
+    pg_lo = (uint32_t)at;
+    pg_hi = (uint32_t)(at >> 32);
   };
-  // the next pair's tiles: page and tile within it
-  int cur_lp = (2 * (p_beg + kg)) / tpp, cur_tp = 2 * (p_beg + kg) - cur_lp * tpp;
-
+  // The cursor of K: the next pair's first tile and its page. This wave loads one tile of every pair (WR = 4: one plane of it).
+  const int my_tile = WR == 4 ? wr >> 1 : wr, my_plane = wr & 1;
+  int cur_lp = 2 * p_beg / tpp, cur_tp = 2 * p_beg - cur_lp * tpp, cur_p = p_beg;
+  uint32_t bads = 0;  // two bits a pair in flight, the latest lowest: its tiles lie on pages outside the pool
   struct Tile {
-    const unsigned char* k;  // K of the tile's first token; V lies plane_bytes behind
-    int64_t at;              // its token slot in the pool's plane 0
-    int valid;               // tokens
+    const unsigned char* k;  // its K; V lies plane_bytes behind
+    int rows;                // with tokens, at least one: the others are read as the first
+    int64_t slot;            // (int8) its first row in the scales
   };
-  auto tile_of = [&](int lp, int tp, int first_tok) {
-    Tile t;
-    const bool in = lp < k.s.np;
-    const int pid = page_id(in ? lp : max(k.s.np - 1, 0));
-    const bool bad = pid < 0 || pid >= a.num_pages;
-    t.valid = in ? min(kTile, k.s.len - first_tok) : 0;
-    if (bad && t.valid > 0) {
-      if (a.status && lane == 0) *a.status = 1;
-      t.valid = 0;
+  Tile kp, vp;  // of the pair whose K is loaded next, and of the one before it, whose V is
+  auto page_base = [&](int at) {
+    const uint32_t lo = __builtin_amdgcn_readlane(pg_lo, at), hi = __builtin_amdgcn_readlane(pg_hi, at);
+    return reinterpret_cast<const unsigned char*>((uintptr_t)(((uint64_t)hi << 32) | lo));
+  };
+  auto next_pair = [&]() {
+    vp = kp;
+    bads <<= 2;
+    if (cur_tp + 2 <= tpp && (cur_lp >> 6) == chunk && cur_p * kPair + kPair <= k.s.len) {  // two whole tiles of one page
+      const int at = cur_lp & 63;
+      kp.k = page_base(at) + (cur_tp + my_tile) * tile_bytes;
+      kp.rows = kTile;
+      if constexpr (T == kI8) kp.slot = (int64_t)__builtin_amdgcn_readlane(pg_id, at) * 2 * a.page + (cur_tp + my_tile) * kTile;
+      bads |= ((uint32_t)(bad >> at) & 1) * 3;
+    } else {
+      int lp = cur_lp, tp = cur_tp;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (lp >= k.s.np) lp = cur_lp, tp = cur_tp;  // a tile past the sequence: its first one again
+        if ((lp >> 6) != chunk) set_chunk(lp >> 6);
+        const int at = lp & 63;
+        if (i == my_tile) {
+          kp.k = page_base(at) + tp * tile_bytes;
+          kp.rows = max(1, min(kTile, k.s.len - cur_p * kPair - kTile * i));
+          if constexpr (T == kI8) kp.slot = (int64_t)__builtin_amdgcn_readlane(pg_id, at) * 2 * a.page + tp * kTile;
+        }
+        bads |= ((uint32_t)(bad >> at) & 1) << i;
+        if (++tp == tpp) tp = 0, ++lp;
+      }
     }
-    const int64_t page = bad ? 0 : pid;
-    t.at = page * 2 * a.page + tp * kTile;
-    t.k = static_cast<const unsigned char*>(uniform_ptr(head0 + t.at * row_bytes));
-    return t;
-  };
-
-  axk_u32x4 kraw[UNITS], vraw[UNITS];
-  uint32_t vis_tiles = 0;  // rows of the pair in flight that hold tokens
-  uint16_t sraw[2];
-  int tok0 = 0;  // first token of the pair in flight
-  // loads of the group's next pair into registers; a row without a token is read as the tile's first one
-  auto load_pair = [&](int p) {
-    const int lp2 = cur_tp + 1 == tpp ? cur_lp + 1 : cur_lp, tp2 = cur_tp + 1 == tpp ? 0 : cur_tp + 1;
-    tok0 = p * kPair;
-    const Tile ta = tile_of(cur_lp, cur_tp, tok0), tb = tile_of(lp2, tp2, tok0 + kTile);
+    kp.k = static_cast<const unsigned char*>(uniform_ptr(kp.k));
+    cur_p += KG;
     cur_tp += 2 * KG;
     while (cur_tp >= tpp) cur_tp -= tpp, ++cur_lp;
-    const uint32_t rows_a = ta.valid > 0 ? (1u << ta.valid) - 1 : 0, rows_b = tb.valid > 0 ? (1u << tb.valid) - 1 : 0;
-    vis_tiles = (rows_a & 0xffffu) | (rows_b << 16);
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int i = (LOADERS < NT ? gt % LOADERS : gt) + u * NT, row = i / LPR, ch = i % LPR;
-      const bool second = row >= kTile;
-      const int64_t off = ((vis_tiles >> row) & 1) ? (row & 15) * row_bytes : 0;
-      const unsigned char* src = (second ? tb.k : ta.k) + off + ch * 16;
-      kraw[u] = *reinterpret_cast<const axk_u32x4*>(src);
-      vraw[u] = *reinterpret_cast<const axk_u32x4*>(src + plane_bytes);
-    }
-    if constexpr (T == kI8) {
-      const int row = lane & 31;
-      const bool second = row >= kTile;
-      const int64_t at = ((second ? tb.at : ta.at) + (((vis_tiles >> row) & 1) ? (row & 15) : 0)) * a.hkv + kvh;
-      sraw[0] = a.scales[at];
-      sraw[1] = a.scales[at + (int64_t)a.page * a.hkv];
-    }
-  };
-  // the pair in flight into the group's LDS slot; rows without a token are zero (weight 0 times any byte could be NaN)
-  auto store_pair = [&](unsigned char* buf) {
-    if (LOADERS == NT || gt < LOADERS)
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int i = gt + u * NT, row = i / LPR, ch = (i % LPR) * CPU;
-      const uint32_t there = ((vis_tiles >> row) & 1) ? 0xffffffffu : 0u;
-      axk_u32x4 kc[CPU], vc[CPU];
-      as_bf16<T>(kraw[u], a.inv_scale, kc);
-      as_bf16<T>(vraw[u], a.inv_scale, vc);
-#pragma unroll
-      for (int j = 0; j < CPU; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) kc[j][e] &= there, vc[j][e] &= there;
-        *reinterpret_cast<axk_u32x4*>(buf + row * C::RB + (((ch + j) ^ C::kswz(row)) * 16)) = kc[j];
-        *reinterpret_cast<axk_u32x4*>(buf + C::PLANE + row * C::RB + (((ch + j) ^ C::vswz(row)) * 16)) = vc[j];
-      }
-    }
-    if constexpr (T == kI8) {
-      if (gt < 64) {
-        const int row = lane & 31;
-        const float s = bf16_bits_to_f32(sraw[lane >> 5]);
-        reinterpret_cast<float*>(buf + 2 * C::PLANE)[lane] = ((vis_tiles >> row) & 1) ? s : 0.f;
-      }
-    }
   };
 
-  axk_f32x16 o[C::DT];
+  unsigned char* const ring = smem + kg * C::GROUP;  // K slots, V slots, scales
+  const uint32_t lds0 = lds_addr(ring) + my_tile * C::TILE;
+  // A load instruction takes RPI rows of a plane: this lane a 16-byte chunk of one, from where the row's order puts it.
+  // Instruction I's rows are I * RPI behind, which changes the order by the swizzle of I * RPI alone.
+  const int ln_row = lane / C::NCH, ln_ch = lane % C::NCH;
+  const uint32_t ln_k = (ln_ch ^ C::kswz(ln_row)) * 16, ln_v = (ln_ch ^ C::vswz(ln_row)) * 16;
+  const uint32_t row_b = (uint32_t)row_bytes, ln_off = ln_row * row_b;
+  auto load_plane = [&](auto whole, auto index, bool v, const Tile& t, int slot) {  // instruction `index` of the tile's plane
+    constexpr int I = decltype(index)::value, R = I * C::RPI;
+    const uint32_t turn = (v ? C::vswz(R) : C::kswz(R)) * 16;
+    uint32_t at = (v ? ln_v : ln_k) ^ turn;
+    if (decltype(whole)::value || R + ln_row < t.rows) at += ln_off + R * row_b;
+    const unsigned char* from = static_cast<const unsigned char*>(uniform_ptr(v ? t.k + plane_bytes : t.k));
+    lds_dma16_su_cached<I * 1024>(from, at, lds0 + (v ? NS * C::PLANE : 0) + slot * C::PLANE);
+  };
+  // load `index` (0 .. IPW - 1) of an iteration: K of kp into slot ks, V of vp into slot vs
+  auto load_one = [&](auto whole, auto index, int ks, int vs) {
+    constexpr int I = decltype(index)::value;
+    if constexpr (WR == 4) load_plane(whole, index, my_plane, my_plane ? vp : kp, my_plane ? vs : ks);
+    else if constexpr (I < C::IPP) load_plane(whole, index, false, kp, ks);
+    else load_plane(whole, std::integral_constant<int, I - C::IPP>{}, true, vp, vs);
+  };
+  // int8: the scales of step i's pair, of this wave's tile of kp: [tile][K, V][16]
+  auto load_scales = [&](int i) {
+    if constexpr (T == kI8) {
+      const int row = l16 < kp.rows ? l16 : 0;
+      const int64_t at = (kp.slot + row + (lane & 16 ? a.page : 0)) * a.hkv + kvh;
+      if (lane < 32) lds_dma2(a.scales + at, lds_addr(ring) + 2 * NS * C::PLANE + (i & 7) * 256 + my_tile * 128);
+    }
+  };
+  // ... read back: element e of group g for this lane's tokens 8 g + 4 h + e
+  auto scales_of = [&](int i, int v, int g) {
+    return *reinterpret_cast<const axk_u32x4*>(ring + 2 * NS * C::PLANE + (i & 7) * 256 + (g >> 1) * 128 + v * 64 +
+                                               (8 * (g & 1) + 4 * h) * 4);
+  };
+
+  axk_f32x16 o[RT][DT];
+  float m_run[RT], l_run[RT];  // l_run: this lane's half of the tokens
+  float s[RT][16];
 #pragma unroll
-  for (int t = 0; t < C::DT; ++t)
+  for (int t = 0; t < RT; ++t) {
+    m_run[t] = -INFINITY, l_run[t] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;  // l_run: this lane's half of the tokens
-  const int kaddr = l32 * C::RB;
-  const int vrow = 4 * h + (l16 >> 2);
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[t][d][i] = 0.f;
+  }
+  const axk_f32x16 zero16 = {};
+
+  // K row l32 of a pair as the A operand of step ks (8-bit: of steps ks and ks + 1)
+  const int krow = (l32 >> 4) * C::TILE + l16 * C::RBY, kx = C::kswz(l16);
+  auto k_read = [&](const unsigned char* kb, int ks) {
+    const int ch = T == kBf16 ? 2 * ks + h : ks + h;
+    return *reinterpret_cast<const axk_u32x4*>(kb + krow + ((ch ^ kx) * 16));
+  };
+  // V^T tile j % DT of the pair's tile j / DT as the A operand; MFMA k index (h, e) is token 8 (e / 4) + 4 h + e % 4
+  const int vrow = T == kBf16 ? 4 * h + (l16 >> 2) : 8 * (l16 >> 3) + 4 * h + ((l16 >> 1) & 3);
+  const int vx = C::vswz(vrow), vhi = (lane >> 4) & 1;
+  auto v_read = [&](const unsigned char* vb, int j) {
+    const int t = j % DT;
+    const unsigned char* row = vb + (j / DT) * C::TILE + vrow * C::RBY;
+    if constexpr (T == kBf16) {
+      const unsigned char* va = row + (((4 * t + 2 * vhi + ((l16 >> 1) & 1)) ^ vx) * 16) + 8 * (l16 & 1);
+      const axk_s16x4 v0 = lds_read_tr16(va), v1 = lds_read_tr16(va + 8 * C::RBY);  // (rows 8 apart are kept alike)
+      return __builtin_bit_cast(axk_u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const axk_i32x2 v = lds_read_tr8(row + (((2 * t + vhi) ^ vx) * 16) + 8 * (l16 & 1));
+      return axk_u32x4{(uint32_t)v[0], (uint32_t)v[1], 0u, 0u};
+    }
+  };
+  auto v_frag = [&](const axk_u32x4& w) {
+    if constexpr (T == kBf16) return __builtin_bit_cast(axk_bf16x8, w);
+    else return bf16_of<T>(w[0], w[1], a.inv_scale);
+  };
+
+  // what row tile t's row sees of the 32 tokens from `tok` on: history, then the row's ancestors
+  auto visible = [&](int t, int tok, uint32_t bad2) {
+    const uint64_t anc = node[t] >= 0 ? s_anc[node[t]] : 0;
+    const int off = tok - base;
+    uint32_t vis;
+    if (off <= -kPair) vis = 0xffffffffu;
+    else if (off < 0) vis = (0xffffffffu >> (kPair + off)) | ((uint32_t)anc << -off);
+    else vis = off < 64 ? (uint32_t)(anc >> off) : 0u;
+    return vis & ((bad2 & 1) ? 0xffff0000u : 0xffffffffu) & ((bad2 & 2) ? 0x0000ffffu : 0xffffffffu);
+  };
+  auto scale_scores = [&](int i) {  // int8: the K rows' scales
+    if constexpr (T == kI8) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const axk_u32x4 w = scales_of(i, 0, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) s[t][4 * g + e] *= bf16_bits_to_f32(w[e]);
+      }
+    }
+  };
   constexpr float kSlack = 8.0f;  // the reference maximum follows the scores in steps of more than 2^8
-
-  // MASKED: some row may not see some of the pair's tokens
-  auto compute = [&](auto masked, const unsigned char* buf, int tok, uint32_t rows_in) {
-    constexpr bool MASKED = decltype(masked)::value;
-    axk_f32x16 sn = {};
+  auto raise_max = [&](int t, float mx) {
+    const bool raise = mx > m_run[t] + kSlack;
+    if (__builtin_amdgcn_ballot_w64(raise)) {
+      const float alpha = raise ? __builtin_amdgcn_exp2f(m_run[t] - mx) : 1.0f;
+      if (raise) m_run[t] = mx;
+      l_run[t] *= alpha;
 #pragma unroll
-    for (int s = 0; s < C::KS; ++s) {
-      const axk_bf16x8 kf = *reinterpret_cast<const axk_bf16x8*>(buf + kaddr + (((2 * s + h) ^ C::kswz(l32)) * 16));
-      sn = mfma_bf16_32x32x16(kf, qb[s], sn);
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][d][i] *= alpha;
     }
-    float s[16], sv[16];
+  };
+  // the scores of step i are in s: masked, and their maximum taken up
+  auto masked_pair = [&](int i, uint32_t bad2) { return (p_beg + i * KG) * kPair + kPair > base || bad2; };
+  auto finish_scores = [&](auto hot, int i, uint32_t bad2, float (&mx)[RT]) {  // mx: the maxima of s, if nothing changes them
+    scale_scores(i);
+    const bool masked = !decltype(hot)::value && masked_pair(i, bad2);
+    if (masked) {
+      const int tok = (p_beg + i * KG) * kPair;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = sn[i];
-    if constexpr (T == kI8) {
-      const float* sc = reinterpret_cast<const float*>(buf + 2 * C::PLANE);
+      for (int t = 0; t < RT; ++t) {
+        const uint32_t vis = visible(t, tok, bad2) >> (4 * h);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const axk_f32x4 ks = *reinterpret_cast<const axk_f32x4*>(sc + 8 * i + 4 * h);
-        const axk_f32x4 vs = *reinterpret_cast<const axk_f32x4*>(sc + kPair + 8 * i + 4 * h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[4 * i + e] *= ks[e], sv[4 * i + e] = vs[e];
+        for (int e = 0; e < 16; ++e)
+          if (!((vis >> (8 * (e >> 2) + (e & 3))) & 1)) s[t][e] = -INFINITY;
       }
     }
-    uint32_t vis = 0;  // what the row sees of the pair's tokens: history, then its ancestors
-    if constexpr (MASKED) {
-      const int off = tok - base;
-      if (off <= -kPair) vis = 0xffffffffu;
-      else if (off < 0) vis = (0xffffffffu >> (kPair + off)) | ((uint32_t)anc << -off);
-      else vis = off < 64 ? (uint32_t)(anc >> off) : 0u;
-      vis &= rows_in;
-      const uint32_t mine = vis >> (4 * h);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if (masked || T == kI8) {
+        mx[t] = s[t][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx[t] = fmaxf(mx[t], s[t][e]);
+      }
+      raise_max(t, xor32_max(mx[t]) * c);
+    }
+  };
+  constexpr int KSTEP = T == kBf16 ? 1 : 2;  // steps of a K read
+  auto qk_step = [&](const axk_u32x4& w, int ks, axk_f32x16 (&sn)[RT]) {
+    if constexpr (T == kBf16) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) sn[t] = mfma_bf16_32x32x16(__builtin_bit_cast(axk_bf16x8, w), qb[t][ks], sn[t]);
+    } else {
+      const axk_bf16x8 f0 = bf16_of<T>(w[0], w[1], a.inv_scale), f1 = bf16_of<T>(w[2], w[3], a.inv_scale);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) sn[t] = mfma_bf16_32x32x16(f0, qb[t][ks], sn[t]);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) sn[t] = mfma_bf16_32x32x16(f1, qb[t][ks + 1], sn[t]);
+    }
+  };
+
+  if (wave == 0) {  // (a bad tree sets *status whatever piece sees it)
+    const uint64_t anc = ancestors(parent, a.nodes, a.status);
+    s_anc[lane] = base >= 0 ? anc : 0;
+  }
+  // K of pair 0, then an iteration's loads NS - 1 times: K of pair i + 1, V of pair i
+  const std::false_type any{};
+  if (steps > 0) {
+    next_pair();
+    vp = kp;
+    for_each_index<C::IPP>([&](auto i) {
+      if (WR == 2 || !my_plane) load_plane(any, i, false, kp, 0);
+    });
+    load_scales(0);
+#pragma unroll
+    for (int j = 1; j < NS; ++j) {
+      if (j < steps) next_pair();
+      else vp = kp, bads <<= 2;
+      if (j <= steps) {  // V of the last pair comes without another K
+        for_each_index<C::IPW>([&](auto i) { load_one(any, i, j, j - 1); });
+        if (j < steps) load_scales(j);
+      }
+    }
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+  if (steps > 0) {
+    // scores of pair 0
+    axk_f32x16 sn[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) sn[t] = zero16;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks += KSTEP) {
+      qk_step(k_read(ring, ks), ks, sn);
+      if (ks % 4 == 2) __builtin_amdgcn_sched_barrier(0);  // (few fragments at a time: registers)
+    }
+    float mx[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      mx[t] = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const bool seen = (mine >> (8 * (i >> 2) + (i & 3))) & 1;
-        s[i] = seen ? s[i] : -INFINITY;
-        if constexpr (T == kI8) sv[i] = seen ? sv[i] : 0.f;
+        s[t][i] = sn[t][i];
+        mx[t] = fmaxf(mx[t], s[t][i]);
       }
     }
-    float mx = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    mx = xor32_max(mx) * c;
-    const bool raise = mx > m_run + kSlack;
-    if (__builtin_amdgcn_ballot_w64(raise)) {
-      const float alpha = raise ? __builtin_amdgcn_exp2f(m_run - mx) : 1.0f;
-      if (raise) m_run = mx;
-      l_run *= alpha;
-#pragma unroll
-      for (int t = 0; t < C::DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[t][i] *= alpha;
+    finish_scores(any, 0, (bads >> (2 * (NS - 1))) & 3, mx);
+  }
+
+  // One step: pair i is weighted, pair i + 1 scored. HOT: whole pairs of history inside the pool, loads and a next pair to score,
+  // so that the loop of nearly all steps is free of masks and of the copies of O that meeting paths bring.
+  auto iteration = [&](auto hot, const int i) {
+    constexpr bool HOT = decltype(hot)::value;
+    // K of pair i + 1 and V of pair i have landed for every wave, and pair i - 1 has been read
+    if (i > 0) {
+      // (int8 at the end: an iteration without scales waits for all)
+      if (HOT || i + NS < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * (C::IPW + (T == kI8))) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
     }
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;
-    axk_bf16x8 pf[2];
+    const bool more = HOT || i + 1 < steps;  // wave-uniform: a next pair to score
+    const int ld = i + NS;                   // K of this pair and V of the one before it are loaded now
+    const bool loads = HOT || ld <= steps;
+    if (HOT || ld < steps) next_pair();
+    else vp = kp, bads <<= 2;
+    const int kslot = ld % NS, vslot = (ld - 1) % NS;
+    if (!HOT && i >= steps) return;
+    const uint32_t bad_i = (bads >> (2 * NS)) & 3, bad_n = (bads >> (2 * (NS - 1))) & 3;
+    const unsigned char* kb = ring + ((i + 1) % NS) * C::PLANE;
+    const unsigned char* vb = ring + NS * C::PLANE + (i % NS) * C::PLANE;
+    // One MFMA step a stage, with the LDS read of a later one, a share of the loads and of the vector work beside it: the
+    // scores of pair i + 1 run while pair i's become probabilities, and their maxima are taken while pair i is weighted. The
+    // compiler orders inside a stage only.
+    constexpr int NST = KS / KSTEP, KA = NST >= 8 ? 4 : NST / 2, VA = DT >= 4 ? 4 : DT;
+    axk_f32x16 sn[RT];
+    axk_u32x4 vf[VA];
+    float m_use[RT];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -m_use));
-      l_run += s[i];
-      if constexpr (T == kI8) s[i] *= sv[i];
+    for (int t = 0; t < RT; ++t) {
+      m_use[t] = m_run[t] == -INFINITY ? 0.f : m_run[t];
+      sn[t] = zero16;
     }
+    auto probs = [&](int lo, int hi) {
 #pragma unroll
-    for (int ti = 0; ti < 2; ++ti) {
-      axk_u32x4 w;
+      for (int e = lo; e < hi; ++e) {
+        const int t = e / 16, x = e % 16;
+        s[t][x] = __builtin_amdgcn_exp2f(fmaf(s[t][x], c, -m_use[t]));
+        l_run[t] += s[t][x];
+      }
+    };
+    if (HOT || ld < steps) load_scales(ld);
+    if (more) {
+      axk_u32x4 kf[KA];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(s[8 * ti + 2 * i], s[8 * ti + 2 * i + 1]);
-      pf[ti] = __builtin_bit_cast(axk_bf16x8, w);
+      for (int x = 0; x < KA; ++x) kf[x] = k_read(kb, x * KSTEP);
+      __builtin_amdgcn_sched_barrier(0);
+      for_each_index<NST>([&](auto stage) {
+        constexpr int I = decltype(stage)::value;
+        qk_step(kf[I % KA], I * KSTEP, sn);
+        if constexpr (I + KA < NST) kf[I % KA] = k_read(kb, (I + KA) * KSTEP);
+        else if constexpr (I + KA - NST < VA) vf[I + KA - NST] = v_read(vb, I + KA - NST);
+        if constexpr (I < C::IPW)
+          if (loads) load_one(hot, stage, kslot, vslot);
+        probs(I * 16 * RT / NST, (I + 1) * 16 * RT / NST);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) asm volatile("" : "+v"(l_run[t]));  // the sums stay in this stage
+        __builtin_amdgcn_sched_barrier(0);
+      });
+#pragma unroll
+      for (int x = KA; x < VA; ++x) vf[x] = v_read(vb, x);
+    } else {
+      if (loads) for_each_index<C::IPW>([&](auto x) { load_one(hot, x, kslot, vslot); });
+      probs(0, 16 * RT);
+#pragma unroll
+      for (int x = 0; x < VA; ++x) vf[x] = v_read(vb, x);
     }
-    uint32_t odd = 0;
-    const unsigned char* vb = buf + C::PLANE + vrow * C::RB + 8 * (l16 & 1);
-    const int vch = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+    axk_bf16x8 pf[RT][2];
 #pragma unroll
-    for (int ti = 0; ti < 2; ++ti)
+    for (int t = 0; t < RT; ++t) {
+      if constexpr (T == kI8) {  // the V rows' scales; what is not seen stays zero whatever they hold
 #pragma unroll
-      for (int t = 0; t < C::DT; ++t) {
-        const unsigned char* va = vb + ti * kTile * C::RB + (((4 * t + vch) ^ C::vswz(vrow)) * 16);
-        const axk_s16x4 v0 = lds_read_tr16(va), v1 = lds_read_tr16(va + 8 * C::RB);
-        axk_u32x4 vw = __builtin_bit_cast(axk_u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-        if constexpr (MASKED && T != kI8) {  // infinities and NaN left out: weight 0 times them would be NaN
+        for (int g = 0; g < 4; ++g) {
+          const axk_u32x4 w = scales_of(i, 1, g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t lo = (vw[e] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
-            const uint32_t hi = (vw[e] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
-            odd |= lo | hi;
-            vw[e] &= ~(lo | hi);
-          }
+          for (int e = 0; e < 4; ++e) s[t][4 * g + e] = s[t][4 * g + e] == 0.f ? 0.f : s[t][4 * g + e] * bf16_bits_to_f32(w[e]);
         }
-        o[t] = mfma_bf16_32x32x16(__builtin_bit_cast(axk_bf16x8, vw), pf[ti], o[t]);
       }
-    if constexpr (MASKED && T != kI8) {
-      if (__builtin_amdgcn_ballot_w64(odd != 0)) {  // .. and added for the rows that do see them
-        for (int j = 0; j < kPair; ++j) {
-          const unsigned char* row = buf + C::PLANE + j * C::RB + 8 * h;
-          const bool seen = (vis >> j) & 1;
 #pragma unroll
-          for (int i = 0; i < 4 * C::DT; ++i) {
-            const uint2 w = *reinterpret_cast<const uint2*>(row + ((i ^ C::vswz(j)) * 16));
-            const float x[4] = {__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                                __uint_as_float(w.y & 0xffff0000u)};
+      for (int x = 0; x < 2; ++x) {
+        axk_u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(s[t][8 * x + 2 * e], s[t][8 * x + 2 * e + 1]);
+        pf[t][x] = __builtin_bit_cast(axk_bf16x8, w);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float mx[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) mx[t] = -INFINITY;
+    auto take_scores = [&](int lo, int hi) {
+#pragma unroll
+      for (int e = lo; e < hi; ++e) {
+        const int t = e / 16, x = e % 16;
+        s[t][x] = sn[t][x];
+        asm volatile("" : "+v"(s[t][x]));  // one copy out of the accumulator
+        mx[t] = fmaxf(mx[t], s[t][x]);
+      }
+    };
+    if (!HOT && T != kI8 && masked_pair(i, bad_i)) {
+      // infinities and NaN of V are left out, since weight 0 times them would be NaN, and added for the rows that see them
+      uint32_t odd = 0;
+#pragma unroll
+      for (int j = 0; j < 2 * DT; ++j) {
+        axk_u32x4 w = __builtin_bit_cast(axk_u32x4, v_frag(v_read(vb, j)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t lo = (w[e] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
+          const uint32_t hi = (w[e] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
+          odd |= lo | hi;
+          w[e] &= ~(lo | hi);
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          o[t][j % DT] = mfma_bf16_32x32x16(__builtin_bit_cast(axk_bf16x8, w), pf[t][j / DT], o[t][j % DT]);
+          if constexpr (RT * D >= 256) asm volatile("" : "+a"(o[t][j % DT]));
+        }
+        if (j % 2) __builtin_amdgcn_sched_barrier(0);
+      }
+      if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+        uint32_t vis[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) vis[t] = visible(t, (p_beg + i * KG) * kPair, bad_i);
+        for (int j = 0; j < kPair; ++j) {
+          const unsigned char* row = vb + j * C::RBY;
+          const int x = C::vswz(j & 15);
+#pragma unroll
+          for (int g = 0; g < 4 * DT; ++g) {  // channels 8 g + 4 h .. + 3
+            float y[4];
+            if constexpr (T == kBf16) {
+              const uint2 w = *reinterpret_cast<const uint2*>(row + ((g ^ x) * 16) + 8 * h);
+              y[0] = __uint_as_float(w.x << 16), y[1] = __uint_as_float(w.x & 0xffff0000u);
+              y[2] = __uint_as_float(w.y << 16), y[3] = __uint_as_float(w.y & 0xffff0000u);
+            } else {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(row + (((g >> 1) ^ x) * 16) + 8 * (g & 1) + 4 * h);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = ((w >> (8 * e)) & 0x7f) == 0x7f ? NAN : 0.f;
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              o[i / 4][4 * (i % 4) + e] += seen && (__float_as_uint(x[e]) & 0x7f800000u) == 0x7f800000u ? x[e] : 0.f;
+#pragma unroll
+              for (int t = 0; t < RT; ++t)
+                o[t][g / 4][4 * (g % 4) + e] += ((vis[t] >> j) & 1) && !(fabsf(y[e]) < INFINITY) ? y[e] : 0.f;
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
-    }
-  };
-
-  unsigned char* const mine = smem + kg * SLOTS * C::BUF;
-  if (steps > 0) load_pair(p_beg + kg);  // (past p_end for a group without a pair: a tile without tokens)
-  for (int i = 0; i < steps; ++i) {
-    unsigned char* buf = mine + (i % SLOTS) * C::BUF;
-    const int p = p_beg + kg + i * KG, tok = tok0;
-    const uint32_t rows_in = p < p_end ? vis_tiles : 0u;
-    store_pair(buf);
-    if (i + 1 < steps) load_pair(p + KG);
-    if constexpr (WR == 1) {
-      __builtin_amdgcn_wave_barrier();
+      take_scores(0, 16 * RT);
     } else {
-      __syncthreads();
+      constexpr int PV = 2 * DT;
+      for_each_index<PV>([&](auto stage) {
+        constexpr int J = decltype(stage)::value;
+        const axk_bf16x8 w = v_frag(vf[J % VA]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          o[t][J % DT] = mfma_bf16_32x32x16(w, pf[t][J / DT], o[t][J % DT]);
+          if constexpr (RT * D >= 256) asm volatile("" : "+a"(o[t][J % DT]));  // (keeps the accumulators in AGPRs, and the stage)
+          else asm volatile("" : "+v"(o[t][J % DT]));
+        }
+        if constexpr (J + VA < PV) vf[J % VA] = v_read(vb, J + VA);
+        if constexpr (J >= 2) take_scores((J - 2) * 16 * RT / (PV - 2), (J - 1) * 16 * RT / (PV - 2));
+        __builtin_amdgcn_sched_barrier(0);
+      });
     }
-    if (p < p_end) {
-      if (tok + kPair > base || rows_in != 0xffffffffu) compute(std::true_type{}, buf, tok, rows_in);
-      else compute(std::false_type{}, buf, tok, rows_in);
+    if (more) finish_scores(hot, i + 1, bad_n, mx);
+  };
+  // steps whose pair lies wholly before token x
+  auto whole_steps = [&](int x) { return max((max(x, 0) / kPair - p_beg + KG - 1) / KG, 0); };
+  const int hot_end = min(steps - NS, min(whole_steps(k.s.len) - NS, whole_steps(base) - 1));
+  int step = 0;
+  for (; step < hot_end && !(bads & ((4u << (2 * NS)) - 1)); ++step) iteration(std::true_type{}, step);
+  for (; step < all_steps; ++step) iteration(any, step);
+
+
+  bool live[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    l_run[t] = xor32_sum(l_run[t]);
+    live[t] = node[t] >= 0 && s_anc[max(node[t], 0)] != 0;
+    if (__builtin_amdgcn_ballot_w64(!live[t])) {  // rows of no node may have attended the history: they get zeros
+      if (!live[t]) m_run[t] = -INFINITY, l_run[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][d][i] = live[t] ? o[t][d][i] : 0.f;
     }
   }
-  l_run = xor32_sum(l_run);
-  if (__builtin_amdgcn_ballot_w64(!live)) {  // rows of no node have attended with zero queries: they get zeros
-    if (!live) m_run = -INFINITY, l_run = 0.f;
+  if constexpr (KG == 2) {  // the second group's results through LDS to the first's waves, which hold the same rows
+    __syncthreads();
+    float2* const s_ml = reinterpret_cast<float2*>(smem);                       // [WR][RT][64]
+    axk_f32x4* const s_o = reinterpret_cast<axk_f32x4*>(smem + WR * RT * 512);  // [WR][RT * DT * 4][64]
+    if (kg == 1) {
 #pragma unroll
-    for (int t = 0; t < C::DT; ++t)
+      for (int t = 0; t < RT; ++t) {
+        if (h == 0) s_ml[(wr * RT + t) * 32 + l32] = make_float2(m_run[t], l_run[t]);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[t][i] = live ? o[t][i] : 0.f;
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            s_o[((wr * RT + t) * DT * 4 + d * 4 + g) * 64 + lane] =
+                axk_f32x4{o[t][d][4 * g], o[t][d][4 * g + 1], o[t][d][4 * g + 2], o[t][d][4 * g + 3]};
+      }
+    }
+    __syncthreads();
+    if (kg == 1) return;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const float2 ml = s_ml[(wr * RT + t) * 32 + l32];
+      const float m = fmaxf(m_run[t], ml.x);
+      const float f0 = m_run[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[t] - m);
+      const float f1 = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
+      m_run[t] = m;
+      l_run[t] = l_run[t] * f0 + ml.y * f1;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const axk_f32x4 x = s_o[((wr * RT + t) * DT * 4 + d * 4 + g) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][d][4 * g + e] = o[t][d][4 * g + e] * f0 + x[e] * f1;
+        }
+    }
   }
 
-  const int64_t slot0 = ((int64_t)(k.first + k.j) * a.hkv + kvh) * a.nb + blk;  // of this piece's rows in the workspace
-  if constexpr (KG == 1) {
-    if (!inside) return;
+  const int64_t slot0 = ((int64_t)gi * a.nb + blk) * RB;  // of this piece's rows in the workspace
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    if (node[t] < 0) continue;
     if (k.ns > 1) {
-      const int64_t slot = slot0 * RB + 32 * wr + l32;
-      if (h == 0) a.ml[slot] = make_float2(m_run, l_run);
+      const int64_t slot = slot0 + 32 * (RT * wr + t) + l32;
+      if (h == 0) a.ml[slot] = make_float2(m_run[t], l_run[t]);
 #pragma unroll
-      for (int t = 0; t < C::DT; ++t)
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<float4*>(a.po + slot * D + 32 * t + 8 * i + 4 * h) =
-              make_float4(o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]);
-      return;
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<axk_f32x4*>(a.po + slot * D + 32 * d + 8 * g + 4 * h) =
+              axk_f32x4{o[t][d][4 * g], o[t][d][4 * g + 1], o[t][d][4 * g + 2], o[t][d][4 * g + 3]};
+      continue;
     }
-    // lanes l and l + 32 exchange halves, so that each holds 8 columns of two: 32 t + 16 i + 8 h of its row
-    const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+    // lanes l and l + 32 exchange halves, so that each holds 8 columns of two: 16 i + 8 h of its row
+    const float inv = l_run[t] > 0.f ? 1.0f / l_run[t] : 0.f;
 #pragma unroll
-    for (int i = 0; i < 2 * C::DT; ++i) {
-      const auto& ot = o[i / 2];
+    for (int i = 0; i < 2 * DT; ++i) {
+      const auto& ot = o[t][i / 2];
       const int e = 8 * (i % 2);
       const auto w0 = __builtin_amdgcn_permlane32_swap(pack_bf16x2(ot[e] * inv, ot[e + 1] * inv),
                                                        pack_bf16x2(ot[e + 4] * inv, ot[e + 5] * inv), false, false);
       const auto w1 = __builtin_amdgcn_permlane32_swap(pack_bf16x2(ot[e + 2] * inv, ot[e + 3] * inv),
                                                        pack_bf16x2(ot[e + 6] * inv, ot[e + 7] * inv), false, false);
-      *reinterpret_cast<axk_u32x4*>(a.out + qrow * D + 16 * i + 8 * h) = axk_u32x4{w0[0], w1[0], w0[1], w1[1]};
-    }
-  } else {
-    // the groups' outputs of each row joined in LDS: every wave against the row's common maximum, then summed
-    __syncthreads();  // the pairs have been read
-    float2* const s_ml = reinterpret_cast<float2*>(smem);                   // [KG][RB]
-    float* const s_o = reinterpret_cast<float*>(smem + KG * RB * sizeof(float2));  // [KG][RB][OLD]
-    const int lr = 32 * wr + l32;
-    if (h == 0) s_ml[kg * RB + lr] = make_float2(m_run, l_run);
-    __syncthreads();
-    float m_all = -INFINITY;
-#pragma unroll
-    for (int g = 0; g < KG; ++g) m_all = fmaxf(m_all, s_ml[g * RB + lr].x);
-    const float f = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_all);
-#pragma unroll
-    for (int t = 0; t < C::DT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<axk_f32x4*>(s_o + (kg * RB + lr) * C::OLD + 32 * t + 8 * i + 4 * h) =
-            axk_f32x4{o[t][4 * i] * f, o[t][4 * i + 1] * f, o[t][4 * i + 2] * f, o[t][4 * i + 3] * f};
-    __syncthreads();
-    constexpr int VPR = D / 4;  // groups of four columns
-    for (int i = threadIdx.x; i < RB * VPR; i += 256) {
-      const int row = i / VPR, col = i % VPR * 4, rr = blk * RB + row;
-      if (rr >= rows) break;
-      axk_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-      float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-      for (int g = 0; g < KG; ++g) mm = fmaxf(mm, s_ml[g * RB + row].x);
-#pragma unroll
-      for (int g = 0; g < KG; ++g) {
-        const float2 x = s_ml[g * RB + row];
-        ll += x.x == -INFINITY ? 0.f : x.y * __builtin_amdgcn_exp2f(x.x - mm);
-        const axk_f32x4 v = *reinterpret_cast<const axk_f32x4*>(s_o + (g * RB + row) * C::OLD + col);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += v[e];
-      }
-      if (k.ns > 1) {
-        const int64_t slot = slot0 * RB + row;
-        if (col == 0) a.ml[slot] = make_float2(mm, ll);
-        *reinterpret_cast<axk_f32x4*>(a.po + slot * D + col) = sum;
-      } else {
-        const float inv = ll > 0.f ? 1.0f / ll : 0.f;
-        const int t = rr / group;
-        const int64_t at = (((int64_t)k.b * a.nodes + t) * a.hq + kvh * group + rr - t * group) * D + col;
-        *reinterpret_cast<uint2*>(a.out + at) = make_uint2(pack_bf16x2(sum[0] * inv, sum[1] * inv),
-                                                           pack_bf16x2(sum[2] * inv, sum[3] * inv));
-      }
+      *reinterpret_cast<axk_u32x4*>(a.out + qrow[t] * D + 16 * i + 8 * h) = axk_u32x4{w0[0], w1[0], w0[1], w1[1]};
     }
   }
 }
@@ -600,42 +845,45 @@ __global__ __launch_bounds__(64 * kMergeRows) void paged_tree_merge_kernel(TreeA
   for (int e = 0; e < PER; ++e) out[e] = (uint16_t)f32_to_bf16_bits(acc[e] * inv);
 }
 
-template <int D, int T, int WR>
+template <int D, int T, int RT, int WR>
 int launch(const TreeArgs& a, hipStream_t st) {
-  using C = TreeCfg<D>;
-  constexpr int KG = 4 / WR, RB = 32 * WR, SLOTS = WR == 1 ? 1 : 2;
-  constexpr size_t pairs = (size_t)KG * SLOTS * C::BUF;
-  constexpr size_t join = KG > 1 ? (size_t)KG * RB * (sizeof(float2) + sizeof(float) * C::OLD) : 0;
-  constexpr size_t lds = pairs > join ? pairs : join;
-  static_assert(lds <= 160 * 1024, "LDS of a CU");
-  if constexpr (lds > 64 * 1024) {  // to be allowed once on each device
+  using C = TreeCfg<D, T, RT, WR>;
+  if constexpr (C::LDS > 64 * 1024) {  // to be allowed once on each device
     static AxkOnce once[64];
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return AXK_E_LAUNCH;
-    if (const int e = axk_raise_lds(once[dev & 63], reinterpret_cast<const void*>(&paged_tree_kernel<D, T, WR>), lds)) return e;
+    if (const int e = axk_raise_lds(once[dev & 63], reinterpret_cast<const void*>(&paged_tree_kernel<D, T, RT, WR>), C::LDS))
+      return e;
   }
   AXK_LAUNCH_GATE();
   const int64_t grid = 8 * (int64_t)a.nb * ((a.groups + 7) / 8);
-  hipLaunchKernelGGL((paged_tree_kernel<D, T, WR>), dim3((unsigned)grid), dim3(256), lds, st, a);
+  hipLaunchKernelGGL((paged_tree_kernel<D, T, RT, WR>), dim3((unsigned)grid), dim3(256), C::LDS, st, a);
   if (a.split) {
     const int64_t rows = (int64_t)a.batch * a.nodes * a.hq;
     hipLaunchKernelGGL((paged_tree_merge_kernel<D>), dim3((unsigned)((rows + kMergeRows - 1) / kMergeRows)),
-                       dim3(64 * kMergeRows), 0, st, a, RB, KG);
+                       dim3(64 * kMergeRows), 0, st, a, C::RB, C::KG);
   }
   return axk_launch_status();
 }
 
+// The variant by the rows of a workgroup.
+template <int D, int T>
+int launch_rows(const TreeArgs& a, int rb, hipStream_t st) {
+  if (rb == 64) return launch<D, T, 1, 2>(a, st);
+  if constexpr (D == 256) return launch<D, T, 1, 4>(a, st);
+  else return rb == 128 ? launch<D, T, 2, 2>(a, st) : launch<D, T, 2, 4>(a, st);
+}
 template <int T>
-int launch_type(const TreeArgs& a, int d, int wr, hipStream_t st) {
+int launch_type(const TreeArgs& a, int d, int rb, hipStream_t st) {
   switch (d) {
-    case 64: return wr == 1 ? launch<64, T, 1>(a, st) : wr == 2 ? launch<64, T, 2>(a, st) : launch<64, T, 4>(a, st);
-    case 128: return wr == 1 ? launch<128, T, 1>(a, st) : wr == 2 ? launch<128, T, 2>(a, st) : launch<128, T, 4>(a, st);
-    default: return wr == 1 ? launch<256, T, 1>(a, st) : wr == 2 ? launch<256, T, 2>(a, st) : launch<256, T, 4>(a, st);
+    case 64: return launch_rows<64, T>(a, rb, st);
+    case 128: return launch_rows<128, T>(a, rb, st);
+    default: return launch_rows<256, T>(a, rb, st);
   }
 }
 
-__attribute__((visibility("hidden"))) int launch_bf16(const TreeArgs& a, int d, int wr, hipStream_t st);
-__attribute__((visibility("hidden"))) int launch_fp8(const TreeArgs& a, int d, int wr, hipStream_t st);
-__attribute__((visibility("hidden"))) int launch_i8(const TreeArgs& a, int d, int wr, hipStream_t st);
+__attribute__((visibility("hidden"))) int launch_bf16(const TreeArgs& a, int d, int rb, hipStream_t st);
+__attribute__((visibility("hidden"))) int launch_fp8(const TreeArgs& a, int d, int rb, hipStream_t st);
+__attribute__((visibility("hidden"))) int launch_i8(const TreeArgs& a, int d, int rb, hipStream_t st);
 
 }  // namespace axk_tree

@@ -239,28 +239,24 @@ int write_rope(const uint16_t* q, int64_t ldq, int64_t hdq, const uint16_t* k, i
 // ---- the tree's attention: how it is cut, from what the host knows ----
 constexpr int kMinPiece = 8;  // pairs: 256 tokens
 struct TreePlan {
-  int wr, nb, den, split;
+  int rb, nb, den, split;
   int64_t groups;
   size_t ml, po;
 };
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Waves over the rows of a workgroup: as many as the tree's rows of one KV head need, the others over its tokens.
-int waves_of(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
-
 TreePlan tree_plan(int64_t batch, int64_t nodes, int64_t hq, int64_t hkv, int64_t d, int64_t max_pairs) {
   TreePlan p;
   const int64_t rows = nodes * (hq / hkv);
-  p.wr = waves_of(rows);
-  const int64_t rb = 32 * p.wr, nb = (rows + rb - 1) / rb;
+  p.rb = rows <= 64 ? 64 : rows <= 128 || d == 256 ? 128 : 256;
+  const int64_t nb = (rows + p.rb - 1) / p.rb;
   p.nb = (int)nb;
-  const int64_t slots = d == 256 ? 256 : 512, each = hkv * nb;  // workgroups that run at once; those of one piece
-  int64_t den = (slots - batch * each) / each;
-  den = den > slots / 2 / each ? den : slots / 2 / each;
+  const int64_t slots = p.rb == 64 && d <= 128 ? 512 : 256;  // workgroups that run at once
+  const int64_t den = slots / (hkv * nb);
   p.den = (int)(den > 1 ? den : 1);
   p.split = p.den > 1 && max_pairs > kMinPiece;
   p.groups = (batch + (p.split ? p.den : 0)) * hkv;
-  const size_t slot_rows = (size_t)p.groups * nb * rb;
+  const size_t slot_rows = (size_t)p.groups * nb * p.rb;
   p.ml = p.split ? round256(slot_rows * sizeof(float2)) : 0;
   p.po = p.split ? slot_rows * d * sizeof(float) : 0;
   return p;
@@ -310,9 +306,9 @@ int tree_verify(const uint16_t* q, const void* cache, int type, float kv_scale, 
   a.scale = sm_scale * axk_tree::kLog2e;
   a.inv_scale = type == kFp8 ? 1.0f / kv_scale : 1.0f;
   hipStream_t st = axk_stream(stream);
-  return type == kBf16 ? axk_tree::launch_bf16(a, (int)d, p.wr, st)
-         : type == kFp8 ? axk_tree::launch_fp8(a, (int)d, p.wr, st)
-                        : axk_tree::launch_i8(a, (int)d, p.wr, st);
+  return type == kBf16 ? axk_tree::launch_bf16(a, (int)d, p.rb, st)
+         : type == kFp8 ? axk_tree::launch_fp8(a, (int)d, p.rb, st)
+                        : axk_tree::launch_i8(a, (int)d, p.rb, st);
 }
 
 }  // namespace

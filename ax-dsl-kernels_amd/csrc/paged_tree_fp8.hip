@@ -2,5 +2,5 @@
 #include "paged_tree.h"
 
 namespace axk_tree {
-int launch_fp8(const TreeArgs& a, int d, int wr, hipStream_t st) { return launch_type<kFp8>(a, d, wr, st); }
+int launch_fp8(const TreeArgs& a, int d, int rb, hipStream_t st) { return launch_type<kFp8>(a, d, rb, st); }
 }  // namespace axk_tree
