@@ -159,12 +159,12 @@ struct TreeCfg {
   static constexpr int GROUP = 2 * NS * PLANE + SCALES;
   static constexpr int RING = KG * GROUP;
   static constexpr int JOIN = KG == 2 ? WR * RT * 32 * (D * 4 + 8) : 0;  // one group's results
-  static constexpr int LDS = (RING > JOIN ? RING : JOIN) + kMaxNodes * 8;  // and the ancestors
+  static constexpr int LDS = (RING > JOIN ? RING : JOIN) + kMaxNodes * 8 + 16;  // and the ancestors, and a flag
   static_assert(KG * 4 * PLANE <= LDS_MAX && LDS <= 160 * 1024 && KG <= 2 && NS < 8, "LDS");
   // Where chunk c of a tile's row r is kept: K fragment reads (32 rows, one or two chunks each) and transposing V reads (4 rows
   // x 64 bytes of bf16, 8 rows x 32 bytes of 8 bits) then cover all LDS banks.
-  static AXK_DEV int kswz(int r) { return NCH == 4 ? (r >> 1) & 3 : r & (NCH < 16 ? NCH - 1 : 15); }
-  static AXK_DEV int vswz(int r) {
+  static constexpr __host__ __device__ int kswz(int r) { return NCH == 4 ? (r >> 1) & 3 : r & (NCH < 16 ? NCH - 1 : 15); }
+  static constexpr __host__ __device__ int vswz(int r) {
     if constexpr (T == kBf16) return 4 * (NCH < 16 ? (r >> 1) & 1 : r & 3);
     return 2 * (NCH < 8 ? (r >> 1) & 1 : r & 3);
   }
@@ -217,7 +217,8 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   using C = TreeCfg<D, T, RT, WR>;
   constexpr int KG = C::KG, RB = C::RB, KS = C::KS, DT = C::DT, NS = C::NS;
   extern __shared__ __align__(16) unsigned char smem[];
-  uint64_t* const s_anc = reinterpret_cast<uint64_t*>(smem + C::LDS - kMaxNodes * 8);
+  uint64_t* const s_anc = reinterpret_cast<uint64_t*>(smem + C::LDS - kMaxNodes * 8 - 16);
+  int* const s_odd = reinterpret_cast<int*>(smem + C::LDS - 16);
 
   const int sl = blockIdx.x >> 3;
   const int gi = sl / a.nb * 8 + (blockIdx.x & 7), blk = sl % a.nb;
@@ -288,7 +289,8 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   auto set_chunk = [&](int ck) {
     chunk = ck;
     const int j = (ck << 6) + lane;
-    const int pid = j < k.s.np ? a.indices[k.s.pb + j] : 0;
+    int pid = j < k.s.np ? a.indices[k.s.pb + j] : 0;
+    asm volatile("" : "+v"(pid));  // the compiler's wait for the load stays here, behind no loop of direct loads
     const bool out = pid < 0 || pid >= a.num_pages;
     bad = __ballot(out);
     if (bad && a.status && lane == 0) *a.status = 1;
@@ -301,25 +303,29 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   const int my_tile = WR == 4 ? wr >> 1 : wr, my_plane = wr & 1;
   int cur_lp = 2 * p_beg / tpp, cur_tp = 2 * p_beg - cur_lp * tpp, cur_p = p_beg;
   uint32_t bads = 0;  // two bits a pair in flight, the latest lowest: its tiles lie on pages outside the pool
-  struct Tile {
-    const unsigned char* k;  // its K; V lies plane_bytes behind
-    int rows;                // with tokens, at least one: the others are read as the first
-    int64_t slot;            // (int8) its first row in the scales
-  };
-  Tile kp, vp;  // of the pair whose K is loaded next, and of the one before it, whose V is
+  // That tile of the pair whose K is loaded next (k_), and of the one before it, whose V is (v_): its K (V lies plane_bytes
+  // behind), its rows with tokens, at least one (the others are read as the first), and (int8) its first row in the scales.
+  const unsigned char *k_at = head0, *v_at = head0;
+  int k_rows = 1, v_rows = 1;
+  int64_t k_slot = 0;
   auto page_base = [&](int at) {
     const uint32_t lo = __builtin_amdgcn_readlane(pg_lo, at), hi = __builtin_amdgcn_readlane(pg_hi, at);
     return reinterpret_cast<const unsigned char*>((uintptr_t)(((uint64_t)hi << 32) | lo));
   };
-  auto next_pair = [&]() {
-    vp = kp;
+  // Whether the next pair is whole and its pages are among those at hand.
+  auto at_hand = [&]() {
+    return ((cur_lp + (cur_tp + 1 == tpp)) >> 6) == chunk && (cur_lp >> 6) == chunk && cur_p * kPair + kPair <= k.s.len;
+  };
+  auto next_pair = [&](auto hot) {  // hot: at_hand() holds
+    v_at = k_at, v_rows = k_rows;
     bads <<= 2;
-    if (cur_tp + 2 <= tpp && (cur_lp >> 6) == chunk && cur_p * kPair + kPair <= k.s.len) {  // two whole tiles of one page
-      const int at = cur_lp & 63;
-      kp.k = page_base(at) + (cur_tp + my_tile) * tile_bytes;
-      kp.rows = kTile;
-      if constexpr (T == kI8) kp.slot = (int64_t)__builtin_amdgcn_readlane(pg_id, at) * 2 * a.page + (cur_tp + my_tile) * kTile;
-      bads |= ((uint32_t)(bad >> at) & 1) * 3;
+    if constexpr (decltype(hot)::value) {
+      const int wrap = cur_tp + 1 == tpp, at1 = (cur_lp + wrap) & 63, at = my_tile ? at1 : cur_lp & 63;
+      const int tp = my_tile ? (wrap ? 0 : cur_tp + 1) : cur_tp;
+      k_at = page_base(at) + tp * tile_bytes;
+      k_rows = kTile;
+      if constexpr (T == kI8) k_slot = (int64_t)__builtin_amdgcn_readlane(pg_id, at) * 2 * a.page + tp * kTile;
+      bads |= (uint32_t)((bad >> (cur_lp & 63)) & 1) | (uint32_t)((bad >> at1) & 1) << 1;
     } else {
       int lp = cur_lp, tp = cur_tp;
 #pragma unroll
@@ -328,15 +334,15 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
         if ((lp >> 6) != chunk) set_chunk(lp >> 6);
         const int at = lp & 63;
         if (i == my_tile) {
-          kp.k = page_base(at) + tp * tile_bytes;
-          kp.rows = max(1, min(kTile, k.s.len - cur_p * kPair - kTile * i));
-          if constexpr (T == kI8) kp.slot = (int64_t)__builtin_amdgcn_readlane(pg_id, at) * 2 * a.page + tp * kTile;
+          k_at = page_base(at) + tp * tile_bytes;
+          k_rows = max(1, min(kTile, k.s.len - cur_p * kPair - kTile * i));
+          if constexpr (T == kI8) k_slot = (int64_t)__builtin_amdgcn_readlane(pg_id, at) * 2 * a.page + tp * kTile;
         }
         bads |= ((uint32_t)(bad >> at) & 1) << i;
         if (++tp == tpp) tp = 0, ++lp;
       }
     }
-    kp.k = static_cast<const unsigned char*>(uniform_ptr(kp.k));
+    k_at = static_cast<const unsigned char*>(uniform_ptr(k_at));
     cur_p += KG;
     cur_tp += 2 * KG;
     while (cur_tp >= tpp) cur_tp -= tpp, ++cur_lp;
@@ -349,26 +355,37 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   const int ln_row = lane / C::NCH, ln_ch = lane % C::NCH;
   const uint32_t ln_k = (ln_ch ^ C::kswz(ln_row)) * 16, ln_v = (ln_ch ^ C::vswz(ln_row)) * 16;
   const uint32_t row_b = (uint32_t)row_bytes, ln_off = ln_row * row_b;
-  auto load_plane = [&](auto whole, auto index, bool v, const Tile& t, int slot) {  // instruction `index` of the tile's plane
-    constexpr int I = decltype(index)::value, R = I * C::RPI;
-    const uint32_t turn = (v ? C::vswz(R) : C::kswz(R)) * 16;
-    uint32_t at = (v ? ln_v : ln_k) ^ turn;
-    if (decltype(whole)::value || R + ln_row < t.rows) at += ln_off + R * row_b;
-    const unsigned char* from = static_cast<const unsigned char*>(uniform_ptr(v ? t.k + plane_bytes : t.k));
-    lds_dma16_su_cached<I * 1024>(from, at, lds0 + (v ? NS * C::PLANE : 0) + slot * C::PLANE);
+  struct Stream {  // where an iteration's loads of this wave come from and go to (K, V; WR = 4: the one it loads, in k)
+    const unsigned char *k, *v;
+    uint32_t lds_k, lds_v;
+    int rows_k, rows_v;
   };
-  // load `index` (0 .. IPW - 1) of an iteration: K of kp into slot ks, V of vp into slot vs
-  auto load_one = [&](auto whole, auto index, int ks, int vs) {
-    constexpr int I = decltype(index)::value;
-    if constexpr (WR == 4) load_plane(whole, index, my_plane, my_plane ? vp : kp, my_plane ? vs : ks);
-    else if constexpr (I < C::IPP) load_plane(whole, index, false, kp, ks);
-    else load_plane(whole, std::integral_constant<int, I - C::IPP>{}, true, vp, vs);
+  const uint32_t vmask = my_plane ? 0xffffffffu : 0u;
+  auto stream = [&](int ks, int vs) {  // the next K into slot ks, the V before it into slot vs
+    const uint32_t lk = lds0 + ks * C::PLANE, lv = lds0 + (NS + vs) * C::PLANE;
+    if constexpr (WR == 4) {
+      const int rk = k_rows, rv = v_rows;
+      const unsigned char *ka = k_at, *va = v_at + plane_bytes;
+      return Stream{static_cast<const unsigned char*>(uniform_ptr(my_plane ? va : ka)), nullptr, my_plane ? lv : lk, 0u,
+                    my_plane ? rv : rk, 0};
+    }
+    return Stream{k_at, static_cast<const unsigned char*>(uniform_ptr(v_at + plane_bytes)), lk, lv, k_rows, v_rows};
   };
-  // int8: the scales of step i's pair, of this wave's tile of kp: [tile][K, V][16]
+  const uint32_t ln_one = WR == 4 && my_plane ? ln_v : ln_k;
+  // load `index` (0 .. IPW - 1) of an iteration
+  auto load_one = [&](auto whole, auto index, const Stream& st) {
+    constexpr int I0 = decltype(index)::value, I = I0 % C::IPP, R = I * C::RPI;
+    constexpr uint32_t TK = C::kswz(R) * 16, TV = C::vswz(R) * 16;
+    constexpr bool V = I0 >= C::IPP;  // (WR = 2: K first)
+    uint32_t at = WR == 4 ? ln_one ^ (TK ^ (vmask & (TK ^ TV))) : V ? ln_v ^ TV : ln_k ^ TK;
+    if (decltype(whole)::value || R + ln_row < (V ? st.rows_v : st.rows_k)) at += ln_off + R * row_b;
+    lds_dma16_su_cached<I * 1024>(V ? st.v : st.k, at, V ? st.lds_v : st.lds_k);
+  };
+  // int8: the scales of step i's pair, of this wave's tile: [tile][K, V][16]
   auto load_scales = [&](int i) {
     if constexpr (T == kI8) {
-      const int row = l16 < kp.rows ? l16 : 0;
-      const int64_t at = (kp.slot + row + (lane & 16 ? a.page : 0)) * a.hkv + kvh;
+      const int row = l16 < k_rows ? l16 : 0;
+      const int64_t at = (k_slot + row + (lane & 16 ? a.page : 0)) * a.hkv + kvh;
       if (lane < 32) lds_dma2(a.scales + at, lds_addr(ring) + 2 * NS * C::PLANE + (i & 7) * 256 + my_tile * 128);
     }
   };
@@ -390,25 +407,30 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       for (int i = 0; i < 16; ++i) o[t][d][i] = 0.f;
   }
   const axk_f32x16 zero16 = {};
+  bool odd_any = false;  // whether V of a masked pair held what is no number
 
+  // LDS addresses in bytes: a fragment's chunk is an exclusive or with a constant, as rows are powers of two of bytes.
+  typedef const __attribute__((address_space(3))) axk_u32x4* LdsVec;
+  typedef __attribute__((address_space(3))) axk_s16x4* LdsTr16;
+  typedef __attribute__((address_space(3))) axk_i32x2* LdsTr8;
+  const uint32_t ring0 = lds_addr(ring);
   // K row l32 of a pair as the A operand of step ks (8-bit: of steps ks and ks + 1)
-  const int krow = (l32 >> 4) * C::TILE + l16 * C::RBY, kx = C::kswz(l16);
-  auto k_read = [&](const unsigned char* kb, int ks) {
-    const int ch = T == kBf16 ? 2 * ks + h : ks + h;
-    return *reinterpret_cast<const axk_u32x4*>(kb + krow + ((ch ^ kx) * 16));
+  const uint32_t k_lane = ring0 + (l32 >> 4) * C::TILE + l16 * C::RBY + ((h ^ C::kswz(l16)) * 16);
+  auto k_read = [&](uint32_t kb, int ks) {  // kb: k_lane of the pair's slot
+    return *(LdsVec)(uintptr_t)(kb ^ ((T == kBf16 ? 32 : 16) * ks));
   };
   // V^T tile j % DT of the pair's tile j / DT as the A operand; MFMA k index (h, e) is token 8 (e / 4) + 4 h + e % 4
   const int vrow = T == kBf16 ? 4 * h + (l16 >> 2) : 8 * (l16 >> 3) + 4 * h + ((l16 >> 1) & 3);
-  const int vx = C::vswz(vrow), vhi = (lane >> 4) & 1;
-  auto v_read = [&](const unsigned char* vb, int j) {
-    const int t = j % DT;
-    const unsigned char* row = vb + (j / DT) * C::TILE + vrow * C::RBY;
+  const int vch = T == kBf16 ? 2 * ((lane >> 4) & 1) + ((l16 >> 1) & 1) : (lane >> 4) & 1;
+  const uint32_t v_lane = ring0 + NS * C::PLANE + vrow * C::RBY + ((vch ^ C::vswz(vrow)) * 16) + 8 * (l16 & 1);
+  auto v_read = [&](uint32_t vb, int j) {  // vb: v_lane of the pair's slot
+    const uint32_t at = (vb ^ ((T == kBf16 ? 64 : 32) * (j % DT))) + (j / DT) * C::TILE;
     if constexpr (T == kBf16) {
-      const unsigned char* va = row + (((4 * t + 2 * vhi + ((l16 >> 1) & 1)) ^ vx) * 16) + 8 * (l16 & 1);
-      const axk_s16x4 v0 = lds_read_tr16(va), v1 = lds_read_tr16(va + 8 * C::RBY);  // (rows 8 apart are kept alike)
+      const axk_s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr16)(uintptr_t)at);
+      const axk_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr16)(uintptr_t)(at + 8 * C::RBY));  // (kept alike)
       return __builtin_bit_cast(axk_u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      const axk_i32x2 v = lds_read_tr8(row + (((2 * t + vhi) ^ vx) * 16) + 8 * (l16 & 1));
+      const axk_i32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsTr8)(uintptr_t)at);
       return axk_u32x4{(uint32_t)v[0], (uint32_t)v[1], 0u, 0u};
     }
   };
@@ -439,6 +461,10 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       }
     }
   };
+  auto pin = [](axk_f32x16& x) {  // a result stays where it is written; large ones in AGPRs
+    if constexpr (RT * D >= 256) asm volatile("" : "+a"(x));
+    else asm volatile("" : "+v"(x));
+  };
   constexpr float kSlack = 8.0f;  // the reference maximum follows the scores in steps of more than 2^8
   auto raise_max = [&](int t, float mx) {
     const bool raise = mx > m_run[t] + kSlack;
@@ -447,9 +473,12 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       if (raise) m_run[t] = mx;
       l_run[t] *= alpha;
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][d][i] *= alpha;
+        pin(o[t][d]);  // (tile by tile: all at once they would push what the loop keeps out of its registers)
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   };
   // the scores of step i are in s: masked, and their maximum taken up
@@ -494,22 +523,23 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   if (wave == 0) {  // (a bad tree sets *status whatever piece sees it)
     const uint64_t anc = ancestors(parent, a.nodes, a.status);
     s_anc[lane] = base >= 0 ? anc : 0;
+    if (lane == 0) *s_odd = 0;
   }
   // K of pair 0, then an iteration's loads NS - 1 times: K of pair i + 1, V of pair i
   const std::false_type any{};
   if (steps > 0) {
-    next_pair();
-    vp = kp;
-    for_each_index<C::IPP>([&](auto i) {
-      if (WR == 2 || !my_plane) load_plane(any, i, false, kp, 0);
-    });
+    next_pair(any);
+    v_at = k_at, v_rows = k_rows;
+    const Stream st = stream(0, 0);
+    if (WR == 2 || !my_plane) for_each_index<C::IPP>([&](auto i) { load_one(any, i, st); });
     load_scales(0);
 #pragma unroll
     for (int j = 1; j < NS; ++j) {
-      if (j < steps) next_pair();
-      else vp = kp, bads <<= 2;
+      if (j < steps) next_pair(any);
+      else v_at = k_at, v_rows = k_rows, bads <<= 2;
       if (j <= steps) {  // V of the last pair comes without another K
-        for_each_index<C::IPW>([&](auto i) { load_one(any, i, j, j - 1); });
+        const Stream sj = stream(j, j - 1);
+        for_each_index<C::IPW>([&](auto i) { load_one(any, i, sj); });
         if (j < steps) load_scales(j);
       }
     }
@@ -523,7 +553,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     for (int t = 0; t < RT; ++t) sn[t] = zero16;
 #pragma unroll
     for (int ks = 0; ks < KS; ks += KSTEP) {
-      qk_step(k_read(ring, ks), ks, sn);
+      qk_step(k_read(k_lane, ks), ks, sn);
       if (ks % 4 == 2) __builtin_amdgcn_sched_barrier(0);  // (few fragments at a time: registers)
     }
     float mx[RT];
@@ -553,13 +583,12 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     const bool more = HOT || i + 1 < steps;  // wave-uniform: a next pair to score
     const int ld = i + NS;                   // K of this pair and V of the one before it are loaded now
     const bool loads = HOT || ld <= steps;
-    if (HOT || ld < steps) next_pair();
-    else vp = kp, bads <<= 2;
-    const int kslot = ld % NS, vslot = (ld - 1) % NS;
+    if (HOT || ld < steps) next_pair(hot);
+    else v_at = k_at, v_rows = k_rows, bads <<= 2;
+    const Stream st = stream(ld % NS, (ld - 1) % NS);
     if (!HOT && i >= steps) return;
     const uint32_t bad_i = (bads >> (2 * NS)) & 3, bad_n = (bads >> (2 * (NS - 1))) & 3;
-    const unsigned char* kb = ring + ((i + 1) % NS) * C::PLANE;
-    const unsigned char* vb = ring + NS * C::PLANE + (i % NS) * C::PLANE;
+    const uint32_t kb = k_lane + ((i + 1) % NS) * C::PLANE, vb = v_lane + (i % NS) * C::PLANE;
     // One MFMA step a stage, with the LDS read of a later one, a share of the loads and of the vector work beside it: the
     // scores of pair i + 1 run while pair i's become probabilities, and their maxima are taken while pair i is weighted. The
     // compiler orders inside a stage only.
@@ -592,16 +621,19 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
         if constexpr (I + KA < NST) kf[I % KA] = k_read(kb, (I + KA) * KSTEP);
         else if constexpr (I + KA - NST < VA) vf[I + KA - NST] = v_read(vb, I + KA - NST);
         if constexpr (I < C::IPW)
-          if (loads) load_one(hot, stage, kslot, vslot);
+          if (loads) load_one(hot, stage, st);
         probs(I * 16 * RT / NST, (I + 1) * 16 * RT / NST);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) asm volatile("" : "+v"(l_run[t]));  // the sums stay in this stage
+        for (int t = 0; t < RT; ++t) {
+          asm volatile("" : "+v"(l_run[t]));  // the sums and products stay in this stage
+          pin(sn[t]);
+        }
         __builtin_amdgcn_sched_barrier(0);
       });
 #pragma unroll
       for (int x = KA; x < VA; ++x) vf[x] = v_read(vb, x);
     } else {
-      if (loads) for_each_index<C::IPW>([&](auto x) { load_one(hot, x, kslot, vslot); });
+      if (loads) for_each_index<C::IPW>([&](auto x) { load_one(hot, x, st); });
       probs(0, 16 * RT);
 #pragma unroll
       for (int x = 0; x < VA; ++x) vf[x] = v_read(vb, x);
@@ -639,7 +671,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       }
     };
     if (!HOT && T != kI8 && masked_pair(i, bad_i)) {
-      // infinities and NaN of V are left out, since weight 0 times them would be NaN, and added for the rows that see them
+      // infinities and NaN of V are left out, since weight 0 times them would be NaN; the rows that see them get them at the end
       uint32_t odd = 0;
 #pragma unroll
       for (int j = 0; j < 2 * DT; ++j) {
@@ -654,38 +686,11 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           o[t][j % DT] = mfma_bf16_32x32x16(__builtin_bit_cast(axk_bf16x8, w), pf[t][j / DT], o[t][j % DT]);
-          if constexpr (RT * D >= 256) asm volatile("" : "+a"(o[t][j % DT]));
+          pin(o[t][j % DT]);
         }
         if (j % 2) __builtin_amdgcn_sched_barrier(0);
       }
-      if (__builtin_amdgcn_ballot_w64(odd != 0)) {
-        uint32_t vis[RT];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) vis[t] = visible(t, (p_beg + i * KG) * kPair, bad_i);
-        for (int j = 0; j < kPair; ++j) {
-          const unsigned char* row = vb + j * C::RBY;
-          const int x = C::vswz(j & 15);
-#pragma unroll
-          for (int g = 0; g < 4 * DT; ++g) {  // channels 8 g + 4 h .. + 3
-            float y[4];
-            if constexpr (T == kBf16) {
-              const uint2 w = *reinterpret_cast<const uint2*>(row + ((g ^ x) * 16) + 8 * h);
-              y[0] = __uint_as_float(w.x << 16), y[1] = __uint_as_float(w.x & 0xffff0000u);
-              y[2] = __uint_as_float(w.y << 16), y[3] = __uint_as_float(w.y & 0xffff0000u);
-            } else {
-              const uint32_t w = *reinterpret_cast<const uint32_t*>(row + (((g >> 1) ^ x) * 16) + 8 * (g & 1) + 4 * h);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[e] = ((w >> (8 * e)) & 0x7f) == 0x7f ? NAN : 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int t = 0; t < RT; ++t)
-                o[t][g / 4][4 * (g % 4) + e] += ((vis[t] >> j) & 1) && !(fabsf(y[e]) < INFINITY) ? y[e] : 0.f;
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
-      }
+      odd_any |= __builtin_amdgcn_ballot_w64(odd != 0) != 0;
       take_scores(0, 16 * RT);
     } else {
       constexpr int PV = 2 * DT;
@@ -695,8 +700,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           o[t][J % DT] = mfma_bf16_32x32x16(w, pf[t][J / DT], o[t][J % DT]);
-          if constexpr (RT * D >= 256) asm volatile("" : "+a"(o[t][J % DT]));  // (keeps the accumulators in AGPRs, and the stage)
-          else asm volatile("" : "+v"(o[t][J % DT]));
+          pin(o[t][J % DT]);
         }
         if constexpr (J + VA < PV) vf[J % VA] = v_read(vb, J + VA);
         if constexpr (J >= 2) take_scores((J - 2) * 16 * RT / (PV - 2), (J - 1) * 16 * RT / (PV - 2));
@@ -705,13 +709,24 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     }
     if (more) finish_scores(hot, i + 1, bad_n, mx);
   };
+  auto whole_pair = [&](int p) {  // whether both tiles of pair p lie on pages of the pool
+    bool good = true;
+    for (int i = 0; i < 2; ++i) {
+      const int tok = p * kPair + kTile * i;
+      if (tok >= k.s.len) continue;
+      const int pid = a.indices[k.s.pb + tok / a.page];
+      good &= pid >= 0 && pid < a.num_pages;
+    }
+    return good;
+  };
   // steps whose pair lies wholly before token x
   auto whole_steps = [&](int x) { return max((max(x, 0) / kPair - p_beg + KG - 1) / KG, 0); };
   const int hot_end = min(steps - NS, min(whole_steps(k.s.len) - NS, whole_steps(base) - 1));
-  int step = 0;
-  for (; step < hot_end && !(bads & ((4u << (2 * NS)) - 1)); ++step) iteration(std::true_type{}, step);
-  for (; step < all_steps; ++step) iteration(any, step);
-
+  for (int step = 0; step < all_steps; ++step) {
+    // (no load that the compiler counts is in this loop: its waits would be waits for the direct loads too)
+    for (; step < hot_end && !(bads & ((4u << (2 * NS)) - 1)) && at_hand(); ++step) iteration(std::true_type{}, step);
+    iteration(any, step);
+  }
 
   bool live[RT];
 #pragma unroll
@@ -727,7 +742,9 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     }
   }
   if constexpr (KG == 2) {  // the second group's results through LDS to the first's waves, which hold the same rows
+    if (odd_any && lane == 0) *s_odd = 1;
     __syncthreads();
+    odd_any = *s_odd != 0;
     float2* const s_ml = reinterpret_cast<float2*>(smem);                       // [WR][RT][64]
     axk_f32x4* const s_o = reinterpret_cast<axk_f32x4*>(smem + WR * RT * 512);  // [WR][RT * DT * 4][64]
     if (kg == 1) {
@@ -790,6 +807,53 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
                                                        pack_bf16x2(ot[e + 6] * inv, ot[e + 7] * inv), false, false);
       *reinterpret_cast<axk_u32x4*>(a.out + qrow[t] * D + 16 * i + 8 * h) = axk_u32x4{w0[0], w1[0], w0[1], w1[1]};
     }
+  }
+  // What was left out of V, added to the rows that see it (each lane to four of every eight channels of its rows).
+  if (T != kI8 && __builtin_expect(odd_any, 0)) {
+    wait_vmcnt<0>();
+    for (int p = k.j * k.size; p < p_end; ++p)
+      for (int i = 0; i < 2; ++i) {
+        const int tok = p * kPair + kTile * i;
+        if (tok >= k.s.len) continue;
+        const int pid = a.indices[k.s.pb + tok / a.page];
+        if (pid < 0 || pid >= a.num_pages) continue;  // (no row sees its tokens)
+        const unsigned char* v0 = head0 + ((int64_t)pid * 2 * a.page + tok % a.page) * row_bytes + plane_bytes;
+        for (int j = 0; j < min(kTile, k.s.len - tok); ++j) {
+          const unsigned char* row = v0 + j * row_bytes;
+          bool odd = false;
+          if (lane * 16 < C::RBY) {
+            const axk_u32x4 w = *reinterpret_cast<const axk_u32x4*>(row + lane * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (T == kBf16) {
+                odd |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
+              } else {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) odd |= ((w[e] >> (8 * y)) & 0x7f) == 0x7f;
+              }
+            }
+          }
+          if (!__builtin_amdgcn_ballot_w64(odd) || !(tok / kPair * kPair + kPair > base || !whole_pair(p))) continue;
+#pragma unroll 1
+          for (int t = 0; t < RT; ++t) {
+            const int r = blk * RB + 32 * (RT * wr + t) + l32, nd = r < rows ? r / group : 0;
+            const uint64_t anc = r < rows ? s_anc[nd] : 0;
+            const int rel = tok + j - base;
+            if (!anc || (rel >= 0 && !((anc >> rel) & 1))) continue;
+            const int64_t out0 = (((int64_t)k.b * a.nodes + nd) * a.hq + kvh * group + r - nd * group) * D;
+            const int64_t po0 = (slot0 + 32 * (RT * wr + t) + l32) * D;
+            for (int g = 0; g < D / 8; ++g)
+              for (int e = 0; e < 4; ++e) {
+                const int ch = 8 * g + 4 * h + e;
+                const float x = T == kBf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[ch])
+                                           : (row[ch] & 0x7f) == 0x7f ? NAN : 0.f;
+                if (fabsf(x) < INFINITY) continue;
+                if (k.ns > 1) a.po[po0 + ch] += x;
+                else a.out[out0 + ch] = (uint16_t)f32_to_bf16_bits(bf16_bits_to_f32(a.out[out0 + ch]) + x);
+              }
+          }
+        }
+      }
   }
 }
 
