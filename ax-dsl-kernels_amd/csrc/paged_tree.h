@@ -160,7 +160,7 @@ struct TreeCfg {
   static constexpr int RING = KG * GROUP;
   static constexpr int JOIN = KG == 2 ? WR * RT * 32 * (D * 4 + 8) : 0;  // one group's results
   static constexpr int LDS = (RING > JOIN ? RING : JOIN) + kMaxNodes * 8 + 16;  // and the ancestors, and a flag
-  static_assert(KG * 4 * PLANE <= LDS_MAX && LDS <= 160 * 1024 && KG <= 2 && NS < 8, "LDS");
+  static_assert(KG * 4 * PLANE <= LDS_MAX && LDS <= 160 * 1024 && KG <= 2 && (NS == 2 || NS == 4), "LDS");
   // Where chunk c of a tile's row r is kept: K fragment reads (32 rows, one or two chunks each) and transposing V reads (4 rows
   // x 64 bytes of bf16, 8 rows x 32 bytes of 8 bits) then cover all LDS banks.
   static constexpr __host__ __device__ int kswz(int r) { return NCH == 4 ? (r >> 1) & 3 : r & (NCH < 16 ? NCH - 1 : 15); }
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       bads |= (uint32_t)((bad >> (cur_lp & 63)) & 1) | (uint32_t)((bad >> at1) & 1) << 1;
     } else {
       int lp = cur_lp, tp = cur_tp;
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (lp >= k.s.np) lp = cur_lp, tp = cur_tp;  // a tile past the sequence: its first one again
         if ((lp >> 6) != chunk) set_chunk(lp >> 6);
@@ -525,48 +525,28 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     s_anc[lane] = base >= 0 ? anc : 0;
     if (lane == 0) *s_odd = 0;
   }
-  // K of pair 0, then an iteration's loads NS - 1 times: K of pair i + 1, V of pair i
+  // K of pair 0, then an iteration's loads NS - 2 times (K of pair j, V of the one before); step -1 scores pair 0
   const std::false_type any{};
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[t][e] = -INFINITY;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qb[t][ks]));  // the compiler's wait for q stays ahead of the loads
+  }
   if (steps > 0) {
     next_pair(any);
-    v_at = k_at, v_rows = k_rows;
     const Stream st = stream(0, 0);
     if (WR == 2 || !my_plane) for_each_index<C::IPP>([&](auto i) { load_one(any, i, st); });
     load_scales(0);
-#pragma unroll
-    for (int j = 1; j < NS; ++j) {
+#pragma unroll 1
+    for (int j = 1; j < NS - 1 && j <= steps; ++j) {
       if (j < steps) next_pair(any);
       else v_at = k_at, v_rows = k_rows, bads <<= 2;
-      if (j <= steps) {  // V of the last pair comes without another K
-        const Stream sj = stream(j, j - 1);
-        for_each_index<C::IPW>([&](auto i) { load_one(any, i, sj); });
-        if (j < steps) load_scales(j);
-      }
+      const Stream sj = stream(j, j - 1);  // (V of the last pair comes with its K again)
+      for_each_index<C::IPW>([&](auto i) { load_one(any, i, sj); });
+      load_scales(min(j, steps - 1));
     }
-  }
-  wait_vmcnt<0>();
-  __syncthreads();
-  if (steps > 0) {
-    // scores of pair 0
-    axk_f32x16 sn[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) sn[t] = zero16;
-#pragma unroll
-    for (int ks = 0; ks < KS; ks += KSTEP) {
-      qk_step(k_read(k_lane, ks), ks, sn);
-      if (ks % 4 == 2) __builtin_amdgcn_sched_barrier(0);  // (few fragments at a time: registers)
-    }
-    float mx[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      mx[t] = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[t][i] = sn[t][i];
-        mx[t] = fmaxf(mx[t], s[t][i]);
-      }
-    }
-    finish_scores(any, 0, (bads >> (2 * (NS - 1))) & 3, mx);
   }
 
   // One step: pair i is weighted, pair i + 1 scored. HOT: whole pairs of history inside the pool, loads and a next pair to score,
@@ -574,21 +554,18 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   auto iteration = [&](auto hot, const int i) {
     constexpr bool HOT = decltype(hot)::value;
     // K of pair i + 1 and V of pair i have landed for every wave, and pair i - 1 has been read
-    if (i > 0) {
-      // (int8 at the end: an iteration without scales waits for all)
-      if (HOT || i + NS < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * (C::IPW + (T == kI8))) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-    }
+    if (HOT || i + NS <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * (C::IPW + (T == kI8))) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
     const bool more = HOT || i + 1 < steps;  // wave-uniform: a next pair to score
     const int ld = i + NS;                   // K of this pair and V of the one before it are loaded now
     const bool loads = HOT || ld <= steps;
     if (HOT || ld < steps) next_pair(hot);
     else v_at = k_at, v_rows = k_rows, bads <<= 2;
-    const Stream st = stream(ld % NS, (ld - 1) % NS);
+    const Stream st = stream(ld & (NS - 1), (ld - 1) & (NS - 1));
     if (!HOT && i >= steps) return;
     const uint32_t bad_i = (bads >> (2 * NS)) & 3, bad_n = (bads >> (2 * (NS - 1))) & 3;
-    const uint32_t kb = k_lane + ((i + 1) % NS) * C::PLANE, vb = v_lane + (i % NS) * C::PLANE;
+    const uint32_t kb = k_lane + ((i + 1) & (NS - 1)) * C::PLANE, vb = v_lane + (i & (NS - 1)) * C::PLANE;
     // One MFMA step a stage, with the LDS read of a later one, a share of the loads and of the vector work beside it: the
     // scores of pair i + 1 run while pair i's become probabilities, and their maxima are taken while pair i is weighted. The
     // compiler orders inside a stage only.
@@ -609,7 +586,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
         l_run[t] += s[t][x];
       }
     };
-    if (HOT || ld < steps) load_scales(ld);
+    if (loads) load_scales(HOT ? ld : min(ld, steps - 1));
     if (more) {
       axk_u32x4 kf[KA];
 #pragma unroll
@@ -670,7 +647,9 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
         mx[t] = fmaxf(mx[t], s[t][x]);
       }
     };
-    if (!HOT && T != kI8 && masked_pair(i, bad_i)) {
+    if (!HOT && i < 0) {
+      take_scores(0, 16 * RT);
+    } else if (!HOT && T != kI8 && masked_pair(i, bad_i)) {
       // infinities and NaN of V are left out, since weight 0 times them would be NaN; the rows that see them get them at the end
       uint32_t odd = 0;
 #pragma unroll
@@ -722,9 +701,9 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   // steps whose pair lies wholly before token x
   auto whole_steps = [&](int x) { return max((max(x, 0) / kPair - p_beg + KG - 1) / KG, 0); };
   const int hot_end = min(steps - NS, min(whole_steps(k.s.len) - NS, whole_steps(base) - 1));
-  for (int step = 0; step < all_steps; ++step) {
+  for (int step = -1; step < all_steps; ++step) {
     // (no load that the compiler counts is in this loop: its waits would be waits for the direct loads too)
-    for (; step < hot_end && !(bads & ((4u << (2 * NS)) - 1)) && at_hand(); ++step) iteration(std::true_type{}, step);
+    for (; step >= 0 && step < hot_end && !(bads & ((4u << (2 * NS)) - 1)) && at_hand(); ++step) iteration(std::true_type{}, step);
     iteration(any, step);
   }
 
