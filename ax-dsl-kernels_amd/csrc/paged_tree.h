@@ -304,9 +304,10 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   int cur_lp = 2 * p_beg / tpp, cur_tp = 2 * p_beg - cur_lp * tpp, cur_p = p_beg;
   uint32_t bads = 0;  // two bits a pair in flight, the latest lowest: its tiles lie on pages outside the pool
   // That tile of the pair whose K is loaded next (k_), and of the one before it, whose V is (v_): its K (V lies plane_bytes
-  // behind), its rows with tokens, at least one (the others are read as the first), and (int8) its first row in the scales.
+  // behind), its rows with tokens (none past the sequence or on a page outside the pool), and (int8) its first row in the
+  // scales.
   const unsigned char *k_at = head0, *v_at = head0;
-  int k_rows = 1, v_rows = 1;
+  int k_rows = 0, v_rows = 0;
   int64_t k_slot = 0;
   auto page_base = [&](int at) {
     const uint32_t lo = __builtin_amdgcn_readlane(pg_lo, at), hi = __builtin_amdgcn_readlane(pg_hi, at);
@@ -314,35 +315,38 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   };
   // Whether the next pair is whole and its pages are among those at hand.
   auto at_hand = [&]() {
-    return ((cur_lp + (cur_tp + 1 == tpp)) >> 6) == chunk && (cur_lp >> 6) == chunk && cur_p * kPair + kPair <= k.s.len;
+    return (cur_lp >> 6) == chunk && ((cur_lp + (cur_tp + 1 == tpp)) >> 6) == chunk && cur_p * kPair + kPair <= k.s.len;
   };
   auto next_pair = [&](auto hot) {  // hot: at_hand() holds
     v_at = k_at, v_rows = k_rows;
     bads <<= 2;
-    if constexpr (decltype(hot)::value) {
-      const int wrap = cur_tp + 1 == tpp, at1 = (cur_lp + wrap) & 63, at = my_tile ? at1 : cur_lp & 63;
-      const int tp = my_tile ? (wrap ? 0 : cur_tp + 1) : cur_tp;
-      k_at = page_base(at) + tp * tile_bytes;
-      k_rows = kTile;
-      if constexpr (T == kI8) k_slot = (int64_t)__builtin_amdgcn_readlane(pg_id, at) * 2 * a.page + tp * kTile;
-      bads |= (uint32_t)((bad >> (cur_lp & 63)) & 1) | (uint32_t)((bad >> at1) & 1) << 1;
-    } else {
-      int lp = cur_lp, tp = cur_tp;
+    const int wrap = cur_tp + 1 == tpp, lp1 = cur_lp + wrap, tp1 = wrap ? 0 : cur_tp + 1;
+    const int tok = cur_p * kPair + kTile * my_tile;
+    int lp = my_tile ? lp1 : cur_lp, tp = my_tile ? tp1 : cur_tp;
+    k_rows = decltype(hot)::value ? kTile : min(kTile, k.s.len - tok);
+    uint32_t bad2;
+    if (decltype(hot)::value || ((cur_lp >> 6) == chunk && (lp1 >> 6) == chunk)) {
+      bad2 = (uint32_t)((bad >> (cur_lp & 63)) & 1) | (uint32_t)((bad >> (lp1 & 63)) & 1) << 1;
+    } else {  // (the other tile first, so that this wave's pages are at hand afterwards; none past the sequence)
+      const int other = my_tile ? cur_lp : lp1;
+      uint32_t b_other = 0, b_mine = 0;
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
-        if (lp >= k.s.np) lp = cur_lp, tp = cur_tp;  // a tile past the sequence: its first one again
-        if ((lp >> 6) != chunk) set_chunk(lp >> 6);
-        const int at = lp & 63;
-        if (i == my_tile) {
-          k_at = page_base(at) + tp * tile_bytes;
-          k_rows = max(1, min(kTile, k.s.len - cur_p * kPair - kTile * i));
-          if constexpr (T == kI8) k_slot = (int64_t)__builtin_amdgcn_readlane(pg_id, at) * 2 * a.page + tp * kTile;
-        }
-        bads |= ((uint32_t)(bad >> at) & 1) << i;
-        if (++tp == tpp) tp = 0, ++lp;
+        const int l = i ? lp : other;
+        if (l >= k.s.np) continue;
+        if ((l >> 6) != chunk) set_chunk(l >> 6);
+        const uint32_t x = (uint32_t)((bad >> (l & 63)) & 1);
+        if (i) b_mine = x;
+        else b_other = x;
       }
+      bad2 = my_tile ? b_other | b_mine << 1 : b_mine | b_other << 1;
     }
-    k_at = static_cast<const unsigned char*>(uniform_ptr(k_at));
+    bads |= bad2;
+    if ((bad2 >> my_tile) & 1) k_rows = 0;  // (hot: K is loaded all the same, from page 0, and masked; V is not any more)
+    if (decltype(hot)::value || k_rows > 0) {
+      k_at = static_cast<const unsigned char*>(uniform_ptr(page_base(lp & 63) + tp * tile_bytes));
+      if constexpr (T == kI8) k_slot = (int64_t)__builtin_amdgcn_readlane(pg_id, lp & 63) * 2 * a.page + tp * kTile;
+    }
     cur_p += KG;
     cur_tp += 2 * KG;
     while (cur_tp >= tpp) cur_tp -= tpp, ++cur_lp;
@@ -355,6 +359,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   const int ln_row = lane / C::NCH, ln_ch = lane % C::NCH;
   const uint32_t ln_k = (ln_ch ^ C::kswz(ln_row)) * 16, ln_v = (ln_ch ^ C::vswz(ln_row)) * 16;
   const uint32_t row_b = (uint32_t)row_bytes, ln_off = ln_row * row_b;
+  typedef __attribute__((address_space(3))) axk_u32x4* LdsPut;
   struct Stream {  // where an iteration's loads of this wave come from and go to (K, V; WR = 4: the one it loads, in k)
     const unsigned char *k, *v;
     uint32_t lds_k, lds_v;
@@ -373,18 +378,26 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   };
   const uint32_t ln_one = WR == 4 && my_plane ? ln_v : ln_k;
   // load `index` (0 .. IPW - 1) of an iteration
-  auto load_one = [&](auto whole, auto index, const Stream& st) {
+  auto load_one = [&](auto index, const Stream& st) {
     constexpr int I0 = decltype(index)::value, I = I0 % C::IPP, R = I * C::RPI;
     constexpr uint32_t TK = C::kswz(R) * 16, TV = C::vswz(R) * 16;
     constexpr bool V = I0 >= C::IPP;  // (WR = 2: K first)
-    uint32_t at = WR == 4 ? ln_one ^ (TK ^ (vmask & (TK ^ TV))) : V ? ln_v ^ TV : ln_k ^ TK;
-    if (decltype(whole)::value || R + ln_row < (V ? st.rows_v : st.rows_k)) at += ln_off + R * row_b;
+    const uint32_t at = (WR == 4 ? ln_one ^ (TK ^ (vmask & (TK ^ TV))) : V ? ln_v ^ TV : ln_k ^ TK) + ln_off + R * row_b;
     lds_dma16_su_cached<I * 1024>(V ? st.v : st.k, at, V ? st.lds_v : st.lds_k);
   };
+  // ... where a row has no token: zeros in its place (weight 0 times whatever lay there could be NaN)
+  auto load_part = [&](auto index, const Stream& st) {
+    constexpr int I0 = decltype(index)::value, I = I0 % C::IPP, R = I * C::RPI;
+    constexpr bool V = I0 >= C::IPP;
+    const int rows_in = V ? st.rows_v : st.rows_k;
+    if (R + ln_row < rows_in) load_one(index, st);
+    else *(LdsPut)(uintptr_t)((V ? st.lds_v : st.lds_k) + I * 1024 + lane * 16) = axk_u32x4{0u, 0u, 0u, 0u};
+  };
+  auto whole = [&](const Stream& st) { return st.rows_k == kTile && (WR == 4 || st.rows_v == kTile); };
   // int8: the scales of step i's pair, of this wave's tile: [tile][K, V][16]
   auto load_scales = [&](int i) {
     if constexpr (T == kI8) {
-      const int row = l16 < k_rows ? l16 : 0;
+      const int row = l16 < k_rows ? l16 : 0;  // (past the last token its scale again: those scores are masked, weights zero)
       const int64_t at = (k_slot + row + (lane & 16 ? a.page : 0)) * a.hkv + kvh;
       if (lane < 32) lds_dma2(a.scales + at, lds_addr(ring) + 2 * NS * C::PLANE + (i & 7) * 256 + my_tile * 128);
     }
@@ -407,7 +420,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       for (int i = 0; i < 16; ++i) o[t][d][i] = 0.f;
   }
   const axk_f32x16 zero16 = {};
-  bool odd_any = false;  // whether V of a masked pair held what is no number
+  bool odd_any = false;  // whether V of a pair with nodes held what is no number
 
   // LDS addresses in bytes: a fragment's chunk is an exclusive or with a constant, as rows are powers of two of bytes.
   typedef const __attribute__((address_space(3))) axk_u32x4* LdsVec;
@@ -483,9 +496,8 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   };
   // the scores of step i are in s: masked, and their maximum taken up
   auto masked_pair = [&](int i, uint32_t bad2) { return (p_beg + i * KG) * kPair + kPair > base || bad2; };
-  auto finish_scores = [&](auto hot, int i, uint32_t bad2, float (&mx)[RT]) {  // mx: the maxima of s, if nothing changes them
-    scale_scores(i);
-    const bool masked = !decltype(hot)::value && masked_pair(i, bad2);
+  auto mask_scores = [&](int i, uint32_t bad2) {
+    const bool masked = masked_pair(i, bad2);
     if (masked) {
       const int tok = (p_beg + i * KG) * kPair;
 #pragma unroll
@@ -496,6 +508,11 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
           if (!((vis >> (8 * (e >> 2) + (e & 3))) & 1)) s[t][e] = -INFINITY;
       }
     }
+    return masked;
+  };
+  auto finish_scores = [&](auto hot, int i, uint32_t bad2, float (&mx)[RT]) {  // mx: the maxima of s, if nothing changes them
+    scale_scores(i);
+    const bool masked = !decltype(hot)::value && mask_scores(i, bad2);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       if (masked || T == kI8) {
@@ -526,7 +543,6 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     if (lane == 0) *s_odd = 0;
   }
   // K of pair 0, then an iteration's loads NS - 2 times (K of pair j, V of the one before); step -1 scores pair 0
-  const std::false_type any{};
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
 #pragma unroll
@@ -534,37 +550,120 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qb[t][ks]));  // the compiler's wait for q stays ahead of the loads
   }
+  const std::false_type any{};
+  int full = 0;  // iterations' loads in a row, up to the latest, that were all issued: they may be counted
   if (steps > 0) {
     next_pair(any);
     const Stream st = stream(0, 0);
-    if (WR == 2 || !my_plane) for_each_index<C::IPP>([&](auto i) { load_one(any, i, st); });
+    if (WR == 2 || !my_plane) for_each_index<C::IPP>([&](auto i) { load_part(i, st); });
     load_scales(0);
 #pragma unroll 1
     for (int j = 1; j < NS - 1 && j <= steps; ++j) {
       if (j < steps) next_pair(any);
       else v_at = k_at, v_rows = k_rows, bads <<= 2;
       const Stream sj = stream(j, j - 1);  // (V of the last pair comes with its K again)
-      for_each_index<C::IPW>([&](auto i) { load_one(any, i, sj); });
+      full = whole(sj) ? full + 1 : 0;
+      if (full) for_each_index<C::IPW>([&](auto i) { load_one(i, sj); });
+      else for_each_index<C::IPW>([&](auto i) { load_part(i, sj); });
       load_scales(min(j, steps - 1));
     }
   }
 
-  // One step: pair i is weighted, pair i + 1 scored. HOT: whole pairs of history inside the pool, loads and a next pair to score,
-  // so that the loop of nearly all steps is free of masks and of the copies of O that meeting paths bring.
-  auto iteration = [&](auto hot, const int i) {
-    constexpr bool HOT = decltype(hot)::value;
-    // K of pair i + 1 and V of pair i have landed for every wave, and pair i - 1 has been read
-    if (HOT || i + NS <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * (C::IPW + (T == kI8))) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  // K of pair i + 1 and V of pair i have landed for every wave, and pair i - 1 has been read
+  auto arrive = [&](auto hot) {
+    if (decltype(hot)::value || full >= NS - 2)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * (C::IPW + (T == kI8))) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    const bool more = HOT || i + 1 < steps;  // wave-uniform: a next pair to score
-    const int ld = i + NS;                   // K of this pair and V of the one before it are loaded now
-    const bool loads = HOT || ld <= steps;
+  };
+  // K of pair ld and V of the one before it are loaded; `full` then says whether their instructions are left to be issued
+  auto issue = [&](auto hot, int ld) {
+    constexpr bool HOT = decltype(hot)::value;
     if (HOT || ld < steps) next_pair(hot);
     else v_at = k_at, v_rows = k_rows, bads <<= 2;
     const Stream st = stream(ld & (NS - 1), (ld - 1) & (NS - 1));
-    if (!HOT && i >= steps) return;
-    const uint32_t bad_i = (bads >> (2 * NS)) & 3, bad_n = (bads >> (2 * (NS - 1))) & 3;
+    if constexpr (HOT) {
+      load_scales(ld);
+      return st;
+    }
+    const bool loads = ld <= steps;
+    full = loads && whole(st) ? full + 1 : 0;
+    if (loads) {
+      if (!full) for_each_index<C::IPW>([&](auto x) { load_part(x, st); });
+      load_scales(min(ld, steps - 1));
+    }
+    return st;
+  };
+  // every wave meets this barrier where a pair of either group holds a node
+  auto holds_nodes = [&](int i) { return T != kI8 && (k.j * k.size + (i + 1) * KG) * kPair > base; };
+  arrive(any);
+  if (steps > 0) {  // the scores of pair 0
+    const Stream st = issue(any, NS - 1);
+    if (full) for_each_index<C::IPW>([&](auto x) { load_one(x, st); });
+    axk_f32x16 sn[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) sn[t] = zero16;
+    axk_u32x4 kf[2] = {k_read(k_lane, 0), k_read(k_lane, KSTEP)};
+#pragma unroll
+    for (int ks = 0; ks < KS; ks += KSTEP) {
+      qk_step(kf[ks / KSTEP % 2], ks, sn);
+      if (ks + 2 * KSTEP < KS) kf[ks / KSTEP % 2] = k_read(k_lane, ks + 2 * KSTEP);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) pin(sn[t]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t][e] = sn[t][e];
+    scale_scores(0);
+    mask_scores(0, (bads >> (2 * (NS - 1))) & 3);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      float mx = s[t][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
+      m_run[t] = xor32_max(mx) * c;
+    }
+  }
+  // Step i: pair i is weighted, pair i + 1 scored. No path leads around the products, since O would be copied where it meets the
+  // others. HOT: whole pairs of history inside the pool, loads, and a next pair to score.
+  auto step = [&](auto hot, const int i) {
+    constexpr bool HOT = decltype(hot)::value;
+    arrive(hot);
+    // V of nodes: infinities and NaN are taken out, since weight 0 times them would be NaN; the rows that see them get them at
+    // the end.
+    if (!HOT && holds_nodes(i)) {
+        const uint32_t at = ring0 + (NS + (i & (NS - 1))) * C::PLANE + (wr * 64 + lane) * 16;
+        bool odd = false;
+#pragma unroll
+        for (int x = 0; x < C::PLANE / (WR * 1024); ++x) {
+          axk_u32x4 w = *(LdsVec)(uintptr_t)(at + x * WR * 1024);
+          uint32_t out = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t drop = 0;
+            if constexpr (T == kBf16) {
+              drop = ((w[e] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w[e] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; ++y) drop |= ((w[e] >> (8 * y)) & 0x7f) == 0x7f ? 0xffu << (8 * y) : 0u;
+            }
+            out |= drop;
+            w[e] &= ~drop;
+          }
+          if (out) *(LdsPut)(uintptr_t)(at + x * WR * 1024) = w;
+          odd |= out != 0;
+        }
+        odd_any |= __builtin_amdgcn_ballot_w64(odd) != 0;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+    }
+    const bool more = HOT || i + 1 < steps;  // wave-uniform: a next pair to score
+    const Stream st = issue(hot, i + NS);
+    const bool staged = HOT || full > 0;
+    const uint32_t bad_n = (bads >> (2 * (NS - 1))) & 3;
     const uint32_t kb = k_lane + ((i + 1) & (NS - 1)) * C::PLANE, vb = v_lane + (i & (NS - 1)) * C::PLANE;
     // One MFMA step a stage, with the LDS read of a later one, a share of the loads and of the vector work beside it: the
     // scores of pair i + 1 run while pair i's become probabilities, and their maxima are taken while pair i is weighted. The
@@ -586,7 +685,6 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
         l_run[t] += s[t][x];
       }
     };
-    if (loads) load_scales(HOT ? ld : min(ld, steps - 1));
     if (more) {
       axk_u32x4 kf[KA];
 #pragma unroll
@@ -598,7 +696,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
         if constexpr (I + KA < NST) kf[I % KA] = k_read(kb, (I + KA) * KSTEP);
         else if constexpr (I + KA - NST < VA) vf[I + KA - NST] = v_read(vb, I + KA - NST);
         if constexpr (I < C::IPW)
-          if (loads) load_one(hot, stage, st);
+          if (staged) load_one(stage, st);
         probs(I * 16 * RT / NST, (I + 1) * 16 * RT / NST);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -610,7 +708,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
 #pragma unroll
       for (int x = KA; x < VA; ++x) vf[x] = v_read(vb, x);
     } else {
-      if (loads) for_each_index<C::IPW>([&](auto x) { load_one(hot, x, st); });
+      if (staged) for_each_index<C::IPW>([&](auto x) { load_one(x, st); });
       probs(0, 16 * RT);
 #pragma unroll
       for (int x = 0; x < VA; ++x) vf[x] = v_read(vb, x);
@@ -647,31 +745,6 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
         mx[t] = fmaxf(mx[t], s[t][x]);
       }
     };
-    if (!HOT && i < 0) {
-      take_scores(0, 16 * RT);
-    } else if (!HOT && T != kI8 && masked_pair(i, bad_i)) {
-      // infinities and NaN of V are left out, since weight 0 times them would be NaN; the rows that see them get them at the end
-      uint32_t odd = 0;
-#pragma unroll
-      for (int j = 0; j < 2 * DT; ++j) {
-        axk_u32x4 w = __builtin_bit_cast(axk_u32x4, v_frag(v_read(vb, j)));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t lo = (w[e] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
-          const uint32_t hi = (w[e] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
-          odd |= lo | hi;
-          w[e] &= ~(lo | hi);
-        }
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          o[t][j % DT] = mfma_bf16_32x32x16(__builtin_bit_cast(axk_bf16x8, w), pf[t][j / DT], o[t][j % DT]);
-          pin(o[t][j % DT]);
-        }
-        if (j % 2) __builtin_amdgcn_sched_barrier(0);
-      }
-      odd_any |= __builtin_amdgcn_ballot_w64(odd != 0) != 0;
-      take_scores(0, 16 * RT);
-    } else {
       constexpr int PV = 2 * DT;
       for_each_index<PV>([&](auto stage) {
         constexpr int J = decltype(stage)::value;
@@ -685,26 +758,19 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
         if constexpr (J >= 2) take_scores((J - 2) * 16 * RT / (PV - 2), (J - 1) * 16 * RT / (PV - 2));
         __builtin_amdgcn_sched_barrier(0);
       });
-    }
     if (more) finish_scores(hot, i + 1, bad_n, mx);
   };
-  auto whole_pair = [&](int p) {  // whether both tiles of pair p lie on pages of the pool
-    bool good = true;
-    for (int i = 0; i < 2; ++i) {
-      const int tok = p * kPair + kTile * i;
-      if (tok >= k.s.len) continue;
-      const int pid = a.indices[k.s.pb + tok / a.page];
-      good &= pid >= 0 && pid < a.num_pages;
-    }
-    return good;
-  };
-  // steps whose pair lies wholly before token x
+  // steps whose pair lies wholly before token x; the last step that finds all it needs in the history
   auto whole_steps = [&](int x) { return max((max(x, 0) / kPair - p_beg + KG - 1) / KG, 0); };
-  const int hot_end = min(steps - NS, min(whole_steps(k.s.len) - NS, whole_steps(base) - 1));
-  for (int step = -1; step < all_steps; ++step) {
+  const int hot_end = min(steps - NS, min(whole_steps(k.s.len) - NS, whole_steps(base) - KG));
+  for (int i = 0; i < steps; ++i) {
     // (no load that the compiler counts is in this loop: its waits would be waits for the direct loads too)
-    for (; step >= 0 && step < hot_end && !(bads & ((4u << (2 * NS)) - 1)) && at_hand(); ++step) iteration(std::true_type{}, step);
-    iteration(any, step);
+    for (; i < hot_end && full >= NS - 2 && !(bads & ((4u << (2 * NS)) - 1)) && at_hand(); ++i) step(std::true_type{}, i);
+    step(any, i);
+  }
+  for (int i = steps; i < all_steps; ++i) {  // (the other group has one more)
+    arrive(any);
+    if (holds_nodes(i)) __builtin_amdgcn_s_barrier();
   }
 
   bool live[RT];
@@ -787,52 +853,34 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       *reinterpret_cast<axk_u32x4*>(a.out + qrow[t] * D + 16 * i + 8 * h) = axk_u32x4{w0[0], w1[0], w0[1], w1[1]};
     }
   }
-  // What was left out of V, added to the rows that see it (each lane to four of every eight channels of its rows).
+  // What was taken out of V, added to the rows that see it (each lane to four of every eight channels of its rows). Whole pairs
+  // were looked through, from the first that holds a node (KG = 2: of the two of its step).
   if (T != kI8 && __builtin_expect(odd_any, 0)) {
     wait_vmcnt<0>();
-    for (int p = k.j * k.size; p < p_end; ++p)
-      for (int i = 0; i < 2; ++i) {
-        const int tok = p * kPair + kTile * i;
-        if (tok >= k.s.len) continue;
-        const int pid = a.indices[k.s.pb + tok / a.page];
-        if (pid < 0 || pid >= a.num_pages) continue;  // (no row sees its tokens)
-        const unsigned char* v0 = head0 + ((int64_t)pid * 2 * a.page + tok % a.page) * row_bytes + plane_bytes;
-        for (int j = 0; j < min(kTile, k.s.len - tok); ++j) {
-          const unsigned char* row = v0 + j * row_bytes;
-          bool odd = false;
-          if (lane * 16 < C::RBY) {
-            const axk_u32x4 w = *reinterpret_cast<const axk_u32x4*>(row + lane * 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (T == kBf16) {
-                odd |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
-              } else {
-#pragma unroll
-                for (int y = 0; y < 4; ++y) odd |= ((w[e] >> (8 * y)) & 0x7f) == 0x7f;
-              }
-            }
-          }
-          if (!__builtin_amdgcn_ballot_w64(odd) || !(tok / kPair * kPair + kPair > base || !whole_pair(p))) continue;
+    const int p0 = k.j * k.size, first = p0 + max((max(base, 0) / kPair - p0) / KG * KG, 0);
+    for (int tok = first * kPair; tok < min(k.s.len, p_end * kPair); ++tok) {
+      const int pid = a.indices[k.s.pb + tok / a.page];
+      if (pid < 0 || pid >= a.num_pages) continue;
+      const unsigned char* row = head0 + ((int64_t)pid * 2 * a.page + tok % a.page) * row_bytes + plane_bytes;
+      const int rel = tok - base;
 #pragma unroll 1
-          for (int t = 0; t < RT; ++t) {
-            const int r = blk * RB + 32 * (RT * wr + t) + l32, nd = r < rows ? r / group : 0;
-            const uint64_t anc = r < rows ? s_anc[nd] : 0;
-            const int rel = tok + j - base;
-            if (!anc || (rel >= 0 && !((anc >> rel) & 1))) continue;
-            const int64_t out0 = (((int64_t)k.b * a.nodes + nd) * a.hq + kvh * group + r - nd * group) * D;
-            const int64_t po0 = (slot0 + 32 * (RT * wr + t) + l32) * D;
-            for (int g = 0; g < D / 8; ++g)
-              for (int e = 0; e < 4; ++e) {
-                const int ch = 8 * g + 4 * h + e;
-                const float x = T == kBf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[ch])
-                                           : (row[ch] & 0x7f) == 0x7f ? NAN : 0.f;
-                if (fabsf(x) < INFINITY) continue;
-                if (k.ns > 1) a.po[po0 + ch] += x;
-                else a.out[out0 + ch] = (uint16_t)f32_to_bf16_bits(bf16_bits_to_f32(a.out[out0 + ch]) + x);
-              }
-          }
+      for (int t = 0; t < RT; ++t) {
+        const int r = blk * RB + 32 * (RT * wr + t) + l32, nd = r < rows ? r / group : 0;
+        const uint64_t anc = r < rows ? s_anc[nd] : 0;
+        if (!anc || (rel >= 0 && !((anc >> rel) & 1))) continue;
+        const int64_t out0 = (((int64_t)k.b * a.nodes + nd) * a.hq + kvh * group + r - nd * group) * D;
+        const int64_t po0 = (slot0 + 32 * (RT * wr + t) + l32) * D;
+#pragma unroll 1
+        for (int x = 0; x < D / 2; ++x) {
+          const int ch = 8 * (x >> 2) + 4 * h + (x & 3);
+          const float v = T == kBf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[ch])
+                                     : (row[ch] & 0x7f) == 0x7f ? NAN : 0.f;
+          if (fabsf(v) < INFINITY) continue;
+          if (k.ns > 1) a.po[po0 + ch] += v;
+          else a.out[out0 + ch] = (uint16_t)f32_to_bf16_bits(bf16_bits_to_f32(a.out[out0 + ch]) + v);
         }
       }
+    }
   }
 }
 
