@@ -479,20 +479,28 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     else asm volatile("" : "+v"(x));
   };
   constexpr float kSlack = 8.0f;  // the reference maximum follows the scores in steps of more than 2^8
-  auto raise_max = [&](int t, float mx) {
-    const bool raise = mx > m_run[t] + kSlack;
-    if (__builtin_amdgcn_ballot_w64(raise)) {
-      const float alpha = raise ? __builtin_amdgcn_exp2f(m_run[t] - mx) : 1.0f;
-      if (raise) m_run[t] = mx;
+  float top[RT];         // the scores' maxima
+  bool higher = false;   // wave-uniform: one has outgrown its reference
+  auto raise_max = [&]() {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const bool raise = top[t] > m_run[t] + kSlack;
+      const float alpha = raise ? __builtin_amdgcn_exp2f(m_run[t] - top[t]) : 1.0f;
+      if (raise) m_run[t] = top[t];
       l_run[t] *= alpha;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
+      for (int d = 0; d < DT; ++d) {  // (tile by tile: all at once they would push what the loop keeps out of its registers)
+        axk_f32x16 x = o[t][d];
+        asm volatile("" : "+v"(x));
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[t][d][i] *= alpha;
-        pin(o[t][d]);  // (tile by tile: all at once they would push what the loop keeps out of its registers)
+        for (int i = 0; i < 16; ++i) x[i] *= alpha;
+        asm volatile("" : "+v"(x));
+        o[t][d] = x;
+        pin(o[t][d]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    higher = false;
   };
   // the scores of step i are in s: masked, and their maximum taken up
   auto masked_pair = [&](int i, uint32_t bad2) { return (p_beg + i * KG) * kPair + kPair > base || bad2; };
@@ -520,7 +528,8 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
 #pragma unroll
         for (int e = 1; e < 16; ++e) mx[t] = fmaxf(mx[t], s[t][e]);
       }
-      raise_max(t, xor32_max(mx[t]) * c);
+      top[t] = xor32_max(mx[t]) * c;
+      higher |= __builtin_amdgcn_ballot_w64(top[t] > m_run[t] + kSlack) != 0;
     }
   };
   constexpr int KSTEP = T == kBf16 ? 1 : 2;  // steps of a K read
@@ -616,7 +625,10 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[t][e] = sn[t][e];
+      for (int e = 0; e < 16; ++e) {
+        s[t][e] = sn[t][e];
+        asm volatile("" : "+v"(s[t][e]));  // (else the loop would carry s in AGPRs)
+      }
     scale_scores(0);
     mask_scores(0, (bads >> (2 * (NS - 1))) & 3);
 #pragma unroll
@@ -721,7 +733,8 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
         for (int g = 0; g < 4; ++g) {
           const axk_u32x4 w = scales_of(i, 1, g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[t][4 * g + e] = s[t][4 * g + e] == 0.f ? 0.f : s[t][4 * g + e] * bf16_bits_to_f32(w[e]);
+          for (int e = 0; e < 4; ++e)
+            s[t][4 * g + e] = !HOT && s[t][4 * g + e] == 0.f ? 0.f : s[t][4 * g + e] * bf16_bits_to_f32(w[e]);
         }
       }
 #pragma unroll
@@ -755,7 +768,8 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
           pin(o[t][J % DT]);
         }
         if constexpr (J + VA < PV) vf[J % VA] = v_read(vb, J + VA);
-        if constexpr (J >= 2) take_scores((J - 2) * 16 * RT / (PV - 2), (J - 1) * 16 * RT / (PV - 2));
+        // (after the last tile's first product: sn and O then share no register)
+        if constexpr (J >= DT) take_scores((J - DT) * 16 * RT / DT, (J - DT + 1) * 16 * RT / DT);
         __builtin_amdgcn_sched_barrier(0);
       });
     if (more) finish_scores(hot, i + 1, bad_n, mx);
@@ -763,10 +777,12 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   // steps whose pair lies wholly before token x; the last step that finds all it needs in the history
   auto whole_steps = [&](int x) { return max((max(x, 0) / kPair - p_beg + KG - 1) / KG, 0); };
   const int hot_end = min(steps - NS, min(whole_steps(k.s.len) - NS, whole_steps(base) - KG));
-  for (int i = 0; i < steps; ++i) {
-    // (no load that the compiler counts is in this loop: its waits would be waits for the direct loads too)
-    for (; i < hot_end && full >= NS - 2 && !(bads & ((4u << (2 * NS)) - 1)) && at_hand(); ++i) step(std::true_type{}, i);
-    step(any, i);
+  for (int i = 0; i < steps;) {
+    // (no load that the compiler counts is in this loop: its waits would be waits for the direct loads too; and no raise, whose
+    // 16 DT RT products would take the loop's registers)
+    while (!higher && i < hot_end && full >= NS - 2 && !(bads & ((4u << (2 * NS)) - 1)) && at_hand()) step(std::true_type{}, i++);
+    if (!higher) step(any, i++);
+    if (higher) raise_max();
   }
   for (int i = steps; i < all_steps; ++i) {  // (the other group has one more)
     arrive(any);

@@ -237,7 +237,7 @@ int write_rope(const uint16_t* q, int64_t ldq, int64_t hdq, const uint16_t* k, i
 }
 
 // ---- the tree's attention: how it is cut, from what the host knows ----
-constexpr int kMinPiece = 8;  // pairs: 256 tokens
+constexpr int kMinPiece = 4;  // pairs: 128 tokens
 struct TreePlan {
   int rb, nb, den, split;
   int64_t groups;
