@@ -54,8 +54,13 @@ AXK_DEV void split3(const float (&x)[8], axk_bf16x8& hi, axk_bf16x8& mid, axk_bf
 // TT 16-node tiles, W waves of 32 state columns each. Lane (l16, g) holds, as an MFMA operand's row, node 16 tt + l16; of a
 // result, column l16 and rows 4 g + r. A result's register r is the right operand of the fp32 step over the rows 4 g + r, so
 // u goes from one product into the next without leaving its registers.
+//
+// Bound by the state's bytes for many short trees (64 sequences x 8 nodes x 32 heads: 150 MB in 41.5 us, 3.6 TB/s; three waves a
+// SIMD, since the rows of the inversion are read one ahead instead of all at once, against 50.1 us with two), by the chain from
+// the state's arrival through the weights and the triangular solve to the outputs for wide ones (8 x 64 nodes 27 us, of which one
+// sequence takes 24).
 template <int TT, int W>
-__global__ __launch_bounds__(64 * W, TT == 4 ? 1 : 2) void gdn_tree_verify_kernel(TreeGdn p) {
+__global__ __launch_bounds__(64 * W, TT == 1 ? 3 : TT == 2 ? 2 : 1) void gdn_tree_verify_kernel(TreeGdn p) {
   constexpr int N = 16 * TT, LD = N + 4;
   __shared__ __align__(16) float s_a[N * LD];  // the system's lower part, its diagonal tiles inverted in place
   __shared__ __align__(16) float s_p[N * LD];  // the outputs' weights
@@ -72,12 +77,13 @@ __global__ __launch_bounds__(64 * W, TT == 4 ? 1 : 2) void gdn_tree_verify_kerne
 
   // the state's columns: rows 32 s + 8 g + j
   float2 st[4][8];
-  const float* sp = p.state + (int64_t)bh * kD * kD + col;
+  const char* sp = reinterpret_cast<const char*>(p.state + (int64_t)bh * kD * kD);
+  const uint32_t at0 = (8 * g * kD + col) * 4;
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const double w = __builtin_nontemporal_load(reinterpret_cast<const double*>(sp + (32 * s + 8 * g + j) * kD));
+      const double w = __builtin_nontemporal_load(reinterpret_cast<const double*>(sp + (at0 + (32 * s + j) * kD * 4)));
       st[s][j] = __builtin_bit_cast(float2, w);
     }
 
@@ -98,6 +104,15 @@ __global__ __launch_bounds__(64 * W, TT == 4 ? 1 : 2) void gdn_tree_verify_kerne
       qf[tt][s] = __builtin_bit_cast(axk_bf16x8, y);
     }
   }
+
+  // v of the nodes 4 g + r of every tile
+  uint32_t vf[TT][4];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      vf[tt][r] = *reinterpret_cast<const uint32_t*>(
+          p.v + (((int64_t)b * p.nodes + min(16 * tt + 4 * g + r, p.nodes - 1)) * p.nv + hd) * kD + col);
 
   // gates, and the tree (wave 0; lane t is node t)
   if (wave == 0) {
@@ -182,12 +197,18 @@ __global__ __launch_bounds__(64 * W, TT == 4 ? 1 : 2) void gdn_tree_verify_kerne
   for (int tt = wave; tt < TT; tt += W) {
     float x[16];
     float* at = s_a + 16 * tt * LD + 16 * tt;
+    axk_f32x4 row[2][4];  // a row ahead; all at once would take 120 registers, and occupancy with them
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (i + 1 < 16 && 4 * c <= i) row[(i + 1) & 1][c] = *reinterpret_cast<const axk_f32x4*>(at + (i + 1) * LD + 4 * c);
       float v = i == l16 ? 1.0f : 0.f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) v = fmaf(-at[i * LD + j], x[j], v);
+      for (int j = 0; j < i; ++j) v = fmaf(-row[i & 1][j / 4][j % 4], x[j], v);
       x[i] = v;
+      asm volatile("" : "+v"(x[i])::"memory");
+      __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_wave_barrier();
     if (g == 0)
@@ -218,6 +239,7 @@ __global__ __launch_bounds__(64 * W, TT == 4 ? 1 : 2) void gdn_tree_verify_kerne
           ks[tt][c] = mfma_bf16_16x16x32(kf[tt][s], part[i], ks[tt][c]);
           qs[tt][c] = mfma_bf16_16x16x32(qf[tt][s], part[i], qs[tt][c]);
         }
+      __builtin_amdgcn_sched_barrier(0);  // (one split at a time: their parts would take as many registers as the state)
     }
 
   // what is no number is taken out before a product that other nodes share and kept as the bits of its nodes, per column
@@ -248,7 +270,7 @@ __global__ __launch_bounds__(64 * W, TT == 4 ? 1 : 2) void gdn_tree_verify_kerne
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * tt + 4 * g + r;
       const bool live = (s_anc[t].x | s_anc[t].y) != 0 && !((lost >> t) & 1);  // (no ancestors past the last node)
-      const uint32_t vw = *reinterpret_cast<const uint32_t*>(p.v + (((int64_t)b * p.nodes + min(t, p.nodes - 1)) * p.nv + hd) * kD + col);
+      const uint32_t vw = vf[tt][r];
       const float be = s_beta[t], dk = s_dec[t] * s_rk[t], dq = s_dec[t] * s_rq[t];
       rhs[0][r] = live ? be * (__uint_as_float(vw << 16) - dk * ks[tt][0][r]) : 0.f;
       rhs[1][r] = live ? be * (__uint_as_float(vw & 0xffff0000u) - dk * ks[tt][1][r]) : 0.f;
@@ -300,7 +322,8 @@ __global__ __launch_bounds__(64 * W, TT == 4 ? 1 : 2) void gdn_tree_verify_kerne
 }
 
 // The accepted branch applied to the state: S' = e^{G_n} S_0 + sum_{i in A(n)} e^{G_n - G_i} k_i u_i^T, each workgroup 32 rows
-// of one head's state, each thread 4 of them x 4 columns.
+// of one head's state, each thread 4 of them x 4 columns. One read and one write of the state and the branch's rows of u bound it:
+// 32 sequences x 32 heads in 23 us, 5.9 TB/s; a single sequence's 4 MB take 5.7 us, a launch's latency and two dependent loads.
 struct TreeCommit {
   const float* state;
   const uint16_t* k;
@@ -404,11 +427,15 @@ int check(int64_t batch, int64_t nodes, int64_t nk, int64_t nv, int64_t dk, int6
 
 template <int TT>
 void launch_verify(const TreeGdn& p, int64_t heads, hipStream_t st) {
-  // one wave a workgroup where whole heads would leave CUs idle
-  if (heads <= 128)
-    hipLaunchKernelGGL((gdn_tree_verify_kernel<TT, 1>), dim3((unsigned)(4 * heads)), dim3(64), 0, st, p);
-  else
-    hipLaunchKernelGGL((gdn_tree_verify_kernel<TT, 4>), dim3((unsigned)heads), dim3(256), 0, st, p);
+  // One wave a workgroup spreads few heads over the CUs, but every wave then works out the heads' weights alone. Us for W = 1 and
+  // W = 4, at 32 heads a sequence: 8 nodes x 1 sequence 7.8 and 9.0, x 8 9.5 and 10.0, x 16 13.9 and 13.1; 32 nodes x 1 12.8 and
+  // 12.5, x 8 18.0 and 14.9; 64 nodes x 1 29.2 and 23.8, x 8 39.6 and 27.2.
+  if constexpr (TT == 1)
+    if (heads <= 256) {
+      hipLaunchKernelGGL((gdn_tree_verify_kernel<1, 1>), dim3((unsigned)(4 * heads)), dim3(64), 0, st, p);
+      return;
+    }
+  hipLaunchKernelGGL((gdn_tree_verify_kernel<TT, 4>), dim3((unsigned)heads), dim3(256), 0, st, p);
 }
 
 }  // namespace
