@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   constexpr int KG = C::KG, RB = C::RB, KS = C::KS, DT = C::DT, NS = C::NS;
   extern __shared__ __align__(16) unsigned char smem[];
   uint64_t* const s_anc = reinterpret_cast<uint64_t*>(smem + C::LDS - kMaxNodes * 8 - 16);
-  int* const s_odd = reinterpret_cast<int*>(smem + C::LDS - 16);
+  volatile int* const s_odd = reinterpret_cast<int*>(smem + C::LDS - 16);  // whether V of a node held what is no number
 
   const int sl = blockIdx.x >> 3;
   const int gi = sl / a.nb * 8 + (blockIdx.x & 7), blk = sl % a.nb;
@@ -420,7 +420,6 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       for (int i = 0; i < 16; ++i) o[t][d][i] = 0.f;
   }
   const axk_f32x16 zero16 = {};
-  bool odd_any = false;  // whether V of a pair with nodes held what is no number
 
   // LDS addresses in bytes: a fragment's chunk is an exclusive or with a constant, as rows are powers of two of bytes.
   typedef const __attribute__((address_space(3))) axk_u32x4* LdsVec;
@@ -647,28 +646,29 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     // V of nodes: infinities and NaN are taken out, since weight 0 times them would be NaN; the rows that see them get them at
     // the end.
     if (!HOT && holds_nodes(i)) {
-        const uint32_t at = ring0 + (NS + (i & (NS - 1))) * C::PLANE + (wr * 64 + lane) * 16;
-        bool odd = false;
+      const uint32_t at = ring0 + (NS + (i & (NS - 1))) * C::PLANE + (wr * 64 + lane) * 16;
+      bool odd = false;
 #pragma unroll
-        for (int x = 0; x < C::PLANE / (WR * 1024); ++x) {
-          axk_u32x4 w = *(LdsVec)(uintptr_t)(at + x * WR * 1024);
-          uint32_t out = 0;
+      for (int x = 0; x < (C::PLANE + WR * 1024 - 1) / (WR * 1024); ++x) {
+        if (C::PLANE % (WR * 1024) && wr * 1024 >= C::PLANE) break;  // (8-bit rows of 64: two waves hold the pair)
+        axk_u32x4 w = *(LdsVec)(uintptr_t)(at + x * WR * 1024);
+        uint32_t out = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t drop = 0;
-            if constexpr (T == kBf16) {
-              drop = ((w[e] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w[e] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
-            } else {
+        for (int e = 0; e < 4; ++e) {
+          uint32_t drop = 0;
+          if constexpr (T == kBf16) {
+            drop = ((w[e] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w[e] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+          } else {
 #pragma unroll
-              for (int y = 0; y < 4; ++y) drop |= ((w[e] >> (8 * y)) & 0x7f) == 0x7f ? 0xffu << (8 * y) : 0u;
-            }
-            out |= drop;
-            w[e] &= ~drop;
+            for (int y = 0; y < 4; ++y) drop |= ((w[e] >> (8 * y)) & 0x7f) == 0x7f ? 0xffu << (8 * y) : 0u;
           }
-          if (out) *(LdsPut)(uintptr_t)(at + x * WR * 1024) = w;
-          odd |= out != 0;
+          out |= drop;
+          w[e] &= ~drop;
         }
-        odd_any |= __builtin_amdgcn_ballot_w64(odd) != 0;
+        if (out) *(LdsPut)(uintptr_t)(at + x * WR * 1024) = w;
+        odd |= out != 0;
+      }
+      if (odd) *s_odd = 1;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
     }
@@ -803,11 +803,10 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     }
   }
   if constexpr (KG == 2) {  // the second group's results through LDS to the first's waves, which hold the same rows
-    if (odd_any && lane == 0) *s_odd = 1;
     __syncthreads();
-    odd_any = *s_odd != 0;
-    float2* const s_ml = reinterpret_cast<float2*>(smem);                       // [WR][RT][64]
-    axk_f32x4* const s_o = reinterpret_cast<axk_f32x4*>(smem + WR * RT * 512);  // [WR][RT * DT * 4][64]
+    float2* const s_ml = reinterpret_cast<float2*>(smem);                       // [WR][RT][32]
+    axk_f32x4* const s_o = reinterpret_cast<axk_f32x4*>(smem + WR * RT * 256);  // [WR][RT * DT * 4][64]
+    static_assert(WR * RT * (256 + DT * 4 * 64 * 16) == C::JOIN, "the join's LDS");
     if (kg == 1) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
@@ -871,7 +870,8 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
   }
   // What was taken out of V, added to the rows that see it (each lane to four of every eight channels of its rows). Whole pairs
   // were looked through, from the first that holds a node (KG = 2: of the two of its step).
-  if (T != kI8 && __builtin_expect(odd_any, 0)) {
+  // s_odd was last written before the last step's barrier.
+  if (T != kI8 && __builtin_expect(*s_odd != 0, 0)) {
     wait_vmcnt<0>();
     const int p0 = k.j * k.size, first = p0 + max((max(base, 0) / kPair - p0) / KG * KG, 0);
     for (int tok = first * kPair; tok < min(k.s.len, p_end * kPair); ++tok) {
