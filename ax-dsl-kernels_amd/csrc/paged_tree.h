@@ -160,6 +160,7 @@ struct TreeCfg {
   static constexpr int RING = KG * GROUP;
   static constexpr int JOIN = KG == 2 ? WR * RT * 32 * (D * 4 + 8) : 0;  // one group's results
   static constexpr int LDS = (RING > JOIN ? RING : JOIN) + kMaxNodes * 8 + 16;  // and the ancestors, and a flag
+  static_assert(PLANE % (WR * 1024) == 0, "V is looked through by all of a group's waves");
   static_assert(KG * 4 * PLANE <= LDS_MAX && LDS <= 160 * 1024 && KG <= 2 && (NS == 2 || NS == 4), "LDS");
   // Where chunk c of a tile's row r is kept: K fragment reads (32 rows, one or two chunks each) and transposing V reads (4 rows
   // x 64 bytes of bf16, 8 rows x 32 bytes of 8 bits) then cover all LDS banks.
@@ -649,8 +650,7 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       const uint32_t at = ring0 + (NS + (i & (NS - 1))) * C::PLANE + (wr * 64 + lane) * 16;
       bool odd = false;
 #pragma unroll
-      for (int x = 0; x < (C::PLANE + WR * 1024 - 1) / (WR * 1024); ++x) {
-        if (C::PLANE % (WR * 1024) && wr * 1024 >= C::PLANE) break;  // (8-bit rows of 64: two waves hold the pair)
+      for (int x = 0; x < C::PLANE / (WR * 1024); ++x) {
         axk_u32x4 w = *(LdsVec)(uintptr_t)(at + x * WR * 1024);
         uint32_t out = 0;
 #pragma unroll
@@ -978,7 +978,8 @@ template <int D, int T>
 int launch_rows(const TreeArgs& a, int rb, hipStream_t st) {
   if (rb == 64) return launch<D, T, 1, 2>(a, st);
   if constexpr (D == 256) return launch<D, T, 1, 4>(a, st);
-  else return rb == 128 ? launch<D, T, 2, 2>(a, st) : launch<D, T, 2, 4>(a, st);
+  else if constexpr (D == 128) return rb == 128 ? launch<D, T, 2, 2>(a, st) : launch<D, T, 2, 4>(a, st);
+  else return launch<D, T, 2, 2>(a, st);
 }
 template <int T>
 int launch_type(const TreeArgs& a, int d, int rb, hipStream_t st) {

@@ -237,7 +237,9 @@ int write_rope(const uint16_t* q, int64_t ldq, int64_t hdq, const uint16_t* k, i
 }
 
 // ---- the tree's attention: how it is cut, from what the host knows ----
-constexpr int kMinPiece = 4;  // pairs: 128 tokens
+// A piece's least pairs of tokens. Us with 8, 4 and 2, 16 heads of 256: one sequence of 600 tokens 21.7, 18.9 and 16.5; of 5003
+// tokens 24.1, 23.8 and 27.6, where shorter pieces cost more in the merge than their loops save.
+constexpr int kMinPiece = 4;
 struct TreePlan {
   int rb, nb, den, split;
   int64_t groups;
@@ -248,10 +250,15 @@ size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 TreePlan tree_plan(int64_t batch, int64_t nodes, int64_t hq, int64_t hkv, int64_t d, int64_t max_pairs) {
   TreePlan p;
   const int64_t rows = nodes * (hq / hkv);
-  p.rb = rows <= 64 ? 64 : rows <= 128 || d == 256 ? 128 : 256;
+  // Rows of a workgroup: two waves of rows and two of tokens up to 64 rows, as many rows as the registers hold beyond. Us with the
+  // other choice, for up to 64 rows 128: 16 sequences of 8000 tokens x 8 heads of 128 x 64 rows 89.6 against 107.8, 2 heads of 256
+  // x 64 rows 51.2 against 55.0 (FP8 45.5 against 54.7); for 96 rows of 128 channels 256: 67.3 against 98.3 (INT8 86.7 against
+  // 139.8). Beyond 128 rows: 256 rows of 128 channels 124.8 against 133.7 with 128, but of 64 channels 282 against 242 (K and V of
+  // a step are then so short that the larger block waits for them); 512 rows of 256 channels 587 against 810 with 64.
+  p.rb = rows <= 64 ? 64 : rows > 128 && d == 128 ? 256 : 128;
   const int64_t nb = (rows + p.rb - 1) / p.rb;
   p.nb = (int)nb;
-  const int64_t slots = p.rb == 64 && d <= 128 ? 512 : 256;  // workgroups that run at once
+  const int64_t slots = p.rb == 64 && d <= 128 ? 512 : 256;  // workgroups that run at once: two a CU where LDS and registers let them
   const int64_t den = slots / (hkv * nb);
   p.den = (int)(den > 1 ? den : 1);
   p.split = p.den > 1 && max_pairs > kMinPiece;
