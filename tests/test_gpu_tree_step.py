@@ -260,6 +260,14 @@ def test_gdn_many_heads(dev, bsz, t, nk, nv):
     check_gdn(gdn_case(bsz, t, nk, nv, seed=t), dev)
 
 
+@pytest.mark.parametrize("batch,longest", [(90, 200), (200, 2500), (256, 60), (257, 60), (700, 12)])
+def test_large_batches(dev, batch, longest):
+    """Sequences left whole because they are even, cut although they are many, and too many to be cut."""
+    rng = random.Random(batch)
+    lens = [longest] + [rng.randint(longest // 2, longest) if batch < 100 else rng.randint(0, 40) for _ in range(batch - 1)]
+    check_tree(tree_case(lens, [rng.randint(0, 2) for _ in lens], 2, 4, 2, 64, 16, seed=batch), dev)
+
+
 def test_no_rows_and_one_node(dev):
     """Nothing to append; a batch of nodes alone, without history; a chain of one."""
     cache = torch.zeros(2, 2, 16, 1, 64, dtype=torch.bfloat16, device=dev)
