@@ -88,8 +88,8 @@ AXK_DEV int wave_scan(int v) {
 // How the batch is cut: every sequence into pieces of P pairs, P such that the pieces of all row blocks and KV heads run at
 // once: total / den pairs, or more until no more than den pieces come out (a sequence's last piece is shorter, so there are at
 // most den + batch). Where that would cut the longest sequence once and not far from its end, all are left whole: 128 sequences of
-// up to 1000 tokens, 4 nodes x 16 heads of 256, 65 us with the cut and 49 without. Every wave of both launches derives the same cut from the page table: the total is a float sum in a fixed
-// order.
+// up to 1000 tokens, 4 nodes x 16 heads of 256, 65 us with the cut and 49 without. Every wave of both launches derives the same
+// cut from the page table: the total is a float sum in a fixed order.
 struct Piece {
   int b;       // sequence (-1: none)
   int j, ns;   // piece of the sequence, and how many it has

@@ -264,7 +264,7 @@ TreePlan tree_plan(int64_t batch, int64_t nodes, int64_t hq, int64_t hkv, int64_
   p.rb = rows <= 64 ? 64 : rows > 128 && d == 128 ? 256 : 128;
   const int64_t nb = (rows + p.rb - 1) / p.rb;
   p.nb = (int)nb;
-  const int64_t slots = p.rb == 64 && d <= 128 ? 512 : 256;  // workgroups that run at once: two a CU where LDS and registers let them
+  const int64_t slots = p.rb == 64 && d <= 128 ? 512 : 256;  // workgroups at once: one or two a CU
   const int64_t den = slots / (hkv * nb);
   p.den = (int)(den > 1 ? den : 1);
   p.split = p.den > 1 && max_pairs > kMinPiece && batch <= kSplitBatch;
