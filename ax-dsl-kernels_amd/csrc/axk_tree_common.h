@@ -13,6 +13,12 @@ AXK_DEV int node_count(int parent) {
   return there ? 64 - __builtin_clzll(there) : 0;
 }
 
+// A log decay g whose e^g is zero in 32 bits (-inf too): nothing of what came before it is left. Such a g stays out of sums over
+// a branch, where -inf less -inf would be NaN and a huge one would swallow the others; what lies before the branch's last one has
+// weight 0 instead. (Parents come before their children, so the last one of a branch has the highest index.)
+AXK_DEV bool forgets(float g) { return g < -104.0f; }
+AXK_DEV int last_of(uint64_t nodes) { return 63 - __builtin_clzll(nodes | 1); }
+
 // Lane t: node t and its ancestors, by doubling the distance to the farthest known one; zero where t is no node. A parent
 // that is no node before it makes t none, and sets *status. With SUM, x becomes its sum over the same nodes.
 template <bool SUM>

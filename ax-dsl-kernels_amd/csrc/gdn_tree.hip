@@ -6,6 +6,7 @@
 //   S_t = e^{G_t} S_0 + sum_{i in A(t)} e^{G_t - G_i} k_i u_i^T
 //   u_t = beta_t (v_t - e^{G_t} k_t^T S_0) - sum_{i in A(t) - t} beta_t e^{G_t - G_i} (k_t . k_i) u_i
 //   o_t = e^{G_t} q_t^T S_0 + sum_{i in A(t)} e^{G_t - G_i} (q_t . k_i) u_i
+// (a g whose e^g is zero is left out of the sums, and what came before it gets weight 0: axk_tree::forgets)
 // so no node's state is ever formed: the verify kernel reads S_0 once, solves the unit lower triangular system for u and
 // leaves u and g; the commit kernel applies the accepted node's branch to S_0.
 #include "axk_host.h"
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(64 * W, TT == 1 ? 3 : TT == 2 ? 2 : 1) void gdn_tre
   __shared__ __align__(16) float s_a[N * LD];  // the system's lower part, its diagonal tiles inverted in place
   __shared__ __align__(16) float s_p[N * LD];  // the outputs' weights
   __shared__ double s_sum[N];                  // G
-  __shared__ uint2 s_anc[N];
+  __shared__ uint2 s_anc[N], s_kept[N];        // A(t), and those of it whose updates are left at t
   __shared__ float s_beta[N], s_rk[N], s_rq[N], s_dec[N];
 
   const int slices = kD / (kCols * W);
@@ -121,13 +122,16 @@ __global__ __launch_bounds__(64 * W, TT == 1 ? 3 : TT == 2 ? 2 : 1) void gdn_tre
     const int parent = in ? p.parents[tok] : -2;
     const float x = bf16_bits_to_f32(p.a[tok * p.nv + hd]) + p.dt_bias[hd], be = bf16_bits_to_f32(p.b[tok * p.nv + hd]);
     const float gt = -expf(p.a_log[hd]) * (x > 20.0f ? x : log1pf(expf(x)));
-    double sum = (double)gt;
+    const uint64_t zero = __ballot(axk_tree::forgets(gt));
+    double sum = axk_tree::forgets(gt) ? 0.0 : (double)gt;
     const uint64_t anc = axk_tree::ancestors_sum<true>(parent, p.nodes, slice == 0 && hd == 0 ? p.status : nullptr, sum);
     if (lane < N) {
       s_sum[lane] = sum;
+      const uint64_t kept = anc & (~0ull << axk_tree::last_of(anc & zero));
+      s_kept[lane] = make_uint2((uint32_t)kept, (uint32_t)(kept >> 32));
       s_anc[lane] = make_uint2((uint32_t)anc, (uint32_t)(anc >> 32));
       s_beta[lane] = 1.0f / (1.0f + expf(-be));
-      s_dec[lane] = expf((float)sum);
+      s_dec[lane] = expf((float)sum) * (anc & zero ? 0.f : 1.0f);  // (0 times a NaN stays one, as in the recurrence)
     }
     if (in && slice == 0) p.gates[tok * p.nv + hd] = anc ? gt : 0.f;
   }
@@ -185,8 +189,8 @@ __global__ __launch_bounds__(64 * W, TT == 1 ? 3 : TT == 2 ? 2 : 1) void gdn_tre
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * tt + 4 * g + r;
-      const uint2 anc = s_anc[t];
-      const bool sees = ((i < 32 ? anc.x >> i : anc.y >> (i - 32)) & 1) != 0 && !((lost >> t) & 1);  // (then i is not either)
+      const uint2 kept = s_kept[t];
+      const bool sees = ((i < 32 ? kept.x >> i : kept.y >> (i - 32)) & 1) != 0 && !((lost >> t) & 1);  // (then i is not either)
       const float w = sees ? expf((float)(s_sum[t] - si)) * rk : 0.f;
       s_a[t * LD + i] = sees && i != t ? s_beta[t] * s_rk[t] * w * kk[r] : 0.f;
       s_p[t * LD + i] = sees ? s_rq[t] * w * qk[r] : 0.f;

@@ -1,0 +1,68 @@
+"""Trees of drafted tokens where decays vanish, a piece of the cache holds nothing or no number for a row, and pages lie outside
+the pool; on the GPU against the 64-bit oracle."""
+import math
+
+import pytest
+import torch
+
+import axk
+from oracle import tree as ot
+
+from test_gpu_tree import BF16_HALF, GDN, NAN, U, chain, gdn_case, within
+
+pytestmark = pytest.mark.gpu
+
+# node 1 is followed by 3 and 6; 2, 4, 5 and the rest are other branches, in the same tile of 16 nodes and in later ones
+FORGETS = [-1, 0, 0, 1, 2, -1, 3] + [5 if i % 2 else 4 for i in range(7, 40)]
+
+
+def forgetting(t, value, where=1):
+    """A case whose node `where` has the gate input `value`, and the same with a decay of e^-300 there: no state or update that
+    it meets leaves a trace in 64 bits either (the values are below 10, a double's half step 2^-53)."""
+    c = gdn_case(2, t, 1, 2, trees=[FORGETS[:t], chain(t, t)], seed=t)
+    c["a_log"], c["dt_bias"] = torch.full((2,), -0.5), torch.zeros(2)
+    c["a"][:, where, 1] = value
+    ref = dict(c, a=c["a"].clone())
+    ref["a"][:, where, 1] = 300.0 * math.exp(0.5)
+    return c, ref
+
+
+@pytest.mark.parametrize("value", [math.inf, 3e38, 1e20, 1e9])
+@pytest.mark.parametrize("t", [7, 20, 40])
+def test_a_decay_to_nothing_stays_in_its_branch(dev, t, value):
+    """e^-inf is zero, as in the recurrence: the node and its descendants know nothing of what came before it, other branches are
+    as they were."""
+    c, finite = forgetting(t, value)
+    o, u, g = (x.cpu() for x in axk.gdn_tree_verify(*(c[n].to(dev) for n in GDN)))
+    (ro, ru, rg), (eo, eu, eg) = ot.gdn_tree(*(finite[n] for n in GDN))
+    within(u, ru, eu, U)
+    within(o, ro, eo, BF16_HALF)
+    assert (g[:, 1, 1] < -5e8).all()
+    g[:, 1, 1], rg[:, 1, 1], eg[:, 1, 1] = 0.0, 0.0, 0.0
+    within(g, rg, eg, U)
+
+
+def test_a_chain_with_a_decay_to_nothing_is_the_recurrence(dev):
+    c, finite = forgetting(20, math.inf, where=9)
+    c["parents"] = torch.tensor([chain(20, 20)] * 2, dtype=torch.int32)
+    o = axk.gdn_tree_verify(*(c[n].to(dev) for n in GDN))[0].double().cpu()
+    ro = axk.gdn_recurrent(*(c[n].to(dev) for n in GDN[:-1]))[0].double().cpu()
+    finite["parents"] = c["parents"]
+    eo = ot.gdn_tree(*(finite[n] for n in GDN))[1][0]
+    # both are within their fp32 errors of the same values, then rounded: a bf16 step apart at most
+    assert not ro.isnan().any() and ((o - ro).abs() <= 2 * eo + 2.01 * BF16_HALF * ro.abs()).all()
+
+
+@pytest.mark.parametrize("name", ["a", "v"])
+def test_nan_is_not_forgotten(dev, name):
+    """0 times NaN: what is no number before such a decay stays none behind it, as in the recurrence."""
+    c, _ = forgetting(20, math.inf, where=3)
+    ref = axk.gdn_tree_verify(*(c[n].to(dev) for n in GDN))
+    c[name][0, 1, 1] = NAN
+    got = axk.gdn_tree_verify(*(c[n].to(dev) for n in GDN))
+    inside = [t for t, m in enumerate(ot.branches(FORGETS[:20])) if 1 in m]
+    outside = [t for t in range(20) if t not in inside]
+    assert 3 in inside and 6 in inside
+    for x, y in zip(got[:2], ref[:2]):
+        assert torch.equal(x[0, outside], y[0, outside]) and torch.equal(x[1], y[1])
+        assert x[0, inside, 1].isnan().all() and torch.equal(x[0, inside, 0], y[0, inside, 0])
