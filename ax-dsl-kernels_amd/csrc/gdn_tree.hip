@@ -357,7 +357,8 @@ __global__ __launch_bounds__(256) void gdn_tree_commit_kernel(TreeCommit p) {
   const int64_t tok = (int64_t)b * p.nodes + min(lane, p.nodes - 1);
   const int parent = in ? p.parents[tok] : -2;
   const int node = p.accepted[b];
-  double sum = in ? (double)p.gates[tok * p.nv + hd] : 0.0;
+  const float gt = in ? p.gates[tok * p.nv + hd] : 0.f;
+  double sum = axk_tree::forgets(gt) ? 0.0 : (double)gt;
   const uint64_t anc = axk_tree::ancestors_sum<true>(parent, p.nodes, hd == 0 && part == 0 ? p.status : nullptr, sum);
   const int from = min(max(node, 0), kMaxNodes - 1);
   const uint64_t all = ((uint64_t)__shfl((uint32_t)(anc >> 32), from) << 32) | __shfl((uint32_t)anc, from);
@@ -374,7 +375,8 @@ __global__ __launch_bounds__(256) void gdn_tree_commit_kernel(TreeCommit p) {
   }
   // the branch in order: its i-th node by wave i % 4, lanes two channels each
   const int rank = __builtin_popcountll(path & ((1ull << lane) - 1));
-  const float w = expf((float)(total - sum));
+  const uint64_t zero = path & __ballot(axk_tree::forgets(gt));
+  const float w = lane < axk_tree::last_of(zero) ? 0.f : expf((float)(total - sum));
   if (((path >> lane) & 1) && wave == 0) s_node[rank] = lane;
   for (int i = wave; i < m; i += 4) {
     const int t = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(((path >> lane) & 1) && rank == i)) - 1);
@@ -387,7 +389,7 @@ __global__ __launch_bounds__(256) void gdn_tree_commit_kernel(TreeCommit p) {
     }
   }
   __syncthreads();
-  const float dec = expf((float)total);
+  const float dec = expf((float)total) * (zero ? 0.f : 1.0f);
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll

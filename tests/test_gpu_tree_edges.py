@@ -66,3 +66,22 @@ def test_nan_is_not_forgotten(dev, name):
     for x, y in zip(got[:2], ref[:2]):
         assert torch.equal(x[0, outside], y[0, outside]) and torch.equal(x[1], y[1])
         assert x[0, inside, 1].isnan().all() and torch.equal(x[0, inside, 0], y[0, inside, 0])
+
+
+@pytest.mark.parametrize("value", [-math.inf, -3e38, -1e20, -105.0])
+def test_commit_of_a_branch_with_a_decay_to_nothing(dev, value):
+    c = gdn_case(3, 20, 1, 2, trees=[chain(20, 20)] * 3, seed=3)
+    g = torch.Generator().manual_seed(7)
+    u, gt = torch.randn(c["v"].shape, generator=g), -torch.rand(c["a"].shape, generator=g)
+    gt[0, 5, 1], gt[1, 19, 0], gt[2, 0] = value, value, value
+    gt[2, 7, 0] = value
+    acc = torch.tensor([19, 19, 9], dtype=torch.int32)
+    finite = gt.clamp(min=-300.0)
+    ref, err = ot.gdn_commit(c["state"], c["k"], u, finite, c["parents"], acc)
+    got = axk.gdn_tree_commit(*(x.to(dev) for x in (c["state"], c["k"], u, gt, c["parents"], acc)))
+    within(got, ref, err, U)
+    u[0, 2, 1, 3], u[0, 10, 0, 4] = NAN, NAN  # before the decay, and of the other head
+    bad = axk.gdn_tree_commit(*(x.to(dev) for x in (c["state"], c["k"], u, gt, c["parents"], acc)))
+    assert bad[0, 1, :, 3].isnan().all() and bad[0, 0, :, 4].isnan().all()
+    bad[0, 1, :, 3], bad[0, 0, :, 4] = got[0, 1, :, 3], got[0, 0, :, 4]
+    assert torch.equal(bad, got)
