@@ -950,7 +950,8 @@ __global__ __launch_bounds__(64 * kMergeRows) void paged_tree_merge_kernel(TreeA
     m = wave_max(m);
     for (int j0 = 0; j0 < ns; j0 += 64) {
       const float2 x = j0 + lane < ns ? a.ml[slot + (j0 + lane) * step] : make_float2(-INFINITY, 0.f);
-      const float w = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - m);
+      // (a maximum of -inf: no score, and a sum of 0, or none but NaN, and a sum that is one)
+      const float w = x.x == -INFINITY ? x.y : __builtin_amdgcn_exp2f(x.x - m);
       l += wave_sum(x.y * w);
       const int here = min(64, ns - j0);
       for (int i0 = 0; i0 < here; i0 += 8) {  // eight pieces' loads in flight

@@ -8,7 +8,7 @@ import torch
 import axk
 from oracle import tree as ot
 
-from test_gpu_tree import BF16_HALF, GDN, NAN, U, chain, gdn_case, within
+from test_gpu_tree import BF16_HALF, GDN, NAN, U, attend, chain, gdn_case, tree_case, within
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,38 @@ def test_commit_of_a_branch_with_a_decay_to_nothing(dev, value):
     assert bad[0, 1, :, 3].isnan().all() and bad[0, 0, :, 4].isnan().all()
     bad[0, 1, :, 3], bad[0, 0, :, 4] = got[0, 1, :, 3], got[0, 0, :, 4]
     assert torch.equal(bad, got)
+
+
+# ---- attention ----
+def where(c, b, pos):
+    """(page, slot) of a cached token."""
+    page = c["cache"].shape[2]
+    return int(c["idx"][int(c["ptr"][b]) + pos // page]), pos % page
+
+
+def put(c, b, pos, plane, value):
+    """A cached row (fp8: its bytes, i8: its scale) of every head set to `value`, NaN or a number."""
+    p, s = where(c, b, pos)
+    if isinstance(c["scale"], torch.Tensor):
+        c["scale"][p, plane, s] = value
+    else:
+        c["cache"][p, plane, s] = 0x7F if c["cache"].dtype is torch.uint8 else value
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "i8"])
+@pytest.mark.parametrize("t,hq,hkv,d,hist", [(64, 4, 4, 64, 500), (64, 8, 4, 64, 500), (64, 2, 2, 128, 500),
+                                             (64, 4, 2, 128, 500), (64, 16, 2, 128, 2932), (64, 2, 2, 256, 884),
+                                             (64, 16, 2, 256, 2932)])
+def test_a_key_that_is_no_number_behind_a_cut(dev, kv, t, hq, hkv, d, hist):
+    """A row that sees nothing but one NaN score in a piece is NaN, whatever the other pieces hold; rows that do not see the key
+    stay as they were. (Pieces of 128 tokens: the last one begins with node 12.)"""
+    tree = chain(t, t)
+    tree[50] = -1
+    tree[51:] = [49 - i for i in range(t - 51)]  # nobody behind it sees node 50
+    c = tree_case([hist], [t], t, hq, hkv, d, 16, kv, seed=d, trees=[tree])
+    ref = attend(c, dev)
+    put(c, 0, hist + 50, 0, NAN)
+    got = attend(c, dev)
+    assert got[0, 50].isnan().all()
+    rest = [i for i in range(t) if i != 50]
+    assert not ref.isnan().any() and torch.equal(got[0, rest], ref[0, rest])
