@@ -965,7 +965,7 @@ __global__ __launch_bounds__(64 * kMergeRows) void paged_tree_merge_kernel(TreeA
           const float wi = i0 + i < here ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w),
                                                                                              min(i0 + i, 63))) : 0.f;
 #pragma unroll
-          for (int e = 0; e < PER; ++e) acc[e] += wi != 0.f ? v[i][e] * wi : 0.f;
+          for (int e = 0; e < PER; ++e) acc[e] += i0 + i < here ? v[i][e] * wi : 0.f;  // (0 times a NaN is one)
         }
       }
     }

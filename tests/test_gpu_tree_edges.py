@@ -120,3 +120,19 @@ def test_a_key_that_is_no_number_behind_a_cut(dev, kv, t, hq, hkv, d, hist):
     assert got[0, 50].isnan().all()
     rest = [i for i in range(t) if i != 50]
     assert not ref.isnan().any() and torch.equal(got[0, rest], ref[0, rest])
+
+
+@pytest.mark.parametrize("hist", [60, 500])  # whole and cut
+def test_a_value_that_is_no_number_counts_whatever_its_weight(dev, hist):
+    """0 times NaN: also where a whole piece's weights are zero in 32 bits."""
+    c = tree_case([hist], [3], 3, 4, 2, 64, 16, trees=[[-1, 0, -1]])
+    c["q"].fill_(1.0)
+    c["cache"][:, 0] = 8.0
+    for pos in range(32 if hist < 128 else 128):  # a pair of tiles, or a piece
+        put(c, 0, pos, 0, -8.0)  # scores of -512 against 512: weights of e^-1024
+    p, s = where(c, 0, 10)
+    c["cache"][p, 1, s, :, 5] = NAN
+    got = attend(c, dev, 1.0)
+    assert got[..., 5].isnan().all()
+    got[..., 5] = 0.0
+    assert not got.isnan().any()
