@@ -589,9 +589,10 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
     if (WR == 2 || !my_plane) for_each_index<C::IPP>([&](auto i) { load_part(i, st); });
     load_scales(0);
 #pragma unroll 1
-    for (int j = 1; j < NS - 1 && j <= steps; ++j) {
+    for (int j = 1; j < NS - 1; ++j) {
       if (j < steps) next_pair(any);
-      else v_at = k_at, v_rows = k_rows, bads <<= 2;
+      else v_at = k_at, v_rows = k_rows, bads <<= 2;  // (NS - 1 shifts before pair 0 is masked, however few pairs there are)
+      if (j > steps) continue;
       const Stream sj = stream(j, j - 1);  // (V of the last pair comes with its K again)
       full = whole(sj) ? full + 1 : 0;
       if (full) for_each_index<C::IPW>([&](auto i) { load_one(i, sj); });

@@ -8,7 +8,7 @@ import torch
 import axk
 from oracle import tree as ot
 
-from test_gpu_tree import BF16_HALF, GDN, NAN, U, attend, chain, gdn_case, tree_case, within
+from test_gpu_tree import BF16_HALF, GDN, NAN, U, attend, chain, check_tree, gdn_case, tree_case, within
 
 pytestmark = pytest.mark.gpu
 
@@ -136,3 +136,28 @@ def test_a_value_that_is_no_number_counts_whatever_its_weight(dev, hist):
     assert got[..., 5].isnan().all()
     got[..., 5] = 0.0
     assert not got.isnan().any()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "i8"])
+@pytest.mark.parametrize("t,hq,hkv,d", [(4, 4, 4, 64), (20, 4, 1, 64), (6, 6, 2, 128), (20, 8, 2, 128), (20, 16, 1, 128),
+                                        (5, 16, 2, 256), (20, 8, 2, 256)])
+def test_pages_outside_the_pool_in_short_caches(dev, kv, t, hq, hkv, d):
+    """Sequences and last pieces of one or two pairs of tiles, in which any page lies outside the pool; no row of the pool's first
+    page may be read in its place."""
+    for total in (t + 3, 30, 32, 50, 64, 528, 550):
+        for at in sorted({0, 1, (total - 1) // 16 - 1, (total - 1) // 16}):
+            if not 0 <= at <= (total - 1) // 16 or total < t:
+                continue
+            c = tree_case([total - t], [t], t, hq, hkv, d, 16, kv, seed=total)
+            for i, pid in enumerate(c["idx"].tolist()):  # page 0 is nobody's
+                if pid == 0:
+                    c["idx"][i] = next(x for x in range(1, c["cache"].shape[0]) if x not in c["idx"].tolist())
+                    c["cache"][c["idx"][i]] = c["cache"][0]
+                    if kv == "i8":
+                        c["scale"][c["idx"][i]] = c["scale"][0]
+            if kv == "i8":
+                c["cache"][0], c["scale"][0] = 1, NAN
+            else:
+                c["cache"][0] = 0x7F if kv == "fp8" else NAN
+            c["idx"][at] = -1 if total % 4 else c["cache"].shape[0]
+            check_tree(c, dev, want_status=1)
