@@ -85,11 +85,18 @@ AXK_DEV int wave_scan(int v) {
   return v;
 }
 
+// A batch of more sequences is not cut: it fills the device by its number, and looking a piece up among its sequences would cost more than
+// the rounds that long ones stand out by. Us with and without, 2 heads of 128: 512 sequences of up to 1000 tokens 128 and 88, 1000
+// of them 295 and 167; 48 sequences of up to 2000 tokens (2 heads of 256) 39.7 and 49.4.
+constexpr int kSplitBatch = 256;
+
 // How the batch is cut: every sequence into pieces of P pairs, P such that the pieces of all row blocks and KV heads run at
-// once: total / den pairs, or more until no more than den pieces come out (a sequence's last piece is shorter, so there are at
-// most den + batch). Where that would cut the longest sequence once and not far from its end, all are left whole: 128 sequences of
-// up to 1000 tokens, 4 nodes x 16 heads of 256, 65 us with the cut and 49 without. Every wave of both launches derives the same
-// cut from the page table: the total is a float sum in a fixed order.
+// once: total / den pairs, or up to twice as many, if no more than den pieces come out so (65 sequences of 1000 to 8000 tokens,
+// 2 heads of 256: 128 us, with total / den 167). Else P is total / den, and pieces follow one another: short sequences are pieces
+// of their own, and a P that keeps their number down leaves a long one whole (131072 tokens beside 63 of 200, 8 heads of 256:
+// 248 us, as one piece 3480). There are at most den + batch. Where the first P would cut the longest sequence once and not far
+// from its end, all are left whole: 128 sequences of up to 1000 tokens, 4 nodes x 16 heads of 256, 65 us with the cut and 49
+// without. Every wave of both launches derives the same cut from the page table: the total is a float sum in a fixed order.
 struct Piece {
   int b;       // sequence (-1: none)
   int j, ns;   // piece of the sequence, and how many it has
@@ -115,40 +122,57 @@ AXK_DEV Piece find_piece(const TreeArgs& a, int want, bool by_piece, int kg) {
     k.s = seq_from(a.indptr[b], a.indptr[b + 1], a.last[b], a.page, a.nnz);
     return k;
   }
-  auto pairs_at = [&](int b0) { return b0 + lane < a.batch ? pairs_of(seq_from(lo, hi, tail, a.page, a.nnz)) : 0; };
   float total = 0.f, longest = 0.f;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    load(b0);
-    const float n = (float)pairs_at(b0);
+  float pairs[kSplitBatch / 64];  // of sequences lane, lane + 64, .., less one half
+#pragma unroll
+  for (int i = 0; i < kSplitBatch / 64; ++i) {
+    pairs[i] = -0.5f;
+    if (i && a.batch <= 64 * i) continue;
+    load(64 * i);
+    const float n = 64 * i + lane < a.batch ? (float)pairs_of(seq_from(lo, hi, tail, a.page, a.nnz)) : 0.f;
+    pairs[i] += n;
     total += wave_sum(n);
     longest = fmaxf(longest, wave_max(n));
   }
+  int p = max(a.min_piece, (int)fminf(total / (float)a.den, 0x1p28f) + 1);  // (offsets that fall back may add up to any total)
+  if (longest <= 1.5f * (float)p) p = max(p, (int)longest);  // sequences even enough to be left whole
+  auto whole_groups = [&](int x) { return (x + kg - 1) / kg * kg; };
+  // How many pieces: n / size rounded up is (n - 1/2) / size rounded down, and 1 (to 2^21 pairs a sequence; beyond, the number may
+  // be off by one, which changes the cut, not its bound).
+  auto pieces = [&](int size) {
+    const float each = __builtin_amdgcn_rcpf((float)size);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kSplitBatch / 64; ++i)
+      if (!i || a.batch > 64 * i) n += 64 * i + lane < a.batch ? (int)(pairs[i] * each) + 1 : 0;
+    return __builtin_amdgcn_readlane(wave_scan(n), 63);
+  };
   Piece k;
   k.b = -1;
-  auto pieces = [&](int b0, int size) {  // at least one each, which writes the zeros of a sequence without tokens
-    return b0 + lane < a.batch ? max(1, (int)((unsigned)(pairs_at(b0) + size - 1) / (unsigned)size)) : 0;
-  };
-  int p = max(a.min_piece, (int)(total / (float)a.den) + 1);
-  if (longest <= 1.5f * (float)p) p = max(p, (int)longest);  // sequences even enough to be left whole
-  k.size = (p + kg - 1) / kg * kg;
-  if (a.batch <= 64)  // (a larger batch has up to den + batch pieces)
-    for (int i = 0; i < 8; ++i) {
-      const int n = __builtin_amdgcn_readlane(wave_scan(pieces(0, k.size)), 63);
-      if (n <= a.den || k.size >= (int)total) break;
-      p = (int)((float)k.size * (float)n / (float)a.den) + 1;
-      k.size = (p + kg - 1) / kg * kg;
+  k.size = whole_groups(p);
+  const int most = 2 * k.size;
+  int n = a.batch <= a.den ? pieces(k.size) : 0;  // (a sequence is at least a piece)
+  // (up to den / 2 sequences no size has to be tried: with the most, full pieces and last ones are den / 2 each)
+  if (n > a.den && (2 * a.batch <= a.den || pieces(most) <= a.den))
+    for (int i = 0; i < 8 && n > a.den; ++i) {
+      const int more = whole_groups((int)((float)k.size * (float)n / (float)a.den) + 1);
+      k.size = i < 7 ? min(more, most) : most;
+      if (k.size == most) break;
+      n = pieces(k.size);
     }
   int base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     if (a.batch > 64) load(b0);
-    const int n = pieces(b0, k.size);
-    const int incl = wave_scan(n), excl = base + incl - n;
-    const bool mine = by_piece ? n > 0 && want >= excl && want < excl + n : b0 + lane == want;
-    const uint64_t hit = __ballot(mine);
+    // (at least one each, which writes the zeros of a sequence without tokens)
+    const int here = pairs_of(seq_from(lo, hi, tail, a.page, a.nnz));
+    const int mine = b0 + lane < a.batch ? max(1, (int)((unsigned)(here + k.size - 1) / (unsigned)k.size)) : 0;
+    const int incl = wave_scan(mine), excl = base + incl - mine;
+    const bool found = by_piece ? want >= excl && want < excl + mine : b0 + lane == want;
+    const uint64_t hit = __ballot(found);
     if (hit) {
       const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)hit) - 1);
       k.b = b0 + src;
-      k.ns = __builtin_amdgcn_readlane(n, src);
+      k.ns = __builtin_amdgcn_readlane(mine, src);
       k.first = __builtin_amdgcn_readlane(excl, src);
       k.j = by_piece ? want - k.first : 0;
       k.s = seq_from(__builtin_amdgcn_readlane(lo, src), __builtin_amdgcn_readlane(hi, src),

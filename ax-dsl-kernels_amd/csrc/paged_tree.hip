@@ -8,6 +8,7 @@ using axk_tree::kBf16;
 using axk_tree::kFp8;
 using axk_tree::kI8;
 using axk_tree::kMaxNodes;
+using axk_tree::kSplitBatch;
 
 // ---- rows into the cache ----
 struct RopeArgs {
@@ -242,10 +243,6 @@ int write_rope(const uint16_t* q, int64_t ldq, int64_t hdq, const uint16_t* k, i
 // A piece's least pairs of tokens. Us with 8, 4 and 2, 16 heads of 256: one sequence of 600 tokens 21.7, 18.9 and 16.5; of 5003
 // tokens 24.1, 23.8 and 27.6, where shorter pieces cost more in the merge than their loops save.
 constexpr int kMinPiece = 4;
-// A larger batch is not cut: it fills the device by its number, and looking a piece up among its sequences would cost more than
-// the rounds that long ones stand out by. Us with and without, 2 heads of 128: 512 sequences of up to 1000 tokens 128 and 88, 1000
-// of them 295 and 167; 48 sequences of up to 2000 tokens (2 heads of 256) 39.7 and 49.4.
-constexpr int kSplitBatch = 256;
 struct TreePlan {
   int rb, nb, den, split;
   int64_t groups;

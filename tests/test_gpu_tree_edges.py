@@ -161,3 +161,24 @@ def test_pages_outside_the_pool_in_short_caches(dev, kv, t, hq, hkv, d):
                 c["cache"][0] = 0x7F if kv == "fp8" else NAN
             c["idx"][at] = -1 if total % 4 else c["cache"].shape[0]
             check_tree(c, dev, want_status=1)
+
+
+def pieces(dev, lens, hkv, d):
+    """The pieces that a batch is cut into, by what they leave in a workspace: each row's maximum, sum and output."""
+    n = len(lens)
+    c = tree_case(lens, [1] * n, 1, hkv, hkv, d, 64)
+    ws = axk.paged_tree_verify_workspace(n, 1, hkv, hkv, d, dev)
+    ws.fill_(255)
+    out = attend(c, dev, ws=ws)
+    assert not out.isnan().any()
+    left = int((ws[:ws.numel() // 4 * 4].view(torch.int32) != -1).sum())
+    assert left % (hkv * (d + 2)) == 0
+    return left // (hkv * (d + 2))
+
+
+@pytest.mark.parametrize("batch", [1, 20, 40, 64, 65, 200])
+def test_a_long_sequence_is_cut_beside_any_number_of_short_ones(dev, batch):
+    """64 pieces of eight KV heads run at once: of 32768 tokens beside sequences of 40, the share that their work has, to within
+    a factor of two (sequences of two pairs of tiles are not cut)."""
+    pairs = 1025 + 2 * (batch - 1)
+    assert 64 * 1025 / pairs / 2 - 1 <= pieces(dev, [32768] + [40] * (batch - 1), 8, 64) <= 64
