@@ -292,7 +292,9 @@ int tree_verify(const uint16_t* q, const void* cache, int type, float kv_scale, 
                   axk_aligned(status, 4),
               AXK_E_ALIGN);
   const TreePlan p = tree_plan(batch, nodes, hq, hkv, d, (nnz * page + 31) / 32);
-  AXK_REQUIRE(launch_fits(p.nb * (p.groups + 7)) && launch_fits(batch * nodes * hq), AXK_E_SHAPE);
+  // (a merge always fits: where a sequence may be cut, den > 1, so that it has at most 128 blocks of up to 256 rows, or 256 of 64,
+  // in at most kSplitBatch sequences: 2^23 waves)
+  AXK_REQUIRE(launch_fits(p.nb * (p.groups + 7)), AXK_E_SHAPE);
   const size_t need = p.ml + p.po;
   AXK_REQUIRE(!need || (workspace && workspace_bytes >= need && axk_aligned(workspace, 256)), AXK_E_WORKSPACE);
   const size_t qb = (size_t)batch * nodes * hq * d * 2, slots = (size_t)num_pages * page * 2 * hkv;

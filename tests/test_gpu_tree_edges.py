@@ -182,3 +182,17 @@ def test_a_long_sequence_is_cut_beside_any_number_of_short_ones(dev, batch):
     a factor of two (sequences of two pairs of tiles are not cut)."""
     pairs = 1025 + 2 * (batch - 1)
     assert 64 * 1025 / pairs / 2 - 1 <= pieces(dev, [32768] + [40] * (batch - 1), 8, 64) <= 64
+
+
+def test_rows_past_what_a_merge_launch_holds(dev):
+    """2^24 rows of nodes in a batch that is not cut."""
+    few = tree_case([3, 0, 17, 40], [64, 9, 64, 30], 64, 1, 1, 64, 16)
+    ref = attend(few, dev).cpu()
+    n = 1 << 16  # times the four
+    up = {x: few[x].to(dev) for x in ("q", "cache", "idx", "last", "parents", "ptr")}
+    ptr = torch.cat([(up["ptr"][:4] + int(few["ptr"][4]) * torch.arange(n, device=dev)[:, None]).flatten().to(torch.int32),
+                     torch.tensor([n * int(few["ptr"][4])], dtype=torch.int32, device=dev)])
+    got = axk.paged_tree_verify(up["q"].repeat(n, 1, 1, 1), up["cache"], ptr, up["idx"].repeat(n), up["last"].repeat(n),
+                                up["parents"].repeat(n, 1))
+    assert torch.equal(got[:4].cpu(), ref) and torch.equal(got[-4:].cpu(), ref)
+    assert (got.view(n, -1) == got[:4].view(1, -1)).all()

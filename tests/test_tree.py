@@ -110,6 +110,14 @@ def test_tree_int8_and_workspace_size():
     assert size(4096, 64, 512, 512, 256) == 0
 
 
+def test_a_batch_that_is_not_cut_needs_no_merge():
+    """2^24 rows of nodes were taken for more than a merge launch holds, but such a batch makes none. (The check of overlaps comes
+    behind that of sizes, and nothing is launched.)"""
+    assert tree(batch=1 << 18, t=64, hq=1, hkv=1, nnz=0, out=at(1)) == ALIAS
+    assert tree(batch=256, t=64, hq=4096, hkv=256, nnz=1 << 20, out=at(1)) == ALIAS
+    assert tree(batch=1 << 20, t=64, hq=16 * 64, hkv=64, nnz=0, out=at(1)) == SHAPE  # 2^29 workgroups
+
+
 @pytest.mark.parametrize("kw,want", [
     *[({n: None}, NULL) for n in GDN],
     (dict(batch=0), SHAPE), (dict(t=0), SHAPE), (dict(t=65), SHAPE), (dict(nk=3), SHAPE), (dict(nk=0), SHAPE), (dict(nv=0), SHAPE),
