@@ -11,12 +11,16 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+#include <utility>
+
 #define AXK_DEV __device__ __forceinline__
 
 typedef __bf16 axk_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 axk_bf16x2 __attribute__((ext_vector_type(2)));
 typedef float axk_f32x4 __attribute__((ext_vector_type(4)));
 typedef float axk_f32x2 __attribute__((ext_vector_type(2)));
+typedef float axk_f32x16 __attribute__((ext_vector_type(16)));
 
 AXK_DEV float bf16_bits_to_f32(uint32_t b) { return __uint_as_float(b << 16); }
 
@@ -255,6 +259,19 @@ AXK_DEV void wait_vmcnt() {
 AXK_DEV axk_f32x4 mfma_bf16_16x16x32(axk_bf16x8 a, axk_bf16x8 b, axk_f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
+AXK_DEV axk_f32x16 mfma_bf16_32x32x16(axk_bf16x8 a, axk_bf16x8 b, axk_f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// f(std::integral_constant<int, 0>) .. f(<N - 1>): an unrolled loop whose index is a constant expression.
+template <typename F, int... I>
+AXK_DEV void for_each_index_of(F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+AXK_DEV void for_each_index(F&& f) {
+  for_each_index_of(f, std::make_integer_sequence<int, N>{});
+}
 
 // Wave-wide reductions (wave64) on DPP lane moves inside rows of 16 lanes, then two row broadcasts that leave
 // the total in lane 63, read back as a uniform value. Control codes (GFX9 DPP): quad_perm [1,0,3,2] = 0xB1,
@@ -276,6 +293,17 @@ AXK_DEV float wave_sum(float v) {
   v += dpp_move<0x142, 0xA>(0.f, v);
   v += dpp_move<0x143, 0xC>(0.f, v);
   return lane63(v);
+}
+// Inclusive sum over the lanes of a wave: shifts within rows of 16 lanes, then the rows' totals passed on.
+AXK_DEV int wave_scan(int x) {
+  unsigned v = (unsigned)x;
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+  return (int)v;
 }
 // Cross-row exchanges on VALU (gfx950 v_permlane16_swap / v_permlane32_swap, which swap the odd rows of 16 lanes
 // (upper 32 lanes) of the first operand with the even rows (lower 32 lanes) of the second): given v twice, the

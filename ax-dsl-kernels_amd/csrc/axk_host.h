@@ -1,6 +1,7 @@
 // Host-side helpers for the C-ABI entry points: argument checks and launch status.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <atomic>
@@ -25,6 +26,38 @@ static inline bool axk_overlap(const void* a, size_t na, const void* b, size_t n
   if (!a || !b || !na || !nb) return false;
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return x < y + nb && y < x + na;
+}
+
+// Arrays that a call writes overlap neither what it reads nor each other.
+struct AxkSpan {
+  const void* p;
+  size_t n;
+};
+template <int W, int R>
+static inline bool axk_disjoint(const AxkSpan (&writes)[W], const AxkSpan (&reads)[R]) {
+  for (int i = 0; i < W; ++i) {
+    for (const AxkSpan& r : reads)
+      if (axk_overlap(writes[i].p, writes[i].n, r.p, r.n)) return false;
+    for (int j = 0; j < i; ++j)
+      if (axk_overlap(writes[i].p, writes[i].n, writes[j].p, writes[j].n)) return false;
+  }
+  return true;
+}
+
+// Whether a dimension of a launch holds these workgroups: its threads are counted in 32 bits.
+static inline bool axk_launch_fits(int64_t workgroups, int threads = 256) {
+  return workgroups <= (int64_t)0xffffffff / threads;
+}
+
+// What a paged cache stores: bf16, E4M3 of x * kv_scale, or int8 codes with a bf16 scale per row and KV head.
+enum { AXK_KV_BF16 = 0, AXK_KV_FP8 = 1, AXK_KV_I8 = 2 };
+// By its dtype code (AXK_KV_BF16, or AXK_KV_FP8 with a power-of-two scale); negative: refused.
+static inline int axk_kv_type(int kv_dtype, float kv_scale) {
+  if (kv_dtype == AXK_DT_BF16) return AXK_KV_BF16;
+  if (kv_dtype != AXK_DT_FP8E4M3) return -AXK_E_DTYPE;
+  int e = 0;
+  const float m = frexpf(kv_scale, &e);
+  return kv_scale > 0.f && m == 0.5f && e >= -125 && e <= 126 ? AXK_KV_FP8 : -AXK_E_SHAPE;
 }
 
 static inline hipStream_t axk_stream(axk_stream_t s) { return reinterpret_cast<hipStream_t>(s); }

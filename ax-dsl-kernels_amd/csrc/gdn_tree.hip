@@ -409,22 +409,6 @@ __global__ __launch_bounds__(256) void gdn_tree_commit_kernel(TreeCommit p) {
     __builtin_nontemporal_store(s[j], reinterpret_cast<axk_f32x4*>(p.out + at0 + (r0 + 8 * j) * kD));
 }
 
-// Arrays that a call writes overlap neither what it reads nor each other.
-struct Span {
-  const void* p;
-  size_t n;
-};
-template <int W, int R>
-bool disjoint(const Span (&writes)[W], const Span (&reads)[R]) {
-  for (int i = 0; i < W; ++i) {
-    for (const Span& r : reads)
-      if (axk_overlap(writes[i].p, writes[i].n, r.p, r.n)) return false;
-    for (int j = 0; j < i; ++j)
-      if (axk_overlap(writes[i].p, writes[i].n, writes[j].p, writes[j].n)) return false;
-  }
-  return true;
-}
-
 int check(int64_t batch, int64_t nodes, int64_t nk, int64_t nv, int64_t dk, int64_t dv) {
   AXK_REQUIRE(batch > 0 && nodes > 0 && nodes <= kMaxNodes && nk > 0 && nv > 0 && nv % nk == 0, AXK_E_SHAPE);
   AXK_REQUIRE(dk == kD && dv == kD && nv <= 4096 && batch <= (1 << 20) && batch * nv <= (1 << 20), AXK_E_SHAPE);
@@ -460,10 +444,10 @@ extern "C" int axk_gdn_tree_verify(const uint16_t* q, const uint16_t* k, const u
               AXK_E_ALIGN);
   const size_t toks = (size_t)batch * nodes, vb = toks * num_v_heads * kD * 2, kb = toks * num_k_heads * kD * 2;
   const size_t gb = toks * num_v_heads * 2, hb = (size_t)num_v_heads * 4;
-  const Span writes[] = {{out, vb}, {updates, 2 * vb}, {gates, 2 * gb}, {status, 4}};
-  const Span reads[] = {{q, kb}, {k, kb}, {v, vb}, {a, gb}, {b, gb}, {a_log, hb}, {dt_bias, hb},
-                        {state, (size_t)batch * num_v_heads * kD * kD * 4}, {parents, toks * 4}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{out, vb}, {updates, 2 * vb}, {gates, 2 * gb}, {status, 4}};
+  const AxkSpan reads[] = {{q, kb}, {k, kb}, {v, vb}, {a, gb}, {b, gb}, {a_log, hb}, {dt_bias, hb},
+                           {state, (size_t)batch * num_v_heads * kD * kD * 4}, {parents, toks * 4}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   const TreeGdn p = {q, k, v, a, b, a_log, dt_bias, state, parents, out, updates, gates, status, (int)nodes, (int)num_k_heads,
                      (int)num_v_heads};
   AXK_LAUNCH_GATE();
@@ -485,11 +469,11 @@ extern "C" int axk_gdn_tree_commit(const float* state_in, const uint16_t* k, con
                   axk_aligned(gates, 4) && axk_aligned(parents, 4) && axk_aligned(accepted, 4) && axk_aligned(status, 4),
               AXK_E_ALIGN);
   const size_t toks = (size_t)batch * nodes, sb = (size_t)batch * num_v_heads * kD * kD * 4;
-  const Span writes[] = {{state_out, sb}, {status, 4}};
-  const Span reads[] = {{state_in == state_out ? nullptr : state_in, sb}, {k, toks * num_k_heads * kD * 2},
-                        {updates, toks * num_v_heads * kD * 4}, {gates, toks * num_v_heads * 4}, {parents, toks * 4},
-                        {accepted, (size_t)batch * 4}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{state_out, sb}, {status, 4}};
+  const AxkSpan reads[] = {{state_in == state_out ? nullptr : state_in, sb}, {k, toks * num_k_heads * kD * 2},
+                           {updates, toks * num_v_heads * kD * 4}, {gates, toks * num_v_heads * 4}, {parents, toks * 4},
+                           {accepted, (size_t)batch * 4}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   const TreeCommit p = {state_in, k, updates, gates, parents, accepted, state_out, status, (int)nodes, (int)num_k_heads,
                         (int)num_v_heads};
   AXK_LAUNCH_GATE();

@@ -1126,7 +1126,6 @@ __global__ __launch_bounds__(256) void paged_kv_write_fp8_kernel(const uint16_t*
 // (816 us before: 32 row blocks on 256 CUs). Short calls are bound by their chain: 1.4 us to the block's numbers, 0.9 to
 // the page ids, 2 to the first K / V, 1.1 a pair and 1.5 for the rows' way out (4 x 4 tokens of 64 cached ones 10.7 us).
 typedef short axk_s16x8 __attribute__((ext_vector_type(8)));
-typedef float axk_f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kPfWaves = 4;
 constexpr int kPfRows = 32 * kPfWaves;
 constexpr int kPfRing = 4;       // tile pairs in the LDS ring
@@ -1153,20 +1152,6 @@ struct PfCfg {
   static AXK_DEV int kswz(int r) { return r & (NCH < 16 ? NCH - 1 : 15); }
   static AXK_DEV int vswz(int r) { return NCH < 16 ? ((r >> 1) & 1) : (r & 3); }  // in units of 4 chunks
 };
-
-AXK_DEV axk_f32x16 mfma_bf16_32x32x16(axk_bf16x8 a, axk_bf16x8 b, axk_f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
-// f(std::integral_constant<int, 0>) .. f(<N - 1>): an unrolled loop whose index is a constant expression.
-template <typename F, int... I>
-AXK_DEV void for_each_index_of(F& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-AXK_DEV void for_each_index(F& f) {
-  for_each_index_of(f, std::make_integer_sequence<int, N>{});
-}
 
 // Row block `want` of one KV head: the blocks of each sequence in turn, its last (longest) block first. Every wave
 // derives the same answer; the grid is an upper bound and surplus workgroups get b = -1. Without qo_indptr every sequence

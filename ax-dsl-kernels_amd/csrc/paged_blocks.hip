@@ -64,17 +64,7 @@ AXK_DEV Owner owner_of(const int* __restrict__ indptr, const int* __restrict__ l
   return {batch, {0, 0, 0}};
 }
 
-// Inclusive sum over the lanes of a wave: shifts within rows of 16 lanes, then the rows' totals passed on.
-AXK_DEV unsigned wave_scan(unsigned v) {
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
-  return v;
-}
-AXK_DEV int wave_total(int v) { return __builtin_amdgcn_readlane((int)wave_scan((unsigned)v), 63); }
+AXK_DEV int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 
 // Two bf16 values (one dword) as two 16-bit integers of the same order, and back (the map is its own inverse): the 15
 // low bits of a negative value are flipped. NaN lies beyond the infinity of its sign.
@@ -87,7 +77,7 @@ AXK_DEV uint32_t bf16_unorder(axk_s16x2 x) { return __builtin_bit_cast(uint32_t,
 
 // What a cache stores: bf16; E4M3 bytes, attended as stored * inv_scale (a power of two: exact in bf16); or int8 codes with a
 // bf16 scale per row and KV head, attended as code * scale.
-enum { kBf16 = 0, kFp8 = 1, kI8 = 2 };
+enum { kBf16 = AXK_KV_BF16, kFp8 = AXK_KV_FP8, kI8 = AXK_KV_I8 };
 
 // Byte i of w, an int8 code, as a float.
 AXK_DEV float i8_code(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
@@ -795,7 +785,7 @@ AXK_DEV PieceOf find_piece(const BlkArgs& a, int it) {
     for (int i = 0; i < 4; ++i) {
       if (b0 + 64 * i >= a.batch) break;
       const int n = b0 + 64 * i + lane < a.batch ? pieces_of(seq_from(lo[i], hi[i], last[i], a.page, a.nnz), a.ps) : 0;
-      const int before = base + (int)wave_scan((unsigned)n) - n;
+      const int before = base + wave_scan(n) - n;
       // (offsets of indptr that fall back can make the sums pass 32 bits: such pieces are nobody's)
       const uint64_t mine = __ballot(before >= 0 && it >= before && it - before < n);
       if (mine) {
@@ -1485,25 +1475,6 @@ namespace {
 
 constexpr int64_t kMaxSubs = 1 << 30;  // subtiles of a page table, or of a row's listed blocks: sums of them fit 32 bits
 
-// Arrays that a call writes overlap neither what it reads nor each other.
-struct Span {
-  const void* p;
-  size_t n;
-};
-template <int W, int R>
-bool disjoint(const Span (&writes)[W], const Span (&reads)[R]) {
-  for (int i = 0; i < W; ++i) {
-    for (const Span& r : reads)
-      if (axk_overlap(writes[i].p, writes[i].n, r.p, r.n)) return false;
-    for (int j = 0; j < i; ++j)
-      if (axk_overlap(writes[i].p, writes[i].n, writes[j].p, writes[j].n)) return false;
-  }
-  return true;
-}
-
-// Whether a dimension of a launch holds these workgroups: its threads are counted in 32 bits.
-bool launch_fits(int64_t workgroups, int threads) { return workgroups <= (int64_t)0xffffffff / threads; }
-
 int check_blocks(int64_t batch, int64_t hkv, int64_t d, int64_t page_size, int64_t block, int64_t num_pages, int64_t nnz) {
   AXK_REQUIRE(batch > 0 && batch <= (1 << 20) && hkv > 0 && hkv <= 4096, AXK_E_SHAPE);
   AXK_REQUIRE(d == 64 || d == 128 || d == 256, AXK_E_SHAPE);
@@ -1511,15 +1482,6 @@ int check_blocks(int64_t batch, int64_t hkv, int64_t d, int64_t page_size, int64
   AXK_REQUIRE(block >= kSub && block % kSub == 0 && page_size % block == 0, AXK_E_SHAPE);
   AXK_REQUIRE(num_pages > 0 && nnz >= 0 && nnz * (page_size / kSub) <= kMaxSubs, AXK_E_SHAPE);
   return AXK_OK;
-}
-
-// The stored type of a cache by its dtype code (kBf16 or kFp8, the latter with a power-of-two scale); negative: refused.
-int cache_type(int kv_dtype, float kv_scale) {
-  if (kv_dtype == AXK_DT_BF16) return kBf16;
-  if (kv_dtype != AXK_DT_FP8E4M3) return -AXK_E_DTYPE;
-  int e = 0;
-  const float m = frexpf(kv_scale, &e);
-  return kv_scale > 0.f && m == 0.5f && e >= -125 && e <= 126 ? kFp8 : -AXK_E_SHAPE;
 }
 
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -1553,8 +1515,8 @@ BlkPlan blk_plan(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t page
   p.po = p.direct ? 0 : round256(items * group * d * sizeof(float));
   p.stat = weights ? round256((size_t)(n ? rows : hkv) * subs * group * sizeof(float2)) : 0;
   p.split = (int)((group * d / 4 + 63) / 64);
-  p.fits = launch_fits(n ? rows * p.pieces : p.pieces, 256) &&
-           (p.direct || launch_fits(rows * p.split + (weights ? (n ? rows : hkv * p.pieces) : 0), 256));
+  p.fits = axk_launch_fits(n ? rows * p.pieces : p.pieces, 256) &&
+           (p.direct || axk_launch_fits(rows * p.split + (weights ? (n ? rows : hkv * p.pieces) : 0), 256));
   return p;
 }
 
@@ -1588,10 +1550,10 @@ int kv_write_bounds(const uint16_t* k, const uint16_t* v, void* kv_cache, int ty
                   axk_aligned(kv_scales, 2),
               AXK_E_ALIGN);
   const size_t row = (size_t)hkv * d, slots = (size_t)num_pages * page_size * 2;
-  const Span writes[] = {{kv_cache, slots * row * (type ? 1 : 2)},
-                         {bounds, (size_t)num_pages * (page_size / block_size) * row * 4}, {kv_scales, slots * hkv * 2}};
-  const Span reads[] = {{k, rows * row * 2}, {v, rows * row * 2}, {loc, (size_t)rows * 8}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{kv_cache, slots * row * (type ? 1 : 2)},
+                            {bounds, (size_t)num_pages * (page_size / block_size) * row * 4}, {kv_scales, slots * hkv * 2}};
+  const AxkSpan reads[] = {{k, rows * row * 2}, {v, rows * row * 2}, {loc, (size_t)rows * 8}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   if (rows == 0) return AXK_OK;
   AXK_LAUNCH_GATE();
   auto* fn = type == kI8 ? &paged_kv_write_bounds_kernel<kI8>
@@ -1610,15 +1572,15 @@ int key_bounds(const void* kv_cache, int type, float kv_scale, const uint16_t* k
               AXK_E_NULL);
   const int rc = check_blocks(batch, hkv, d, page_size, block_size, num_pages, nnz);
   if (rc != AXK_OK) return rc;
-  AXK_REQUIRE(launch_fits(nnz * (page_size / block_size), 256), AXK_E_SHAPE);
+  AXK_REQUIRE(axk_launch_fits(nnz * (page_size / block_size)), AXK_E_SHAPE);
   if (type < 0) return -type;
   AXK_REQUIRE(axk_aligned(kv_cache, 16) && axk_aligned(bounds, 16) && axk_aligned(kv_scales, 2), AXK_E_ALIGN);
   const size_t row = (size_t)hkv * d, slots = (size_t)num_pages * page_size * 2;
   const size_t tb = (size_t)batch * 4;
-  const Span writes[] = {{bounds, (size_t)num_pages * (page_size / block_size) * row * 4}};
-  const Span reads[] = {{kv_cache, slots * row * (type ? 1 : 2)}, {kv_scales, slots * hkv * 2}, {indptr, tb + 4},
-                        {indices, (size_t)nnz * 4}, {last_page_len, tb}, {start, tb}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{bounds, (size_t)num_pages * (page_size / block_size) * row * 4}};
+  const AxkSpan reads[] = {{kv_cache, slots * row * (type ? 1 : 2)}, {kv_scales, slots * hkv * 2}, {indptr, tb + 4},
+                           {indices, (size_t)nnz * 4}, {last_page_len, tb}, {start, tb}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   if (nnz == 0) return AXK_OK;
   AXK_LAUNCH_GATE();
   auto* fn = type == kI8 ? &paged_key_bounds_kernel<kI8>
@@ -1636,7 +1598,7 @@ extern "C" int axk_paged_kv_write_bounds(const uint16_t* k, const uint16_t* v, v
                                          float kv_scale, uint16_t* bounds, const int32_t* cache_location, int64_t rows,
                                          int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t block_size,
                                          int64_t num_pages, int32_t* status, axk_stream_t stream) {
-  return kv_write_bounds(k, v, kv_cache, cache_type(kv_dtype, kv_scale), kv_scale, nullptr, bounds, cache_location, rows,
+  return kv_write_bounds(k, v, kv_cache, axk_kv_type(kv_dtype, kv_scale), kv_scale, nullptr, bounds, cache_location, rows,
                          num_kv_heads, head_dim, page_size, block_size, num_pages, status, stream);
 }
 
@@ -1654,7 +1616,7 @@ extern "C" int axk_paged_key_bounds(const void* kv_cache, int kv_dtype, float kv
                                     const int32_t* start, int64_t nnz, int64_t batch, int64_t num_kv_heads,
                                     int64_t head_dim, int64_t page_size, int64_t block_size, int64_t num_pages,
                                     int32_t* status, axk_stream_t stream) {
-  return key_bounds(kv_cache, cache_type(kv_dtype, kv_scale), kv_scale, nullptr, bounds, indptr, indices, last_page_len,
+  return key_bounds(kv_cache, axk_kv_type(kv_dtype, kv_scale), kv_scale, nullptr, bounds, indptr, indices, last_page_len,
                     start, nnz, batch, num_kv_heads, head_dim, page_size, block_size, num_pages, status, stream);
 }
 
@@ -1677,15 +1639,15 @@ extern "C" int axk_paged_block_scores(const uint16_t* q, const uint16_t* bounds,
   if (rc != AXK_OK) return rc;
   AXK_REQUIRE(num_qo_heads > 0 && num_qo_heads % num_kv_heads == 0 && num_qo_heads / num_kv_heads <= kMaxGroup, AXK_E_SHAPE);
   const int64_t total = nnz * (page_size / block_size), units = (total + 15) / 16 * num_kv_heads;
-  AXK_REQUIRE(launch_fits((units + 3) / 4, 256), AXK_E_SHAPE);
+  AXK_REQUIRE(axk_launch_fits((units + 3) / 4), AXK_E_SHAPE);
   AXK_REQUIRE(axk_aligned(q, 16) && axk_aligned(bounds, 16) && axk_aligned(scores, 4), AXK_E_ALIGN);
   if (nnz == 0) return AXK_OK;
   const size_t tb = (size_t)batch * 4;
-  const Span writes[] = {{scores, (size_t)num_kv_heads * total * 4}};
-  const Span reads[] = {{q, tb / 2 * num_qo_heads * head_dim},
-                        {bounds, (size_t)num_pages * (page_size / block_size) * num_kv_heads * head_dim * 4},
-                        {indptr, tb + 4}, {indices, (size_t)nnz * 4}, {last_page_len, tb}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{scores, (size_t)num_kv_heads * total * 4}};
+  const AxkSpan reads[] = {{q, tb / 2 * num_qo_heads * head_dim},
+                           {bounds, (size_t)num_pages * (page_size / block_size) * num_kv_heads * head_dim * 4},
+                           {indptr, tb + 4}, {indices, (size_t)nnz * 4}, {last_page_len, tb}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   AXK_LAUNCH_GATE();
   auto* fn = head_dim == 64 ? &paged_block_scores_kernel<64>
                             : head_dim == 128 ? &paged_block_scores_kernel<128> : &paged_block_scores_kernel<256>;
@@ -1707,12 +1669,12 @@ extern "C" int axk_paged_select_blocks(const float* scores, const int32_t* indpt
               AXK_E_SHAPE);
   const int64_t total = nnz * (page_size / block_size);
   const bool small = total <= 2048;  // every row at most eight keys a thread of 256
-  AXK_REQUIRE(launch_fits(batch * num_kv_heads, small ? 256 : 1024), AXK_E_SHAPE);
+  AXK_REQUIRE(axk_launch_fits(batch * num_kv_heads, small ? 256 : 1024), AXK_E_SHAPE);
   AXK_REQUIRE(axk_aligned(scores, 4) && axk_aligned(blocks, 4), AXK_E_ALIGN);
   const size_t tb = (size_t)batch * 4;
-  const Span writes[] = {{blocks, tb * num_kv_heads * num_select}};
-  const Span reads[] = {{scores, (size_t)num_kv_heads * total * 4}, {indptr, tb + 4}, {last_page_len, tb}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{blocks, tb * num_kv_heads * num_select}};
+  const AxkSpan reads[] = {{scores, (size_t)num_kv_heads * total * 4}, {indptr, tb + 4}, {last_page_len, tb}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   AXK_LAUNCH_GATE();
   const dim3 grid((unsigned)(batch * num_kv_heads));
   if (small)
@@ -1770,11 +1732,11 @@ int decode_blocks(const uint16_t* q, const void* kv_cache, int type, float kv_sc
   // (The merge reads the page table and the lists again, after the first kernel has written the workspace.)
   const size_t tb = (size_t)batch * 4, qb = tb / 2 * num_qo_heads * head_dim, wb = (size_t)num_kv_heads * nnz * 4;
   const size_t slots = (size_t)num_pages * page_size * 2 * num_kv_heads;
-  const Span writes[] = {{out, qb}, {weights_out, wb}, {workspace, need}};
-  const Span reads[] = {{q, qb}, {kv_cache, slots * head_dim * (type ? 1 : 2)}, {kv_scales, slots * 2}, {indptr, tb + 4},
-                        {indices, (size_t)nnz * 4}, {last_page_len, tb}, {blocks, tb * num_kv_heads * num_select},
-                        {weights_in == weights_out ? nullptr : weights_in, wb}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{out, qb}, {weights_out, wb}, {workspace, need}};
+  const AxkSpan reads[] = {{q, qb}, {kv_cache, slots * head_dim * (type ? 1 : 2)}, {kv_scales, slots * 2}, {indptr, tb + 4},
+                           {indices, (size_t)nnz * 4}, {last_page_len, tb}, {blocks, tb * num_kv_heads * num_select},
+                           {weights_in == weights_out ? nullptr : weights_in, wb}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   BlkArgs a;
   a.q = q;
   a.cache = static_cast<const unsigned char*>(kv_cache);
@@ -1828,7 +1790,7 @@ extern "C" int axk_paged_decode_blocks(const uint16_t* q, const void* kv_cache, 
                                        int64_t batch, int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim,
                                        int64_t page_size, int64_t num_pages, float sm_scale, int32_t* status,
                                        void* workspace, size_t workspace_bytes, axk_stream_t stream) {
-  return decode_blocks(q, kv_cache, cache_type(kv_dtype, kv_scale), kv_scale, nullptr, indptr, indices, last_page_len,
+  return decode_blocks(q, kv_cache, axk_kv_type(kv_dtype, kv_scale), kv_scale, nullptr, indptr, indices, last_page_len,
                        blocks, block_size, num_select, out, weights_in, weights_out, decay, nnz, batch, num_qo_heads,
                        num_kv_heads, head_dim, page_size, num_pages, sm_scale, status, workspace, workspace_bytes, stream);
 }
@@ -1856,9 +1818,9 @@ extern "C" int axk_paged_evict_pages(const float* weights, const int32_t* indptr
   const size_t ib = (size_t)nnz * 4, pb = (size_t)(batch + 1) * 4, wb = (size_t)num_kv_heads * nnz * 4;
   AXK_REQUIRE(axk_aligned(out_indptr, 4) && axk_aligned(out_indices, 4) && axk_aligned(out_weights, 4) && axk_aligned(freed, 4),
               AXK_E_ALIGN);
-  const Span writes[] = {{out_indptr, pb}, {out_indices, ib}, {out_weights, wb}, {freed, ib}};
-  const Span reads[] = {{weights, wb}, {indptr, pb}, {indices, ib}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{out_indptr, pb}, {out_indices, ib}, {out_weights, wb}, {freed, ib}};
+  const AxkSpan reads[] = {{weights, wb}, {indptr, pb}, {indices, ib}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   AXK_LAUNCH_GATE();
   hipLaunchKernelGGL(paged_evict_kernel, dim3((unsigned)batch), dim3(kEvict), 0, axk_stream(stream), weights, indptr, indices,
                      out_indptr, out_indices, out_weights, freed, (int)nnz, (int)batch, (int)num_kv_heads, (int)budget,

@@ -23,20 +23,15 @@
 // read 1.04 times (a KV head's row blocks read a piece through one L2). Its nodes fill 25 of 32 blocks; cutting the work into
 // equal shares of the 25 measured the same time (594 and 611 us), with twice the partials.
 #pragma once
-#include <math.h>
-
-#include <type_traits>
-
 #include "axk_common.h"
 #include "axk_host.h"
 #include "axk_tree_common.h"
 
 namespace axk_tree {
 
-typedef float axk_f32x16 __attribute__((ext_vector_type(16)));
 typedef int axk_i32x4 __attribute__((ext_vector_type(4)));
 
-enum { kBf16 = 0, kFp8 = 1, kI8 = 2 };  // stored as bf16, as E4M3 of x * kv_scale, as int8 codes with a bf16 scale per row
+enum { kBf16 = AXK_KV_BF16, kFp8 = AXK_KV_FP8, kI8 = AXK_KV_I8 };
 constexpr int kTile = 16;
 constexpr int kPair = 32;
 constexpr int kMergeRows = 4;           // rows (waves) of a merge workgroup
@@ -74,20 +69,9 @@ AXK_DEV Seq seq_from(int lo, int hi, int last, int page, int nnz) {
 }
 AXK_DEV int pairs_of(const Seq& s) { return (s.len + kPair - 1) / kPair; }
 
-// Inclusive sum over the lanes of a wave.
-AXK_DEV int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-  return v;
-}
-
-// A batch of more sequences is not cut: it fills the device by its number, and looking a piece up among its sequences would cost more than
-// the rounds that long ones stand out by. Us with and without, 2 heads of 128: 512 sequences of up to 1000 tokens 128 and 88, 1000
-// of them 295 and 167; 48 sequences of up to 2000 tokens (2 heads of 256) 39.7 and 49.4.
+// A batch of more sequences is not cut: it fills the device by its number, and looking a piece up among its sequences would cost
+// more than the rounds that long ones stand out by. Us with and without, 2 heads of 128: 512 sequences of up to 1000 tokens 128
+// and 88, 1000 of them 295 and 167; 48 sequences of up to 2000 tokens (2 heads of 256) 39.7 and 49.4.
 constexpr int kSplitBatch = 256;
 
 // How the batch is cut: every sequence into pieces of P pairs, P such that the pieces of all row blocks and KV heads run at
@@ -137,8 +121,8 @@ AXK_DEV Piece find_piece(const TreeArgs& a, int want, bool by_piece, int kg) {
   int p = max(a.min_piece, (int)fminf(total / (float)a.den, 0x1p28f) + 1);  // (offsets that fall back may add up to any total)
   if (longest <= 1.5f * (float)p) p = max(p, (int)longest);  // sequences even enough to be left whole
   auto whole_groups = [&](int x) { return (x + kg - 1) / kg * kg; };
-  // How many pieces: n / size rounded up is (n - 1/2) / size rounded down, and 1 (to 2^21 pairs a sequence; beyond, the number may
-  // be off by one, which changes the cut, not its bound).
+  // How many pieces: n / size rounded up is (n - 1/2) / size rounded down, and 1 (to 2^21 pairs a sequence; beyond, the number
+  // may be off by one, which changes the cut, not its bound).
   auto pieces = [&](int size) {
     const float each = __builtin_amdgcn_rcpf((float)size);
     int n = 0;
@@ -217,10 +201,6 @@ struct TreeCfg {
   }
 };
 
-AXK_DEV axk_f32x16 mfma_bf16_32x32x16(axk_bf16x8 a, axk_bf16x8 b, axk_f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
 // Eight stored 8-bit values (two dwords) as bf16: E4M3 times a power of two, or int8 codes, both exact.
 template <int T>
 AXK_DEV axk_bf16x8 bf16_of(uint32_t w0, uint32_t w1, float inv_scale) {
@@ -247,16 +227,6 @@ AXK_DEV void lds_dma2(const void* gptr, uint32_t lds_base_any) {
       :
       : "s"(lds_base), "v"(gptr)
       : "memory");
-}
-
-// f(std::integral_constant<int, 0>) .. f(<N - 1>): an unrolled loop whose index is a constant expression.
-template <typename F, int... I>
-AXK_DEV void for_each_index_of(F& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-AXK_DEV void for_each_index(F&& f) {
-  for_each_index_of(f, std::make_integer_sequence<int, N>{});
 }
 
 template <int D, int T, int RT, int WR>

@@ -143,34 +143,6 @@ void launch_rope(const RopeArgs& a, int d, int64_t grid, hipStream_t st) {
   }
 }
 
-// Arrays that a call writes overlap neither what it reads nor each other.
-struct Span {
-  const void* p;
-  size_t n;
-};
-template <int W, int R>
-bool disjoint(const Span (&writes)[W], const Span (&reads)[R]) {
-  for (int i = 0; i < W; ++i) {
-    for (const Span& r : reads)
-      if (axk_overlap(writes[i].p, writes[i].n, r.p, r.n)) return false;
-    for (int j = 0; j < i; ++j)
-      if (axk_overlap(writes[i].p, writes[i].n, writes[j].p, writes[j].n)) return false;
-  }
-  return true;
-}
-
-// Whether a launch of 256 threads holds these workgroups: its threads are counted in 32 bits.
-bool launch_fits(int64_t workgroups) { return workgroups <= (int64_t)0xffffffff / 256; }
-
-// The stored type of a cache by its dtype code (kBf16 or kFp8, the latter with a power-of-two scale); negative: refused.
-int cache_type(int kv_dtype, float kv_scale) {
-  if (kv_dtype == AXK_DT_BF16) return kBf16;
-  if (kv_dtype != AXK_DT_FP8E4M3) return -AXK_E_DTYPE;
-  int e = 0;
-  const float m = frexpf(kv_scale, &e);
-  return kv_scale > 0.f && m == 0.5f && e >= -125 && e <= 126 ? kFp8 : -AXK_E_SHAPE;
-}
-
 bool head_dim_ok(int64_t d) { return d == 64 || d == 128 || d == 256; }
 bool page_ok(int64_t page) { return page >= 16 && page % 16 == 0 && page <= 4096; }
 
@@ -203,16 +175,16 @@ int write_rope(const uint16_t* q, int64_t ldq, int64_t hdq, const uint16_t* k, i
               AXK_E_ALIGN);
   if (rows == 0) return AXK_OK;
   const int64_t grid = (rows * (hq + 2 * hkv) * (d / 8) + 255) / 256;
-  AXK_REQUIRE(launch_fits(grid), AXK_E_SHAPE);
+  AXK_REQUIRE(axk_launch_fits(grid), AXK_E_SHAPE);
   const size_t slots = (size_t)num_pages * page_size * 2 * hkv, tab = (size_t)table_rows * (rot / 2) *
                                                                      (table_dtype == AXK_DT_F32 ? 4 : 2);
-  const Span writes[] = {{q_out, (size_t)rows * hq * d * 2}, {cache, slots * d * (type == kBf16 ? 2 : 1)}, {scales, slots * 2},
-                         {status, 4}};
-  const Span reads[] = {{q, q ? span_of(rows, hq, ldq, hdq, d) * 2 : 0}, {k, span_of(rows, hkv, ldk, hdk, d) * 2},
-                        {v, span_of(rows, hkv, ldv, hdv, d) * 2}, {q_norm, (size_t)d * 4}, {k_norm, (size_t)d * 4},
-                        {rot ? cos : nullptr, tab}, {rot ? sin : nullptr, tab}, {positions, (size_t)rows * 4},
-                        {loc, (size_t)rows * 8}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{q_out, (size_t)rows * hq * d * 2}, {cache, slots * d * (type == kBf16 ? 2 : 1)}, {scales, slots * 2},
+                            {status, 4}};
+  const AxkSpan reads[] = {{q, q ? span_of(rows, hq, ldq, hdq, d) * 2 : 0}, {k, span_of(rows, hkv, ldk, hdk, d) * 2},
+                           {v, span_of(rows, hkv, ldv, hdv, d) * 2}, {q_norm, (size_t)d * 4}, {k_norm, (size_t)d * 4},
+                           {rot ? cos : nullptr, tab}, {rot ? sin : nullptr, tab}, {positions, (size_t)rows * 4},
+                           {loc, (size_t)rows * 8}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   RopeArgs a;
   a.q = q, a.k = k, a.v = v;
   a.ldq = ldq, a.hdq = hdq, a.ldk = ldk, a.hdk = hdk, a.ldv = ldv, a.hdv = hdv;
@@ -294,15 +266,15 @@ int tree_verify(const uint16_t* q, const void* cache, int type, float kv_scale, 
   const TreePlan p = tree_plan(batch, nodes, hq, hkv, d, (nnz * page + 31) / 32);
   // (a merge always fits: where a sequence may be cut, den > 1, so that it has at most 128 blocks of up to 256 rows, or 256 of 64,
   // in at most kSplitBatch sequences: 2^23 waves)
-  AXK_REQUIRE(launch_fits(p.nb * (p.groups + 7)), AXK_E_SHAPE);
+  AXK_REQUIRE(axk_launch_fits(p.nb * (p.groups + 7)), AXK_E_SHAPE);
   const size_t need = p.ml + p.po;
   AXK_REQUIRE(!need || (workspace && workspace_bytes >= need && axk_aligned(workspace, 256)), AXK_E_WORKSPACE);
   const size_t qb = (size_t)batch * nodes * hq * d * 2, slots = (size_t)num_pages * page * 2 * hkv;
-  const Span writes[] = {{out, qb}, {workspace, need}, {status, 4}};
-  const Span reads[] = {{q, qb}, {cache, slots * d * (type == kBf16 ? 2 : 1)}, {scales, slots * 2},
-                        {indptr, (size_t)(batch + 1) * 4}, {indices, (size_t)nnz * 4}, {last, (size_t)batch * 4},
-                        {parents, (size_t)batch * nodes * 4}};
-  AXK_REQUIRE(disjoint(writes, reads), AXK_E_ALIAS);
+  const AxkSpan writes[] = {{out, qb}, {workspace, need}, {status, 4}};
+  const AxkSpan reads[] = {{q, qb}, {cache, slots * d * (type == kBf16 ? 2 : 1)}, {scales, slots * 2},
+                           {indptr, (size_t)(batch + 1) * 4}, {indices, (size_t)nnz * 4}, {last, (size_t)batch * 4},
+                           {parents, (size_t)batch * nodes * 4}};
+  AXK_REQUIRE(axk_disjoint(writes, reads), AXK_E_ALIAS);
   axk_tree::TreeArgs a;
   a.q = q;
   a.cache = static_cast<const unsigned char*>(cache);
@@ -333,7 +305,7 @@ extern "C" int axk_paged_kv_write_rope(const uint16_t* q, int64_t ldq, int64_t h
                                        int64_t head_dim, int64_t rot, int64_t page_size, int64_t num_pages, float eps,
                                        int32_t* status, axk_stream_t stream) {
   return write_rope(q, ldq, hdq, k, ldk, hdk, v, ldv, hdv, q_norm, k_norm, cos, sin, table_dtype, table_rows, positions,
-                    cache_location, q_out, kv_cache, cache_type(kv_dtype, kv_scale), kv_scale, nullptr, rows, num_qo_heads,
+                    cache_location, q_out, kv_cache, axk_kv_type(kv_dtype, kv_scale), kv_scale, nullptr, rows, num_qo_heads,
                     num_kv_heads, head_dim, rot, page_size, num_pages, eps, status, stream);
 }
 
@@ -363,7 +335,7 @@ extern "C" int axk_paged_tree_verify(const uint16_t* q, const void* kv_cache, in
                                      int64_t num_qo_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
                                      int64_t num_pages, float sm_scale, int32_t* status, void* workspace,
                                      size_t workspace_bytes, axk_stream_t stream) {
-  return tree_verify(q, kv_cache, cache_type(kv_dtype, kv_scale), kv_scale, nullptr, indptr, indices, last_page_len, parents,
+  return tree_verify(q, kv_cache, axk_kv_type(kv_dtype, kv_scale), kv_scale, nullptr, indptr, indices, last_page_len, parents,
                      out, nnz, batch, nodes, num_qo_heads, num_kv_heads, head_dim, page_size, num_pages, sm_scale, status,
                      workspace, workspace_bytes, stream);
 }
