@@ -13,6 +13,13 @@ been accepted, its rows go to their final places, and the states to its last nod
     store_paged_kv_rope(k, v, kv_cache, final_loc, cos, sin, positions, k_norm=kn)  # page -1: rows that are not kept
     gdn_tree_commit(state, k, updates, gates, parents, accepted, state_out=state)
 
+The GDN calls take q, k and v behind the layer's causal convolution, contiguous. Along a tree a node's window holds the inputs
+before it on its branch, not in the rows before: causal_conv1d_silu computes it with every node as a sequence of one row,
+x.view(B * T, 1, C), and as its state the K - 1 inputs before the node, gathered from [conv state | x] along its parents; those up
+to the accepted node are the next conv state. Value head h reads key head h // (NV // NK), the "grouped" order, as in
+gdn_recurrent. In a layer of the "tiled" order (the default of axk.layer), where it reads head h % NK, q and k are passed repeated
+to NV heads: q.repeat(1, 1, NV // NK, 1). The calls of whole layers, attn_layer_verify and gdn_layer_verify, verify chains.
+
 Caches are those of paged_decode (bf16), paged_decode_fp8 (u8 / float8_e4m3fn with ``kv_scale``) and paged_decode_i8 (int8 with
 ``kv_scales``), page tables theirs too. Nothing is read back to the host, so a step can be captured in a HIP graph. Contract
 violations raise ValueError; what only the device sees (a bad parent, page, slot, position) sets ``status`` (int32 [1]) to 1.
@@ -217,9 +224,10 @@ def gdn_tree_verify(
     status: Optional[torch.Tensor] = None,
 ):
     """gdn_recurrent along every branch of the trees: q, k [B, T, NK, 128] bf16; v [B, T, NV, 128] bf16; a, b [B, T, NV] bf16;
-    a_log, dt_bias [NV] f32; state [B, NV, 128, 128] f32, the state before the trees, only read; parents int32 [B, T]. Returns
+    a_log, dt_bias [NV] f32; state [B, NV, 128, 128] f32, the state before the trees, only read; parents int32 [B, T]; all
+    contiguous, value heads in the grouped order (the module's head says what a layer of the other order passes). Returns
     (output bf16 [B, T, NV, 128], updates f32 [B, T, NV, 128], gates f32 [B, T, NV]): every node's output, its rank-1 update
-    and log decay, which gdn_tree_commit takes; zeros where there is no node."""
+    and log decay (may be -inf), which gdn_tree_commit takes; zeros where there is no node."""
     if v.dim() != 4 or v.dtype is not _BF16 or not v.is_contiguous():
         raise ValueError("v must be contiguous bf16 [B, T, NV, 128]")
     nv = v.shape[2]

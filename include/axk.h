@@ -555,7 +555,9 @@ int axk_paged_tree_verify_i8(const uint16_t* q, const int8_t* kv_cache, const ui
  * 128], a, b [batch, nodes, num_v_heads]; node t continues the state after its parent, a node with parent -1 state f32 [batch,
  * num_v_heads, 128, 128], which is only read. out bf16 like v; updates f32 like v, each node's rank-1 update u = beta (v - k^T
  * S); gates f32 [batch, nodes, num_v_heads], its log decay g, which may be -inf; all zero where there is no node. A chain's
- * outputs are those of axk_gdn_recurrent. Value head h reads key head h / (num_v_heads / num_k_heads). batch * num_v_heads <= 2^20. */
+ * outputs are those of axk_gdn_recurrent. q, k and v are those behind a layer's causal convolution (along a tree: of each node's
+ * branch). Value head h reads key head h / (num_v_heads / num_k_heads), AXK_VORDER_GROUPED; for AXK_VORDER_TILED pass q and k with
+ * their heads repeated to num_v_heads. batch * num_v_heads <= 2^20. */
 int axk_gdn_tree_verify(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* a, const uint16_t* b,
                         const float* a_log, const float* dt_bias, const float* state, const int32_t* parents, uint16_t* out,
                         float* updates, float* gates, int64_t batch, int64_t nodes, int64_t num_k_heads, int64_t num_v_heads,
