@@ -327,7 +327,7 @@ __global__ __launch_bounds__(64 * W, TT == 1 ? 3 : TT == 2 ? 2 : 1) void gdn_tre
 
 // The accepted branch applied to the state: S' = e^{G_n} S_0 + sum_{i in A(n)} e^{G_n - G_i} k_i u_i^T, each workgroup 32 rows
 // of one head's state, each thread 4 of them x 4 columns. One read and one write of the state and the branch's rows of u bound it:
-// 32 sequences x 32 heads in 23 us, 5.9 TB/s; a single sequence's 4 MB take 5.7 us, a launch's latency and two dependent loads.
+// 32 sequences x 32 heads in 24.4 us, 5.7 TB/s; a single sequence's 4 MB take 5.5 us, a launch's latency and two dependent loads.
 struct TreeCommit {
   const float* state;
   const uint16_t* k;
@@ -418,8 +418,8 @@ int check(int64_t batch, int64_t nodes, int64_t nk, int64_t nv, int64_t dk, int6
 template <int TT>
 void launch_verify(const TreeGdn& p, int64_t heads, hipStream_t st) {
   // One wave a workgroup spreads few heads over the CUs, but every wave then works out the heads' weights alone. Us for W = 1 and
-  // W = 4, at 32 heads a sequence: 8 nodes x 1 sequence 7.8 and 9.0, x 8 9.5 and 10.0, x 16 13.9 and 13.1; 32 nodes x 1 12.8 and
-  // 12.5, x 8 18.0 and 14.9; 64 nodes x 1 29.2 and 23.8, x 8 39.6 and 27.2.
+  // W = 4, at 32 heads a sequence: 8 nodes x 1 sequence 7.9 and 9.2, x 8 10.4 and 10.4, x 16 14.1 and 13.4; 32 nodes x 1 13.4 and
+  // 13.0, x 8 18.3 and 15.0; 64 nodes x 1 29.8 and 24.4, x 8 39.5 and 27.0.
   if constexpr (TT == 1)
     if (heads <= 256) {
       hipLaunchKernelGGL((gdn_tree_verify_kernel<1, 1>), dim3((unsigned)(4 * heads)), dim3(64), 0, st, p);

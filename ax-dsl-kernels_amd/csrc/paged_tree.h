@@ -17,11 +17,13 @@
 // are exact in bf16; scores, maxima, sums, O and the pieces' partials are fp32. The maximum that weights refer to follows the
 // scores only in steps of more than 2^8, which rescales O rarely and changes no bit of what is represented.
 //
-// What bounds it. Few rows: HBM and the start of a piece (lookup, first page, first pair). Many rows: a wave's instructions, not
+// What bounds it. Few rows: the start and the end of a piece (lookup, first page, first pair, join), run once and waiting for 57%
+// of the time: one draft of 8 nodes, pieces of four pairs, takes 16.6 us and a merge of 7. Many rows: a wave's instructions, not
 // the matrix cores: one wave a SIMD (O and Q take 3 RT D / 4 of its registers) issues 381 instructions a pair in the loop without
-// masks, of which 32 are MFMAs. 8 sequences of 32768 tokens x 64 nodes x 32 heads of 256: 570-640 us traced, 560-630 TFLOP/s, HBM
-// read 1.04 times (a KV head's row blocks read a piece through one L2). Its nodes fill 25 of 32 blocks; cutting the work into
-// equal shares of the 25 measured the same time (594 and 611 us), with twice the partials.
+// masks, of which 32 are MFMAs; it issues in 58% of its cycles and waits in 30, its matrix core works in 42. 8 sequences of 32768
+// tokens x 64 nodes x 32 heads of 256: 565-580 us a replay, 620-630 TFLOP/s, HBM read 1.1 times (a KV head's row blocks read a
+// piece through one L2). Its nodes fill 25 of 32 blocks; cutting the work into equal shares of the 25 measured the same time (594
+// and 611 us), with twice the partials.
 #pragma once
 #include "axk_common.h"
 #include "axk_host.h"
@@ -70,8 +72,8 @@ AXK_DEV Seq seq_from(int lo, int hi, int last, int page, int nnz) {
 AXK_DEV int pairs_of(const Seq& s) { return (s.len + kPair - 1) / kPair; }
 
 // A batch of more sequences is not cut: it fills the device by its number, and looking a piece up among its sequences would cost
-// more than the rounds that long ones stand out by. Us with and without, 2 heads of 128: 512 sequences of up to 1000 tokens 128
-// and 88, 1000 of them 295 and 167; 48 sequences of up to 2000 tokens (2 heads of 256) 39.7 and 49.4.
+// more than the rounds that long ones stand out by. Us with and without, 2 heads of 128: 512 sequences of up to 1000 tokens 121
+// and 67, 1000 of them 313 and 137; 48 sequences of up to 2000 tokens (2 heads of 256) 38 and 49.
 constexpr int kSplitBatch = 256;
 
 // How the batch is cut: every sequence into pieces of P pairs, P such that the pieces of all row blocks and KV heads run at
@@ -79,7 +81,7 @@ constexpr int kSplitBatch = 256;
 // 2 heads of 256: 128 us, with total / den 167). Else P is total / den, and pieces follow one another: short sequences are pieces
 // of their own, and a P that keeps their number down leaves a long one whole (131072 tokens beside 63 of 200, 8 heads of 256:
 // 248 us, as one piece 3480). There are at most den + batch. Where the first P would cut the longest sequence once and not far
-// from its end, all are left whole: 128 sequences of up to 1000 tokens, 4 nodes x 16 heads of 256, 65 us with the cut and 49
+// from its end, all are left whole: 128 sequences of 500 to 1000 tokens, 4 nodes x 16 heads of 256, 55 us with the cut and 52
 // without. Every wave of both launches derives the same cut from the page table: the total is a float sum in a fixed order.
 struct Piece {
   int b;       // sequence (-1: none)

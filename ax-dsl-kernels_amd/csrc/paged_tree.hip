@@ -48,8 +48,8 @@ AXK_DEV axk_u32x4 pack8(const float (&x)[8]) {
 // (y = x rsqrt(mean x^2 + eps) w) and channel pairs (i, i + rot / 2), i < rot / 2, turned by the row's angle, all in fp32 and
 // rounded once, to what is stored: bf16, E4M3 of y * kv_scale, or int8 codes of the row's scale. A lane of a turned chunk
 // loads its partner chunk too, which costs a cached load and no exchange. One launch for what a norm, a rotation and a store do in
-// three: 4096 rows of 32 + 8 + 8 heads of 128 in 22.5 us, 4.6 TB/s of the 103 MB that they cannot do without; 16 rows in 3.9 us,
-// a launch and two dependent loads.
+// three: 4096 rows of 32 + 8 + 8 heads of 128 in 22.6 us (FP8 25.4, INT8 23.2), 4.5 TB/s of the 103 MB that they cannot do without;
+// 16 rows in 4.1 us (4.6, 4.2), a launch and two dependent loads.
 template <int D, int T, typename TAB>
 __global__ __launch_bounds__(256) void paged_kv_write_rope_kernel(RopeArgs a) {
   constexpr int LPH = D / 8;  // lanes of a head
@@ -212,8 +212,8 @@ int write_rope(const uint16_t* q, int64_t ldq, int64_t hdq, const uint16_t* k, i
 }
 
 // ---- the tree's attention: how it is cut, from what the host knows ----
-// A piece's least pairs of tokens. Us with 8, 4 and 2, 16 heads of 256: one sequence of 600 tokens 21.7, 18.9 and 16.5; of 5003
-// tokens 24.1, 23.8 and 27.6, where shorter pieces cost more in the merge than their loops save.
+// A piece's least pairs of tokens. Us with 8, 4 and 2, 16 heads of 256: one sequence of 600 tokens 20.6, 20.4 and 19.0; of 5003
+// tokens 24.8, 24.6 and 28.1, where shorter pieces cost more in the merge than their loops save.
 constexpr int kMinPiece = 4;
 struct TreePlan {
   int rb, nb, den, split;
@@ -226,10 +226,11 @@ TreePlan tree_plan(int64_t batch, int64_t nodes, int64_t hq, int64_t hkv, int64_
   TreePlan p;
   const int64_t rows = nodes * (hq / hkv);
   // Rows of a workgroup: two waves of rows and two of tokens up to 64 rows, as many rows as the registers hold beyond. Us with the
-  // other choice, for up to 64 rows 128: 16 sequences of 8000 tokens x 8 heads of 128 x 64 rows 89.6 against 107.8, 2 heads of 256
-  // x 64 rows 51.2 against 55.0 (FP8 45.5 against 54.7); for 96 rows of 128 channels 256: 67.3 against 98.3 (INT8 86.7 against
-  // 139.8). Beyond 128 rows: 256 rows of 128 channels 124.8 against 133.7 with 128, but of 64 channels 282 against 242 (K and V of
-  // a step are then so short that the larger block waits for them); 512 rows of 256 channels 587 against 810 with 64.
+  // rule and the other choice, 16 sequences of 8000 tokens: 64 rows of 128 channels (8 KV heads) with 64 and 128 115 and 124 (FP8 69
+  // and 115, INT8 90 and 150), of 256 channels (2 heads) 59 and 63 (FP8 49 and 62, INT8 61 and 88); 96 rows of 128 channels (4
+  // heads) with 128 and 256 75 and 106 (INT8 91 and 142). Beyond 128 rows, 8 sequences of 32768 tokens: of 128 channels with 256 and
+  // 128 160 rows 370 and 409, 256 rows 399 and 413, 1024 rows 364 and 369 (256 rows of 16 x 8000 135 and 132); 512 rows of 256
+  // channels with 128 and 64 653 and 804. Blocks of 256 rows of 64 channels measured 494 against 511, too little for a variant.
   p.rb = rows <= 64 ? 64 : rows > 128 && d == 128 ? 256 : 128;
   const int64_t nb = (rows + p.rb - 1) / p.rb;
   p.nb = (int)nb;
