@@ -226,10 +226,10 @@ TreePlan tree_plan(int64_t batch, int64_t nodes, int64_t hq, int64_t hkv, int64_
   TreePlan p;
   const int64_t rows = nodes * (hq / hkv);
   // Rows of a workgroup: two waves of rows and two of tokens up to 64 rows, as many rows as the registers hold beyond. Us with the
-  // rule and the other choice, 16 sequences of 8000 tokens: 64 rows of 128 channels (8 KV heads) with 64 and 128 115 and 124 (FP8 69
-  // and 115, INT8 90 and 150), of 256 channels (2 heads) 59 and 63 (FP8 49 and 62, INT8 61 and 88); 96 rows of 128 channels (4
-  // heads) with 128 and 256 75 and 106 (INT8 91 and 142). Beyond 128 rows, 8 sequences of 32768 tokens: of 128 channels with 256 and
-  // 128 160 rows 370 and 409, 256 rows 399 and 413, 1024 rows 364 and 369 (256 rows of 16 x 8000 135 and 132); 512 rows of 256
+  // rule and the other choice, 16 sequences of 8000 tokens: 64 rows of 128 channels (8 KV heads) with 64 and 128 115 and 124 (FP8
+  // 69 and 115, INT8 90 and 150), of 256 channels (2 heads) 59 and 63 (FP8 49 and 62, INT8 61 and 88); 96 rows of 128 channels
+  // (4 heads) with 128 and 256 75 and 106 (INT8 91 and 142). Beyond 128 rows, 8 sequences of 32768 tokens: of 128 channels with 256
+  // and 128 160 rows 370 and 409, 256 rows 399 and 413, 1024 rows 364 and 369 (256 rows of 16 x 8000 135 and 132); 512 rows of 256
   // channels with 128 and 64 653 and 804. Blocks of 256 rows of 64 channels measured 494 against 511, too little for a variant.
   p.rb = rows <= 64 ? 64 : rows > 128 && d == 128 ? 256 : 128;
   const int64_t nb = (rows + p.rb - 1) / p.rb;

@@ -530,11 +530,12 @@ int axk_paged_kv_write_rope_i8(const uint16_t* q, int64_t ldq, int64_t hdq, cons
 
 /* Attention of a tree's nodes over the paged cache: q, out bf16 [batch, nodes, num_qo_heads, head_dim]. The page table covers
  * the history and the sequence's n nodes (those up to its last that is one), whose K / V are its last n cached tokens, node t
- * at n - t from the end; node t attends the history, its ancestors and itself. Rows that attend nothing are zero. A chain
- * (parents -1, 0, 1, ..) is axk_paged_prefill over the same rows. Cache, page table and page size as axk_paged_decode;
- * num_qo_heads / num_kv_heads <= 16, num_kv_heads <= 4096, batch <= 2^20. nnz: the entries of indices; offsets of indptr past it
- * are read as nnz, negative ones as 0, a last_page_len past page_size as page_size; nnz * page_size < 2^31 - 256. A page id
- * outside [0, num_pages) is skipped, never read, and a sequence of fewer cached tokens than nodes gets zeros; both set *status.
+ * at n - t from the end; node t attends the history, its ancestors and itself. Rows that attend nothing, or nothing but scores
+ * of -inf, are zero. A chain (parents -1, 0, 1, ..) is axk_paged_prefill over the same rows. Cache, page table and page size as
+ * axk_paged_decode; num_qo_heads / num_kv_heads <= 16, num_kv_heads <= 4096, batch <= 2^20. nnz: the entries of indices; offsets
+ * of indptr past it are read as nnz, negative ones as 0, a last_page_len past page_size as page_size; nnz * page_size < 2^31 -
+ * 256. A page id outside [0, num_pages) is skipped, never read, and a sequence of fewer cached tokens than nodes gets zeros; both
+ * set *status.
  * workspace: the fp32 partial outputs of sequences that are cut into pieces, 256-byte aligned, of
  * axk_paged_tree_verify_workspace_size bytes (0: may be NULL, or an unsupported shape); it carries nothing from call to call,
  * and calls that may run at the same time need one each. Equal calls give equal bits. */
