@@ -887,8 +887,9 @@ __global__ __launch_bounds__(256, (TreeCfg<D, T, RT, WR>::OCC)) void paged_tree_
       *reinterpret_cast<axk_u32x4*>(a.out + qrow[t] * D + 16 * i + 8 * h) = axk_u32x4{w0[0], w1[0], w0[1], w1[1]};
     }
   }
-  // What was taken out of V, added to the rows that see it (each lane to four of every eight channels of its rows). Whole pairs
-  // were looked through, from the first that holds a node (KG = 2: of the two of its step).
+  // What was taken out of V, added to the rows that see it (each lane to four of every eight channels of its rows; an infinity
+  // under a score of -inf, too, counts as one and not as 0 times it). Whole pairs were looked through, from the first that holds a
+  // node (KG = 2: of the two of its step).
   // s_odd was last written before the last step's barrier.
   if (T != kI8 && __builtin_expect(*s_odd != 0, 0)) {
     wait_vmcnt<0>();
